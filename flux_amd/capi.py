@@ -32,7 +32,7 @@ EXPORTS = (
     "fluxmi_grouped_gemm_dual_tiles",
     "fluxmi_grouped_gemm_multi", "fluxmi_grouped_gemm_topk_reduce_workspace_bytes",
     "fluxmi_grouped_gemm_topk_reduce", "fluxmi_grouped_gemm_blockscale",
-    "fluxmi_topk_gather_reduce", "fluxmi_quant_e4m3_rowwise", "fluxmi_quant_e4m3_square",
+    "fluxmi_topk_gather_reduce", "fluxmi_moe_permute", "fluxmi_moe_unpermute", "fluxmi_moe_unpermute_backward", "fluxmi_quant_e4m3_rowwise", "fluxmi_quant_e4m3_square",
     "fluxmi_quant_e4m3_block128", "fluxmi_quant_e4m3_block128_filled", "fluxmi_calib_stream_sink_bytes", "fluxmi_calib_stream",
 )
 
@@ -98,6 +98,9 @@ def load():
     lib.fluxmi_grouped_gemm_blockscale.argtypes = [ctypes.POINTER(GroupedGemmArgs), vp, i32, vp, i32, vp]
     lib.fluxmi_grouped_gemm_multi.argtypes = [ctypes.POINTER(GroupedGemmArgs), i32, vp, vp, vp, vp, sz, vp]
     lib.fluxmi_topk_gather_reduce.argtypes = [ctypes.POINTER(vp), i32, i32, vp, vp, f32, i32, i32, i32, vp, vp]
+    lib.fluxmi_moe_permute.argtypes = [vp, vp, i32, i32, i64, vp, vp]
+    lib.fluxmi_moe_unpermute.argtypes = [vp, i32, vp, vp, i32, i32, i32, i32, vp, vp]
+    lib.fluxmi_moe_unpermute_backward.argtypes = [vp, vp, i32, vp, vp, i32, i32, i32, i32, vp, vp, vp]
     lib.fluxmi_quant_e4m3_rowwise.argtypes = [vp, i64, i64, i32, f32, vp, vp, i32, vp]
     lib.fluxmi_quant_e4m3_square.argtypes = [vp, i64, i64, i64, f32, vp, vp, vp, vp, vp]
     lib.fluxmi_quant_e4m3_block128.argtypes = [vp, i64, i64, f32, vp, vp, vp, vp, vp]
@@ -389,6 +392,46 @@ def topk_gather_reduce(inputs, routing_idx, topk, row_weight=None, scale=1.0, ou
     _check(lib.fluxmi_topk_gather_reduce(ptrs, len(inputs), io_format, _ptr(routing_idx), _ptr(row_weight),
                                          float(scale), ntokens, topk, n, _ptr(out), _stream()),
            "fluxmi_topk_gather_reduce")
+    return out
+
+
+_ROW_TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+
+
+def moe_permute(x, scatter_index, out=None):
+    """rows[scatter_index[t, j]] = x[t] (fluxmi_moe_permute); rows that no entry names are 0."""
+    lib = load()
+    _dev_tensor(x, x.dtype, "x")
+    _dev_tensor(scatter_index, torch.int32, "scatter_index")
+    tokens, topk = scatter_index.shape
+    if x.shape[0] != tokens:
+        raise ValueError(f"x has {x.shape[0]} rows, scatter_index {tokens}")
+    if out is None:
+        out = torch.empty(tokens * topk, x.shape[1], dtype=x.dtype, device=x.device)
+    _dev_tensor(out, x.dtype, "out")
+    if out.shape != (tokens * topk, x.shape[1]):
+        raise ValueError(f"out {tuple(out.shape)} is not [{tokens * topk}, {x.shape[1]}]")
+    _check(lib.fluxmi_moe_permute(_ptr(x), _ptr(scatter_index), tokens, topk, x.shape[1] * x.element_size(), _ptr(out), _stream()),
+           "fluxmi_moe_permute")
+    return out
+
+
+def moe_unpermute(rows, scatter_index, weights=None):
+    """out[t] = sum_j weights[t, j] * rows[scatter_index[t, j]] (fluxmi_moe_unpermute)."""
+    lib = load()
+    _dev_tensor(rows, rows.dtype, "rows")
+    _dev_tensor(scatter_index, torch.int32, "scatter_index")
+    tokens, topk = scatter_index.shape
+    if rows.dtype not in _ROW_TYPES or rows.shape[0] != tokens * topk:
+        raise ValueError(f"rows must be bf16, fp16 or fp32 [{tokens * topk}, N], got {rows.dtype} {tuple(rows.shape)}")
+    if weights is not None:
+        _dev_tensor(weights, weights.dtype, "weights")
+        if weights.dtype not in _ROW_TYPES or weights.shape != scatter_index.shape:
+            raise ValueError(f"weights must be bf16, fp16 or fp32 {tuple(scatter_index.shape)}")
+    out = torch.empty(tokens, rows.shape[1], dtype=rows.dtype, device=rows.device)
+    _check(lib.fluxmi_moe_unpermute(_ptr(rows), _ROW_TYPES[rows.dtype], _ptr(scatter_index), _ptr(weights),
+                                    1 if weights is None else _ROW_TYPES[weights.dtype], tokens, topk, rows.shape[1], _ptr(out),
+                                    _stream()), "fluxmi_moe_unpermute")
     return out
 
 

@@ -175,6 +175,11 @@ PYBIND11_MODULE(flux_ths_pybind, m) {
   m.def("topk_scatter_reduce", &topk_scatter_reduce, py::arg("inputs"), py::arg("scatter_idx"), py::arg("TOPK"));
   m.def("topk_weighted_gather_reduce", &topk_weighted_gather_reduce, py::arg("inputs"), py::arg("routing_idx"),
         py::arg("topk"), py::arg("row_weight") = py::none(), py::arg("scale") = 1.0);
+  m.def("moe_permute", &moe_permute, py::arg("input"), py::arg("scatter_index"));
+  m.def("moe_permute_backward", &moe_permute_backward, py::arg("grad_rows"), py::arg("scatter_index"));
+  m.def("moe_unpermute", &moe_unpermute, py::arg("rows"), py::arg("scatter_index"), py::arg("weights") = py::none());
+  m.def("moe_unpermute_backward", &moe_unpermute_backward, py::arg("grad_out"), py::arg("rows"), py::arg("scatter_index"),
+        py::arg("weights"));
   m.def("bitwise_check", &bitwise_check);
   m.def("init_flux_shm", [](py::object) {}, py::arg("group") = py::none());  // nothing to set up on one GPU
   // Test helper of the reference (src/ths_op/helper_ops.cc:33-44, src/cuda/random_initialize.cu:27-51): fills a

@@ -152,6 +152,14 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> moe_route
 torch::Tensor topk_scatter_reduce(std::vector<torch::Tensor> inputs, torch::Tensor scatter_idx, int64_t topk);
 torch::Tensor topk_weighted_gather_reduce(std::vector<torch::Tensor> inputs, torch::Tensor routing_idx,
                                           int64_t topk, std::optional<torch::Tensor> row_weight, double scale);
+// Tokens to the rows of their experts and back (permute_ops.cc).  scatter_index int32 [tokens, topk], as calc_scatter_index gives it; entries
+// outside [0, tokens * topk) are dropped pairs, the others are distinct.  Both are differentiable once; the *_backward functions are the same
+// gradients for callers without autograd.
+torch::Tensor moe_permute(torch::Tensor input, torch::Tensor scatter_index);
+torch::Tensor moe_permute_backward(torch::Tensor grad_rows, torch::Tensor scatter_index);
+torch::Tensor moe_unpermute(torch::Tensor rows, torch::Tensor scatter_index, std::optional<torch::Tensor> weights);
+std::tuple<torch::Tensor, torch::Tensor> moe_unpermute_backward(torch::Tensor grad_out, torch::Tensor rows, torch::Tensor scatter_index,
+                                                                torch::Tensor weights);
 bool bitwise_check(torch::Tensor a, torch::Tensor b);
 
 }  // namespace flux_amd

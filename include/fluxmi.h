@@ -314,6 +314,37 @@ int fluxmi_topk_gather_reduce(const void *const *in, int32_t ngroups, int32_t io
                               int32_t ntokens, int32_t topk, int32_t n, void *out, void *stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Tokens to the rows of their experts and back, and the gradients of both.  No counterpart in the reference, whose GEMM gathers
+ * while it loads and whose reduction has no gradient.
+ *
+ * `scatter_index` [ntokens, topk] int32 names the row of each pair, as fluxmi_moe_route_sort writes it; there are ntokens * topk rows.
+ * Entries outside [0, ntokens * topk) name no row (dropped pairs).  The others have to be distinct; with two pairs on one row, that row
+ * is one of the two or a mixture of both.
+ *
+ *   fluxmi_moe_permute             rows[scatter_index[t, j]] = in[t], rows of `row_bytes` bytes of any type; rows that no entry names are 0.
+ *                                  Its gradient is fluxmi_moe_unpermute without weights.
+ *   fluxmi_moe_unpermute           out[t] = sum_j weights[t, j] * rows[scatter_index[t, j]]   (weights NULL: 1), j ascending, fp32
+ *                                  multiply-adds, one rounding
+ *   fluxmi_moe_unpermute_backward  grad_rows[scatter_index[t, j]] = weights[t, j] * grad_out[t]; rows that no entry names are 0
+ *                                  grad_weights[t, j] = sum_n grad_out[t, n] * rows[scatter_index[t, j], n] (fp32 sums in a fixed order;
+ *                                  0 for a dropped pair)
+ *                                  grad_rows or grad_weights may be NULL: it is not computed (and rows not read without grad_weights).
+ *
+ * `row_type` is the type of rows, out, grad_out and grad_rows, `weight_type` that of weights [ntokens, topk] and grad_weights (FLUXMI_ROWS_*).
+ * Pointers are aligned to their elements, no more; any n; 1 <= topk <= 64; ntokens * topk <= 2^30.
+ * ---------------------------------------------------------------------------------------------- */
+#define FLUXMI_ROWS_BF16 0
+#define FLUXMI_ROWS_FP32 1
+#define FLUXMI_ROWS_FP16 2
+int fluxmi_moe_permute(const void *in, const int32_t *scatter_index, int32_t ntokens, int32_t topk, int64_t row_bytes, void *rows,
+                       void *stream);
+int fluxmi_moe_unpermute(const void *rows, int32_t row_type, const int32_t *scatter_index, const void *weights, int32_t weight_type,
+                         int32_t ntokens, int32_t topk, int32_t n, void *out, void *stream);
+int fluxmi_moe_unpermute_backward(const void *grad_out, const void *rows, int32_t row_type, const int32_t *scatter_index,
+                                  const void *weights, int32_t weight_type, int32_t ntokens, int32_t topk, int32_t n, void *grad_rows,
+                                  void *grad_weights, void *stream);
+
+/* ------------------------------------------------------------------------------------------------
  * bf16 -> fp8-e4m3 absmax quantisation, one scale per (row, block of `block_cols` columns).
  *
  * Stands in for `block_scaled_1d_cast_transpose_impl` behind `Quantization::quantize_vector_blockwise`
