@@ -29,7 +29,7 @@ def _load_ths():
 
 _THS_NAMES = (
     "MoeArguments", "DistEnvTPWithEP", "GemmGroupedV3AGScatter", "GemmGroupedV3GatherRS", "GemmGroupedV3",
-    "Quantization", "BlockScaleGemm", "calc_scatter_index", "topk_scatter_reduce", "bitwise_check", "init_flux_shm",
+    "Quantization", "BlockScaleGemm", "MxGemm", "calc_scatter_index", "topk_scatter_reduce", "bitwise_check", "init_flux_shm",
     "moe_route_sort", "topk_weighted_gather_reduce", "moe_permute", "moe_permute_backward", "moe_unpermute",
     "moe_unpermute_backward", "uniform_initialize", "load_tuning_record",
     "ProfilingContext", "TuningRecord", "load_tuning_text",

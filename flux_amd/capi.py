@@ -34,6 +34,7 @@ EXPORTS = (
     "fluxmi_grouped_gemm_topk_reduce", "fluxmi_grouped_gemm_blockscale",
     "fluxmi_topk_gather_reduce", "fluxmi_moe_permute", "fluxmi_moe_unpermute", "fluxmi_moe_unpermute_backward", "fluxmi_quant_e4m3_rowwise", "fluxmi_quant_e4m3_square",
     "fluxmi_quant_e4m3_block128", "fluxmi_quant_e4m3_block128_filled", "fluxmi_calib_stream_sink_bytes", "fluxmi_calib_stream",
+    "fluxmi_quant_mx", "fluxmi_dequant_mx", "fluxmi_grouped_gemm_mx_workspace_bytes", "fluxmi_grouped_gemm_mx",
 )
 
 
@@ -49,6 +50,11 @@ class GroupedGemmArgs(ctypes.Structure):
         ("cu_margin", ctypes.c_int32), ("raster_rows", ctypes.c_int32), ("sched_flags", ctypes.c_int32),
         ("reserved", ctypes.c_int32),
     ]
+
+
+class MxGemmArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("nexperts", "max_rows", "n", "k", "a_rows", "d_type")] + [
+        (n, ctypes.c_void_p) for n in ("a", "a_scale", "b", "b_scale", "d", "splits", "gather_a", "row_scale")]
 
 
 class GemmLaunchInfo(ctypes.Structure):
@@ -105,6 +111,11 @@ def load():
     lib.fluxmi_quant_e4m3_square.argtypes = [vp, i64, i64, i64, f32, vp, vp, vp, vp, vp]
     lib.fluxmi_quant_e4m3_block128.argtypes = [vp, i64, i64, f32, vp, vp, vp, vp, vp]
     lib.fluxmi_quant_e4m3_block128_filled.argtypes = lib.fluxmi_quant_e4m3_block128.argtypes
+    lib.fluxmi_quant_mx.argtypes = [vp, i32, i64, i64, i64, vp, vp, vp, vp, vp]
+    lib.fluxmi_dequant_mx.argtypes = [vp, vp, i64, i64, i32, vp, vp]
+    lib.fluxmi_grouped_gemm_mx_workspace_bytes.restype = sz
+    lib.fluxmi_grouped_gemm_mx_workspace_bytes.argtypes = [ctypes.POINTER(MxGemmArgs)]
+    lib.fluxmi_grouped_gemm_mx.argtypes = [ctypes.POINTER(MxGemmArgs), vp, sz, vp]
     lib.fluxmi_calib_stream_sink_bytes.restype = sz
     lib.fluxmi_calib_stream.argtypes = [vp, vp, sz, i32, vp]
     _lib = lib

@@ -1,0 +1,458 @@
+// MXFP4: blocks of 32 values along a row share a power of two, a value is one of sixteen.
+//
+//   f = biased fp32 exponent of the block's largest magnitude, b = f == 255 ? 255 : max(f - 2, 0)
+//   code = e2m1(x / 2^(b - 127)), ties to the even code, saturating; all codes 0 where b = 255 (the block holds an infinity or a NaN)
+//
+// Everything is exact up to the code's own rounding: the exponent is read from the bits of the maximum, the division is one by a power of
+// two inside the conversion instruction (checked against the definition for every bf16 and fp16 value and millions of fp32 ones, subnormal ones
+// and scales at both ends of the range among them).  The maximum is taken over the patterns without sign, where infinities and NaN are largest.
+//
+// Bound by HBM: a value is read once and becomes 17 / 32 bytes.  Along the rows a lane converts 8 neighbours (fp32: two vectors) and four lanes
+// join their maxima; rows whose length is a multiple of 32 are one flat array.  With the transposed copy a lane holds 32 rows of one vector's
+// columns in registers, which gives both directions from one read with no exchange but that of the maxima along the rows; eight lanes side by side and
+// eight row blocks below each other make a wave, so that its loads and its transposed stores are whole 128-byte lines.
+#include "rows.hpp"
+
+namespace fluxmi {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBlock = 32;
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// Lanes that share a block when each has one vector.
+template <Row T>
+constexpr int kShare = kBlock / kVec<T>;
+
+// Running maximum over the magnitudes' patterns: of each half, or of the whole word.
+template <Row T>
+__device__ __forceinline__ uint32_t max_pattern(uint32_t a, uint32_t b) {
+  if constexpr (T == Row::F32) return a > b ? a : b;
+  else return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+template <Row T>
+__device__ __forceinline__ uint32_t magnitude(uint32_t v) {
+  return v & (T == Row::F32 ? 0x7fffffffu : 0x7fff7fffu);
+}
+template <Row T>
+__device__ __forceinline__ uint32_t join_halves(uint32_t m) {
+  if constexpr (T == Row::F32) return m;
+  else return (m >> 16) > (m & 0xffffu) ? m >> 16 : m & 0xffffu;
+}
+
+// The maximum of 2, 4 or 8 neighbouring lanes, in each of them.
+template <int LANES>
+__device__ __forceinline__ uint32_t max_of_lanes(uint32_t m) {
+  auto with = [&](uint32_t o) { return m > o ? m : o; };
+  m = with(__builtin_amdgcn_mov_dpp(m, 0xb1, 0xf, 0xf, false));                    // quad_perm [1,0,3,2]
+  if constexpr (LANES >= 4) m = with(__builtin_amdgcn_mov_dpp(m, 0x4e, 0xf, 0xf, false));   // quad_perm [2,3,0,1]
+  if constexpr (LANES >= 8) m = with(__builtin_amdgcn_mov_dpp(m, 0x141, 0xf, 0xf, false));  // row_half_mirror: lane 7 - i of every 8
+  return m;
+}
+
+// Scale byte of a block from the largest pattern of its magnitudes.
+template <Row T>
+__device__ __forceinline__ uint32_t scale_byte(uint32_t largest) {
+  uint32_t f;
+  if constexpr (T == Row::F32) f = largest >> 23;
+  else if constexpr (T == Row::BF16) f = largest >> 7;
+  else f = __float_as_uint(f16_bits_to_float(static_cast<uint16_t>(largest))) >> 23;
+  return f == 255 ? 255 : (f > 2 ? f - 2 : 0);
+}
+
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  return __uint_as_float(byte == 0 ? 0x00400000u : (byte == 255 ? 0x7fc00000u : byte << 23));
+}
+
+// Two values (16-bit types: a pair in one word) to byte SEL of `old`.
+template <Row T, int SEL>
+__device__ __forceinline__ uint32_t convert2(uint32_t old, uint32_t pair, float scale) {
+  if constexpr (T == Row::BF16) return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(old, __builtin_bit_cast(bf16x2, pair), scale, SEL);
+  else return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(old, __builtin_bit_cast(f16x2, pair), scale, SEL);
+}
+template <int SEL>
+__device__ __forceinline__ uint32_t convert2f(uint32_t old, uint32_t lo, uint32_t hi, float scale) {
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(old, __uint_as_float(lo), __uint_as_float(hi), scale, SEL);
+}
+
+// A vector's codes: 4 bytes, fp32 the lower 2.
+template <Row T>
+__device__ __forceinline__ uint32_t convert_vector(const u32x4 v, float scale) {
+  uint32_t c = 0;
+  if constexpr (T == Row::F32) {
+    c = convert2f<0>(c, v[0], v[1], scale);
+    return convert2f<1>(c, v[2], v[3], scale);
+  } else {
+    c = convert2<T, 0>(c, v[0], scale);
+    c = convert2<T, 1>(c, v[1], scale);
+    c = convert2<T, 2>(c, v[2], scale);
+    return convert2<T, 3>(c, v[3], scale);
+  }
+}
+
+template <Row T>
+__device__ __forceinline__ uint32_t vector_max(const u32x4 v) {
+  uint32_t m = magnitude<T>(v[0]);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) m = max_pattern<T>(m, magnitude<T>(v[i]));
+  return m;
+}
+
+// `count` elements (fewer than a vector) from p, zeros behind them.
+template <Row T>
+__device__ __forceinline__ u32x4 load_part(const uint8_t *p, int count) {
+  u32x4 v = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) {
+    if (i >= count) continue;
+    if constexpr (T == Row::F32) v[i] = reinterpret_cast<const uint32_t *>(p)[i];
+    else v[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(p)[i]) << (16 * (i & 1));
+  }
+  return v;
+}
+
+// ---- along the rows --------------------------------------------------------------------------------------------
+
+// Eight neighbours, four lanes to a block.
+template <Row T>
+struct Eight {
+  u32x4 v[T == Row::F32 ? 2 : 1];
+};
+
+template <Row T>
+__device__ __forceinline__ Eight<T> load_eight(const uint8_t *p, int count) {
+  Eight<T> e;
+  if (count >= 8) {
+    e.v[0] = load16(p);
+    if constexpr (T == Row::F32) e.v[1] = load16(p + 16);
+  } else {
+    e.v[0] = load_part<T>(p, count);
+    if constexpr (T == Row::F32) e.v[1] = load_part<T>(p + 16, count - 4);
+  }
+  return e;
+}
+
+template <Row T>
+__device__ __forceinline__ void quantise_eight(const Eight<T> &e, uint8_t *codes, uint8_t *scale, bool first_lane) {
+  uint32_t m = vector_max<T>(e.v[0]);
+  if constexpr (T == Row::F32) m = max_pattern<T>(m, vector_max<T>(e.v[1]));
+  const uint32_t byte = scale_byte<T>(max_of_lanes<4>(join_halves<T>(m)));
+  const float s = scale_value(byte);
+  uint32_t c = convert_vector<T>(e.v[0], s);
+  if constexpr (T == Row::F32) c = (c & 0xffffu) | convert_vector<T>(e.v[1], s) << 16;
+  *reinterpret_cast<uint32_t *>(codes) = byte == 255 ? 0u : c;
+  if (first_lane) *scale = static_cast<uint8_t>(byte);
+}
+
+// Rows of whole blocks: eight values to a lane, U of them in flight.
+template <Row T, int U>
+__global__ __launch_bounds__(kThreads) void quant_flat_kernel(const uint8_t *__restrict__ x, size_t eights, uint8_t *__restrict__ codes, uint8_t *__restrict__ scale) {
+  const size_t at = static_cast<size_t>(blockIdx.x) * (kThreads * U) + threadIdx.x;
+  Eight<T> e[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (at + u * kThreads < eights) e[u] = load_eight<T>(x + (at + u * kThreads) * 8 * kElt<T>, 8);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const size_t i = at + u * kThreads;
+    if (i < eights) quantise_eight<T>(e[u], codes + i * 4, scale + (i >> 2), (threadIdx.x & 3) == 0);
+  }
+}
+
+// Rows that end inside a block: a row to `1 << shift` lanes.
+template <Row T>
+__global__ __launch_bounds__(kThreads) void quant_rows_kernel(const uint8_t *__restrict__ x, int64_t rows, int cols, int shift, uint8_t *__restrict__ codes,
+                                                              uint8_t *__restrict__ scale) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads >> shift) + (threadIdx.x >> shift);
+  if (row >= rows) return;
+  const int kb = (cols + kBlock - 1) / kBlock;
+  const uint8_t *const src = x + static_cast<size_t>(row) * cols * kElt<T>;
+  for (int i = threadIdx.x & ((1 << shift) - 1); i < kb * 4; i += 1 << shift) {
+    const size_t at = static_cast<size_t>(row) * kb * 4 + i;
+    quantise_eight<T>(load_eight<T>(src + static_cast<size_t>(i) * 8 * kElt<T>, cols - i * 8), codes + at * 4, scale + (at >> 2), (i & 3) == 0);
+  }
+}
+
+// ---- along the rows and along the columns -----------------------------------------------------------------------------
+
+// One matrix of the batch.  A wave covers 8 vectors of columns x 8 blocks of 32 rows, a workgroup 4 waves side by side.
+template <Row T>
+__global__ __launch_bounds__(kThreads, 2) void quant_both_kernel(const uint8_t *__restrict__ x, int rows, int cols, int row_tiles, int col_tiles,
+                                                              uint8_t *__restrict__ codes, uint8_t *__restrict__ scale, uint8_t *__restrict__ codes_t,
+                                                              uint8_t *__restrict__ scale_t) {
+  constexpr int V = kVec<T>;
+  // Neighbouring column tiles on one XCD (workgroups are dealt to the eight of them in turn): they share lines of the codes and of the scales.
+  const int tiles = row_tiles * col_tiles, per_xcd = (tiles + 7) / 8, tile = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if (static_cast<int>(blockIdx.x >> 3) >= per_xcd || tile >= tiles) return;
+  const int rt = tile / col_tiles, ct = tile - rt * col_tiles;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r0 = (rt * 8 + (lane >> 3)) * kBlock, c0 = ((ct * 4 + wave) * 8 + (lane & 7)) * V;
+  const int kb = (cols + kBlock - 1) / kBlock, rb = (rows + kBlock - 1) / kBlock;
+  const size_t matrix = static_cast<size_t>(blockIdx.y);
+  x += matrix * rows * cols * kElt<T>;
+  codes += matrix * rows * kb * 16;
+  scale += matrix * rows * kb;
+  codes_t += matrix * cols * rb * 16;
+  scale_t += matrix * cols * rb;
+  const int rows_here = rows - r0 < kBlock ? rows - r0 : kBlock, cols_here = cols - c0;  // (either may be negative)
+  u32x4 v[kBlock];
+  const uint8_t *const src = x + (static_cast<size_t>(r0) * cols + c0) * kElt<T>;
+#pragma unroll
+  for (int r = 0; r < kBlock; ++r) {
+    v[r] = u32x4{0u, 0u, 0u, 0u};
+    if (r < rows_here && cols_here > 0) {
+      const uint8_t *const p = src + static_cast<size_t>(r) * cols * kElt<T>;
+      v[r] = cols_here >= V ? load16(p) : load_part<T>(p, cols_here);
+    }
+  }
+  // Along the rows: kShare lanes have a block.
+#pragma unroll
+  for (int r = 0; r < kBlock; ++r) {
+    const uint32_t byte = scale_byte<T>(max_of_lanes<kShare<T>>(join_halves<T>(vector_max<T>(v[r]))));
+    const uint32_t c = byte == 255 ? 0u : convert_vector<T>(v[r], scale_value(byte));
+    if (r < rows_here && c0 < kb * kBlock) {
+      uint8_t *const to = codes + (static_cast<size_t>(r0 + r) * kb * kBlock + c0) / 2;
+      if constexpr (T == Row::F32) *reinterpret_cast<uint16_t *>(to) = static_cast<uint16_t>(c);
+      else *reinterpret_cast<uint32_t *>(to) = c;
+      if ((lane & (kShare<T> - 1)) == 0) scale[static_cast<size_t>(r0 + r) * kb + c0 / kBlock] = static_cast<uint8_t>(byte);
+    }
+  }
+  // Along the columns: 32 values of each are this lane's.
+  u32x4 most = v[0];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    most[i] = magnitude<T>(v[0][i]);
+#pragma unroll
+    for (int r = 1; r < kBlock; ++r) most[i] = max_pattern<T>(most[i], magnitude<T>(v[r][i]));
+  }
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    uint32_t largest;
+    if constexpr (T == Row::F32) largest = most[c];
+    else largest = c & 1 ? most[c / 2] >> 16 : most[c / 2] & 0xffffu;
+    const uint32_t byte = scale_byte<T>(largest);
+    const float s = scale_value(byte);
+    u32x4 o;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t w = 0;
+      if constexpr (T == Row::F32) {
+        w = convert2f<0>(w, v[8 * q][c], v[8 * q + 1][c], s);
+        w = convert2f<1>(w, v[8 * q + 2][c], v[8 * q + 3][c], s);
+        w = convert2f<2>(w, v[8 * q + 4][c], v[8 * q + 5][c], s);
+        w = convert2f<3>(w, v[8 * q + 6][c], v[8 * q + 7][c], s);
+      } else {
+        // The column's halves of two rows to one word.
+        auto pair = [&](int r) { return __builtin_amdgcn_perm(v[r + 1][c / 2], v[r][c / 2], c & 1 ? 0x07060302u : 0x05040100u); };
+        w = convert2<T, 0>(w, pair(8 * q), s);
+        w = convert2<T, 1>(w, pair(8 * q + 2), s);
+        w = convert2<T, 2>(w, pair(8 * q + 4), s);
+        w = convert2<T, 3>(w, pair(8 * q + 6), s);
+      }
+      o[q] = byte == 255 ? 0u : w;
+    }
+    if (rows_here > 0 && c < cols_here) {
+      const size_t at = static_cast<size_t>(c0 + c) * rb + r0 / kBlock;
+      store16(codes_t + at * 16, o);
+      scale_t[at] = static_cast<uint8_t>(byte);
+    }
+  }
+}
+
+// ---- back ------------------------------------------------------------------------------------------------------
+
+template <Row T>
+__device__ __forceinline__ void dequantise_eight(uint32_t c, uint32_t byte, uint8_t *out, int count) {
+  const float s = scale_value(byte);
+  u32x4 v[T == Row::F32 ? 2 : 1];
+  if constexpr (T == Row::F32) {
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1),
+                d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 3);
+    v[0] = u32x4{__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(b[0]), __float_as_uint(b[1])};
+    v[1] = u32x4{__float_as_uint(d[0]), __float_as_uint(d[1]), __float_as_uint(e[0]), __float_as_uint(e[1])};
+    if (byte == 255) v[0] = v[1] = u32x4{0x7fc00000u, 0x7fc00000u, 0x7fc00000u, 0x7fc00000u};
+  } else if constexpr (T == Row::BF16) {
+    v[0] = u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0)), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2)), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3))};
+    if (byte == 255) v[0] = u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+  } else {
+    // Through fp32, which holds every value: the one rounding is that to fp16.
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f32x2 p;
+      if (i == 0) p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 0);
+      else if (i == 1) p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1);
+      else if (i == 2) p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 2);
+      else p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 3);
+      v[0][i] = float_to_f16_bits(p[0]) | static_cast<uint32_t>(float_to_f16_bits(p[1])) << 16;
+    }
+    if (byte == 255) v[0] = u32x4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
+  }
+  if (count >= 8) {
+    store16(out, v[0]);
+    if constexpr (T == Row::F32) store16(out + 16, v[1]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 7; ++i) {
+    if (i >= count) continue;
+    if constexpr (T == Row::F32) reinterpret_cast<uint32_t *>(out)[i] = v[i / 4][i % 4];
+    else reinterpret_cast<uint16_t *>(out)[i] = static_cast<uint16_t>(v[0][i / 2] >> (16 * (i & 1)));
+  }
+}
+
+template <Row T, int U>
+__global__ __launch_bounds__(kThreads) void dequant_flat_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scale, size_t eights, uint8_t *__restrict__ out) {
+  const size_t at = static_cast<size_t>(blockIdx.x) * (kThreads * U) + threadIdx.x;
+  uint32_t c[U], b[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const size_t i = at + u * kThreads;
+    if (i < eights) {
+      c[u] = reinterpret_cast<const uint32_t *>(codes)[i];
+      b[u] = scale[i >> 2];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const size_t i = at + u * kThreads;
+    if (i < eights) dequantise_eight<T>(c[u], b[u], out + i * 8 * kElt<T>, 8);
+  }
+}
+
+template <Row T>
+__global__ __launch_bounds__(kThreads) void dequant_rows_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scale, int64_t rows, int cols, int shift,
+                                                                uint8_t *__restrict__ out) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads >> shift) + (threadIdx.x >> shift);
+  if (row >= rows) return;
+  const int kb = (cols + kBlock - 1) / kBlock;
+  uint8_t *const dst = out + static_cast<size_t>(row) * cols * kElt<T>;
+  for (int i = threadIdx.x & ((1 << shift) - 1); i * 8 < cols; i += 1 << shift) {
+    const size_t at = static_cast<size_t>(row) * kb * 4 + i;
+    dequantise_eight<T>(reinterpret_cast<const uint32_t *>(codes)[at], scale[at >> 2], dst + static_cast<size_t>(i) * 8 * kElt<T>, cols - i * 8);
+  }
+}
+
+// Lanes of a row that ends inside a block, as a power of two from 4 to 256.
+int row_shift(int64_t cols) {
+  const int64_t eights = (cols + kBlock - 1) / kBlock * 4;
+  int shift = 2;
+  while (shift < 8 && (int64_t{1} << shift) < eights) ++shift;
+  return shift;
+}
+
+// Workgroups of `items` work items, `per` to a workgroup; false: more than a launch has.
+bool grid_of(int64_t items, int64_t per, dim3 *grid) {
+  const int64_t n = (items + per - 1) / per;
+  *grid = dim3(static_cast<unsigned>(n));
+  return n * kThreads < (int64_t{1} << 32);
+}
+
+// From this many values on a lane has four groups of eight in flight: below, one each spreads the work wider.
+constexpr size_t kManyEights = size_t{1} << 19;
+
+int check_sizes(const char *who, int64_t rows, int64_t cols) {
+  FLUXMI_REQUIRE(rows >= 0 && cols >= 0, FLUXMI_ERR_INVALID_ARG, "%s: negative size (rows=%lld, cols=%lld)", who, static_cast<long long>(rows),
+                 static_cast<long long>(cols));
+  FLUXMI_REQUIRE(cols <= (int64_t{1} << 30), FLUXMI_ERR_UNSUPPORTED, "%s: cols=%lld exceeds 2^30", who, static_cast<long long>(cols));
+  FLUXMI_REQUIRE(cols == 0 || rows <= (int64_t{1} << 40) / cols, FLUXMI_ERR_UNSUPPORTED, "%s: more than 2^40 values", who);
+  return FLUXMI_OK;
+}
+
+}  // namespace
+}  // namespace fluxmi
+
+extern "C" int fluxmi_quant_mx(const void *x, int32_t row_type, int64_t batch, int64_t rows, int64_t cols, void *codes, void *scale, void *codes_t, void *scale_t,
+                               void *stream) {
+  using namespace fluxmi;
+  Row type;
+  int rc = check_type("quant_mx", row_type, &type);
+  if (rc == FLUXMI_OK) rc = check_sizes("quant_mx", rows, cols);
+  if (rc != FLUXMI_OK) return rc;
+  FLUXMI_REQUIRE(batch >= 0 && batch <= 65535, FLUXMI_ERR_INVALID_ARG, "quant_mx: batch=%lld outside [0,65535]", static_cast<long long>(batch));
+  FLUXMI_REQUIRE((codes_t == nullptr) == (scale_t == nullptr), FLUXMI_ERR_INVALID_ARG, "quant_mx: codes_t and scale_t go together");
+  if (batch == 0 || rows == 0 || cols == 0) return FLUXMI_OK;
+  rc = check_sizes("quant_mx", batch * rows, cols);
+  if (rc != FLUXMI_OK) return rc;
+  FLUXMI_REQUIRE(x != nullptr && codes != nullptr && scale != nullptr, FLUXMI_ERR_INVALID_ARG, "quant_mx: null pointer argument");
+  FLUXMI_REQUIRE(aligned_to(x, type) && (reinterpret_cast<uintptr_t>(codes) & 3) == 0 && aligned16(codes_t), FLUXMI_ERR_INVALID_ARG,
+                 "quant_mx: x is not aligned to its elements, codes to 4 or codes_t to 16 bytes");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const auto *const in = static_cast<const uint8_t *>(x);
+  auto *const q = static_cast<uint8_t *>(codes), *const sc = static_cast<uint8_t *>(scale);
+  dim3 grid;
+  bool fits = true;
+  if (codes_t != nullptr) {
+    FLUXMI_REQUIRE(rows <= (int64_t{1} << 30), FLUXMI_ERR_UNSUPPORTED, "quant_mx: rows=%lld exceeds 2^30 with a transposed copy", static_cast<long long>(rows));
+    by_type(type, [&](auto t) {
+      constexpr Row T = decltype(t)::value;
+      const int64_t row_tiles = (rows + 8 * kBlock - 1) / (8 * kBlock), col_tiles = (cols + 32 * kVec<T> - 1) / (32 * kVec<T>);
+      fits = grid_of((row_tiles * col_tiles + 7) / 8 * 8, 1, &grid) && row_tiles * col_tiles < (int64_t{1} << 23);
+      if (!fits) return;
+      grid.y = static_cast<unsigned>(batch);
+      hipLaunchKernelGGL(quant_both_kernel<T>, grid, dim3(kThreads), 0, s, in, static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(row_tiles),
+                         static_cast<int>(col_tiles), q, sc, static_cast<uint8_t *>(codes_t), static_cast<uint8_t *>(scale_t));
+    });
+  } else if (cols % kBlock == 0) {
+    const size_t eights = static_cast<size_t>(batch * rows) * cols / 8;
+    by_type(type, [&](auto t) {
+      constexpr Row T = decltype(t)::value;
+      fits = grid_of(eights, kThreads * (eights >= kManyEights ? 4 : 1), &grid);
+      if (!fits) return;
+      if (eights >= kManyEights) hipLaunchKernelGGL((quant_flat_kernel<T, 4>), grid, dim3(kThreads), 0, s, in, eights, q, sc);
+      else hipLaunchKernelGGL((quant_flat_kernel<T, 1>), grid, dim3(kThreads), 0, s, in, eights, q, sc);
+    });
+  } else {
+    const int shift = row_shift(cols);
+    by_type(type, [&](auto t) {
+      constexpr Row T = decltype(t)::value;
+      fits = grid_of(batch * rows, kThreads >> shift, &grid);
+      if (fits) hipLaunchKernelGGL(quant_rows_kernel<T>, grid, dim3(kThreads), 0, s, in, batch * rows, static_cast<int>(cols), shift, q, sc);
+    });
+  }
+  FLUXMI_REQUIRE(fits, FLUXMI_ERR_UNSUPPORTED, "quant_mx: batch=%lld rows=%lld cols=%lld is more than a launch covers", static_cast<long long>(batch),
+                 static_cast<long long>(rows), static_cast<long long>(cols));
+  FLUXMI_HIP_CHECK(hipGetLastError());
+  return FLUXMI_OK;
+}
+
+extern "C" int fluxmi_dequant_mx(const void *codes, const void *scale, int64_t rows, int64_t cols, int32_t row_type, void *out, void *stream) {
+  using namespace fluxmi;
+  Row type;
+  int rc = check_type("dequant_mx", row_type, &type);
+  if (rc == FLUXMI_OK) rc = check_sizes("dequant_mx", rows, cols);
+  if (rc != FLUXMI_OK) return rc;
+  if (rows == 0 || cols == 0) return FLUXMI_OK;
+  FLUXMI_REQUIRE(codes != nullptr && scale != nullptr && out != nullptr, FLUXMI_ERR_INVALID_ARG, "dequant_mx: null pointer argument");
+  FLUXMI_REQUIRE(aligned_to(out, type) && (reinterpret_cast<uintptr_t>(codes) & 3) == 0, FLUXMI_ERR_INVALID_ARG,
+                 "dequant_mx: out is not aligned to its elements or codes to 4 bytes");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const auto *const q = static_cast<const uint8_t *>(codes), *const sc = static_cast<const uint8_t *>(scale);
+  auto *const o = static_cast<uint8_t *>(out);
+  dim3 grid;
+  bool fits = true;
+  if (cols % kBlock == 0) {
+    const size_t eights = static_cast<size_t>(rows) * cols / 8;
+    by_type(type, [&](auto t) {
+      constexpr Row T = decltype(t)::value;
+      fits = grid_of(eights, kThreads * (eights >= kManyEights ? 4 : 1), &grid);
+      if (!fits) return;
+      if (eights >= kManyEights) hipLaunchKernelGGL((dequant_flat_kernel<T, 4>), grid, dim3(kThreads), 0, s, q, sc, eights, o);
+      else hipLaunchKernelGGL((dequant_flat_kernel<T, 1>), grid, dim3(kThreads), 0, s, q, sc, eights, o);
+    });
+  } else {
+    const int shift = row_shift(cols);
+    by_type(type, [&](auto t) {
+      constexpr Row T = decltype(t)::value;
+      fits = grid_of(rows, kThreads >> shift, &grid);
+      if (fits) hipLaunchKernelGGL(dequant_rows_kernel<T>, grid, dim3(kThreads), 0, s, q, sc, rows, static_cast<int>(cols), shift, o);
+    });
+  }
+  FLUXMI_REQUIRE(fits, FLUXMI_ERR_UNSUPPORTED, "dequant_mx: rows=%lld cols=%lld is more than a launch covers", static_cast<long long>(rows), static_cast<long long>(cols));
+  FLUXMI_HIP_CHECK(hipGetLastError());
+  return FLUXMI_OK;
+}

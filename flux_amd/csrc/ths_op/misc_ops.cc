@@ -9,6 +9,11 @@ constexpr int64_t kBlock = 128;  // BLOCK_TILE_DIM of the reference's quantisati
 
 Quantization::Quantization(at::ScalarType input_dtype, at::ScalarType output_dtype, int32_t /*num_streams*/)
     : input_dtype_(input_dtype), output_dtype_(output_dtype) {
+  if (output_dtype == at::ScalarType::Float4_e2m1fn_x2) {
+    TORCH_CHECK(input_dtype == at::kBFloat16 || input_dtype == at::kHalf || input_dtype == at::kFloat,
+                "Quantization: input dtype must be bfloat16, float16 or float32 for float4_e2m1fn_x2, got ", input_dtype);
+    return;
+  }
   // The reference hard-wires the same pair (src/quantization/quantization.cu:1399-1400).
   TORCH_CHECK(input_dtype == at::kBFloat16, "Quantization: input dtype must be bfloat16, got ", input_dtype);
   TORCH_CHECK(output_dtype == at::ScalarType::Float8_e4m3fn, "Quantization: output dtype must be float8_e4m3fn, got ",
@@ -22,7 +27,12 @@ static void quant_call(const torch::Tensor &x, int32_t block_cols, float eps, to
                "fluxmi_quant_e4m3_rowwise");
 }
 
+void Quantization::require_e4m3(const char *method) const {
+  TORCH_CHECK(output_dtype_ == at::ScalarType::Float8_e4m3fn, method, " needs a Quantization whose output dtype is float8_e4m3fn, this one's is ", output_dtype_);
+}
+
 Quantization::Result Quantization::quantize_vector_blockwise(torch::Tensor input, bool return_transpose, float eps) {
+  require_e4m3("quantize_vector_blockwise");
   TORCH_CHECK(input.dim() == 2, "Input must have 2 dimensions.");
   FLUX_AMD_CHECK_INPUT(input, input_dtype_);
   const int64_t rows = input.size(0), cols = input.size(1);
@@ -69,6 +79,7 @@ static Quantization::Result quant_square(const torch::Tensor &input, int64_t bat
 }
 
 Quantization::Result Quantization::quantize_square_blockwise(torch::Tensor input, bool return_transpose, float eps) {
+  require_e4m3("quantize_square_blockwise");
   TORCH_CHECK(input.dim() == 2, "Input must have 2 dimensions.");
   FLUX_AMD_CHECK_INPUT(input, input_dtype_);
   return quant_square(input, 1, input.size(0), input.size(1), false, return_transpose, eps, output_dtype_);
@@ -76,6 +87,7 @@ Quantization::Result Quantization::quantize_square_blockwise(torch::Tensor input
 
 Quantization::Result Quantization::batch_quantize_square_blockwise(torch::Tensor input, bool return_transpose,
                                                                    float eps) {
+  require_e4m3("batch_quantize_square_blockwise");
   TORCH_CHECK(input.dim() == 3, "Input must have 3 dimensions.");
   FLUX_AMD_CHECK_INPUT(input, input_dtype_);
   return quant_square(input, input.size(0), input.size(1), input.size(2), true, return_transpose, eps,
@@ -83,6 +95,7 @@ Quantization::Result Quantization::batch_quantize_square_blockwise(torch::Tensor
 }
 
 std::tuple<torch::Tensor, torch::Tensor> Quantization::quantize_rowwise(torch::Tensor input, float eps) {
+  require_e4m3("quantize_rowwise");
   TORCH_CHECK(input.dim() == 2, "Input must have 2 dimensions.");
   FLUX_AMD_CHECK_INPUT(input, input_dtype_);
   torch::Tensor out = torch::empty(input.sizes(), input.options().dtype(output_dtype_));

@@ -168,7 +168,17 @@ PYBIND11_MODULE(flux_ths_pybind, m) {
            py::arg("return_tranpose") = true, py::arg("eps") = 0.0)
       .def("batch_quantize_square_blockwise", &Quantization::batch_quantize_square_blockwise, py::arg("input"),
            py::arg("return_tranpose") = true, py::arg("eps") = 0.0)
-      .def("quantize_rowwise", &Quantization::quantize_rowwise, py::arg("input"), py::arg("eps") = 0.0);
+      .def("quantize_rowwise", &Quantization::quantize_rowwise, py::arg("input"), py::arg("eps") = 0.0)
+      .def("quantize_mx", &Quantization::quantize_mx, py::arg("input"), py::arg("return_tranpose") = false)
+      .def("dequantize_mx", &Quantization::dequantize_mx, py::arg("codes"), py::arg("scale"), py::arg("cols") = py::none());
+
+  py::class_<MxGemm>(m, "MxGemm")
+      .def(py::init([](py::object output_dtype) { return new MxGemm(to_dtype(output_dtype)); }), py::arg("output_dtype"))
+      .def("forward", &MxGemm::forward, py::arg("input"), py::arg("weight"), py::arg("input_scale"), py::arg("weight_scale"),
+           py::arg("output") = py::none())
+      .def("forward_grouped", &MxGemm::forward_grouped, py::arg("input"), py::arg("input_splits"), py::arg("weight"),
+           py::arg("input_scale"), py::arg("weight_scale"), py::arg("gather_index") = py::none(), py::arg("row_scale") = py::none(),
+           py::arg("output") = py::none());
 
   m.def("calc_scatter_index", &calc_scatter_index, py::arg("choosed_experts"), py::arg("splits"));
   m.def("moe_route_sort", &moe_route_sort, py::arg("choosed_experts"), py::arg("nexperts"));

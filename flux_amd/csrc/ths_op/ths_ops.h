@@ -141,9 +141,31 @@ class Quantization {
   Result quantize_square_blockwise(torch::Tensor input, bool return_transpose, float eps);
   Result batch_quantize_square_blockwise(torch::Tensor input, bool return_transpose, float eps);
   std::tuple<torch::Tensor, torch::Tensor> quantize_rowwise(torch::Tensor input, float eps);
+  // MXFP4, for output dtype float4_e2m1fn_x2 (mx_ops.cc): input [rows, cols] or [batch, rows, cols] of the input dtype -> codes [.., rows,
+  // 16 kb] (two a byte), scales float8_e8m0fnu [.., rows, kb], kb = ceil(cols / 32), and with return_transpose the same of the
+  // transposed matrices.
+  Result quantize_mx(torch::Tensor input, bool return_transpose);
+  // The values that codes and scales stand for, in the input dtype; cols: the row's length where the last block is not full.
+  torch::Tensor dequantize_mx(torch::Tensor codes, torch::Tensor scale, std::optional<int64_t> cols);
 
  private:
+  void require_e4m3(const char *method) const;
   at::ScalarType input_dtype_, output_dtype_;
+};
+
+// Products of MXFP4 operands as quantize_mx returns them, one launch on the current stream (mx_ops.cc).
+class MxGemm {
+ public:
+  explicit MxGemm(at::ScalarType output_dtype);
+  // input [M, K/2], weight [N, K/2], scales [M, K/32] and [N, K/32] -> [M, N].
+  torch::Tensor forward(torch::Tensor input, torch::Tensor weight, torch::Tensor input_scale, torch::Tensor weight_scale, std::optional<torch::Tensor> output);
+  // Rows sorted by expert; input_splits int32 [E] on the device or on the host, weight [E, N, K/2], weight_scale [E, N, K/32].  gather_index int32
+  // [M]: the row of input that a sorted row reads; row_scale fp32 [M]: a factor of each sorted row.  Rows past the splits' sum are not touched.
+  torch::Tensor forward_grouped(torch::Tensor input, torch::Tensor input_splits, torch::Tensor weight, torch::Tensor input_scale, torch::Tensor weight_scale,
+                                std::optional<torch::Tensor> gather_index, std::optional<torch::Tensor> row_scale, std::optional<torch::Tensor> output);
+
+ private:
+  at::ScalarType output_dtype_;
 };
 
 torch::Tensor calc_scatter_index(torch::Tensor choosed_experts, torch::Tensor splits);

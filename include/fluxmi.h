@@ -404,6 +404,50 @@ int fluxmi_quant_e4m3_block128_filled(const void *x_bf16, int64_t rows, int64_t 
                                       float *scale_inv_out, void *q_t_out, float *scale_inv_t_out, void *stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Microscaled 4-bit floating point (MXFP4: the OCP Microscaling Formats' E2M1 elements with E8M0 scales).  No counterpart in the
+ * reference.
+ *
+ * Along the last dimension 32 values share a scale byte b that stands for 2^(b - 127); 255 stands for NaN.  A code is a sign and the index of one of
+ * 0, 0.5, 1, 1.5, 2, 3, 4, 6; two codes are packed in a byte, the lower half first.  A row of `cols` values has kb = ceil(cols / 32) scale bytes and 16 kb
+ * bytes of codes; what lies past the end is zero codes.
+ *
+ * fluxmi_quant_mx: x [batch, rows, cols] (FLUXMI_ROWS_*) -> codes [batch, rows, 16 kb], scale [batch, rows, kb].  With f the biased fp32 exponent
+ *   of a block's largest magnitude: b = 255 and zero codes if the block holds an infinity or a NaN, else b = max(f - 2, 0) (the largest
+ *   magnitude lies in [4, 8) times the scale), and a code is the one nearest to x / 2^(b - 127), ties to the even code, beyond 6 the
+ *   code of 6; the sign is kept, that of zeros too.
+ *   codes_t / scale_t (both or neither): the same of the transposed matrix, [batch, cols, 16 ceil(rows / 32)] and
+ *   [batch, cols, ceil(rows / 32)], from the same read of x.
+ * fluxmi_dequant_mx: codes, scale -> out [rows, cols] (FLUXMI_ROWS_*), the values they stand for (rounded where the type does not hold them: fp16).
+ * Pointers are aligned to their elements, codes to 4 bytes (fluxmi_quant_mx with codes_t: that to 16); any rows and cols.
+ * ---------------------------------------------------------------------------------------------- */
+int fluxmi_quant_mx(const void *x, int32_t row_type, int64_t batch, int64_t rows, int64_t cols, void *codes, void *scale, void *codes_t,
+                    void *scale_t, void *stream);
+int fluxmi_dequant_mx(const void *codes, const void *scale, int64_t rows, int64_t cols, int32_t row_type, void *out, void *stream);
+
+/* Grouped product of MXFP4 operands, one dense product without splits:
+ *
+ *   for sorted row r of expert e (offsets = prefix sums of splits):
+ *     D[r, n] = row_scale[r] * sum_k A[gather_a ? gather_a[r] : r, k] * B[e, n, k]        (fp32 sums, one rounding to the type of D)
+ *
+ * A [a_rows, 16 kb] codes with scales [a_rows, kb], B [nexperts, N, 16 kb] with scales [nexperts, N, kb], kb = ceil(k / 32) (what fluxmi_quant_mx writes
+ * along k).  `splits`: DEVICE int32 row counts; NULL: nexperts is 1 and all max_rows rows are its own.  Negative counts are 0.  max_rows is an upper bound
+ * of their sum; rows past the sum are not touched.  Entries of gather_a are clamped into [0, a_rows).
+ * Requirements: 1 <= nexperts <= 1024; a, b 16-byte aligned, d aligned to its elements; any n, k >= 1; one expert's codes and all of A below 2 GiB.
+ * `workspace`: fluxmi_grouped_gemm_mx_workspace_bytes() bytes, 16-byte aligned, of any content; not shared by calls that may overlap. */
+typedef struct fluxmi_mx_gemm_args {
+  int32_t nexperts, max_rows, n, k, a_rows;
+  int32_t d_type;           /* FLUXMI_ROWS_* */
+  const void *a, *a_scale;
+  const void *b, *b_scale;
+  void *d;                  /* [max_rows, n] */
+  const int32_t *splits;    /* device [nexperts] or NULL */
+  const int32_t *gather_a;  /* device [max_rows] or NULL */
+  const float *row_scale;   /* device [max_rows] or NULL */
+} fluxmi_mx_gemm_args;
+size_t fluxmi_grouped_gemm_mx_workspace_bytes(const fluxmi_mx_gemm_args *args);
+int fluxmi_grouped_gemm_mx(const fluxmi_mx_gemm_args *args, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Calibration streams (no counterpart in the reference; for benchmarks): what the memory system of the GPU at
  * hand gives a kernel that only streams.  copy == 0: every byte of src[0, bytes) is read once (16 bytes per lane
  * and load, eight loads in flight per lane) and fluxmi_calib_stream_sink_bytes() bytes of dst are written;

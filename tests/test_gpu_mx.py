@@ -1,0 +1,353 @@
+"""MXFP4 on the GPU: quantisation bit for bit against the oracle, products against 64 bits.
+
+A product's bound: the terms are exact in fp32 (two 2-bit significands and powers of two), their sum in fp32 is off by at most K roundings of 2^-24 of the
+sum of magnitudes, and the result is rounded to its type once (half a step, eps / 2), after one more rounding by row_scale."""
+import numpy as np
+import pytest
+import torch
+
+import flux_amd
+from oracle import mx
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+FP4, E8M0 = torch.float4_e2m1fn_x2, torch.float8_e8m0fnu
+
+
+def quantiser(dtype):
+    return flux_amd.Quantization(dtype, FP4)
+
+
+def bytes_of(t):
+    return t.view(torch.uint8).cpu().numpy()
+
+
+def hard_values(rows, cols, dtype, seed):
+    """Blocks of every magnitude the type has, ties, zeros of both signs, subnormal values, and a few blocks with an infinity or a NaN."""
+    rng = np.random.default_rng(seed)
+    info = torch.finfo(dtype)
+    lo, hi = np.log2(info.tiny * info.eps), np.log2(info.max) - 1
+    size = np.exp2(rng.uniform(lo, hi, (rows, (cols + 31) // 32))).repeat(32, axis=1)[:, :cols]
+    x = rng.standard_normal((rows, cols)) * size / 4
+    tie = rng.random((rows, cols)) < 0.2
+    quarter = np.exp2(np.floor(np.log2(size)))
+    x = np.where(tie, np.round(x / quarter * 4) / 4 * quarter, x)
+    x = np.where(rng.random((rows, cols)) < 0.05, 0.0, x)
+    x = np.where(rng.random((rows, cols)) < 0.02, -0.0, x)
+    x = np.where(rng.random((rows, 1)) < 0.05, 0.0, x)
+    bad = rng.random((rows, cols)) < 0.0005
+    x = np.where(bad, rng.choice([np.inf, -np.inf, np.nan], (rows, cols)), x)
+    return torch.from_numpy(x).clamp(-info.max, info.max).where(torch.from_numpy(~bad), torch.from_numpy(x)).to(dtype)
+
+
+SHAPES = [(1, 32), (1, 1), (3, 31), (7, 33), (128, 7168), (50, 2048), (33, 1000), (257, 96), (300, 130), (2, 16384), (1000, 64), (515, 2056)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_quantise_bit_for_bit(rows, cols, dtype):
+    print(f"[case] quantise {rows} {cols} {dtype}", flush=True)
+    x = hard_values(rows, cols, dtype, rows + cols)
+    q = quantiser(dtype)
+    want = mx.quantise(x.double().numpy())
+    want_t = mx.quantise(x.double().numpy().T)
+    codes, scale, none, none2 = q.quantize_mx(x.to(DEV))
+    assert none is None and none2 is None and codes.dtype == FP4 and scale.dtype == E8M0
+    assert np.array_equal(bytes_of(scale), want[1]) and np.array_equal(bytes_of(codes), want[0])
+    codes, scale, codes_t, scale_t = q.quantize_mx(x.to(DEV), return_tranpose=True)
+    assert np.array_equal(bytes_of(scale), want[1]) and np.array_equal(bytes_of(codes), want[0])
+    assert np.array_equal(bytes_of(scale_t), want_t[1]) and np.array_equal(bytes_of(codes_t), want_t[0])
+    # and back: the values are held by the type
+    for c, s, n, (wc, ws) in ((codes, scale, cols, want), (codes_t, scale_t, rows, want_t)):
+        back = q.dequantize_mx(c, s, n)
+        assert back.dtype == dtype and np.array_equal(back.double().cpu().numpy(), mx.values(wc, ws)[:, :n], equal_nan=True)
+
+
+def test_large_and_flat_forms():
+    """Enough values for the form with four groups in flight, and a tensor whose last workgroup is not full."""
+    for rows, cols, dtype in ((4099, 1056, BF16), (2051, 4096, F32), (4100, 1056, F16)):
+        x = (torch.randn(rows, cols, generator=torch.Generator().manual_seed(1)) * 3).to(dtype)
+        codes, scale, _, _ = quantiser(dtype).quantize_mx(x.to(DEV))
+        want = mx.quantise(x.double().numpy())
+        assert np.array_equal(bytes_of(scale), want[1]) and np.array_equal(bytes_of(codes), want[0])
+        back = quantiser(dtype).dequantize_mx(codes, scale)
+        assert np.array_equal(back.double().cpu().numpy(), mx.values(*want))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_batch_of_matrices(dtype):
+    x = hard_values(5 * 70, 100, dtype, 4).view(5, 70, 100)
+    for transposed in (False, True):
+        codes, scale, codes_t, scale_t = quantiser(dtype).quantize_mx(x.to(DEV), transposed)
+        want = mx.quantise(x.double().numpy())
+        assert codes.shape == (5, 70, 64) and np.array_equal(bytes_of(codes), want[0]) and np.array_equal(bytes_of(scale), want[1])
+        if transposed:
+            want = mx.quantise(x.double().numpy().transpose(0, 2, 1))
+            assert codes_t.shape == (5, 100, 48) and np.array_equal(bytes_of(codes_t), want[0]) and np.array_equal(bytes_of(scale_t), want[1])
+
+
+def test_dequantise_every_code_and_scale():
+    codes = torch.arange(256, dtype=torch.uint8).repeat_interleave(16).view(1, -1).repeat(256, 1)     # every byte in a block of its own
+    scale = torch.arange(256, dtype=torch.uint8).view(256, 1).repeat(1, 256)
+    want = mx.values(codes.numpy(), scale.numpy())
+    for dtype in (F32, BF16, F16):
+        got = quantiser(dtype).dequantize_mx(codes.to(DEV).view(FP4), scale.to(DEV).view(E8M0))
+        expect = torch.from_numpy(want).to(F32).to(dtype)  # (fp32 holds them all but 6 * 2^127 and 4 * 2^127, infinite there and here)
+        assert torch.equal(got.cpu().nan_to_num(nan=7.0), expect.nan_to_num(nan=7.0))
+        assert torch.equal(got.cpu().isnan(), expect.isnan())
+
+
+def test_values_at_any_element():
+    flat = hard_values(1, 3 + 40 * 70, BF16, 3).view(-1).to(DEV)
+    x = flat[3:].view(40, 70)
+    for t in (False, True):
+        for a, b in zip(quantiser(BF16).quantize_mx(x, t), quantiser(BF16).quantize_mx(x.clone(), t)):
+            assert (a is None and b is None) or np.array_equal(bytes_of(a), bytes_of(b))
+    even = flat[3:3 + 2 * 1024].view(2, 1024)
+    assert np.array_equal(bytes_of(quantiser(BF16).quantize_mx(even)[0]), bytes_of(quantiser(BF16).quantize_mx(even.clone())[0]))
+
+
+def test_nothing_to_quantise():
+    for shape in ((0, 64), (4, 0), (0, 3, 5)):
+        codes, scale, codes_t, scale_t = quantiser(F32).quantize_mx(torch.empty(shape, device=DEV), True)
+        assert codes.numel() == 0 and scale.numel() == 0 and codes_t.numel() == 0
+    assert quantiser(F32).dequantize_mx(torch.empty(0, 16, dtype=torch.uint8, device=DEV).view(FP4),
+                                        torch.empty(0, 1, dtype=torch.uint8, device=DEV).view(E8M0)).shape == (0, 32)
+
+
+# ---- products ----------------------------------------------------------------------------------------------------
+
+
+def operand(*shape, k, seed):
+    """Codes and scales of a tensor [*shape, k]: every code, scales over a few powers of two; and its values, fp64 on the GPU."""
+    g = torch.Generator().manual_seed(seed)
+    kb = mx.blocks(k)
+    codes = torch.randint(0, 256, (*shape, kb, 16), dtype=torch.uint8, generator=g)
+    last = k - 32 * (kb - 1)  # the end of the last block is zero codes
+    codes[..., -1, (last + 1) // 2:] = 0
+    if last % 2:
+        codes[..., -1, last // 2] &= 15
+    scale = torch.randint(122, 130, (*shape, kb), dtype=torch.uint8, generator=g)
+    codes = codes.view(*shape, kb * 16)
+    table = torch.from_numpy(mx.values(np.arange(256, dtype=np.uint8)[:, None].repeat(16, 1), np.full((256, 1), 127, np.uint8)))[:, :2].to(DEV)
+    codes, scale = codes.to(DEV), scale.to(DEV)
+    value = table[codes.long()].flatten(-2) * torch.exp2(scale.double() - 127).repeat_interleave(32, -1)
+    return codes.view(FP4), scale.view(E8M0), value
+
+
+def check(got, a, w, k, factor=None):
+    """got against a [M, K] @ w [N, K]^T in fp64."""
+    want, size = a @ w.t(), a.abs() @ w.abs().t()
+    if factor is not None:
+        want, size = want * factor.double()[:, None], size * factor.double().abs()[:, None]
+    step = torch.finfo(got.dtype).eps / 2 if got.dtype != F32 else 0.0
+    bound = step * want.abs() + (k + 2) * 2.0**-24 * size
+    off = (got.double() - want).abs()
+    assert (off <= bound * 1.0000001).all(), f"off by {(off - bound).max().item():.3g} more than the bound"
+
+
+@pytest.mark.parametrize("out", [BF16, F16, F32])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 64, 32), (16, 16, 128), (17, 65, 544), (5, 1000, 100), (64, 64, 512), (65, 257, 2048), (300, 130, 1056),
+                                   (128, 128, 4096), (513, 520, 640), (1025, 384, 160), (2, 4096, 14336), (700, 1025, 3000)])
+def test_dense_product(m, n, k, out):
+    print(f"[case] dense {m} {n} {k} {out}", flush=True)
+    a, sa, va = operand(m, k=k, seed=1)
+    w, sw, vw = operand(n, k=k, seed=2)
+    got = flux_amd.MxGemm(out).forward(a, w, sa, sw)
+    assert got.shape == (m, n) and got.dtype == out
+    check(got, va, vw, k)
+
+
+SPLITS = [[0, 3, 0, 70], [5], [1, 1, 1, 1, 1], [0, 0, 0], [200, 0, 16, 33], [64, 64, 128], [129, 1, 255, 31, 0, 300], [600, 2, 0, 900], [17] * 70]
+
+
+@pytest.mark.parametrize("n,k", [(96, 224), (257, 1100), (512, 2048)])
+@pytest.mark.parametrize("splits", SPLITS, ids=str)
+@pytest.mark.parametrize("gathered,weighted,out", [(False, False, BF16), (True, False, F16), (False, True, F32), (True, True, BF16)])
+def test_grouped_product(splits, n, k, gathered, weighted, out):
+    print(f"[case] grouped {splits} {n} {k} {gathered} {weighted} {out}", flush=True)
+    rows, experts = sum(splits), len(splits)
+    tokens = max(rows // 3, 1) if gathered else rows
+    a, sa, va = operand(tokens, k=k, seed=3)
+    w, sw, vw = operand(experts, n, k=k, seed=4)
+    extra = 9  # rows past the last routed one are left as they were
+    g = torch.Generator().manual_seed(5)
+    gather = torch.randint(0, tokens, (rows + extra,), generator=g).to(torch.int32).to(DEV) if gathered else None
+    if not gathered:
+        a, sa = (torch.cat([t.view(torch.uint8), t.view(torch.uint8).new_full((extra, t.shape[1]), 255)]).view(t.dtype) for t in (a, sa))
+    factor = torch.rand(rows + extra, generator=g).to(DEV) if weighted else None
+    sp = torch.tensor(splits, dtype=torch.int32)
+    got = torch.full((rows + extra, n), 77.0, dtype=out, device=DEV)
+    same = flux_amd.MxGemm(out).forward_grouped(a, sp.to(DEV), w, sa, sw, gather_index=gather, row_scale=factor, output=got)
+    assert same.data_ptr() == got.data_ptr() and (got[rows:] == 77).all()
+    at = 0
+    for e, r in enumerate(splits):
+        mine = slice(at, at + r)
+        check(got[mine], va[gather[mine].long()] if gathered else va[mine], vw[e], k, factor[mine] if weighted else None)
+        at += r
+    host = flux_amd.MxGemm(out).forward_grouped(a, sp, w, sa, sw, gather_index=gather, row_scale=factor)
+    assert torch.equal(host[:rows], got[:rows])
+
+
+def test_counts_below_zero_and_past_the_rows():
+    a, sa, va = operand(40, k=256, seed=1)
+    w, sw, vw = operand(4, 70, k=256, seed=2)
+    out = torch.full((40, 70), 5.0, device=DEV)
+    flux_amd.MxGemm(F32).forward_grouped(a, torch.tensor([10, -7, 25, 1 << 30], dtype=torch.int32, device=DEV), w, sa, sw, output=out)
+    for e, rows in ((0, slice(0, 10)), (2, slice(10, 35)), (3, slice(35, 40))):
+        check(out[rows], va[rows], vw[e], 256)
+
+
+def test_gather_entries_past_the_input_are_clamped():
+    a, sa, va = operand(6, k=96, seed=1)
+    w, sw, vw = operand(1, 33, k=96, seed=2)
+    gather = torch.tensor([0, -5, 5, 6, 1 << 30, 3], dtype=torch.int32, device=DEV)
+    got = flux_amd.MxGemm(F32).forward_grouped(a, torch.tensor([6], dtype=torch.int32, device=DEV), w, sa, sw, gather_index=gather)
+    check(got, va[[0, 0, 5, 5, 5, 3]], vw[0], 96)
+
+
+@pytest.mark.parametrize("rows,k", [(20, 320), (300, 320), (300, 2048)])
+def test_nan_blocks_stay_in_their_rows_and_columns(rows, k):
+    a, sa, va = operand(rows, k=k, seed=1)
+    w, sw, vw = operand(1, 300, k=k, seed=2)
+    sa.view(torch.uint8)[7, 1] = 255
+    sw.view(torch.uint8)[0, 50, k // 32 - 1] = 255
+    got = flux_amd.MxGemm(F32).forward(a, w[0], sa, sw[0])
+    nan = torch.zeros(rows, 300, dtype=torch.bool, device=DEV)
+    nan[7], nan[:, 50] = True, True
+    assert torch.equal(got.isnan(), nan)
+    keep_r, keep_c = [i for i in range(rows) if i != 7], [i for i in range(300) if i != 50]
+    check(got[keep_r][:, keep_c], va[keep_r], vw[0][keep_c], k)
+
+
+def test_no_rows_no_columns():
+    a, sa, _ = operand(4, k=64, seed=1)
+    w, sw, _ = operand(2, 8, k=64, seed=2)
+    gemm = flux_amd.MxGemm(BF16)
+    assert gemm.forward(a[:0], w[0], sa[:0], sw[0]).shape == (0, 8)
+    assert gemm.forward(a, w[0][:0], sa, sw[0][:0]).shape == (4, 0)
+    assert gemm.forward_grouped(a[:0], torch.zeros(2, dtype=torch.int32, device=DEV), w, sa[:0], sw).shape == (0, 8)
+
+
+def test_weights_past_32_bits():
+    experts, n, k = 90, 14336, 7168  # 4.6 GB of codes
+    w = torch.randint(0, 256, (experts, n, k // 2), dtype=torch.uint8, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+    sw = torch.full((experts, n, k // 32), 120, dtype=torch.uint8, device=DEV)
+    a, sa, va = operand(40, k=k, seed=1)
+    splits = torch.zeros(experts, dtype=torch.int32)
+    splits[0], splits[-1] = 20, 20
+    got = flux_amd.MxGemm(F32).forward_grouped(a, splits.to(DEV), w.view(FP4), sa, sw.view(E8M0))
+    cols = torch.randint(0, n, (300,), device=DEV)
+    q = quantiser(F32)
+    for e, rows in ((0, slice(0, 20)), (experts - 1, slice(20, 40))):
+        vw = q.dequantize_mx(w[e][cols].view(FP4), sw[e][cols].view(E8M0)).double()
+        check(got[rows][:, cols], va[rows], vw, k)
+
+
+def test_graph_of_a_decode_step_replays():
+    """Quantisation and product in one graph, the splits on the device changing between replays."""
+    tokens, topk, experts, n, k = 40, 2, 4, 320, 512
+    w, sw, _ = operand(experts, n, k=k, seed=2)
+    x = torch.randn(tokens, k, device=DEV, dtype=BF16)
+    choosed = torch.randint(0, experts, (tokens, topk), dtype=torch.int32, device=DEV)
+    q, gemm = quantiser(BF16), flux_amd.MxGemm(BF16)
+
+    def step():
+        splits, scatter, gather, _ = flux_amd.moe_route_sort(choosed, experts)
+        codes, scale, _, _ = q.quantize_mx(x)
+        y = gemm.forward_grouped(codes, splits, w, scale, sw, gather_index=gather)
+        return y, flux_amd.moe_unpermute(y, scatter)
+
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    for seed in range(4):
+        gen = torch.Generator(device=DEV).manual_seed(seed)
+        x.copy_(torch.randn(tokens, k, device=DEV, generator=gen))
+        choosed.copy_(torch.randint(0, experts - (seed % 2), (tokens, topk), device=DEV, generator=gen))
+        want = step()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_on_another_stream():
+    a, sa, va = operand(30, k=640, seed=1)
+    w, sw, vw = operand(50, k=640, seed=2)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = flux_amd.MxGemm(F32).forward(a, w, sa, sw)
+    torch.cuda.current_stream().wait_stream(s)
+    check(got, va, vw, 640)
+
+
+@pytest.mark.parametrize("tokens", [1, 29, 600])
+def test_run_of_a_layer(tokens):
+    """Tokens to experts, gated MXFP4 products, and back with the router's weights: each step against 64 bits on the outputs of the one before."""
+    topk, experts, hidden, ffn = 3, 6, 352, 544
+    g = torch.Generator().manual_seed(tokens)
+    x = torch.randn(tokens, hidden, generator=g).to(BF16).to(DEV)
+    weight, choosed = torch.topk(torch.softmax(torch.randn(tokens, experts, generator=g), -1).to(DEV), topk)
+    choosed = choosed.to(torch.int32)
+    q, gemm, gemm32 = quantiser(BF16), flux_amd.MxGemm(BF16), flux_amd.MxGemm(F32)
+    (w1, s1, v1), (w3, s3, v3), (w2, s2, v2) = operand(experts, ffn, k=hidden, seed=1), operand(experts, ffn, k=hidden, seed=2), operand(experts, hidden, k=ffn, seed=3)
+    splits = torch.bincount(choosed.flatten().long(), minlength=experts).to(torch.int32)
+    scatter = flux_amd.calc_scatter_index(choosed, splits)
+    # the rows sorted by expert, quantised after the copy or before it: the same codes
+    rows = flux_amd.moe_permute(x, scatter)
+    codes, scale, _, _ = q.quantize_mx(rows)
+    xc, xs, _, _ = q.quantize_mx(x)
+    assert torch.equal(flux_amd.moe_permute(xc, scatter).view(torch.uint8), codes.view(torch.uint8))
+    assert torch.equal(flux_amd.moe_permute(xs, scatter).view(torch.uint8), scale.view(torch.uint8))
+    gate, up = (gemm.forward_grouped(codes, splits, w, scale, s) for w, s in ((w1, s1), (w3, s3)))
+    act = torch.nn.functional.silu(gate) * up
+    ac, asc, _, _ = q.quantize_mx(act)
+    down = gemm32.forward_grouped(ac, splits, w2, asc, s2)
+    out = flux_amd.moe_unpermute(down, scatter, weight)
+    vx = torch.from_numpy(mx.values(*mx.quantise(rows.double().cpu().numpy()))).to(DEV)
+    va = torch.from_numpy(mx.values(*mx.quantise(act.double().cpu().numpy()))).to(DEV)
+    at = 0
+    for e, r in enumerate(splits.tolist()):
+        mine = slice(at, at + r)
+        check(gate[mine], vx[mine], v1[e], hidden)
+        check(up[mine], vx[mine], v3[e], hidden)
+        check(down[mine], va[mine], v2[e], ffn)
+        at += r
+    terms = down.double()[scatter.long()] * weight.double().unsqueeze(-1)
+    assert ((out.double() - terms.sum(1)).abs() <= (topk + 1) * 2.0**-24 * terms.abs().sum(1)).all()
+
+
+def test_refusals():
+    a, sa, _ = operand(4, k=64, seed=1)
+    w, sw, _ = operand(2, 8, k=64, seed=2)
+    gemm, sp = flux_amd.MxGemm(BF16), torch.tensor([2, 2], dtype=torch.int32, device=DEV)
+    q = quantiser(BF16)
+    x = torch.zeros(4, 64, dtype=BF16, device=DEV)
+    for call, message in (
+        (lambda: q.quantize_mx(x.half()), "Inconsistency"),
+        (lambda: q.quantize_mx(x.t()), "contiguous"),
+        (lambda: q.quantize_mx(x[0]), "2 or 3 dimensions"),
+        (lambda: q.quantize_rowwise(x), "float8_e4m3fn"),
+        (lambda: q.quantize_vector_blockwise(x), "float8_e4m3fn"),
+        (lambda: flux_amd.Quantization(BF16, torch.float8_e4m3fn).quantize_mx(x), "float4_e2m1fn_x2"),
+        (lambda: q.dequantize_mx(a, sa, 32), "last of 2 blocks"),
+        (lambda: q.dequantize_mx(a, sa, 65), "last of 2 blocks"),
+        (lambda: q.dequantize_mx(a, sa[:, :1].contiguous()), "shape mismatch"),
+        (lambda: q.dequantize_mx(a.view(torch.uint8), sa), "float4_e2m1fn_x2"),
+        (lambda: gemm.forward(a, w[0], sa.view(torch.uint8), sw[0]), "float8_e8m0fnu"),
+        (lambda: gemm.forward(a, w[0][:, :16].contiguous(), sa, sw[0][:, :1].contiguous()), "mismatch"),
+        (lambda: gemm.forward(a, w, sa, sw), "2 dimensions"),
+        (lambda: gemm.forward(a, w[0], sa, sw[0], output=torch.empty(4, 8, device=DEV)), "Inconsistency"),
+        (lambda: gemm.forward_grouped(a, sp.long(), w, sa, sw), "int32"),
+        (lambda: gemm.forward_grouped(a, sp[:1], w, sa, sw), "splits 0-dim"),
+        (lambda: gemm.forward_grouped(a, torch.tensor([3, 2], dtype=torch.int32), w, sa, sw), "sum exceeds"),
+        (lambda: gemm.forward_grouped(a, sp, w, sa, sw, row_scale=torch.ones(3, device=DEV)), "row_scale must be"),
+        (lambda: gemm.forward_grouped(a, sp, w, sa, sw, gather_index=torch.zeros(4, dtype=torch.int64, device=DEV)), "Inconsistency"),
+        (lambda: gemm.forward_grouped(a[:0], sp, w, sa[:0], sw, gather_index=torch.zeros(4, dtype=torch.int32, device=DEV)), "empty input"),
+    ):
+        with pytest.raises(RuntimeError, match=message):
+            call()
