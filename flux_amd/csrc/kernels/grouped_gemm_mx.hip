@@ -6,6 +6,10 @@
 //
 // Few rows per expert: the weights are read once and everything else is small.  A workgroup has 64 columns of an expert and up to 64 of its
 // rows; its four waves split K in turns of 512 values and add their sums through LDS in a fixed order.
+//
+// Many rows: tiles of up to 256 x 256 through a ring of four stages in LDS, a stage 128 values of K (64 bytes a row), filled by loads that write LDS three
+// stages ahead.  A wave's fragments are read half a stage ahead of their MFMAs, and one barrier a stage, in its middle, stands between the fills and the
+// reads.  Scales come 16 bytes a row for four stages, into two buffers of their own.
 #include "rows.hpp"
 
 namespace fluxmi {
@@ -25,6 +29,7 @@ struct MxParams {
   const int32_t *splits, *gather_a;
   const float *row_scale;
   int32_t nexperts, max_rows, n, kb, a_rows;  // kb: blocks of a row
+  int32_t scale_stride;                       // bytes from row to row of the scales
   Row d_type;
 };
 
@@ -110,7 +115,276 @@ __device__ __forceinline__ void load_turn(Turn &t, const uint8_t *codes, const u
   }
 }
 
+// ---- tiles -----------------------------------------------------------------------------------------------------
+
+// A tile: rows row0 .. row0 + rows of the sorted rows, all of expert e, columns from n0 on; rows == 0: there is no such tile.
+struct TileItem {
+  int e, row0, rows, n0;
+};
+
+// Workgroup -> tile.  Experts in order; an expert's rows are dealt to its row tiles evenly in units of 32, and its tiles are walked in groups of up to 8 row tiles,
+// column by column.  Workgroups come to the eight XCDs in turn: each XCD has one stretch of that order, so that its L2 holds what its tiles share.
+__device__ __forceinline__ TileItem locate_tile(const MxParams &p, int block, int tiles_n, int bm, int bn) {
+  const int lane = threadIdx.x & 63;
+  int row_carry = 0, piece_carry = 0, begin = 0, rows = 0, pieces_end = 0;
+  auto scan = [&](int e0) {
+    int r = 0;
+    if (e0 + lane < p.nexperts) r = p.splits ? p.splits[e0 + lane] : p.max_rows;
+    r = r < 0 ? 0 : (r > p.max_rows ? p.max_rows : r);
+    const int incl = wave_inclusive_scan(r);
+    int end = row_carry + incl;
+    begin = end - r > p.max_rows ? p.max_rows : end - r;
+    end = end > p.max_rows ? p.max_rows : end;
+    rows = end - begin;
+    row_carry = __builtin_amdgcn_readlane(end, 63);
+    pieces_end = piece_carry + wave_inclusive_scan((rows + bm - 1) / bm);
+    piece_carry = __builtin_amdgcn_readlane(pieces_end, 63);
+  };
+  for (int e0 = 0; e0 < p.nexperts; e0 += 64) scan(e0);
+  const int per_xcd = (piece_carry * tiles_n + 7) / 8, i = block >> 3, item = (block & 7) * per_xcd + i;
+  if (i >= per_xcd || item >= piece_carry * tiles_n) return {0, 0, 0, 0};
+  row_carry = piece_carry = 0;
+  for (int e0 = 0; e0 < p.nexperts; e0 += 64) {
+    if (p.nexperts > 64) scan(e0);
+    const uint64_t hit = __ballot(item < pieces_end * tiles_n);
+    if (hit == 0) continue;
+    const int src = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+    const int e_begin = __builtin_amdgcn_readlane(begin, src), e_rows = __builtin_amdgcn_readlane(rows, src);
+    const int m_tiles = (e_rows + bm - 1) / bm, local = item - (__builtin_amdgcn_readlane(pieces_end, src) - m_tiles) * tiles_n;
+    const int groups = (m_tiles + 7) / 8, per_group = (m_tiles + groups - 1) / groups;
+    const int group = local / (per_group * tiles_n), group_rows = m_tiles - group * per_group < per_group ? m_tiles - group * per_group : per_group;
+    const int in_group = local - group * per_group * tiles_n, nt = in_group / group_rows, mt = group * per_group + in_group - nt * group_rows;
+    const int units = (e_rows + 31) / 32, per = units / m_tiles, longer = units - per * m_tiles;
+    const int m0 = 32 * (mt * per + (mt < longer ? mt : longer)), height = 32 * (per + (mt < longer ? 1 : 0));
+    TileItem t;
+    t.e = __builtin_amdgcn_readfirstlane(e0 + src);
+    t.row0 = __builtin_amdgcn_readfirstlane(e_begin + m0);
+    t.rows = __builtin_amdgcn_readfirstlane(e_rows - m0 < height ? e_rows - m0 : height);
+    t.n0 = __builtin_amdgcn_readfirstlane(nt * bn);
+    return t;
+  }
+  return {0, 0, 0, 0};
+}
+
+#define FLUXMI_VMCNT(vm) __builtin_amdgcn_s_waitcnt(((vm)&15) | (((vm) >> 4) << 14) | (7 << 4) | (15 << 8))
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void *base, int64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, static_cast<int>(bytes), 0x00020000);
+}
+
+// 16 bytes a lane to LDS at `dst` + 16 * lane, zeros from an offset past the buffer.  (The scalar registers may come from vector instructions: five wait states
+// lie between the statement's start and the load.)
+__device__ __forceinline__ void fill(uint32_t dst, uint32_t off, __amdgpu_buffer_rsrc_t r, int soff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(dst), "v"(off), "s"(r), "s"(soff) : "memory");
+}
+
+constexpr uint32_t kNoRow = 0x80000000u;  // a byte offset past every operand
+
+// The column of a tile that row R of B's part of a stage holds: of 32 rows, lane group g finds columns 8 g .. 8 g + 7 in its sums of the two blocks of 16.
+__device__ __forceinline__ int column_of(int R) { return (R & ~31) + 8 * ((R & 15) >> 2) + 4 * ((R >> 4) & 1) + (R & 3); }
+
 #endif  // __HIP_DEVICE_COMPILE__
+
+// MI x NJ blocks of 16 rows x 16 columns to a wave, WM x WN waves to a tile.
+template <int MI, int NJ, int WM, int WN>
+struct Tile {
+  static constexpr int kWaves = WM * WN, BM = MI * 16 * WM, BN = NJ * 16 * WN;
+  static constexpr int XF = BM / 16 / kWaves, WF = BN / 16 / kWaves;                 // fills of a wave for a stage
+  static constexpr int SF = ((BM + BN) / 64 + kWaves - 1) / kWaves;                  // ... for the scales of four stages
+  static constexpr int kStage = (BM + BN) * 64, kStages = 4, kScales = (BM + BN) * 16;
+  static constexpr int kLds = kStage * kStages + 2 * kScales;
+  static_assert(BM % (16 * kWaves) == 0 && BN % (16 * kWaves) == 0 && BM % 64 == 0 && BN % 64 == 0 && MI % 2 == 0 && NJ % 2 == 0, "");
+};
+
+template <int MI, int NJ, int WM, int WN>
+__global__ __launch_bounds__(64 * WM *WN, 2) void mx_tile_kernel(const MxParams p, int tiles_n) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using C = Tile<MI, NJ, WM, WN>;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const TileItem t = locate_tile(p, blockIdx.x, tiles_n, C::BM, C::BN);
+  if (t.rows <= 0) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)smem));
+  const int row_bytes = p.kb * 16, stages = (p.kb + 3) / 4;
+
+  // ---- fills: LDS row R lies at R * 64, its chunk c of 16 bytes at slot c ^ ((R >> 2) & 3); a fill covers 16 rows, lane l row l >> 2 and slot l & 3.
+  const int chunk = (lane & 3) ^ (lane >> 4);
+  const auto xr = buffer_of(p.a, static_cast<int64_t>(p.a_rows) * row_bytes), xsr = buffer_of(p.a_scale, static_cast<int64_t>(p.a_rows) * p.scale_stride);
+  const auto wr = buffer_of(p.b + static_cast<int64_t>(t.e) * p.n * row_bytes, static_cast<int64_t>(p.n) * row_bytes);
+  const auto wsr = buffer_of(p.b_scale + static_cast<int64_t>(t.e) * p.n * p.scale_stride, static_cast<int64_t>(p.n) * p.scale_stride);
+  uint32_t xoff[C::XF], woff[C::WF], soff[C::SF];
+#pragma unroll
+  for (int q = 0; q < C::XF; ++q) {
+    const int m = (wave * C::XF + q) * 16 + (lane >> 2);
+    xoff[q] = m < t.rows ? static_cast<uint32_t>(a_row(p, t.row0 + m)) * row_bytes + chunk * 16 : kNoRow;
+  }
+#pragma unroll
+  for (int q = 0; q < C::WF; ++q) {
+    const int n = t.n0 + column_of((wave * C::WF + q) * 16 + (lane >> 2));
+    woff[q] = n < p.n ? static_cast<uint32_t>(n) * row_bytes + chunk * 16 : kNoRow;
+  }
+#pragma unroll
+  for (int q = 0; q < C::SF; ++q) {  // A's rows, then B's; waves without rows of their own repeat the first ones'
+    const int R = (wave * C::SF + q) % ((C::BM + C::BN) / 64) * 64 + lane;
+    if (R < C::BM) {
+      soff[q] = R < t.rows ? static_cast<uint32_t>(a_row(p, t.row0 + R)) * p.scale_stride : kNoRow;
+    } else {
+      const int n = t.n0 + column_of(R - C::BM);
+      soff[q] = n < p.n ? static_cast<uint32_t>(n) * p.scale_stride : kNoRow;
+    }
+  }
+  // Stage s, into slot s mod 4; blocks past the end of the rows, and stages past the last, are zeros.
+  auto fill_stage = [&](int s, int slot) {
+    if ((slot & 3) == 0) {
+#pragma unroll
+      for (int q = 0; q < C::SF; ++q) {
+        const int group = (wave * C::SF + q) % ((C::BM + C::BN) / 64);
+        fill(lds0 + C::kStage * C::kStages + ((s >> 2) & 1) * C::kScales + group * 1024, soff[q], group * 64 < C::BM ? xsr : wsr, (s >> 2) * 16);
+      }
+    }
+    const bool in = s * 4 + chunk < p.kb;
+    const uint32_t dst = lds0 + slot * C::kStage;
+#pragma unroll
+    for (int q = 0; q < C::XF; ++q) fill(dst + (wave * C::XF + q) * 1024, in ? xoff[q] : kNoRow, xr, s * 64);
+#pragma unroll
+    for (int q = 0; q < C::WF; ++q) fill(dst + C::BM * 64 + (wave * C::WF + q) * 1024, in ? woff[q] : kNoRow, wr, s * 64);
+  };
+
+  // ---- fragments ---------------------------------------------------------------------------------------------
+  typedef const __attribute__((address_space(3))) u32x4 *LdsFrag;
+  typedef const __attribute__((address_space(3))) uint8_t *LdsByte;
+  // Wave rows: of both halves of the tile's rows MI / 2 blocks each, so that few rows are shared out evenly.
+  const uint32_t in_rows = (lane & 15) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3)) * 16);
+  const uint32_t xread = lds0 + wm * (MI * 8) * 64 + in_rows, wread = lds0 + (C::BM + wn * NJ * 16) * 64 + in_rows;
+  const uint32_t in_scales = lds0 + C::kStage * C::kStages + (lane & 15) * 16 + (lane >> 4);
+  const uint32_t xsread = in_scales + wm * (MI * 8) * 16, wsread = in_scales + (C::BM + wn * NJ * 16) * 16;
+  struct XHalf {
+    u32x4 code[MI / 2];
+    uint32_t scale[MI / 2];
+  };
+  struct WAll {
+    u32x4 code[NJ];
+    uint32_t scale[NJ];
+  };
+  auto read_x = [&](XHalf &x, int s, int slot, int half) {
+    const uint32_t at = xread + slot * C::kStage, sc = xsread + ((s >> 2) & 1) * C::kScales + (slot & 3) * 4;
+#pragma unroll
+    for (int i = 0; i < MI / 2; ++i) {
+      x.code[i] = *reinterpret_cast<LdsFrag>(at + half * (C::BM / 2) * 64 + i * 1024);
+      x.scale[i] = *reinterpret_cast<LdsByte>(sc + half * (C::BM / 2) * 16 + i * 256);
+    }
+  };
+  auto read_w = [&](WAll &w, int s, int slot) {
+    const uint32_t at = wread + slot * C::kStage, sc = wsread + ((s >> 2) & 1) * C::kScales + (slot & 3) * 4;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      w.code[j] = *reinterpret_cast<LdsFrag>(at + j * 1024);
+      w.scale[j] = *reinterpret_cast<LdsByte>(sc + j * 256);
+    }
+  };
+  f32x4 acc[MI][NJ] = {};
+  const bool has0 = wm * (MI * 8) < t.rows, has1 = C::BM / 2 + wm * (MI * 8) < t.rows;  // rows of the tile in the wave's halves
+  auto compute = [&](const XHalf &x, const WAll &w, int half) {
+    if (half == 0 ? !has0 : !has1) return;
+#pragma unroll
+    for (int i = 0; i < MI / 2; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[half * (MI / 2) + i][j] = mfma(w.code[j], x.code[i], w.scale[j], x.scale[i], acc[half * (MI / 2) + i][j]);
+  };
+  auto sync = [&]() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  // ---- the loop over K ----------------------------------------------------------------------------------------
+  constexpr int kFills = C::XF + C::WF;
+  fill_stage(0, 0);
+  fill_stage(1, 1);
+  fill_stage(2, 2);
+  FLUXMI_VMCNT(2 * kFills);
+  sync();
+  XHalf x0, x1;
+  WAll wa, wb;
+  read_w(wa, 0, 0);
+  read_x(x0, 0, 0, 0);
+  // One stage: its first rows with what was read before, then, behind the barrier that shows the next stage, the others.
+  auto stage = [&](auto SLOT, int s, WAll &w, WAll &w_next) {
+    constexpr int slot = decltype(SLOT)::value;
+    read_x(x1, s, slot, 1);
+    compute(x0, w, 0);
+    FLUXMI_VMCNT(slot == 2 ? kFills + C::SF : kFills);  // stage s + 1 has come; s + 2 may be on its way
+    sync();
+    fill_stage(s + 3, (slot + 3) & 3);
+    read_w(w_next, s + 1, (slot + 1) & 3);
+    read_x(x0, s + 1, (slot + 1) & 3, 0);
+    compute(x1, w, 1);
+  };
+  for (int s = 0;;) {
+    stage(std::integral_constant<int, 0>{}, s, wa, wb);
+    if (++s == stages) break;
+    stage(std::integral_constant<int, 1>{}, s, wb, wa);
+    if (++s == stages) break;
+    stage(std::integral_constant<int, 2>{}, s, wa, wb);
+    if (++s == stages) break;
+    stage(std::integral_constant<int, 3>{}, s, wb, wa);
+    if (++s == stages) break;
+  }
+  FLUXMI_VMCNT(0);  // fills past the end write zeros: LDS is this workgroup's until they have
+
+  // ---- results: lane group g has columns 8 g .. 8 g + 7 of each 32, of row lane & 15 of each block ------------------
+  float rs[MI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int m = (i / (MI / 2)) * (C::BM / 2) + wm * (MI * 8) + (i % (MI / 2)) * 16 + (lane & 15);
+    rs[i] = p.row_scale && m < t.rows ? p.row_scale[t.row0 + m] : 1.f;
+  }
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int m = (i / (MI / 2)) * (C::BM / 2) + wm * (MI * 8) + (i % (MI / 2)) * 16 + (lane & 15);
+    if (m >= t.rows) continue;
+    const size_t row = static_cast<size_t>(t.row0 + m) * p.n;
+#pragma unroll
+    for (int jg = 0; jg < NJ / 2; ++jg) {
+      const int n = t.n0 + wn * NJ * 16 + jg * 32 + (lane >> 4) * 8;
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = acc[i][2 * jg + k / 4][k % 4] * rs[i];
+      if (n + 8 <= p.n) {
+        if (p.d_type == Row::F32) {
+          store16(p.d + (row + n) * 4, pack<Row::F32>(reinterpret_cast<const float(&)[4]>(v[0])));
+          store16(p.d + (row + n) * 4 + 16, pack<Row::F32>(reinterpret_cast<const float(&)[4]>(v[4])));
+        } else {
+          store16(p.d + (row + n) * 2, p.d_type == Row::BF16 ? pack<Row::BF16>(v) : pack<Row::F16>(v));
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (n + k < p.n) store_one(p.d, p.d_type, row + n + k, v[k]);
+      }
+    }
+  }
+#endif  // __HIP_DEVICE_COMPILE__
+}
+
+// Scales in rows of a multiple of 16 bytes, zeros behind their end, as the tiles read them: A's rows, then those of all experts.
+__global__ __launch_bounds__(kThreads) void mx_pad_scales_kernel(const uint8_t *__restrict__ a, int64_t a_rows, const uint8_t *__restrict__ b, int64_t b_rows, int kb, int stride,
+                                                                 uint8_t *__restrict__ out) {
+  const int per_row = stride / 16;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < (a_rows + b_rows) * per_row; i += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int64_t row = i / per_row;
+    const int c = static_cast<int>(i - row * per_row) * 16;
+    const uint8_t *const src = (row < a_rows ? a + row * kb : b + (row - a_rows) * kb) + c;
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (c + 16 <= kb) {
+      v = load16(src);
+    } else {
+      for (int k = 0; k < kb - c; ++k) v[k / 4] |= static_cast<uint32_t>(src[k]) << (8 * (k & 3));
+    }
+    store16(out + i * 16, v);
+  }
+}
 
 template <int MT>
 __global__ __launch_bounds__(kThreads) void mx_few_rows_kernel(const MxParams p, int tiles_n) {
@@ -215,10 +489,30 @@ int launch_few_rows(const MxParams &p, hipStream_t s) {
   return FLUXMI_OK;
 }
 
+template <int MI, int NJ, int WM, int WN>
+int launch_tiles(const MxParams &p, hipStream_t s) {
+  using C = Tile<MI, NJ, WM, WN>;
+  static std::atomic<uint64_t> lds_done{0};
+  const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(mx_tile_kernel<MI, NJ, WM, WN>), C::kLds, lds_done);
+  if (rc != FLUXMI_OK) return rc;
+  const int tiles_n = (p.n + C::BN - 1) / C::BN;
+  const int64_t pieces = p.max_rows / C::BM + (p.nexperts < p.max_rows ? p.nexperts : p.max_rows), grid = (pieces * tiles_n + 7) / 8 * 8;
+  FLUXMI_REQUIRE(grid * 64 * C::kWaves < (int64_t{1} << 32), FLUXMI_ERR_UNSUPPORTED, "grouped_gemm_mx: max_rows=%d and n=%d are more than a launch covers", p.max_rows, p.n);
+  hipLaunchKernelGGL((mx_tile_kernel<MI, NJ, WM, WN>), dim3(static_cast<unsigned>(grid)), dim3(64 * C::kWaves), C::kLds, s, p, tiles_n);
+  return FLUXMI_OK;
+}
+
+bool takes_tiles(const fluxmi_mx_gemm_args &a) { return a.max_rows / a.nexperts > 64; }
+
 }  // namespace
 }  // namespace fluxmi
 
-extern "C" size_t fluxmi_grouped_gemm_mx_workspace_bytes(const fluxmi_mx_gemm_args *) { return 0; }
+extern "C" size_t fluxmi_grouped_gemm_mx_workspace_bytes(const fluxmi_mx_gemm_args *args) {
+  if (args == nullptr || args->nexperts < 1 || args->max_rows < 1 || args->n < 1 || args->k < 1 || args->a_rows < 0) return 0;
+  const int64_t kb = (int64_t{args->k} + 31) / 32;
+  if (kb % 16 == 0 || !fluxmi::takes_tiles(*args)) return 0;
+  return static_cast<size_t>(args->a_rows + int64_t{args->nexperts} * args->n) * ((kb + 15) / 16 * 16);
+}
 
 extern "C" int fluxmi_grouped_gemm_mx(const fluxmi_mx_gemm_args *args, void *workspace, size_t workspace_bytes, void *stream) {
   using namespace fluxmi;
@@ -244,6 +538,22 @@ extern "C" int fluxmi_grouped_gemm_mx(const fluxmi_mx_gemm_args *args, void *wor
   p.d_type = args->d_type == FLUXMI_ROWS_BF16 ? Row::BF16 : args->d_type == FLUXMI_ROWS_FP32 ? Row::F32 : Row::F16;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int average = p.max_rows / p.nexperts;
+  p.scale_stride = p.kb;
+  if (takes_tiles(*args)) {
+    if (need > 0) {
+      p.scale_stride = (p.kb + 15) / 16 * 16;
+      const int64_t a_rows = p.a_rows, b_rows = int64_t{p.nexperts} * p.n, groups = (a_rows + b_rows) * (p.scale_stride / 16);
+      const unsigned grid = static_cast<unsigned>(groups / kThreads < 8192 ? groups / kThreads + 1 : 8192);
+      uint8_t *const padded = static_cast<uint8_t *>(workspace);
+      hipLaunchKernelGGL(mx_pad_scales_kernel, dim3(grid), dim3(kThreads), 0, s, p.a_scale, a_rows, p.b_scale, b_rows, p.kb, p.scale_stride, padded);
+      p.a_scale = padded;
+      p.b_scale = padded + a_rows * p.scale_stride;
+    }
+    rc = launch_tiles<8, 4, 2, 4>(p, s);
+    if (rc != FLUXMI_OK) return rc;
+    FLUXMI_HIP_CHECK(hipGetLastError());
+    return FLUXMI_OK;
+  }
   rc = average <= 16 ? launch_few_rows<1>(p, s) : average <= 32 ? launch_few_rows<2>(p, s) : launch_few_rows<4>(p, s);
   if (rc != FLUXMI_OK) return rc;
   FLUXMI_HIP_CHECK(hipGetLastError());

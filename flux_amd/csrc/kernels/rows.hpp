@@ -28,6 +28,35 @@ constexpr int kElt = T == Row::F32 ? 4 : 2;
 template <Row T>
 constexpr int kVec = 16 / kElt<T>;  // elements of a vector
 
+template <Row T>
+__device__ __forceinline__ void unpack(const u32x4 v, float (&x)[kVec<T>]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (T == Row::F32) {
+      x[i] = __uint_as_float(v[i]);
+    } else if constexpr (T == Row::F16) {
+      x[2 * i] = f16_bits_to_float(static_cast<uint16_t>(v[i] & 0xffffu));
+      x[2 * i + 1] = f16_bits_to_float(static_cast<uint16_t>(v[i] >> 16));
+    } else {
+      x[2 * i] = __uint_as_float(v[i] << 16);
+      x[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+    }
+  }
+}
+
+// One rounding to the rows' type.
+template <Row T>
+__device__ __forceinline__ u32x4 pack(const float (&x)[kVec<T>]) {
+  u32x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (T == Row::F32) v[i] = __float_as_uint(x[i]);
+    else if constexpr (T == Row::F16) v[i] = float_to_f16_bits(x[2 * i]) | static_cast<uint32_t>(float_to_f16_bits(x[2 * i + 1])) << 16;
+    else v[i] = float_to_bf16_bits(x[2 * i]) | static_cast<uint32_t>(float_to_bf16_bits(x[2 * i + 1])) << 16;
+  }
+  return v;
+}
+
 // ---- host ----------------------------------------------------------------------------------------------------
 inline int check_type(const char *who, int32_t type, Row *row) {
   FLUXMI_REQUIRE(type == FLUXMI_ROWS_BF16 || type == FLUXMI_ROWS_FP32 || type == FLUXMI_ROWS_FP16, FLUXMI_ERR_INVALID_ARG, "%s: unknown type %d", who, type);
