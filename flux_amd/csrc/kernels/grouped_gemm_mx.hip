@@ -7,9 +7,9 @@
 // Few rows per expert: the weights are read once and everything else is small.  A workgroup has 64 columns of an expert and up to 64 of its
 // rows; its four waves split K in turns of 512 values and add their sums through LDS in a fixed order.
 //
-// Many rows: tiles of up to 256 x 256 through a ring of four stages in LDS, a stage 128 values of K (64 bytes a row), filled by loads that write LDS three
-// stages ahead.  A wave's fragments are read half a stage ahead of their MFMAs, and one barrier a stage, in its middle, stands between the fills and the
-// reads.  Scales come 16 bytes a row for four stages, into two buffers of their own.
+// Many rows: tiles of 256 x 256 on eight waves through a ring of four stages in LDS, a stage 128 values of K (64 bytes a row), filled by loads that write
+// LDS.  The waves of a SIMD take turns: while one computes a stage, the other reads its fragments and requests fills.  Scales come 16 bytes a row for four
+// stages, and lie in registers while those are computed.
 #include "rows.hpp"
 
 namespace fluxmi {
@@ -76,10 +76,12 @@ __device__ __forceinline__ int a_row(const MxParams &p, int r) {
   return x < 0 ? 0 : (x >= p.a_rows ? p.a_rows - 1 : x);
 }
 
+// BYTE: the byte of both scale registers that the MFMA takes.
+template <int BYTE>
 __device__ __forceinline__ f32x4 mfma(const u32x4 w, const u32x4 x, uint32_t w_scale, uint32_t x_scale, f32x4 c) {
   const i32x8 wa = {static_cast<int>(w[0]), static_cast<int>(w[1]), static_cast<int>(w[2]), static_cast<int>(w[3]), 0, 0, 0, 0};
   const i32x8 xa = {static_cast<int>(x[0]), static_cast<int>(x[1]), static_cast<int>(x[2]), static_cast<int>(x[3]), 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xa, c, 4, 4, 0, w_scale, 0, x_scale);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xa, c, 4, 4, BYTE, w_scale, BYTE, x_scale);
 }
 
 __device__ __forceinline__ void store_one(uint8_t *d, Row type, size_t i, float v) {
@@ -166,6 +168,7 @@ __device__ __forceinline__ TileItem locate_tile(const MxParams &p, int block, in
   return {0, 0, 0, 0};
 }
 
+#define FLUXMI_LGKM0() __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8))
 #define FLUXMI_VMCNT(vm) __builtin_amdgcn_s_waitcnt(((vm)&15) | (((vm) >> 4) << 14) | (7 << 4) | (15 << 8))
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void *base, int64_t bytes) {
@@ -185,19 +188,19 @@ __device__ __forceinline__ int column_of(int R) { return (R & ~31) + 8 * ((R & 1
 
 #endif  // __HIP_DEVICE_COMPILE__
 
-// MI x NJ blocks of 16 rows x 16 columns to a wave, WM x WN waves to a tile.
+// MI x NJ blocks of 16 rows x 16 columns to a wave, WM x WN = 8 waves to a tile.
 template <int MI, int NJ, int WM, int WN>
 struct Tile {
-  static constexpr int kWaves = WM * WN, BM = MI * 16 * WM, BN = NJ * 16 * WN;
-  static constexpr int XF = BM / 16 / kWaves, WF = BN / 16 / kWaves;                 // fills of a wave for a stage
-  static constexpr int SF = ((BM + BN) / 64 + kWaves - 1) / kWaves;                  // ... for the scales of four stages
-  static constexpr int kStage = (BM + BN) * 64, kStages = 4, kScales = (BM + BN) * 16;
-  static constexpr int kLds = kStage * kStages + 2 * kScales;
-  static_assert(BM % (16 * kWaves) == 0 && BN % (16 * kWaves) == 0 && BM % 64 == 0 && BN % 64 == 0 && MI % 2 == 0 && NJ % 2 == 0, "");
+  static constexpr int BM = MI * 16 * WM, BN = NJ * 16 * WN;
+  static constexpr int XF = BM / 128, WF = BN / 128;            // fills of a wave for a stage
+  static constexpr int kScaleFills = (BM + BN) / 64;             // fills of a tile for the scales of four stages, one or none to a wave
+  static constexpr int kStage = (BM + BN) * 64, kStages = 4;
+  static constexpr int kLds = kStage * kStages + (BM + BN) * 16;  // the ring, and the scales of four stages
+  static_assert(WM * WN == 8 && BM % 128 == 0 && BN % 128 == 0 && kScaleFills <= 8, "");
 };
 
 template <int MI, int NJ, int WM, int WN>
-__global__ __launch_bounds__(64 * WM *WN, 2) void mx_tile_kernel(const MxParams p, int tiles_n) {
+__global__ __launch_bounds__(512, 2) void mx_tile_kernel(const MxParams p, int tiles_n) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using C = Tile<MI, NJ, WM, WN>;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
@@ -209,10 +212,13 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void mx_tile_kernel(const MxParams 
 
   // ---- fills: LDS row R lies at R * 64, its chunk c of 16 bytes at slot c ^ ((R >> 2) & 3); a fill covers 16 rows, lane l row l >> 2 and slot l & 3.
   const int chunk = (lane & 3) ^ (lane >> 4);
-  const auto xr = buffer_of(p.a, static_cast<int64_t>(p.a_rows) * row_bytes), xsr = buffer_of(p.a_scale, static_cast<int64_t>(p.a_rows) * p.scale_stride);
+  const auto xr = buffer_of(p.a, static_cast<int64_t>(p.a_rows) * row_bytes);
   const auto wr = buffer_of(p.b + static_cast<int64_t>(t.e) * p.n * row_bytes, static_cast<int64_t>(p.n) * row_bytes);
-  const auto wsr = buffer_of(p.b_scale + static_cast<int64_t>(t.e) * p.n * p.scale_stride, static_cast<int64_t>(p.n) * p.scale_stride);
-  uint32_t xoff[C::XF], woff[C::WF], soff[C::SF];
+  const int scale_fill = wave % C::kScaleFills;  // (waves without one of their own repeat another's)
+  const bool scales_of_a = scale_fill * 64 < C::BM;
+  const auto sr = buffer_of(scales_of_a ? p.a_scale : p.b_scale + static_cast<int64_t>(t.e) * p.n * p.scale_stride,
+                            static_cast<int64_t>(scales_of_a ? p.a_rows : p.n) * p.scale_stride);
+  uint32_t xoff[C::XF], woff[C::WF], soff;
 #pragma unroll
   for (int q = 0; q < C::XF; ++q) {
     const int m = (wave * C::XF + q) * 16 + (lane >> 2);
@@ -223,25 +229,18 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void mx_tile_kernel(const MxParams 
     const int n = t.n0 + column_of((wave * C::WF + q) * 16 + (lane >> 2));
     woff[q] = n < p.n ? static_cast<uint32_t>(n) * row_bytes + chunk * 16 : kNoRow;
   }
-#pragma unroll
-  for (int q = 0; q < C::SF; ++q) {  // A's rows, then B's; waves without rows of their own repeat the first ones'
-    const int R = (wave * C::SF + q) % ((C::BM + C::BN) / 64) * 64 + lane;
+  {
+    const int R = scale_fill * 64 + lane;  // A's rows, then B's
     if (R < C::BM) {
-      soff[q] = R < t.rows ? static_cast<uint32_t>(a_row(p, t.row0 + R)) * p.scale_stride : kNoRow;
+      soff = R < t.rows ? static_cast<uint32_t>(a_row(p, t.row0 + R)) * p.scale_stride : kNoRow;
     } else {
       const int n = t.n0 + column_of(R - C::BM);
-      soff[q] = n < p.n ? static_cast<uint32_t>(n) * p.scale_stride : kNoRow;
+      soff = n < p.n ? static_cast<uint32_t>(n) * p.scale_stride : kNoRow;
     }
   }
   // Stage s, into slot s mod 4; blocks past the end of the rows, and stages past the last, are zeros.
   auto fill_stage = [&](int s, int slot) {
-    if ((slot & 3) == 0) {
-#pragma unroll
-      for (int q = 0; q < C::SF; ++q) {
-        const int group = (wave * C::SF + q) % ((C::BM + C::BN) / 64);
-        fill(lds0 + C::kStage * C::kStages + ((s >> 2) & 1) * C::kScales + group * 1024, soff[q], group * 64 < C::BM ? xsr : wsr, (s >> 2) * 16);
-      }
-    }
+    if (slot == 0) fill(lds0 + C::kStage * C::kStages + scale_fill * 1024, soff, sr, (s >> 2) * 16);
     const bool in = s * 4 + chunk < p.kb;
     const uint32_t dst = lds0 + slot * C::kStage;
 #pragma unroll
@@ -252,44 +251,47 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void mx_tile_kernel(const MxParams 
 
   // ---- fragments ---------------------------------------------------------------------------------------------
   typedef const __attribute__((address_space(3))) u32x4 *LdsFrag;
-  typedef const __attribute__((address_space(3))) uint8_t *LdsByte;
   // Wave rows: of both halves of the tile's rows MI / 2 blocks each, so that few rows are shared out evenly.
   const uint32_t in_rows = (lane & 15) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3)) * 16);
   const uint32_t xread = lds0 + wm * (MI * 8) * 64 + in_rows, wread = lds0 + (C::BM + wn * NJ * 16) * 64 + in_rows;
-  const uint32_t in_scales = lds0 + C::kStage * C::kStages + (lane & 15) * 16 + (lane >> 4);
+  const uint32_t in_scales = lds0 + C::kStage * C::kStages + (lane & 15) * 16;
   const uint32_t xsread = in_scales + wm * (MI * 8) * 16, wsread = in_scales + (C::BM + wn * NJ * 16) * 16;
-  struct XHalf {
-    u32x4 code[MI / 2];
-    uint32_t scale[MI / 2];
+  const bool has0 = wm * (MI * 8) < t.rows, has1 = C::BM / 2 + wm * (MI * 8) < t.rows;  // rows of the tile in the wave's halves
+  u32x4 x[MI], w[NJ];
+  uint32_t xs[MI], ws[NJ];  // byte s: the scale of this lane's block in stage s of four
+  // 16 bytes of a row's scales, byte 4 s + g for the lanes of group g in stage s -> the lane's four.
+  const uint32_t pick = 0x0c0c0400u + 0x0101u * (lane >> 4);
+  auto scales_of = [&](uint32_t at) {
+    const u32x4 v = *reinterpret_cast<LdsFrag>(at);
+    const uint32_t lo = __builtin_amdgcn_perm(v[1], v[0], pick), hi = __builtin_amdgcn_perm(v[3], v[2], pick);
+    return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
   };
-  struct WAll {
-    u32x4 code[NJ];
-    uint32_t scale[NJ];
-  };
-  auto read_x = [&](XHalf &x, int s, int slot, int half) {
-    const uint32_t at = xread + slot * C::kStage, sc = xsread + ((s >> 2) & 1) * C::kScales + (slot & 3) * 4;
+  auto read_stage = [&](int slot) {
+    const uint32_t xat = xread + slot * C::kStage, wat = wread + slot * C::kStage;
 #pragma unroll
-    for (int i = 0; i < MI / 2; ++i) {
-      x.code[i] = *reinterpret_cast<LdsFrag>(at + half * (C::BM / 2) * 64 + i * 1024);
-      x.scale[i] = *reinterpret_cast<LdsByte>(sc + half * (C::BM / 2) * 16 + i * 256);
-    }
-  };
-  auto read_w = [&](WAll &w, int s, int slot) {
-    const uint32_t at = wread + slot * C::kStage, sc = wsread + ((s >> 2) & 1) * C::kScales + (slot & 3) * 4;
+    for (int j = 0; j < NJ; ++j) w[j] = *reinterpret_cast<LdsFrag>(wat + j * 1024);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      w.code[j] = *reinterpret_cast<LdsFrag>(at + j * 1024);
-      w.scale[j] = *reinterpret_cast<LdsByte>(sc + j * 256);
+    for (int i = 0; i < MI; ++i) x[i] = *reinterpret_cast<LdsFrag>(xat + (i / (MI / 2)) * (C::BM / 2) * 64 + (i % (MI / 2)) * 1024);
+    if (slot == 0) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) ws[j] = scales_of(wsread + j * 256);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) xs[i] = scales_of(xsread + (i / (MI / 2)) * (C::BM / 2) * 16 + (i % (MI / 2)) * 256);
     }
   };
   f32x4 acc[MI][NJ] = {};
-  const bool has0 = wm * (MI * 8) < t.rows, has1 = C::BM / 2 + wm * (MI * 8) < t.rows;  // rows of the tile in the wave's halves
-  auto compute = [&](const XHalf &x, const WAll &w, int half) {
-    if (half == 0 ? !has0 : !has1) return;
+  auto compute = [&](auto SLOT) {
+    constexpr int slot = decltype(SLOT)::value;
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int i = 0; i < MI / 2; ++i)
+    for (int h = 0; h < 2; ++h) {
+      if (h == 0 ? !has0 : !has1) continue;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) acc[half * (MI / 2) + i][j] = mfma(w.code[j], x.code[i], w.scale[j], x.scale[i], acc[half * (MI / 2) + i][j]);
+      for (int i = h * (MI / 2); i < (h + 1) * (MI / 2); ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = mfma<slot>(w[j], x[i], ws[j], xs[i], acc[i][j]);
+    }
+    __builtin_amdgcn_s_setprio(0);
   };
   auto sync = [&]() {
     __builtin_amdgcn_sched_barrier(0);
@@ -299,38 +301,40 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void mx_tile_kernel(const MxParams 
   };
 
   // ---- the loop over K ----------------------------------------------------------------------------------------
+  // The four waves of a group, one to a SIMD, compute a stage while the others read their fragments and request fills; a barrier ends the phase for both.
+  // Both groups run the same code, the second one phase behind: the first reads stage s in phase 2 s - 1 and computes it in 2 s, the second reads it in
+  // 2 s and computes it in 2 s + 1.  Whoever reads stage s requests s + 3, whose slot was that of stage s - 1, which nobody reads after phase 2 s - 2.
+  // Stage s + 1 has to have come when phase 2 s ends; then stages s + 2 and s + 3 of a wave may be on their way.
   constexpr int kFills = C::XF + C::WF;
+  const bool behind = wave >= 4;
   fill_stage(0, 0);
   fill_stage(1, 1);
   fill_stage(2, 2);
   FLUXMI_VMCNT(2 * kFills);
   sync();
-  XHalf x0, x1;
-  WAll wa, wb;
-  read_w(wa, 0, 0);
-  read_x(x0, 0, 0, 0);
-  // One stage: its first rows with what was read before, then, behind the barrier that shows the next stage, the others.
-  auto stage = [&](auto SLOT, int s, WAll &w, WAll &w_next) {
-    constexpr int slot = decltype(SLOT)::value;
-    read_x(x1, s, slot, 1);
-    compute(x0, w, 0);
-    FLUXMI_VMCNT(slot == 2 ? kFills + C::SF : kFills);  // stage s + 1 has come; s + 2 may be on its way
-    sync();
+  if (behind) sync();
+  auto stage = [&](auto SLOT, int s) {
+    constexpr int slot = decltype(SLOT)::value, kYounger = 2 * kFills + (slot == 1 || slot == 2 ? 1 : 0);  // (scales come with every fourth stage)
+    read_stage(slot);
     fill_stage(s + 3, (slot + 3) & 3);
-    read_w(w_next, s + 1, (slot + 1) & 3);
-    read_x(x0, s + 1, (slot + 1) & 3, 0);
-    compute(x1, w, 1);
+    if (behind) FLUXMI_VMCNT(kYounger);
+    FLUXMI_LGKM0();
+    sync();
+    compute(SLOT);
+    if (!behind) FLUXMI_VMCNT(kYounger);
+    sync();
   };
   for (int s = 0;;) {
-    stage(std::integral_constant<int, 0>{}, s, wa, wb);
+    stage(std::integral_constant<int, 0>{}, s);
     if (++s == stages) break;
-    stage(std::integral_constant<int, 1>{}, s, wb, wa);
+    stage(std::integral_constant<int, 1>{}, s);
     if (++s == stages) break;
-    stage(std::integral_constant<int, 2>{}, s, wa, wb);
+    stage(std::integral_constant<int, 2>{}, s);
     if (++s == stages) break;
-    stage(std::integral_constant<int, 3>{}, s, wb, wa);
+    stage(std::integral_constant<int, 3>{}, s);
     if (++s == stages) break;
   }
+  if (!behind) sync();
   FLUXMI_VMCNT(0);  // fills past the end write zeros: LDS is this workgroup's until they have
 
   // ---- results: lane group g has columns 8 g .. 8 g + 7 of each 32, of row lane & 15 of each block ------------------
@@ -423,7 +427,7 @@ __global__ __launch_bounds__(kThreads) void mx_few_rows_kernel(const MxParams p,
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = mfma(wt[j].code[s], xt[i].code[s], wt[j].scale[s], xt[i].scale[s], acc[i][j]);
+        for (int j = 0; j < 4; ++j) acc[i][j] = mfma<0>(wt[j].code[s], xt[i].code[s], wt[j].scale[s], xt[i].scale[s], acc[i][j]);
   }
   // Wave w finishes the blocks of column group w.
 #pragma unroll
@@ -497,8 +501,8 @@ int launch_tiles(const MxParams &p, hipStream_t s) {
   if (rc != FLUXMI_OK) return rc;
   const int tiles_n = (p.n + C::BN - 1) / C::BN;
   const int64_t pieces = p.max_rows / C::BM + (p.nexperts < p.max_rows ? p.nexperts : p.max_rows), grid = (pieces * tiles_n + 7) / 8 * 8;
-  FLUXMI_REQUIRE(grid * 64 * C::kWaves < (int64_t{1} << 32), FLUXMI_ERR_UNSUPPORTED, "grouped_gemm_mx: max_rows=%d and n=%d are more than a launch covers", p.max_rows, p.n);
-  hipLaunchKernelGGL((mx_tile_kernel<MI, NJ, WM, WN>), dim3(static_cast<unsigned>(grid)), dim3(64 * C::kWaves), C::kLds, s, p, tiles_n);
+  FLUXMI_REQUIRE(grid * 512 < (int64_t{1} << 32), FLUXMI_ERR_UNSUPPORTED, "grouped_gemm_mx: max_rows=%d and n=%d are more than a launch covers", p.max_rows, p.n);
+  hipLaunchKernelGGL((mx_tile_kernel<MI, NJ, WM, WN>), dim3(static_cast<unsigned>(grid)), dim3(512), C::kLds, s, p, tiles_n);
   return FLUXMI_OK;
 }
 
