@@ -39,6 +39,9 @@ constexpr int kDualExperts = 128;     // two to a lane
 // Behind the scales: the experts' rows and tiles, and what a wave knows of its next tile's rows.
 constexpr int kTables = kUnit * kRing + 3 * kScaleSlot, kStash = kTables + 2 * kDualExperts * 4;
 constexpr int kDualLds = kStash + 5 * 4 * kDualThreads;
+// MXFP4: behind the ring the scale bytes of two steps, 16 of each row of A and of B, then the tables, then rows and scales of the next tile, each once.
+constexpr int kMxTables = kUnit * kRing + 16 * 2 * kTile, kMxStash = kMxTables + 2 * kDualExperts * 4, kMxStashOfWave = 32 + 64;
+constexpr int kMxLds = kMxStash + 4 * kMxStashOfWave * (kDualThreads / 64);
 constexpr uint32_t kNoRow = 0x80000000u;  // a byte offset past every operand, with offsets along K still below 2^32
 
 struct DualArgs {
@@ -117,9 +120,30 @@ __device__ __forceinline__ void quadrant(f32x4 (&acc)[8][4], const i32x4 (&x)[4]
   }
 }
 
+// MXFP4: the same quadrant, two MFMAs of 128 values to a block.  PAR: the step's place among the two whose scales a register holds, a byte for each of
+// their MFMAs.
+template <bool FIRST, int PAR, int I0, int J0>
+__device__ __forceinline__ void quadrant_mx(f32x4 (&acc)[8][4], const i32x4 (&x)[4][2], const i32x4 (&w)[4][2], const uint32_t (&xs)[8], const uint32_t (&ws)[4]) {
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  auto half = [&](auto H) {
+    constexpr int h = decltype(H)::value, byte = 2 * PAR + h;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const i32x4 a = w[J0 + j][h], b = x[i][h];
+        const i32x8 wa = {a[0], a[1], a[2], a[3], 0, 0, 0, 0}, xa = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
+        acc[I0 + i][J0 + j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xa, FIRST && h == 0 ? zero : acc[I0 + i][J0 + j], 4, 4, byte, ws[J0 + j],
+                                                                               byte, xs[I0 + i]);
+      }
+  };
+  half(std::integral_constant<int, 0>{});
+  half(std::integral_constant<int, 1>{});
+}
+
 template <Elem T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (T == Elem::F16) {
+  if constexpr (T == Elem::F16 || T == Elem::MXFP4_F16) {
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
     const f16x2 h = {static_cast<_Float16>(lo), static_cast<_Float16>(hi)};
     return __builtin_bit_cast(uint32_t, h);
@@ -155,11 +179,11 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
 #if defined(__HIP_DEVICE_COMPILE__)
   const GemmParams &p = args.p;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
-  constexpr bool BS = T == Elem::FP8_BLOCKSCALED;
+  constexpr bool BS = T == Elem::FP8_BLOCKSCALED, MX = is_mx(T);
   constexpr int ELT = is_fp8(T) ? 1 : 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 2, wn = wave & 3;
-  const int kbytes = p.k * ELT, steps = kbytes >> 7;
+  const int kbytes = MX ? p.k / 2 : p.k * ELT, steps = kbytes >> 7;
   const int tiles_n1 = (p.n + kTile - 1) / kTile, tiles_n = tiles_n1 * p.ngroups;
   const int grid = gridDim.x, bid = blockIdx.x;
   const int virt = (grid & 7) == 0 ? (bid & 7) * (grid >> 3) + (bid >> 3) : bid;
@@ -167,7 +191,7 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
   // ---- the experts: rows and tiles up to each of them, in LDS (registers are short) --------------------------
   typedef __attribute__((address_space(3))) int *LdsInt;
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)smem));
-  const LdsInt row_ends = reinterpret_cast<LdsInt>(lds0 + kTables), tile_ends = row_ends + kDualExperts;
+  const LdsInt row_ends = reinterpret_cast<LdsInt>(lds0 + (MX ? kMxTables : kTables)), tile_ends = row_ends + kDualExperts;
   int total_tiles;
   {
     int row_carry = 0, tile_carry = 0, chunks = 0, active = 0;
@@ -302,7 +326,7 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
       if (r + 8 < t.rows) nxt1 = src[8];
       if (r + 16 < t.rows) nxt2 = src[16];
       if (r + 24 < t.rows) nxt3 = src[24];
-      if constexpr (BS) {
+      if constexpr (BS || MX) {
         const int rs = wn * 64 + fresh_lane();
         nxts = 0;
         if (rs < t.rows) nxts = a->gather_a[t.row0 + rs];
@@ -320,7 +344,8 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
         const int x = static_cast<int>(v);
         row = x < 0 ? 0 : (x >= a_rows ? a_rows - 1 : x);
       }
-      return r + 8 * j < t.rows ? row * static_cast<uint32_t>(kbytes) + (chunk0 ^ ((j & 1) * 64)) : kNoRow;
+      const uint32_t chunk = MX ? 0 : chunk0 ^ ((j & 1) * 64);  // (MX: added when the offsets come out of LDS)
+      return r + 8 * j < t.rows ? row * static_cast<uint32_t>(kbytes) + chunk : kNoRow;
     };
     nxt0 = offset(nxt0, 0);
     nxt1 = offset(nxt1, 1);
@@ -334,6 +359,12 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
                                ? static_cast<uint32_t>(((row >> 7) * steps * 128 + (row & 127)) * 4)
                                : static_cast<uint32_t>((static_cast<int64_t>(t.e_row0) * (steps - 1) + row) * 4);
       nxts = rs < t.rows ? off : kNoRow;
+    }
+    if constexpr (MX) {  // the first group's scales: a row of A to each lane
+      const int rs = wn * 64 + l;
+      int row = t.row0 + rs;
+      if (gathered) row = static_cast<int>(nxts) < 0 ? 0 : (static_cast<int>(nxts) >= a_rows ? a_rows - 1 : static_cast<int>(nxts));
+      nxts = rs < t.rows ? static_cast<uint32_t>(row) * (kbytes / 16) : kNoRow;
     }
   };
   __amdgpu_buffer_rsrc_t xrsrc, wrsrc;
@@ -359,21 +390,49 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
     woff2 = w0 + wstep2 + chunk0;
     woff3 = w0 + wstep1 + wstep2 + (chunk0 ^ 64);
   };
-  const LdsInt stash = reinterpret_cast<LdsInt>(lds0 + kStash);
+  const LdsInt stash = reinterpret_cast<LdsInt>(lds0 + (MX ? kMxStash + wave * kMxStashOfWave * 4 : kStash));
   auto put_next = [&]() {
+    if constexpr (MX) {  // the eight lanes of a row have the same offset
+      const int l = fresh_lane(), r = l >> 3;
+      if ((l & 7) == 0) stash[r] = nxt0, stash[8 + r] = nxt1, stash[16 + r] = nxt2, stash[24 + r] = nxt3;
+      stash[32 + l] = nxts;
+      return;
+    }
     const int t = wave * 64 + fresh_lane();
     stash[t] = nxt0, stash[512 + t] = nxt1, stash[1024 + t] = nxt2, stash[1536 + t] = nxt3;
     if constexpr (BS) stash[2048 + t] = nxts;
   };
   auto get_next = [&]() {
+    if constexpr (MX) {
+      const int l = fresh_lane(), r = l >> 3;
+      const uint32_t chunk0 = chunk_of(l);  // (less than 128: an offset past the operand stays past it)
+      nxt0 = stash[r] + chunk0, nxt1 = stash[8 + r] + (chunk0 ^ 64), nxt2 = stash[16 + r] + chunk0, nxt3 = stash[24 + r] + (chunk0 ^ 64);
+      nxts = stash[32 + l];
+      return;
+    }
     const int t = wave * 64 + fresh_lane();
     nxt0 = stash[t], nxt1 = stash[512 + t], nxt2 = stash[1024 + t], nxt3 = stash[1536 + t];
     if constexpr (BS) nxts = stash[2048 + t];
   };
-  uint32_t soff = 0;   // block scales: of the scale that this lane of the first group fetches
+  uint32_t soff = 0;   // block scales: of the scale that this lane of the first group fetches; MXFP4: of the 16 that it fetches for two steps
   int sstep = 0;       // ... and their distance between steps
+  __amdgpu_buffer_rsrc_t srsrc;  // MXFP4: scales of A (first group) or of the tile's expert (second group)
   auto start_scales = [&](const DualTile &t) {
     const KernArgs a = kernel_args();
+    if constexpr (MX) {
+      const int kb = kbytes / 16, n = a->n;
+      const uint8_t *const base = wm == 0 ? reinterpret_cast<const uint8_t *>(a->a_scale)
+                                          : reinterpret_cast<const uint8_t *>(a->b_scale) + static_cast<int64_t>(t.e) * n * kb;
+      srsrc = buffer_of(base, static_cast<int64_t>(wm == 0 ? a->a_rows : n) * kb);
+      soff = nxts;
+      if (wm != 0) {  // the column of LDS row R of the step's W units
+        const int R = wn * 64 + fresh_lane(), in_half = R & 127, q = in_half & 31;
+        const int col = f32_out ? q : ((q >> 2) & 1) * 8 + (q & 3) + ((q >> 3) & 1) * 16 + (q >> 4) * 4;
+        const int first = t.wide ? (in_half >> 5) * 64 + (R >> 7) * 32 : (in_half >> 5) * 32, c = t.n0 + first + col;
+        soff = t.rows > 0 && c < n && (t.wide || R < 128) ? static_cast<uint32_t>(c) * kb : kNoRow;
+      }
+      return;
+    }
     soff = nxts;
     sstep = a->a_scale_layout == FLUXMI_ASCALE_BLOCK128 ? 512 : t.e_rows * 4;
   };
@@ -405,11 +464,31 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
   uint32_t xread[2], wread[2];
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    const uint32_t chunk = ((c * 4 + (lane >> 4)) ^ ((lane >> 1) & 7)) * 16;
+    const uint32_t chunk = ((MX ? (lane >> 4) * 2 + c : c * 4 + (lane >> 4)) ^ ((lane >> 1) & 7)) * 16;
     xread[c] = lds0 + (wm * 64 + (lane & 15)) * 128 + chunk;
     wread[c] = lds0 + (wn * 32 + (lane & 15)) * 128 + chunk;
   }
   const uint32_t sread = lds0 + kRing * kUnit + (wm * 64 + (lane & 15)) * 4;  // row scales of this lane
+  // MXFP4: scale bytes of this lane's blocks, one for each MFMA of two steps.  Lane group g has chunks 2 g and 2 g + 1 of a step's 128 bytes in its two
+  // MFMAs, so of the 16 bytes of a row it wants 2 g, 2 g + 1, 8 + 2 g and 9 + 2 g: halves of two words.
+  uint32_t xs[8], ws[4];
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  auto read_mx_scales = [&](u32x2 (&raw)[12]) {
+    typedef const __attribute__((address_space(3))) uint32_t *LdsWord;
+    const uint32_t at = lds0 + kRing * kUnit + (lane & 15) * 16 + (lane >> 5) * 4, x_at = at + wm * 1024, w_at = at + 4096 + wn * 512;
+    auto of_row = [&](uint32_t a) { return u32x2{*reinterpret_cast<LdsWord>(a), *reinterpret_cast<LdsWord>(a + 8)}; };
+#pragma unroll
+    for (int j = 0; j < 4; ++j) raw[j] = of_row(w_at + (j >> 1) * 2048 + (j & 1) * 256);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) raw[4 + i] = of_row(x_at + (i >> 2) * 2048 + (i & 3) * 256);
+  };
+  auto pick_mx_scales = [&](const u32x2 (&raw)[12]) {
+    const uint32_t pick = 0x05040100u + 0x02020202u * ((lane >> 4) & 1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ws[j] = __builtin_amdgcn_perm(raw[j][1], raw[j][0], pick);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) xs[i] = __builtin_amdgcn_perm(raw[4 + i][1], raw[4 + i][0], pick);
+  };
   // (An opaque address: the distance of the blocks goes into the instructions.)
   auto address = [&](uint32_t at, uint32_t slot) {
     uint32_t a = at + slot;
@@ -446,9 +525,13 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
   if (cur.rows == 0) return;
   load_rows(cur);
   rows_to_offsets(cur);
+  if constexpr (MX) {
+    put_next();
+    get_next();
+  }
   start_x(cur);
   start_w(cur);
-  if constexpr (BS) start_scales(cur);
+  if constexpr (BS || MX) start_scales(cur);
   DualTile nx = next_tile();
   // Row scales of step st into slot st mod 3 (of the launch's steps).
   auto fill_scales = [&](uint32_t slot, int st) {
@@ -457,6 +540,12 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds"
                  : : "s"(lds0 + kRing * kUnit + slot * kScaleSlot + wn * 256), "v"(soff), "s"(r) : "memory");
   };
+  // MXFP4: the scales of steps 2 m and 2 m + 1, 16 bytes of 64 rows to a wave: those of A by the first group, of B by the second.
+  auto fill_mx_scales = [&](int m) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 : : "s"(lds0 + kRing * kUnit + wave * 1024), "v"(soff), "s"(srsrc), "s"(m * 16) : "memory");
+  };
+  if constexpr (MX) fill_mx_scales(0);
   for (int s = 0; s < 2; ++s) {  // units 0 to 6
     if (wm == 0) {
       fill_w(slot_of(4 * s + 1), s * 128);
@@ -495,11 +584,13 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
         bs_step = nblocks;
       }
     }
-    auto step = [&](auto FIRSTSTEP, int s) {
+    auto step = [&](auto FIRSTSTEP, auto PARITY, auto ENDING, int s) {
       constexpr bool FS = decltype(FIRSTSTEP)::value;
+      constexpr int PAR = decltype(PARITY)::value;         // MXFP4: s & 1
+      constexpr bool ENDS = !MX || decltype(ENDING)::value;  // MXFP4: of a tile's last two steps, which request the next tile's first
       // The steps of K whose X and W this wave requests.
       int fw = s + 2, fx = s + 1 + wm;
-      if (fw >= steps) {
+      if (ENDS && fw >= steps) {
         fw -= steps;
         if (fw == 0) {
           start_w(nx);
@@ -509,7 +600,7 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
           }
         }
       }
-      if (fx >= steps) {
+      if (ENDS && fx >= steps) {
         fx -= steps;
         if (fx == 0) {
           get_next();
@@ -538,7 +629,18 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
       // What the waits count: a unit's fills are four instructions of a wave, and with block scales the first group's fills of a step's row
       // scales, one each, follow those of X.  The first steps of a tile were waited for at its start.
       // Read: the first half's rows, all columns.  Reads before fills: the phase ends when the last of them is issued.
-      read_x(slot_of(base));
+      if constexpr (MX && PAR == 0) {
+        // The words lie where B's fragments will; read after these, row for row in the few registers left, they cost 6 % of a long K.
+        u32x2 raw[12];
+        read_mx_scales(raw);
+        __builtin_amdgcn_sched_barrier(0);
+        read_x(slot_of(base));
+        __builtin_amdgcn_sched_barrier(0);
+        pick_mx_scales(raw);
+        __builtin_amdgcn_sched_barrier(0);
+      } else {
+        read_x(slot_of(base));
+      }
       read_w(slot_of(base + 1), 0);
       read_w(slot_of(base + 2), 2);
       read_scales(0);
@@ -549,33 +651,64 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
       sync();
       __builtin_amdgcn_s_setprio(1);
       if (rows0 > 0) {
-        quadrant<T, FS, 0, 0>(acc, x, w, scale);
-        if (wide) quadrant<T, FS, 0, 2>(acc, x, w, scale);
+        if constexpr (MX) {
+          quadrant_mx<FS, PAR, 0, 0>(acc, x, w, xs, ws);
+          if (wide) quadrant_mx<FS, PAR, 0, 2>(acc, x, w, xs, ws);
+        } else {
+          quadrant<T, FS, 0, 0>(acc, x, w, scale);
+          if (wide) quadrant<T, FS, 0, 2>(acc, x, w, scale);
+        }
       }
       __builtin_amdgcn_s_setprio(0);
-      if (wm == 0 && s > 0) FLUXMI_VMCNT(BS ? 10 : 8);  // X's second half, requested in the step before: two units, and scales, since
+      if (wm == 0 && s > 0) FLUXMI_VMCNT(BS ? 10 : (MX && PAR == 1 ? 9 : 8));  // X's second half, requested in the step before: two units, and scales, since
       sync();
       // Read: the second half's rows.
       read_x(slot_of(base + 3));
       read_scales(1);
       fill_w(slot_of(base + wm), fw * 128);
-      if (wm != 0 && s > 0) FLUXMI_VMCNT(8);  // the next step's X and W, requested two units ago and before
+      if constexpr (MX && PAR == 0) {  // both groups have read this pair of steps' scales: the next pair's, or the next tile's first
+        if constexpr (ENDS) {
+          get_next();
+          start_scales(nx);
+        }
+        fill_mx_scales(ENDS ? 0 : (s >> 1) + 1);
+      }
+      if (wm != 0 && s > 0) FLUXMI_VMCNT(MX && PAR == 0 ? 9 : 8);  // the next step's X and W, requested two units ago and before
       FLUXMI_LGKM0();
       scale_rows();
       sync();
       __builtin_amdgcn_s_setprio(1);
       if (rows0 > 128) {
-        quadrant<T, FS, 4, 0>(acc, x, w, scale);
-        if (wide) quadrant<T, FS, 4, 2>(acc, x, w, scale);
+        if constexpr (MX) {
+          quadrant_mx<FS, PAR, 4, 0>(acc, x, w, xs, ws);
+          if (wide) quadrant_mx<FS, PAR, 4, 2>(acc, x, w, xs, ws);
+        } else {
+          quadrant<T, FS, 4, 0>(acc, x, w, scale);
+          if (wide) quadrant<T, FS, 4, 2>(acc, x, w, scale);
+        }
       }
       __builtin_amdgcn_s_setprio(0);
-      if (wm == 0 && s > 0) FLUXMI_VMCNT(BS ? 9 : 8);  // the next step's W, requested in the step before: the same
+      if (wm == 0 && s > 0) FLUXMI_VMCNT(BS || (MX && PAR == 0) ? 9 : 8);  // the next step's W, requested in the step before: the same
       base = base + 4 >= kRing ? base + 4 - kRing : base + 4;
       scale_slot = scale_slot == 2 ? 0 : scale_slot + 1;
-      if (wm == 0 || s + 1 < steps) sync();
+      if (wm == 0 || !ENDS || s + 1 < steps) sync();
     };
-    step(std::true_type{}, 0);
-    for (int s = 1; s < steps; ++s) step(std::false_type{}, s);
+    typedef std::integral_constant<int, 0> Even;
+    typedef std::integral_constant<int, 1> Odd;
+    if constexpr (MX) {  // an even number of steps, four at least
+      step(std::true_type{}, Even{}, std::false_type{}, 0);
+      step(std::false_type{}, Odd{}, std::false_type{}, 1);
+      int s = 2;
+      for (; s < steps - 2; s += 2) {
+        step(std::false_type{}, Even{}, std::false_type{}, s);
+        step(std::false_type{}, Odd{}, std::false_type{}, s + 1);
+      }
+      step(std::false_type{}, Even{}, std::true_type{}, s);
+      step(std::false_type{}, Odd{}, std::true_type{}, s + 1);
+    } else {
+      step(std::true_type{}, Even{}, std::true_type{}, 0);
+      for (int s = 1; s < steps; ++s) step(std::false_type{}, Even{}, std::true_type{}, s);
+    }
 
     // ---- epilogue ------------------------------------------------------------------------------------------
     FLUXMI_VMCNT(0);  // the next tile's first units; this wave's, the others' by the barriers
@@ -667,9 +800,10 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
 template <Elem T>
 int launch(const GemmParams &p, const FewRowsArgs &few, int grid, hipStream_t s) {
   static std::atomic<uint64_t> lds_done{0};
-  const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(grouped_gemm_dual_kernel<T>), kDualLds, lds_done);
+  constexpr int kLds = is_mx(T) ? kMxLds : kDualLds;
+  const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(grouped_gemm_dual_kernel<T>), kLds, lds_done);
   if (rc != FLUXMI_OK) return rc;
-  hipLaunchKernelGGL(grouped_gemm_dual_kernel<T>, dim3(grid), dim3(kDualThreads), kDualLds, s, DualArgs{p, few});
+  hipLaunchKernelGGL(grouped_gemm_dual_kernel<T>, dim3(grid), dim3(kDualThreads), kLds, s, DualArgs{p, few});
   return FLUXMI_OK;
 }
 
@@ -686,6 +820,20 @@ bool dual_takes(const GemmParams &p, int dtype) {
   bool aligned = p.n % 8 == 0;
   for (int g = 0; g < p.ngroups; ++g) aligned = aligned && aligned16(p.d[g]);
   return aligned;
+}
+
+// Whole pairs of steps of K, two at least, scale rows on 16 bytes, offsets below kNoRow; results in stores of 16 bytes.
+bool dual_takes_mx(const GemmParams &p) {
+  const int64_t kbytes = p.k / 2, span = 0x70000000ll;
+  if (p.k % 512 != 0 || p.k < 1024 || p.nexperts > kDualExperts || !aligned16(p.a) || !aligned16(p.b[0]) || !aligned16(p.a_scale) || !aligned16(p.b_scale)) return false;
+  if (kTile * kbytes > span || p.n * kbytes > span || p.a_rows * kbytes > span) return false;
+  return aligned16(p.d[0]) && p.n % (p.d_fp32 ? 4 : 8) == 0;
+}
+
+int launch_grouped_gemm_dual_mx(const GemmParams &p, int grid, hipStream_t s) {
+  FewRowsArgs few{};
+  if (p.splits == nullptr) few.count = 1, few.splits[0] = p.max_rows;  // one expert with all rows
+  return p.half_is_f16 ? launch<Elem::MXFP4_F16>(p, few, grid, s) : launch<Elem::MXFP4>(p, few, grid, s);
 }
 
 int launch_grouped_gemm_dual(const GemmParams &p, const FewRowsArgs &few, int dtype, int grid, hipStream_t s) {

@@ -4,12 +4,16 @@
 // values (lane l: row l & 15, block l >> 4), and the block's scale byte in a register of its own.  B's rows are the MFMA's rows, so that a lane's
 // four sums are neighbouring columns of one row of D.
 //
-// Few rows per expert: the weights are read once and everything else is small.  A workgroup has 64 columns of an expert and up to 64 of its
-// rows; its four waves split K in turns of 512 values and add their sums through LDS in a fixed order.
+// Bound by the weights' bytes with few rows per expert, by the MFMAs and what feeds them with many.  Four kernels:
+//  * streams (mx_stream_kernel): a wave, or two or four that split K, has 16 or 32 rows and 32 or 64 columns of an expert and streams through LDS on its own;
+//  * the dual tiles of 256 x 256 (grouped_gemm_dual.hip);
+//  * for K that is no multiple of 512, and whatever else those do not take, mx_few_rows_kernel, whose four waves split K in turns of 512 values and load straight into
+//    registers, and mx_tile_kernel.
 //
-// Many rows: tiles of 256 x 256 on eight waves through a ring of four stages in LDS, a stage 128 values of K (64 bytes a row), filled by loads that write
+// The tiles of this file: 256 x 256 on eight waves through a ring of four stages in LDS, a stage 128 values of K (64 bytes a row), filled by loads that write
 // LDS.  The waves of a SIMD take turns: while one computes a stage, the other reads its fragments and requests fills.  Scales come 16 bytes a row for four
 // stages, and lie in registers while those are computed.
+#include "grouped_gemm_dual.hpp"
 #include "rows.hpp"
 
 namespace fluxmi {
@@ -22,6 +26,7 @@ constexpr int kThreads = 256;
 constexpr int kCols = 64;    // columns of a workgroup
 constexpr int kTurn = 512;   // values of K a wave takes at a time: 256 bytes of codes, 16 of scales of each row
 constexpr int kMaxExperts = 1024;
+constexpr int kPlanCus = 256;  // compute units that the choice of a kernel reckons with
 
 struct MxParams {
   const uint8_t *a, *a_scale, *b, *b_scale;
@@ -87,6 +92,23 @@ __device__ __forceinline__ f32x4 mfma(const u32x4 w, const u32x4 x, uint32_t w_s
 __device__ __forceinline__ void store_one(uint8_t *d, Row type, size_t i, float v) {
   if (type == Row::F32) reinterpret_cast<float *>(d)[i] = v;
   else reinterpret_cast<uint16_t *>(d)[i] = type == Row::BF16 ? float_to_bf16_bits(v) : float_to_f16_bits(v);
+}
+
+// Eight neighbouring results of one row, from column n on.
+__device__ __forceinline__ void store_eight(const MxParams &p, int r, int n, const float (&v)[8]) {
+  const size_t at = static_cast<size_t>(r) * p.n + n;
+  if (n + 8 <= p.n) {
+    if (p.d_type == Row::F32) {
+      store16(p.d + at * 4, pack<Row::F32>(reinterpret_cast<const float(&)[4]>(v[0])));
+      store16(p.d + at * 4 + 16, pack<Row::F32>(reinterpret_cast<const float(&)[4]>(v[4])));
+    } else {
+      store16(p.d + at * 2, p.d_type == Row::BF16 ? pack<Row::BF16>(v) : pack<Row::F16>(v));
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (n + k < p.n) store_one(p.d, p.d_type, at + k, v[k]);
+  }
 }
 
 // Codes and scales of a lane's blocks of one turn: block 4 s + g of the turn, s = 0 .. 3, with g = lane >> 4.  What lies past the end of the row is zero codes
@@ -179,6 +201,11 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void *base, in
 // lie between the statement's start and the load.)
 __device__ __forceinline__ void fill(uint32_t dst, uint32_t off, __amdgpu_buffer_rsrc_t r, int soff) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(dst), "v"(off), "s"(r), "s"(soff) : "memory");
+}
+
+// The same, of bytes that are read once.
+__device__ __forceinline__ void fill_once(uint32_t dst, uint32_t off, __amdgpu_buffer_rsrc_t r, int soff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds" : : "s"(dst), "v"(off), "s"(r), "s"(soff) : "memory");
 }
 
 constexpr uint32_t kNoRow = 0x80000000u;  // a byte offset past every operand
@@ -348,25 +375,12 @@ __global__ __launch_bounds__(512, 2) void mx_tile_kernel(const MxParams p, int t
   for (int i = 0; i < MI; ++i) {
     const int m = (i / (MI / 2)) * (C::BM / 2) + wm * (MI * 8) + (i % (MI / 2)) * 16 + (lane & 15);
     if (m >= t.rows) continue;
-    const size_t row = static_cast<size_t>(t.row0 + m) * p.n;
 #pragma unroll
     for (int jg = 0; jg < NJ / 2; ++jg) {
-      const int n = t.n0 + wn * NJ * 16 + jg * 32 + (lane >> 4) * 8;
       float v[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = acc[i][2 * jg + k / 4][k % 4] * rs[i];
-      if (n + 8 <= p.n) {
-        if (p.d_type == Row::F32) {
-          store16(p.d + (row + n) * 4, pack<Row::F32>(reinterpret_cast<const float(&)[4]>(v[0])));
-          store16(p.d + (row + n) * 4 + 16, pack<Row::F32>(reinterpret_cast<const float(&)[4]>(v[4])));
-        } else {
-          store16(p.d + (row + n) * 2, p.d_type == Row::BF16 ? pack<Row::BF16>(v) : pack<Row::F16>(v));
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (n + k < p.n) store_one(p.d, p.d_type, row + n + k, v[k]);
-      }
+      store_eight(p, t.row0 + m, t.n0 + wn * NJ * 16 + jg * 32 + (lane >> 4) * 8, v);
     }
   }
 #endif  // __HIP_DEVICE_COMPILE__
@@ -390,9 +404,141 @@ __global__ __launch_bounds__(kThreads) void mx_pad_scales_kernel(const uint8_t *
   }
 }
 
-template <int MT>
+// MT blocks of 16 rows x NJ blocks of 16 columns, P waves that split K.
+template <int MT, int NJ, int P>
+struct Stream {
+  static constexpr int kX = NJ * 4096, kScales = kX + MT * 4096, kStage = kScales + 2048;  // of a stage: codes of B, of A, scales of B, of A
+  static constexpr int kFills = 4 * (NJ + MT) + 2, kWaveLds = 2 * kStage, kLds = P * kWaveLds;
+};
+
+// A wave is on its own until the end: it requests a turn's 512 values of K of its columns and rows into one half of its LDS while it computes the other half's, with
+// no barrier.  Weights come in whole lines, eight rows of 128 bytes to a load, and non-temporally, as nobody else reads them.
+template <int MT, int NJ, int P>
+__global__ __launch_bounds__(64 * P) void mx_stream_kernel(const MxParams p, int tiles_n) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using C = Stream<MT, NJ, P>;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const int lane = threadIdx.x & 63, wave = P == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int item = blockIdx.x / tiles_n, n0 = (blockIdx.x - item * tiles_n) * (NJ * 16);
+  const Item it = locate(p, item, MT * 16);
+  if (it.rows <= 0) return;
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)smem)) + wave * C::kWaveLds;
+  const int row_bytes = p.kb * 16, turns = p.kb / 16;
+  const auto xr = buffer_of(p.a, static_cast<int64_t>(p.a_rows) * row_bytes), xsr = buffer_of(p.a_scale, static_cast<int64_t>(p.a_rows) * p.kb);
+  const auto wr = buffer_of(p.b + static_cast<int64_t>(it.e) * p.n * row_bytes, static_cast<int64_t>(p.n) * row_bytes);
+  const auto wsr = buffer_of(p.b_scale + static_cast<int64_t>(it.e) * p.n * p.kb, static_cast<int64_t>(p.n) * p.kb);
+  // LDS row R of 128 bytes: chunk c of 16 bytes at slot c ^ ((R >> 1) & 7); a fill covers 8 rows, lane l row l >> 3 and slot l & 7.
+  uint32_t xoff[2 * MT], woff[2 * NJ];
+  const uint32_t chunk0 = ((lane & 7) ^ (lane >> 4)) * 16;
+#pragma unroll
+  for (int q = 0; q < 2 * NJ; ++q) {
+    const int n = n0 + column_of(q * 8 + (lane >> 3));
+    woff[q] = n < p.n ? static_cast<uint32_t>(n) * row_bytes + (chunk0 ^ ((q & 1) * 64)) : kNoRow;
+  }
+  const int ns = n0 + column_of(lane);
+  const uint32_t wsoff = lane < NJ * 16 && ns < p.n ? static_cast<uint32_t>(ns) * p.kb : kNoRow;
+#pragma unroll
+  for (int q = 0; q < 2 * MT; ++q) {
+    const int m = q * 8 + (lane >> 3);
+    xoff[q] = m < it.rows ? static_cast<uint32_t>(a_row(p, it.row0 + m)) * row_bytes + (chunk0 ^ ((q & 1) * 64)) : kNoRow;
+  }
+  const uint32_t xsoff = lane < it.rows ? static_cast<uint32_t>(a_row(p, it.row0 + lane)) * p.kb : kNoRow;  // (lanes past the rows' blocks: not read)
+  auto fill_turn = [&](int t, int slot) {
+    const uint32_t dst = lds0 + slot * C::kStage;
+    fill_once(dst + C::kScales, wsoff, wsr, t * 16);
+#pragma unroll
+    for (int q = 0; q < 4 * NJ; ++q) fill_once(dst + q * 1024, woff[q % (2 * NJ)], wr, t * 256 + q / (2 * NJ) * 128);
+    fill(dst + C::kScales + 1024, xsoff, xsr, t * 16);
+#pragma unroll
+    for (int q = 0; q < 4 * MT; ++q) fill(dst + C::kX + q * 1024, xoff[q % (2 * MT)], xr, t * 256 + q / (2 * MT) * 128);
+  };
+  // Lane group g has chunks 2 g and 2 g + 1 of a line in two MFMAs, and their scales are bytes 2 g and 2 g + 1 of the line's 8.
+  typedef const __attribute__((address_space(3))) u32x4 *LdsFrag;
+  typedef const __attribute__((address_space(3))) uint32_t *LdsWord;
+  const int g = lane >> 4, r = lane & 15;
+  const uint32_t in_rows0 = r * 128 + (((2 * g) ^ ((lane >> 1) & 7)) * 16), in_rows1 = r * 128 + (((2 * g + 1) ^ ((lane >> 1) & 7)) * 16);
+  const uint32_t in_scales = C::kScales + r * 16 + (g >> 1) * 4, pick = 0x05040100u + 0x02020202u * (g & 1);
+  f32x4 acc[MT][NJ] = {};
+  int slot = 0;
+  if (wave < turns) fill_turn(wave, 0);
+  if (wave + P < turns) fill_turn(wave + P, 1);
+  for (int t = wave; t < turns; t += P) {
+    if (t + P < turns) FLUXMI_VMCNT(C::kFills);
+    else FLUXMI_VMCNT(0);
+    asm volatile("" ::: "memory");
+    const uint32_t at = lds0 + slot * C::kStage;
+    u32x4 w[NJ][4], x[MT][4];
+    uint32_t ws[NJ], xs[MT];
+    auto scales_of = [&](uint32_t a) { return __builtin_amdgcn_perm(*reinterpret_cast<LdsWord>(a + 8), *reinterpret_cast<LdsWord>(a), pick); };
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) ws[j] = scales_of(at + in_scales + j * 256);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) xs[i] = scales_of(at + in_scales + 1024 + i * 256);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        w[j][2 * h] = *reinterpret_cast<LdsFrag>(at + in_rows0 + h * NJ * 2048 + j * 2048);
+        w[j][2 * h + 1] = *reinterpret_cast<LdsFrag>(at + in_rows1 + h * NJ * 2048 + j * 2048);
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        x[i][2 * h] = *reinterpret_cast<LdsFrag>(at + C::kX + in_rows0 + h * MT * 2048 + i * 2048);
+        x[i][2 * h + 1] = *reinterpret_cast<LdsFrag>(at + C::kX + in_rows1 + h * MT * 2048 + i * 2048);
+      }
+    }
+    FLUXMI_LGKM0();  // all of this half is in registers: the turn after the next may come into it
+    __builtin_amdgcn_sched_barrier(0);
+    if (t + 2 * P < turns) fill_turn(t + 2 * P, slot);
+    auto multiply = [&](auto M) {
+      constexpr int m = decltype(M)::value;
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = mfma<m>(w[j][m], x[i][m], ws[j], xs[i], acc[i][j]);
+    };
+    multiply(std::integral_constant<int, 0>{});
+    multiply(std::integral_constant<int, 1>{});
+    multiply(std::integral_constant<int, 2>{});
+    multiply(std::integral_constant<int, 3>{});
+    slot ^= 1;
+  }
+  // The waves' sums, in their order; wave v stores every P-th group of 16 rows x 32 columns from the v-th on.
+  typedef __attribute__((address_space(3))) f32x4 *LdsSums;
+  if constexpr (P > 1) {
+    FLUXMI_VMCNT(0);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) *reinterpret_cast<LdsSums>(lds0 + (i * NJ + j) * 1024 + lane * 16) = acc[i][j];
+    __syncthreads();
+  }
+#pragma unroll
+  for (int q = 0; q < MT * NJ / 2; ++q) {
+    if (P > 1 && q % P != wave) continue;
+    const int i = q / (NJ / 2), jg = q % (NJ / 2), m = i * 16 + r;
+    f32x4 sum[2] = {acc[i][2 * jg], acc[i][2 * jg + 1]};
+    if constexpr (P > 1) {
+      const uint32_t first = lds0 - wave * C::kWaveLds + (i * NJ + 2 * jg) * 1024 + lane * 16;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        sum[k] = *reinterpret_cast<LdsSums>(first + k * 1024);
+        for (int v = 1; v < P; ++v) sum[k] += *reinterpret_cast<LdsSums>(first + v * C::kWaveLds + k * 1024);
+      }
+    }
+    if (m >= it.rows) continue;
+    const float scale = p.row_scale ? p.row_scale[it.row0 + m] : 1.f;
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = sum[k / 4][k % 4] * scale;
+    store_eight(p, it.row0 + m, n0 + jg * 32 + g * 8, v);
+  }
+#endif  // __HIP_DEVICE_COMPILE__
+}
+
 __global__ __launch_bounds__(kThreads) void mx_few_rows_kernel(const MxParams p, int tiles_n) {
 #if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int MT = 1;
   __shared__ f32x4 sums[3][MT * 4][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int item = blockIdx.x / tiles_n, n0 = (blockIdx.x - item * tiles_n) * kCols;
@@ -483,13 +629,25 @@ int check_args(const fluxmi_mx_gemm_args *args) {
   return FLUXMI_OK;
 }
 
-template <int MT>
 int launch_few_rows(const MxParams &p, hipStream_t s) {
   const int tiles_n = (p.n + kCols - 1) / kCols;
   // Pieces of rows: at most one that is not full for each expert with rows.
-  const int64_t items = p.max_rows / (MT * 16) + (p.nexperts < p.max_rows ? p.nexperts : p.max_rows), grid = items * tiles_n;
+  const int64_t items = p.max_rows / 16 + (p.nexperts < p.max_rows ? p.nexperts : p.max_rows), grid = items * tiles_n;
   FLUXMI_REQUIRE(grid * kThreads < (int64_t{1} << 32), FLUXMI_ERR_UNSUPPORTED, "grouped_gemm_mx: max_rows=%d and n=%d are more than a launch covers", p.max_rows, p.n);
-  hipLaunchKernelGGL(mx_few_rows_kernel<MT>, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, s, p, tiles_n);
+  hipLaunchKernelGGL(mx_few_rows_kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, s, p, tiles_n);
+  return FLUXMI_OK;
+}
+
+template <int MT, int NJ, int P>
+int launch_stream(const MxParams &p, hipStream_t s) {
+  using C = Stream<MT, NJ, P>;
+  static std::atomic<uint64_t> lds_done{0};
+  const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(mx_stream_kernel<MT, NJ, P>), C::kLds, lds_done);
+  if (rc != FLUXMI_OK) return rc;
+  const int tiles_n = (p.n + NJ * 16 - 1) / (NJ * 16);
+  const int64_t items = p.max_rows / (MT * 16) + (p.nexperts < p.max_rows ? p.nexperts : p.max_rows), grid = items * tiles_n;
+  FLUXMI_REQUIRE(grid * 64 * P < (int64_t{1} << 32), FLUXMI_ERR_UNSUPPORTED, "grouped_gemm_mx: max_rows=%d and n=%d are more than a launch covers", p.max_rows, p.n);
+  hipLaunchKernelGGL((mx_stream_kernel<MT, NJ, P>), dim3(static_cast<unsigned>(grid)), dim3(64 * P), C::kLds, s, p, tiles_n);
   return FLUXMI_OK;
 }
 
@@ -506,25 +664,82 @@ int launch_tiles(const MxParams &p, hipStream_t s) {
   return FLUXMI_OK;
 }
 
-bool takes_tiles(const fluxmi_mx_gemm_args &a) { return a.max_rows / a.nexperts > 64; }
+// The call as the dual tiles take it.
+GemmParams dual_params(const fluxmi_mx_gemm_args &a) {
+  GemmParams p{};
+  p.a = static_cast<const uint8_t *>(a.a);
+  p.b[0] = static_cast<const uint8_t *>(a.b);
+  p.d[0] = a.d;
+  p.splits = a.splits;
+  p.gather_a = a.gather_a;
+  p.row_scale = a.row_scale;
+  p.scalar = 1.f;
+  p.nexperts = a.nexperts;
+  p.max_rows = a.max_rows;
+  p.a_rows = a.a_rows;
+  p.n = a.n;
+  p.k = (a.k + 31) / 32 * 32;  // the codes past the end are zeros
+  p.d_fp32 = a.d_type == FLUXMI_ROWS_FP32;
+  p.half_is_f16 = a.d_type == FLUXMI_ROWS_FP16;
+  p.ngroups = 1;
+  p.raster_rows = 8;
+  p.a_scale = static_cast<const float *>(a.a_scale);
+  p.b_scale = static_cast<const float *>(a.b_scale);
+  return p;
+}
+
+// Which kernel computes a call.
+enum class Form { FEW_ROWS, STREAM, DUAL, TILES };
+struct Plan {
+  Form form;
+  int row_blocks, col_blocks, waves;  // STREAM: blocks of 16 rows and of 16 columns of an item, waves that split K
+  bool low;         // TILES: of 128 rows
+  size_t workspace;
+};
+
+// The streams read an expert's weights once for every 16 or 32 of its rows, the tiles once for up to 256.  us, stream of 16 rows / of 32 rows / dual tiles, rows on
+// average and a fifth more or less: 8 experts 14336 x 4096, 9 rows 47 / 55 / 62, 24 rows 90 / 61 / 63, 48 rows - / 102 / 65; 4096 x 14336, 9 rows 50 / 49 / 71, 24
+// rows 95 / 54 / 72; 32 experts 7168 x 2048, 24 rows 86 / 62 / 67; 2048 x 7168, 9 rows 52 / 64 / 53, 24 rows 91 / 70 / 54, where the dual tiles are one
+// to a compute unit: with whole rounds of tiles they are taken from 10 rows on.
+// Few waves (one token with two experts of 4096 x 14336: 256): K is split over two or four of a workgroup, 16.3 -> 13.2 us; with 896 (14336 x 4096) 14.0 -> 15.8.
+// The dual tiles want K in multiples of 512 and N of 8 (fp32 results 4), the streams K only; what neither takes goes to the first kernel up to 16 rows (9 rows: 58,
+// tiles 61) and to the tiles of this file beyond (32 rows 2048 x 7168 of 32 experts: 81, tiles 57), of 128 rows up to 128 on average (194 rows 4096 x 14336 of
+// 8 experts 116 -> 96, 2048 rows 600 -> 750).
+Plan plan_of(const fluxmi_mx_gemm_args &a, const GemmParams &dual, int cus) {
+  const int64_t rows = a.max_rows, experts = a.nexperts, active = rows < experts ? rows : experts, kb = (int64_t{a.k} + 31) / 32;
+  const bool dual_takes = dual_takes_mx(dual), streams = kb % 16 == 0 && aligned16(a.a_scale) && aligned16(a.b_scale);
+  const int64_t tiles = active * ((a.n + 255) / 256);
+  const bool whole_rounds = tiles >= cus && tiles % cus == 0;
+  if (streams && (rows <= 10 * experts || (rows <= 24 * experts && !(dual_takes && whole_rounds)))) {
+    const bool two = rows > 10 * experts;
+    const int64_t waves32 = active * ((a.n + 31) / 32);
+    const bool wide = two && waves32 >= 1024;
+    const int waves = wide || waves32 >= 768 ? 1 : waves32 >= 192 ? 2 : 4;
+    return {Form::STREAM, two ? 2 : 1, wide ? 4 : 2, waves, false, 0};
+  }
+  if (dual_takes) return {Form::DUAL, 0, 0, 0, false, 0};
+  if (rows <= 16 * experts) return {Form::FEW_ROWS, 0, 0, 0, false, 0};
+  const bool padded = kb % 16 != 0 || !aligned16(a.a_scale) || !aligned16(a.b_scale);
+  return {Form::TILES, 0, 0, 0, rows <= 128 * experts, padded ? static_cast<size_t>(a.a_rows + experts * a.n) * ((kb + 15) / 16 * 16) : 0};
+}
 
 }  // namespace
 }  // namespace fluxmi
 
 extern "C" size_t fluxmi_grouped_gemm_mx_workspace_bytes(const fluxmi_mx_gemm_args *args) {
   if (args == nullptr || args->nexperts < 1 || args->max_rows < 1 || args->n < 1 || args->k < 1 || args->a_rows < 0) return 0;
-  const int64_t kb = (int64_t{args->k} + 31) / 32;
-  if (kb % 16 == 0 || !fluxmi::takes_tiles(*args)) return 0;
-  return static_cast<size_t>(args->a_rows + int64_t{args->nexperts} * args->n) * ((kb + 15) / 16 * 16);
+  return fluxmi::plan_of(*args, fluxmi::dual_params(*args), fluxmi::kPlanCus).workspace;
 }
 
 extern "C" int fluxmi_grouped_gemm_mx(const fluxmi_mx_gemm_args *args, void *workspace, size_t workspace_bytes, void *stream) {
   using namespace fluxmi;
   int rc = check_args(args);
   if (rc != FLUXMI_OK || args->max_rows == 0 || args->n == 0) return rc;
-  const size_t need = fluxmi_grouped_gemm_mx_workspace_bytes(args);
-  FLUXMI_REQUIRE(need == 0 || (workspace != nullptr && aligned16(workspace) && workspace_bytes >= need), FLUXMI_ERR_WORKSPACE,
-                 "grouped_gemm_mx: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+  const GemmParams dual = dual_params(*args);
+  const Plan plan = plan_of(*args, dual, kPlanCus);
+  FLUXMI_REQUIRE(plan.workspace == 0 || (workspace != nullptr && aligned16(workspace) && workspace_bytes >= plan.workspace), FLUXMI_ERR_WORKSPACE,
+                 "grouped_gemm_mx: workspace of %zu bytes needed, %zu given", plan.workspace, workspace_bytes);
+  hipStream_t s = static_cast<hipStream_t>(stream);
   MxParams p;
   p.a = static_cast<const uint8_t *>(args->a);
   p.a_scale = static_cast<const uint8_t *>(args->a_scale);
@@ -539,26 +754,36 @@ extern "C" int fluxmi_grouped_gemm_mx(const fluxmi_mx_gemm_args *args, void *wor
   p.n = args->n;
   p.kb = (args->k + 31) / 32;
   p.a_rows = args->a_rows;
-  p.d_type = args->d_type == FLUXMI_ROWS_BF16 ? Row::BF16 : args->d_type == FLUXMI_ROWS_FP32 ? Row::F32 : Row::F16;
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  const int average = p.max_rows / p.nexperts;
   p.scale_stride = p.kb;
-  if (takes_tiles(*args)) {
-    if (need > 0) {
-      p.scale_stride = (p.kb + 15) / 16 * 16;
-      const int64_t a_rows = p.a_rows, b_rows = int64_t{p.nexperts} * p.n, groups = (a_rows + b_rows) * (p.scale_stride / 16);
-      const unsigned grid = static_cast<unsigned>(groups / kThreads < 8192 ? groups / kThreads + 1 : 8192);
-      uint8_t *const padded = static_cast<uint8_t *>(workspace);
-      hipLaunchKernelGGL(mx_pad_scales_kernel, dim3(grid), dim3(kThreads), 0, s, p.a_scale, a_rows, p.b_scale, b_rows, p.kb, p.scale_stride, padded);
-      p.a_scale = padded;
-      p.b_scale = padded + a_rows * p.scale_stride;
+  p.d_type = args->d_type == FLUXMI_ROWS_BF16 ? Row::BF16 : args->d_type == FLUXMI_ROWS_FP32 ? Row::F32 : Row::F16;
+  switch (plan.form) {
+    case Form::STREAM:
+      if (plan.col_blocks == 4) rc = launch_stream<2, 4, 1>(p, s);
+      else if (plan.row_blocks == 2) rc = plan.waves == 1 ? launch_stream<2, 2, 1>(p, s) : plan.waves == 2 ? launch_stream<2, 2, 2>(p, s) : launch_stream<2, 2, 4>(p, s);
+      else rc = plan.waves == 1 ? launch_stream<1, 2, 1>(p, s) : plan.waves == 2 ? launch_stream<1, 2, 2>(p, s) : launch_stream<1, 2, 4>(p, s);
+      break;
+    case Form::DUAL: {
+      // Up to four workgroups to a tile, which is cut in pieces when these still fit the card.
+      const int64_t tiles = (int64_t{p.max_rows} / 256 + (p.nexperts < p.max_rows ? p.nexperts : p.max_rows)) * ((p.n + 255) / 256), cus = fluxmi_device_cu_count();
+      rc = launch_grouped_gemm_dual_mx(dual, static_cast<int>(tiles * 4 < cus ? tiles * 4 : cus), s);
+      break;
     }
-    rc = launch_tiles<8, 4, 2, 4>(p, s);
-    if (rc != FLUXMI_OK) return rc;
-    FLUXMI_HIP_CHECK(hipGetLastError());
-    return FLUXMI_OK;
+    case Form::FEW_ROWS:
+      rc = launch_few_rows(p, s);
+      break;
+    case Form::TILES:
+      if (plan.workspace > 0) {
+        p.scale_stride = (p.kb + 15) / 16 * 16;
+        const int64_t a_rows = p.a_rows, b_rows = int64_t{p.nexperts} * p.n, groups = (a_rows + b_rows) * (p.scale_stride / 16);
+        const unsigned grid = static_cast<unsigned>(groups / kThreads < 8192 ? groups / kThreads + 1 : 8192);
+        uint8_t *const padded = static_cast<uint8_t *>(workspace);
+        hipLaunchKernelGGL(mx_pad_scales_kernel, dim3(grid), dim3(kThreads), 0, s, p.a_scale, a_rows, p.b_scale, b_rows, p.kb, p.scale_stride, padded);
+        p.a_scale = padded;
+        p.b_scale = padded + a_rows * p.scale_stride;
+      }
+      rc = plan.low ? launch_tiles<4, 4, 2, 4>(p, s) : launch_tiles<8, 4, 2, 4>(p, s);
+      break;
   }
-  rc = average <= 16 ? launch_few_rows<1>(p, s) : average <= 32 ? launch_few_rows<2>(p, s) : launch_few_rows<4>(p, s);
   if (rc != FLUXMI_OK) return rc;
   FLUXMI_HIP_CHECK(hipGetLastError());
   return FLUXMI_OK;

@@ -9,8 +9,10 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-enum class Elem { BF16, F16, FP8, FP8_BLOCKSCALED };
+// MXFP4: packed 4-bit codes with a scale byte for every 32 values of both operands; 16-bit results are bf16, of MXFP4_F16 fp16.
+enum class Elem { BF16, F16, FP8, FP8_BLOCKSCALED, MXFP4, MXFP4_F16 };
 constexpr bool is_fp8(Elem t) { return t == Elem::FP8 || t == Elem::FP8_BLOCKSCALED; }
+constexpr bool is_mx(Elem t) { return t == Elem::MXFP4 || t == Elem::MXFP4_F16; }
 
 #if defined(__HIP_DEVICE_COMPILE__)
 
