@@ -7,10 +7,13 @@
 // two inside the conversion instruction (checked against the definition for every bf16 and fp16 value and millions of fp32 ones, subnormal ones
 // and scales at both ends of the range among them).  The maximum is taken over the patterns without sign, where infinities and NaN are largest.
 //
-// Bound by HBM: a value is read once and becomes 17 / 32 bytes.  Along the rows a lane converts 8 neighbours (fp32: two vectors) and four lanes
-// join their maxima; rows whose length is a multiple of 32 are one flat array.  With the transposed copy a lane holds 32 rows of one vector's
+// Bound by HBM: a value is read once and becomes 17 / 32 bytes.  Along the rows a lane converts one vector of 16 bytes and the four lanes (fp32: eight)
+// of a block join their maxima; rows whose length is a multiple of 32 are one flat array.  With the transposed copy a lane holds 32 rows of one vector's
 // columns in registers, which gives both directions from one read with no exchange but that of the maxima along the rows; eight lanes side by side and
 // eight row blocks below each other make a wave, so that its loads and its transposed stores are whole 128-byte lines.
+// Measured at 11000 x 7168 bf16: both directions 57 us (4.2 TB/s; without the stores of the row codes 47, without the transposed ones 45: two sets of
+// writes beside the read are what is left), along the rows 33 (7.4 of values and codes together), back 29 (6.9), back from the transposed copy 38 (5.3).
+// Other tiles of the two-way form (4 x 16 or 2 x 32 lanes, waves stacked instead of side by side) take 56 to 65 us, three waves to a SIMD the same 57.
 #include "rows.hpp"
 
 namespace fluxmi {
@@ -117,70 +120,59 @@ __device__ __forceinline__ u32x4 load_part(const uint8_t *p, int count) {
 
 // ---- along the rows --------------------------------------------------------------------------------------------
 
-// Eight neighbours, four lanes to a block.
-template <Row T>
-struct Eight {
-  u32x4 v[T == Row::F32 ? 2 : 1];
-};
+template <Row T, bool NT>
+__device__ __forceinline__ u32x4 load_vector(const uint8_t *p, int count) {
+  return count >= kVec<T> ? load16<NT>(p) : load_part<T>(p, count);
+}
 
+// A vector's codes.
 template <Row T>
-__device__ __forceinline__ Eight<T> load_eight(const uint8_t *p, int count) {
-  Eight<T> e;
-  if (count >= 8) {
-    e.v[0] = load16(p);
-    if constexpr (T == Row::F32) e.v[1] = load16(p + 16);
-  } else {
-    e.v[0] = load_part<T>(p, count);
-    if constexpr (T == Row::F32) e.v[1] = load_part<T>(p + 16, count - 4);
-  }
-  return e;
+__device__ __forceinline__ void store_codes(uint8_t *to, uint32_t c) {
+  if constexpr (T == Row::F32) *reinterpret_cast<uint16_t *>(to) = static_cast<uint16_t>(c);
+  else *reinterpret_cast<uint32_t *>(to) = c;
 }
 
 template <Row T>
-__device__ __forceinline__ void quantise_eight(const Eight<T> &e, uint8_t *codes, uint8_t *scale, bool first_lane) {
-  uint32_t m = vector_max<T>(e.v[0]);
-  if constexpr (T == Row::F32) m = max_pattern<T>(m, vector_max<T>(e.v[1]));
-  const uint32_t byte = scale_byte<T>(max_of_lanes<4>(join_halves<T>(m)));
-  const float s = scale_value(byte);
-  uint32_t c = convert_vector<T>(e.v[0], s);
-  if constexpr (T == Row::F32) c = (c & 0xffffu) | convert_vector<T>(e.v[1], s) << 16;
-  *reinterpret_cast<uint32_t *>(codes) = byte == 255 ? 0u : c;
+__device__ __forceinline__ void quantise_vector(const u32x4 v, uint8_t *codes, uint8_t *scale, bool first_lane) {
+  const uint32_t byte = scale_byte<T>(max_of_lanes<kShare<T>>(join_halves<T>(vector_max<T>(v))));
+  store_codes<T>(codes, byte == 255 ? 0u : convert_vector<T>(v, scale_value(byte)));
   if (first_lane) *scale = static_cast<uint8_t>(byte);
 }
 
-// Rows of whole blocks: eight values to a lane, U of them in flight.
-template <Row T, int U>
-__global__ __launch_bounds__(kThreads) void quant_flat_kernel(const uint8_t *__restrict__ x, size_t eights, uint8_t *__restrict__ codes, uint8_t *__restrict__ scale) {
+// Rows of whole blocks: a vector to a lane, U of them in flight.
+template <Row T, int U, bool NT>
+__global__ __launch_bounds__(kThreads) void quant_flat_kernel(const uint8_t *__restrict__ x, size_t vectors, uint8_t *__restrict__ codes, uint8_t *__restrict__ scale) {
   const size_t at = static_cast<size_t>(blockIdx.x) * (kThreads * U) + threadIdx.x;
-  Eight<T> e[U];
+  u32x4 v[U];
 #pragma unroll
   for (int u = 0; u < U; ++u)
-    if (at + u * kThreads < eights) e[u] = load_eight<T>(x + (at + u * kThreads) * 8 * kElt<T>, 8);
+    if (at + u * kThreads < vectors) v[u] = load16<NT>(x + (at + u * kThreads) * 16);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const size_t i = at + u * kThreads;
-    if (i < eights) quantise_eight<T>(e[u], codes + i * 4, scale + (i >> 2), (threadIdx.x & 3) == 0);
+    if (i < vectors) quantise_vector<T>(v[u], codes + i * (kVec<T> / 2), scale + i / kShare<T>, (threadIdx.x & (kShare<T> - 1)) == 0);
   }
 }
 
 // Rows that end inside a block: a row to `1 << shift` lanes.
-template <Row T>
+template <Row T, bool NT>
 __global__ __launch_bounds__(kThreads) void quant_rows_kernel(const uint8_t *__restrict__ x, int64_t rows, int cols, int shift, uint8_t *__restrict__ codes,
                                                               uint8_t *__restrict__ scale) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads >> shift) + (threadIdx.x >> shift);
   if (row >= rows) return;
-  const int kb = (cols + kBlock - 1) / kBlock;
+  const int vectors = (cols + kBlock - 1) / kBlock * kShare<T>;
   const uint8_t *const src = x + static_cast<size_t>(row) * cols * kElt<T>;
-  for (int i = threadIdx.x & ((1 << shift) - 1); i < kb * 4; i += 1 << shift) {
-    const size_t at = static_cast<size_t>(row) * kb * 4 + i;
-    quantise_eight<T>(load_eight<T>(src + static_cast<size_t>(i) * 8 * kElt<T>, cols - i * 8), codes + at * 4, scale + (at >> 2), (i & 3) == 0);
+  for (int i = threadIdx.x & ((1 << shift) - 1); i < vectors; i += 1 << shift) {
+    const size_t at = static_cast<size_t>(row) * vectors + i;
+    quantise_vector<T>(load_vector<T, NT>(src + static_cast<size_t>(i) * 16, cols - i * kVec<T>), codes + at * (kVec<T> / 2), scale + at / kShare<T>,
+                       (i & (kShare<T> - 1)) == 0);
   }
 }
 
 // ---- along the rows and along the columns -----------------------------------------------------------------------------
 
 // One matrix of the batch.  A wave covers 8 vectors of columns x 8 blocks of 32 rows, a workgroup 4 waves side by side.
-template <Row T>
+template <Row T, bool NT>
 __global__ __launch_bounds__(kThreads, 2) void quant_both_kernel(const uint8_t *__restrict__ x, int rows, int cols, int row_tiles, int col_tiles,
                                                               uint8_t *__restrict__ codes, uint8_t *__restrict__ scale, uint8_t *__restrict__ codes_t,
                                                               uint8_t *__restrict__ scale_t) {
@@ -206,7 +198,7 @@ __global__ __launch_bounds__(kThreads, 2) void quant_both_kernel(const uint8_t *
     v[r] = u32x4{0u, 0u, 0u, 0u};
     if (r < rows_here && cols_here > 0) {
       const uint8_t *const p = src + static_cast<size_t>(r) * cols * kElt<T>;
-      v[r] = cols_here >= V ? load16(p) : load_part<T>(p, cols_here);
+      v[r] = load_vector<T, NT>(p, cols_here);
     }
   }
   // Along the rows: kShare lanes have a block.
@@ -215,9 +207,7 @@ __global__ __launch_bounds__(kThreads, 2) void quant_both_kernel(const uint8_t *
     const uint32_t byte = scale_byte<T>(max_of_lanes<kShare<T>>(join_halves<T>(vector_max<T>(v[r]))));
     const uint32_t c = byte == 255 ? 0u : convert_vector<T>(v[r], scale_value(byte));
     if (r < rows_here && c0 < kb * kBlock) {
-      uint8_t *const to = codes + (static_cast<size_t>(r0 + r) * kb * kBlock + c0) / 2;
-      if constexpr (T == Row::F32) *reinterpret_cast<uint16_t *>(to) = static_cast<uint16_t>(c);
-      else *reinterpret_cast<uint32_t *>(to) = c;
+      store_codes<T>(codes + (static_cast<size_t>(r0 + r) * kb * kBlock + c0) / 2, c);
       if ((lane & (kShare<T> - 1)) == 0) scale[static_cast<size_t>(r0 + r) * kb + c0 / kBlock] = static_cast<uint8_t>(byte);
     }
   }
@@ -265,20 +255,19 @@ __global__ __launch_bounds__(kThreads, 2) void quant_both_kernel(const uint8_t *
 
 // ---- back ------------------------------------------------------------------------------------------------------
 
-template <Row T>
-__device__ __forceinline__ void dequantise_eight(uint32_t c, uint32_t byte, uint8_t *out, int count) {
+// A vector of values from its codes (4 bytes, fp32 the lower 2); `count` of them are there.
+template <Row T, bool NT>
+__device__ __forceinline__ void dequantise_vector(uint32_t c, uint32_t byte, uint8_t *out, int count) {
   const float s = scale_value(byte);
-  u32x4 v[T == Row::F32 ? 2 : 1];
+  u32x4 v;
   if constexpr (T == Row::F32) {
-    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1),
-                d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 3);
-    v[0] = u32x4{__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(b[0]), __float_as_uint(b[1])};
-    v[1] = u32x4{__float_as_uint(d[0]), __float_as_uint(d[1]), __float_as_uint(e[0]), __float_as_uint(e[1])};
-    if (byte == 255) v[0] = v[1] = u32x4{0x7fc00000u, 0x7fc00000u, 0x7fc00000u, 0x7fc00000u};
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1);
+    v = u32x4{__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(b[0]), __float_as_uint(b[1])};
+    if (byte == 255) v = u32x4{0x7fc00000u, 0x7fc00000u, 0x7fc00000u, 0x7fc00000u};
   } else if constexpr (T == Row::BF16) {
-    v[0] = u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0)), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2)), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3))};
-    if (byte == 255) v[0] = u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+    v = u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0)), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1)),
+              __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2)), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3))};
+    if (byte == 255) v = u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
   } else {
     // Through fp32, which holds every value: the one rounding is that to fp16.
 #pragma unroll
@@ -288,60 +277,67 @@ __device__ __forceinline__ void dequantise_eight(uint32_t c, uint32_t byte, uint
       else if (i == 1) p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1);
       else if (i == 2) p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 2);
       else p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 3);
-      v[0][i] = float_to_f16_bits(p[0]) | static_cast<uint32_t>(float_to_f16_bits(p[1])) << 16;
+      v[i] = float_to_f16_bits(p[0]) | static_cast<uint32_t>(float_to_f16_bits(p[1])) << 16;
     }
-    if (byte == 255) v[0] = u32x4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
+    if (byte == 255) v = u32x4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
   }
-  if (count >= 8) {
-    store16(out, v[0]);
-    if constexpr (T == Row::F32) store16(out + 16, v[1]);
+  if (count >= kVec<T>) {
+    store16<NT>(out, v);
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 7; ++i) {
+  for (int i = 0; i < kVec<T> - 1; ++i) {
     if (i >= count) continue;
-    if constexpr (T == Row::F32) reinterpret_cast<uint32_t *>(out)[i] = v[i / 4][i % 4];
-    else reinterpret_cast<uint16_t *>(out)[i] = static_cast<uint16_t>(v[0][i / 2] >> (16 * (i & 1)));
+    if constexpr (T == Row::F32) reinterpret_cast<uint32_t *>(out)[i] = v[i];
+    else reinterpret_cast<uint16_t *>(out)[i] = static_cast<uint16_t>(v[i / 2] >> (16 * (i & 1)));
   }
 }
 
-template <Row T, int U>
-__global__ __launch_bounds__(kThreads) void dequant_flat_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scale, size_t eights, uint8_t *__restrict__ out) {
+// Codes of vector i.
+template <Row T>
+__device__ __forceinline__ uint32_t load_codes(const uint8_t *codes, size_t i) {
+  if constexpr (T == Row::F32) return reinterpret_cast<const uint16_t *>(codes)[i];
+  else return reinterpret_cast<const uint32_t *>(codes)[i];
+}
+
+template <Row T, int U, bool NT>
+__global__ __launch_bounds__(kThreads) void dequant_flat_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scale, size_t vectors, uint8_t *__restrict__ out) {
   const size_t at = static_cast<size_t>(blockIdx.x) * (kThreads * U) + threadIdx.x;
   uint32_t c[U], b[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const size_t i = at + u * kThreads;
-    if (i < eights) {
-      c[u] = reinterpret_cast<const uint32_t *>(codes)[i];
-      b[u] = scale[i >> 2];
+    if (i < vectors) {
+      c[u] = load_codes<T>(codes, i);
+      b[u] = scale[i / kShare<T>];
     }
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const size_t i = at + u * kThreads;
-    if (i < eights) dequantise_eight<T>(c[u], b[u], out + i * 8 * kElt<T>, 8);
+    if (i < vectors) dequantise_vector<T, NT>(c[u], b[u], out + i * 16, kVec<T>);
   }
 }
 
-template <Row T>
+template <Row T, bool NT>
 __global__ __launch_bounds__(kThreads) void dequant_rows_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scale, int64_t rows, int cols, int shift,
                                                                 uint8_t *__restrict__ out) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads >> shift) + (threadIdx.x >> shift);
   if (row >= rows) return;
-  const int kb = (cols + kBlock - 1) / kBlock;
+  const int vectors = (cols + kBlock - 1) / kBlock * kShare<T>;
   uint8_t *const dst = out + static_cast<size_t>(row) * cols * kElt<T>;
-  for (int i = threadIdx.x & ((1 << shift) - 1); i * 8 < cols; i += 1 << shift) {
-    const size_t at = static_cast<size_t>(row) * kb * 4 + i;
-    dequantise_eight<T>(reinterpret_cast<const uint32_t *>(codes)[at], scale[at >> 2], dst + static_cast<size_t>(i) * 8 * kElt<T>, cols - i * 8);
+  for (int i = threadIdx.x & ((1 << shift) - 1); i * kVec<T> < cols; i += 1 << shift) {
+    const size_t at = static_cast<size_t>(row) * vectors + i;
+    dequantise_vector<T, NT>(load_codes<T>(codes, at), scale[at / kShare<T>], dst + static_cast<size_t>(i) * 16, cols - i * kVec<T>);
   }
 }
 
-// Lanes of a row that ends inside a block, as a power of two from 4 to 256.
+// Lanes of a row that ends inside a block, as a power of two from one block's to 256.
+template <Row T>
 int row_shift(int64_t cols) {
-  const int64_t eights = (cols + kBlock - 1) / kBlock * 4;
+  const int64_t vectors = (cols + kBlock - 1) / kBlock * kShare<T>;
   int shift = 2;
-  while (shift < 8 && (int64_t{1} << shift) < eights) ++shift;
+  while (shift < 8 && (int64_t{1} << shift) < vectors) ++shift;
   return shift;
 }
 
@@ -352,8 +348,13 @@ bool grid_of(int64_t items, int64_t per, dim3 *grid) {
   return n * kThreads < (int64_t{1} << 32);
 }
 
-// From this many values on a lane has four groups of eight in flight: below, one each spreads the work wider.
-constexpr size_t kManyEights = size_t{1} << 19;
+// From this many vectors on a lane has four of them in flight: below, one each spreads the work wider.
+constexpr size_t kManyVectors = size_t{1} << 19;
+
+// Values of this many bytes pass the caches by: they would only push out of them what is used again.
+// Measured (us, ordinary and non-temporal), bf16 of 8192 columns: with both directions 25 and 23 at 64 MB, 41 and 35 at 96 MB, 104 and 96 at 256 MB;
+// along the rows 14 and 16, 24 and 22, 59 and 53; back 15 and 13, 26 and 20, 60 and 49.  fp32 is alike.
+constexpr size_t kStreamBytes = size_t{96} << 20;
 
 int check_sizes(const char *who, int64_t rows, int64_t cols) {
   FLUXMI_REQUIRE(rows >= 0 && cols >= 0, FLUXMI_ERR_INVALID_ARG, "%s: negative size (rows=%lld, cols=%lld)", who, static_cast<long long>(rows),
@@ -386,34 +387,36 @@ extern "C" int fluxmi_quant_mx(const void *x, int32_t row_type, int64_t batch, i
   auto *const q = static_cast<uint8_t *>(codes), *const sc = static_cast<uint8_t *>(scale);
   dim3 grid;
   bool fits = true;
-  if (codes_t != nullptr) {
-    FLUXMI_REQUIRE(rows <= (int64_t{1} << 30), FLUXMI_ERR_UNSUPPORTED, "quant_mx: rows=%lld exceeds 2^30 with a transposed copy", static_cast<long long>(rows));
-    by_type(type, [&](auto t) {
-      constexpr Row T = decltype(t)::value;
+  auto launch = [&](auto t, auto nt) {
+    constexpr Row T = decltype(t)::value;
+    constexpr bool NT = decltype(nt)::value;
+    if (codes_t != nullptr) {
       const int64_t row_tiles = (rows + 8 * kBlock - 1) / (8 * kBlock), col_tiles = (cols + 32 * kVec<T> - 1) / (32 * kVec<T>);
       fits = grid_of((row_tiles * col_tiles + 7) / 8 * 8, 1, &grid) && row_tiles * col_tiles < (int64_t{1} << 23);
       if (!fits) return;
       grid.y = static_cast<unsigned>(batch);
-      hipLaunchKernelGGL(quant_both_kernel<T>, grid, dim3(kThreads), 0, s, in, static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(row_tiles),
+      hipLaunchKernelGGL((quant_both_kernel<T, NT>), grid, dim3(kThreads), 0, s, in, static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(row_tiles),
                          static_cast<int>(col_tiles), q, sc, static_cast<uint8_t *>(codes_t), static_cast<uint8_t *>(scale_t));
-    });
-  } else if (cols % kBlock == 0) {
-    const size_t eights = static_cast<size_t>(batch * rows) * cols / 8;
-    by_type(type, [&](auto t) {
-      constexpr Row T = decltype(t)::value;
-      fits = grid_of(eights, kThreads * (eights >= kManyEights ? 4 : 1), &grid);
+    } else if (cols % kBlock == 0) {
+      const size_t vectors = static_cast<size_t>(batch * rows) * cols / kVec<T>;
+      const bool many = vectors >= kManyVectors;
+      fits = grid_of(vectors, kThreads * (many ? 4 : 1), &grid);
       if (!fits) return;
-      if (eights >= kManyEights) hipLaunchKernelGGL((quant_flat_kernel<T, 4>), grid, dim3(kThreads), 0, s, in, eights, q, sc);
-      else hipLaunchKernelGGL((quant_flat_kernel<T, 1>), grid, dim3(kThreads), 0, s, in, eights, q, sc);
-    });
-  } else {
-    const int shift = row_shift(cols);
-    by_type(type, [&](auto t) {
-      constexpr Row T = decltype(t)::value;
+      if (many) hipLaunchKernelGGL((quant_flat_kernel<T, 4, NT>), grid, dim3(kThreads), 0, s, in, vectors, q, sc);
+      else if constexpr (!NT) hipLaunchKernelGGL((quant_flat_kernel<T, 1, false>), grid, dim3(kThreads), 0, s, in, vectors, q, sc);
+    } else {
+      const int shift = row_shift<T>(cols);
       fits = grid_of(batch * rows, kThreads >> shift, &grid);
-      if (fits) hipLaunchKernelGGL(quant_rows_kernel<T>, grid, dim3(kThreads), 0, s, in, batch * rows, static_cast<int>(cols), shift, q, sc);
-    });
-  }
+      if (fits) hipLaunchKernelGGL((quant_rows_kernel<T, NT>), grid, dim3(kThreads), 0, s, in, batch * rows, static_cast<int>(cols), shift, q, sc);
+    }
+  };
+  if (codes_t != nullptr)
+    FLUXMI_REQUIRE(rows <= (int64_t{1} << 30), FLUXMI_ERR_UNSUPPORTED, "quant_mx: rows=%lld exceeds 2^30 with a transposed copy", static_cast<long long>(rows));
+  const bool streamed = static_cast<size_t>(batch * rows) * cols * (type == Row::F32 ? 4 : 2) >= kStreamBytes;
+  by_type(type, [&](auto t) {
+    if (streamed) launch(t, std::true_type{});
+    else launch(t, std::false_type{});
+  });
   FLUXMI_REQUIRE(fits, FLUXMI_ERR_UNSUPPORTED, "quant_mx: batch=%lld rows=%lld cols=%lld is more than a launch covers", static_cast<long long>(batch),
                  static_cast<long long>(rows), static_cast<long long>(cols));
   FLUXMI_HIP_CHECK(hipGetLastError());
@@ -435,23 +438,27 @@ extern "C" int fluxmi_dequant_mx(const void *codes, const void *scale, int64_t r
   auto *const o = static_cast<uint8_t *>(out);
   dim3 grid;
   bool fits = true;
-  if (cols % kBlock == 0) {
-    const size_t eights = static_cast<size_t>(rows) * cols / 8;
-    by_type(type, [&](auto t) {
-      constexpr Row T = decltype(t)::value;
-      fits = grid_of(eights, kThreads * (eights >= kManyEights ? 4 : 1), &grid);
+  auto launch = [&](auto t, auto nt) {
+    constexpr Row T = decltype(t)::value;
+    constexpr bool NT = decltype(nt)::value;
+    if (cols % kBlock == 0) {
+      const size_t vectors = static_cast<size_t>(rows) * cols / kVec<T>;
+      const bool many = vectors >= kManyVectors;
+      fits = grid_of(vectors, kThreads * (many ? 4 : 1), &grid);
       if (!fits) return;
-      if (eights >= kManyEights) hipLaunchKernelGGL((dequant_flat_kernel<T, 4>), grid, dim3(kThreads), 0, s, q, sc, eights, o);
-      else hipLaunchKernelGGL((dequant_flat_kernel<T, 1>), grid, dim3(kThreads), 0, s, q, sc, eights, o);
-    });
-  } else {
-    const int shift = row_shift(cols);
-    by_type(type, [&](auto t) {
-      constexpr Row T = decltype(t)::value;
+      if (many) hipLaunchKernelGGL((dequant_flat_kernel<T, 4, NT>), grid, dim3(kThreads), 0, s, q, sc, vectors, o);
+      else if constexpr (!NT) hipLaunchKernelGGL((dequant_flat_kernel<T, 1, false>), grid, dim3(kThreads), 0, s, q, sc, vectors, o);
+    } else {
+      const int shift = row_shift<T>(cols);
       fits = grid_of(rows, kThreads >> shift, &grid);
-      if (fits) hipLaunchKernelGGL(dequant_rows_kernel<T>, grid, dim3(kThreads), 0, s, q, sc, rows, static_cast<int>(cols), shift, o);
-    });
-  }
+      if (fits) hipLaunchKernelGGL((dequant_rows_kernel<T, NT>), grid, dim3(kThreads), 0, s, q, sc, rows, static_cast<int>(cols), shift, o);
+    }
+  };
+  const bool streamed = static_cast<size_t>(rows) * cols * (type == Row::F32 ? 4 : 2) >= kStreamBytes;
+  by_type(type, [&](auto t) {
+    if (streamed) launch(t, std::true_type{});
+    else launch(t, std::false_type{});
+  });
   FLUXMI_REQUIRE(fits, FLUXMI_ERR_UNSUPPORTED, "dequant_mx: rows=%lld cols=%lld is more than a launch covers", static_cast<long long>(rows), static_cast<long long>(cols));
   FLUXMI_HIP_CHECK(hipGetLastError());
   return FLUXMI_OK;

@@ -75,6 +75,25 @@ def test_large_and_flat_forms():
         assert np.array_equal(back.double().cpu().numpy(), mx.values(*want))
 
 
+@pytest.mark.parametrize("cols", [2080, 2051])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_values_of_many_megabytes_as_their_parts(dtype, cols):
+    """From 96 MB on the values pass the caches by; parts of 32 x 100 rows are below that."""
+    rows = (112 << 20) // (cols * (4 if dtype == F32 else 2))
+    x = torch.randn(rows, cols, device=DEV, generator=torch.Generator(DEV).manual_seed(cols)).mul_(5).to(dtype)
+    q = quantiser(dtype)
+    codes, scale, codes_t, scale_t = (t.view(torch.uint8) for t in q.quantize_mx(x, True))
+    along = [t.view(torch.uint8) for t in q.quantize_mx(x)[:2]]
+    assert torch.equal(codes, along[0]) and torch.equal(scale, along[1])
+    back = q.dequantize_mx(codes.view(FP4), scale.view(E8M0), cols)
+    for lo in range(0, rows, 3200):
+        part, blocks = x[lo:lo + 3200], slice(lo // 32, lo // 32 + 100)
+        c, s, ct, st = (t.view(torch.uint8) for t in q.quantize_mx(part, True))
+        assert torch.equal(codes[lo:lo + 3200], c) and torch.equal(scale[lo:lo + 3200], s)
+        assert torch.equal(codes_t[:, lo // 2:lo // 2 + 1600], ct) and torch.equal(scale_t[:, blocks], st)
+        assert torch.equal(back[lo:lo + 3200], q.dequantize_mx(c.view(FP4), s.view(E8M0), cols))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 def test_batch_of_matrices(dtype):
     x = hard_values(5 * 70, 100, dtype, 4).view(5, 70, 100)
