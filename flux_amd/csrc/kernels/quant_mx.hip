@@ -12,7 +12,7 @@
 // columns in registers, which gives both directions from one read with no exchange but that of the maxima along the rows; eight lanes side by side and
 // eight row blocks below each other make a wave, so that its loads and its transposed stores are whole 128-byte lines.
 // Measured at 11000 x 7168 bf16: both directions 57 us (4.2 TB/s; without the stores of the row codes 47, without the transposed ones 45: two sets of
-// writes beside the read are what is left), along the rows 33 (7.4 of values and codes together), back 29 (6.9), back from the transposed copy 38 (5.3).
+// writes beside the read are what is left), along the rows 33 (6.1 of values and codes together), back 29 (6.9), back from the transposed copy 38 (5.3).
 // Other tiles of the two-way form (4 x 16 or 2 x 32 lanes, waves stacked instead of side by side) take 56 to 65 us, three waves to a SIMD the same 57.
 #include "rows.hpp"
 

@@ -37,7 +37,7 @@ Quantization::Result Quantization::quantize_mx(torch::Tensor input, bool return_
   const bool batched = input.dim() == 3;
   const int64_t batch = batched ? input.size(0) : 1, rows = input.size(-2), cols = input.size(-1);
   auto make = [&](int64_t r, int64_t c, at::ScalarType st) {
-    return torch::empty(batched ? std::vector<int64_t>{batch, r, c} : std::vector<int64_t>{r, c}, input.options().dtype(st).requires_grad(false));
+    return batched ? empty_on(input, {batch, r, c}, st) : empty_on(input, {r, c}, st);
   };
   torch::Tensor codes = make(rows, blocks_of(cols) * 16, kCodes), scale = make(rows, blocks_of(cols), kScales);
   std::optional<torch::Tensor> codes_t, scale_t;
@@ -62,7 +62,7 @@ torch::Tensor Quantization::dequantize_mx(torch::Tensor codes, torch::Tensor sca
   const c10::DeviceGuard guard(codes.device());
   std::vector<int64_t> shape = codes.sizes().vec();
   shape.back() = n;
-  torch::Tensor out = torch::empty(shape, codes.options().dtype(input_dtype_));
+  torch::Tensor out = empty_on(codes, shape, input_dtype_);
   check_status(fluxmi_dequant_mx(codes.data_ptr(), scale.data_ptr(), codes.dim() == 3 ? codes.size(0) * codes.size(1) : codes.size(0), n, mx_type(input_dtype_),
                                  out.data_ptr(), current_stream()),
                "fluxmi_dequant_mx");
@@ -93,7 +93,7 @@ static torch::Tensor mx_run(const torch::Tensor &input, const torch::Tensor &inp
     FLUX_AMD_CHECK_2D(out, max_rows, n);
     on_device(out, "output");
   } else {
-    out = torch::empty({max_rows, n}, input.options().dtype(out_dtype));
+    out = empty_on(input, {max_rows, n}, out_dtype);
   }
   fluxmi_mx_gemm_args args{};
   if (gather_index.has_value()) {
@@ -123,7 +123,7 @@ static torch::Tensor mx_run(const torch::Tensor &input, const torch::Tensor &inp
   if (splits != nullptr) args.splits = splits->data_ptr<int32_t>();
   const size_t ws_bytes = fluxmi_grouped_gemm_mx_workspace_bytes(&args);
   torch::Tensor ws;
-  if (ws_bytes > 0) ws = torch::empty({static_cast<int64_t>(ws_bytes)}, input.options().dtype(at::kByte));
+  if (ws_bytes > 0) ws = empty_on(input, {static_cast<int64_t>(ws_bytes)}, at::kByte);
   check_status(fluxmi_grouped_gemm_mx(&args, ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, current_stream()), "fluxmi_grouped_gemm_mx");
   return out;
 }

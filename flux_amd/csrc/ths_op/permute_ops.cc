@@ -47,7 +47,7 @@ int32_t topk_of(const torch::Tensor &scatter_index) { return static_cast<int32_t
 
 torch::Tensor permute(const torch::Tensor &input, const torch::Tensor &scatter_index) {
   const c10::DeviceGuard guard(input.device());
-  torch::Tensor rows = torch::empty({scatter_index.numel(), input.size(1)}, input.options().requires_grad(false));
+  torch::Tensor rows = empty_on(input, {scatter_index.numel(), input.size(1)}, input.scalar_type());
   check_status(fluxmi_moe_permute(input.data_ptr(), scatter_index.data_ptr<int32_t>(), tokens_of(scatter_index), topk_of(scatter_index),
                                   input.size(1) * static_cast<int64_t>(input.element_size()), rows.data_ptr(), current_stream()),
                "fluxmi_moe_permute");
@@ -56,7 +56,7 @@ torch::Tensor permute(const torch::Tensor &input, const torch::Tensor &scatter_i
 
 torch::Tensor unpermute(const torch::Tensor &rows, const torch::Tensor &scatter_index, const torch::Tensor &weights) {
   const c10::DeviceGuard guard(rows.device());
-  torch::Tensor out = torch::empty({scatter_index.size(0), rows.size(1)}, rows.options().requires_grad(false));
+  torch::Tensor out = empty_on(rows, {scatter_index.size(0), rows.size(1)}, rows.scalar_type());
   check_status(fluxmi_moe_unpermute(rows.data_ptr(), row_type(rows, "rows"), scatter_index.data_ptr<int32_t>(),
                                     weights.defined() ? weights.data_ptr() : nullptr, weights.defined() ? row_type(weights, "weights") : FLUXMI_ROWS_FP32,
                                     tokens_of(scatter_index), topk_of(scatter_index), static_cast<int32_t>(rows.size(1)), out.data_ptr(), current_stream()),
@@ -69,8 +69,8 @@ std::tuple<torch::Tensor, torch::Tensor> unpermute_backward(const torch::Tensor 
                                                             const torch::Tensor &weights, bool want_rows, bool want_weights) {
   const c10::DeviceGuard guard(grad_out.device());
   torch::Tensor grad_rows, grad_weights;
-  if (want_rows) grad_rows = torch::empty({scatter_index.numel(), grad_out.size(1)}, grad_out.options().requires_grad(false));
-  if (want_weights) grad_weights = torch::empty(weights.sizes(), weights.options().requires_grad(false));
+  if (want_rows) grad_rows = empty_on(grad_out, {scatter_index.numel(), grad_out.size(1)}, grad_out.scalar_type());
+  if (want_weights) grad_weights = empty_on(weights, weights.sizes(), weights.scalar_type());
   check_status(fluxmi_moe_unpermute_backward(grad_out.data_ptr(), want_weights ? rows.data_ptr() : nullptr, row_type(grad_out, "grad_out"),
                                              scatter_index.data_ptr<int32_t>(), weights.data_ptr(), row_type(weights, "weights"), tokens_of(scatter_index),
                                              topk_of(scatter_index), static_cast<int32_t>(grad_out.size(1)), want_rows ? grad_rows.data_ptr() : nullptr,
