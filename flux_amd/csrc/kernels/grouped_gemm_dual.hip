@@ -23,6 +23,12 @@
 // 516 -> 505.  Without block scales long K with many rows stays on the macro tiles: both are at the board's power limit there, and
 // these read half as much again from LDS per MFMA (dense fp8 8192 x 8192 x 8192: 736 k cycles against 771 k, at 1.73 GHz against 1.95;
 // bf16 8 experts 4096 x 14336, 2048 rows each 1361 -> 1540).
+//
+// MXFP4 (K in multiples of 512): 8 experts of 2048 rows 14336 x 4096 556 us, 4096 x 14336 515 (3.5 and 3.7 PFLOP/s); dense 8192 x 8192 x 8192 269 (4.1);
+// the tiles of grouped_gemm_mx.hip, of half a line of K, 650, 600 and 311.  Fills bound it, and the power limit: without the MFMAs 460, 414 and 212 us, with
+// operands of zeros, which draw less, 490, 441 and 226.  The scales' fills, 16 bytes from a line of each row, are 33 us of the first two and 2 of the last.
+// Kept: scales read once in two steps; the last two steps of a tile apart, so that the others choose no source (2 %); chunks off each other's banks
+// (2 %; 8 experts of 194 rows 4096 x 14336 95 -> 91).  Without gain: fills between the reads or half of them beside the MFMAs, scales read a phase earlier.
 #include "grouped_gemm_dual.hpp"
 #include "grouped_gemm_rows.hpp"
 
@@ -313,7 +319,13 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
   // 16-bit results: a lane has columns 8 g .. 8 g + 7 in the two blocks of a group of 32 (g = lane / 16), fp32: 4 g .. in each block
   const bool f32_out = p.d_fp32 != 0;
   const uint32_t wstep1 = (f32_out ? 8u : 16u) * kbytes, wstep2 = (f32_out ? 16u : 4u) * kbytes;
-  auto chunk_of = [&](int l) { return static_cast<uint32_t>(((l & 7) ^ (l >> 4)) * 16); };  // of even fills; odd ones: ^ 64
+  // Of even fills; odd ones: ^ kOdd.  MXFP4: places 0 to 3 of a line have the chunks 0, 2, 4 and 6, places 4 to 7 the others: the lanes that LDS serves
+  // together differ in their place as those of the other types do (with chunks in their order, two of each four meet on a bank).
+  constexpr uint32_t kOdd = MX ? 16 : 64;
+  auto chunk_of = [&](int l) {
+    const int place = (l & 7) ^ (l >> 4);
+    return static_cast<uint32_t>((MX ? (place & 3) * 2 + (place >> 2) : place) * 16);
+  };
   const int row_first = xhalf * 128 + wn * 32;                 // first row of the tile that this wave fills
   uint32_t nxts = 0;  // the same for the row whose scale this lane fetches
   auto load_rows = [&](const DualTile &t) {  // requests the rows of A that X fills of tile t read
@@ -344,7 +356,7 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
         const int x = static_cast<int>(v);
         row = x < 0 ? 0 : (x >= a_rows ? a_rows - 1 : x);
       }
-      const uint32_t chunk = MX ? 0 : chunk0 ^ ((j & 1) * 64);  // (MX: added when the offsets come out of LDS)
+      const uint32_t chunk = MX ? 0 : chunk0 ^ ((j & 1) * kOdd);  // (MX: added when the offsets come out of LDS)
       return r + 8 * j < t.rows ? row * static_cast<uint32_t>(kbytes) + chunk : kNoRow;
     };
     nxt0 = offset(nxt0, 0);
@@ -386,9 +398,9 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
     const int l = fresh_lane(), r = l >> 3, col = f32_out ? r : (r >> 2) * 8 + (r & 3);
     const uint32_t w0 = static_cast<uint32_t>(col) * kbytes + wbase, chunk0 = chunk_of(l);
     woff0 = w0 + chunk0;
-    woff1 = w0 + wstep1 + (chunk0 ^ 64);
+    woff1 = w0 + wstep1 + (chunk0 ^ kOdd);
     woff2 = w0 + wstep2 + chunk0;
-    woff3 = w0 + wstep1 + wstep2 + (chunk0 ^ 64);
+    woff3 = w0 + wstep1 + wstep2 + (chunk0 ^ kOdd);
   };
   const LdsInt stash = reinterpret_cast<LdsInt>(lds0 + (MX ? kMxStash + wave * kMxStashOfWave * 4 : kStash));
   auto put_next = [&]() {
@@ -406,7 +418,7 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
     if constexpr (MX) {
       const int l = fresh_lane(), r = l >> 3;
       const uint32_t chunk0 = chunk_of(l);  // (less than 128: an offset past the operand stays past it)
-      nxt0 = stash[r] + chunk0, nxt1 = stash[8 + r] + (chunk0 ^ 64), nxt2 = stash[16 + r] + chunk0, nxt3 = stash[24 + r] + (chunk0 ^ 64);
+      nxt0 = stash[r] + chunk0, nxt1 = stash[8 + r] + (chunk0 ^ kOdd), nxt2 = stash[16 + r] + chunk0, nxt3 = stash[24 + r] + (chunk0 ^ kOdd);
       nxts = stash[32 + l];
       return;
     }
@@ -464,7 +476,7 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
   uint32_t xread[2], wread[2];
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    const uint32_t chunk = ((MX ? (lane >> 4) * 2 + c : c * 4 + (lane >> 4)) ^ ((lane >> 1) & 7)) * 16;
+    const uint32_t chunk = ((c * 4 + (lane >> 4)) ^ ((lane >> 1) & 7)) * 16;
     xread[c] = lds0 + (wm * 64 + (lane & 15)) * 128 + chunk;
     wread[c] = lds0 + (wn * 32 + (lane & 15)) * 128 + chunk;
   }
@@ -630,7 +642,7 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
       // scales, one each, follow those of X.  The first steps of a tile were waited for at its start.
       // Read: the first half's rows, all columns.  Reads before fills: the phase ends when the last of them is issued.
       if constexpr (MX && PAR == 0) {
-        // The words lie where B's fragments will; read after these, row for row in the few registers left, they cost 6 % of a long K.
+        // The words lie where B's fragments will.
         u32x2 raw[12];
         read_mx_scales(raw);
         __builtin_amdgcn_sched_barrier(0);

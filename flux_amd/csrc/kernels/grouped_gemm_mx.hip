@@ -24,7 +24,6 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kThreads = 256;
 constexpr int kCols = 64;    // columns of a workgroup
-constexpr int kTurn = 512;   // values of K a wave takes at a time: 256 bytes of codes, 16 of scales of each row
 constexpr int kMaxExperts = 1024;
 constexpr int kPlanCus = 256;  // compute units that the choice of a kernel reckons with
 
@@ -237,8 +236,10 @@ __global__ __launch_bounds__(512, 2) void mx_tile_kernel(const MxParams p, int t
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)smem));
   const int row_bytes = p.kb * 16, stages = (p.kb + 3) / 4;
 
-  // ---- fills: LDS row R lies at R * 64, its chunk c of 16 bytes at slot c ^ ((R >> 2) & 3); a fill covers 16 rows, lane l row l >> 2 and slot l & 3.
-  const int chunk = (lane & 3) ^ (lane >> 4);
+  // ---- fills: LDS row R lies at R * 64, its chunk c of 16 bytes at slot c ^ turn(R >> 2); a fill covers 16 rows, lane l row l >> 2 and slot l & 3.  The turns
+  // 0, 3, 2, 1 of every 16 rows keep the 16 lanes that LDS serves together (rows 0 to 3 and 12 to 15 of one lane group, 4 to 11 of the next) off each other's banks.
+  auto turn = [](int q) { return -q & 3; };
+  const int chunk = (lane & 3) ^ turn(lane >> 4);
   const auto xr = buffer_of(p.a, static_cast<int64_t>(p.a_rows) * row_bytes);
   const auto wr = buffer_of(p.b + static_cast<int64_t>(t.e) * p.n * row_bytes, static_cast<int64_t>(p.n) * row_bytes);
   const int scale_fill = wave % C::kScaleFills;  // (waves without one of their own repeat another's)
@@ -279,7 +280,7 @@ __global__ __launch_bounds__(512, 2) void mx_tile_kernel(const MxParams p, int t
   // ---- fragments ---------------------------------------------------------------------------------------------
   typedef const __attribute__((address_space(3))) u32x4 *LdsFrag;
   // Wave rows: of both halves of the tile's rows MI / 2 blocks each, so that few rows are shared out evenly.
-  const uint32_t in_rows = (lane & 15) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3)) * 16);
+  const uint32_t in_rows = (lane & 15) * 64 + (((lane >> 4) ^ turn(lane >> 2)) * 16);
   const uint32_t xread = lds0 + wm * (MI * 8) * 64 + in_rows, wread = lds0 + (C::BM + wn * NJ * 16) * 64 + in_rows;
   const uint32_t in_scales = lds0 + C::kStage * C::kStages + (lane & 15) * 16;
   const uint32_t xsread = in_scales + wm * (MI * 8) * 16, wsread = in_scales + (C::BM + wn * NJ * 16) * 16;
@@ -427,20 +428,22 @@ __global__ __launch_bounds__(64 * P) void mx_stream_kernel(const MxParams p, int
   const auto xr = buffer_of(p.a, static_cast<int64_t>(p.a_rows) * row_bytes), xsr = buffer_of(p.a_scale, static_cast<int64_t>(p.a_rows) * p.kb);
   const auto wr = buffer_of(p.b + static_cast<int64_t>(it.e) * p.n * row_bytes, static_cast<int64_t>(p.n) * row_bytes);
   const auto wsr = buffer_of(p.b_scale + static_cast<int64_t>(it.e) * p.n * p.kb, static_cast<int64_t>(p.n) * p.kb);
-  // LDS row R of 128 bytes: chunk c of 16 bytes at slot c ^ ((R >> 1) & 7); a fill covers 8 rows, lane l row l >> 3 and slot l & 7.
+  // LDS row R of 128 bytes: its chunks of 16 bytes in the order 0, 2, 4, 6, 1, 3, 5, 7, the c-th of them at slot c ^ ((R >> 1) & 7); a fill covers 8 rows, lane l row
+  // l >> 3 and slot l & 7.  (The 16 lanes that LDS serves together, of two lane groups, are so on banks of their own.)
   uint32_t xoff[2 * MT], woff[2 * NJ];
-  const uint32_t chunk0 = ((lane & 7) ^ (lane >> 4)) * 16;
+  const int place = (lane & 7) ^ (lane >> 4);  // of even fills; odd ones: ^ 4
+  const uint32_t chunk0 = ((place & 3) * 2 + (place >> 2)) * 16;
 #pragma unroll
   for (int q = 0; q < 2 * NJ; ++q) {
     const int n = n0 + column_of(q * 8 + (lane >> 3));
-    woff[q] = n < p.n ? static_cast<uint32_t>(n) * row_bytes + (chunk0 ^ ((q & 1) * 64)) : kNoRow;
+    woff[q] = n < p.n ? static_cast<uint32_t>(n) * row_bytes + (chunk0 ^ ((q & 1) * 16)) : kNoRow;
   }
   const int ns = n0 + column_of(lane);
   const uint32_t wsoff = lane < NJ * 16 && ns < p.n ? static_cast<uint32_t>(ns) * p.kb : kNoRow;
 #pragma unroll
   for (int q = 0; q < 2 * MT; ++q) {
     const int m = q * 8 + (lane >> 3);
-    xoff[q] = m < it.rows ? static_cast<uint32_t>(a_row(p, it.row0 + m)) * row_bytes + (chunk0 ^ ((q & 1) * 64)) : kNoRow;
+    xoff[q] = m < it.rows ? static_cast<uint32_t>(a_row(p, it.row0 + m)) * row_bytes + (chunk0 ^ ((q & 1) * 16)) : kNoRow;
   }
   const uint32_t xsoff = lane < it.rows ? static_cast<uint32_t>(a_row(p, it.row0 + lane)) * p.kb : kNoRow;  // (lanes past the rows' blocks: not read)
   auto fill_turn = [&](int t, int slot) {
@@ -456,7 +459,7 @@ __global__ __launch_bounds__(64 * P) void mx_stream_kernel(const MxParams p, int
   typedef const __attribute__((address_space(3))) u32x4 *LdsFrag;
   typedef const __attribute__((address_space(3))) uint32_t *LdsWord;
   const int g = lane >> 4, r = lane & 15;
-  const uint32_t in_rows0 = r * 128 + (((2 * g) ^ ((lane >> 1) & 7)) * 16), in_rows1 = r * 128 + (((2 * g + 1) ^ ((lane >> 1) & 7)) * 16);
+  const uint32_t in_rows0 = r * 128 + ((g ^ ((lane >> 1) & 7)) * 16), in_rows1 = r * 128 + (((4 + g) ^ ((lane >> 1) & 7)) * 16);
   const uint32_t in_scales = C::kScales + r * 16 + (g >> 1) * 4, pick = 0x05040100u + 0x02020202u * (g & 1);
   f32x4 acc[MT][NJ] = {};
   int slot = 0;
