@@ -1,6 +1,7 @@
 // Tokens sorted by expert and back, with gradients: moe_permute, moe_unpermute and their backward passes.  The reference gathers inside its GEMM
 // and reduces without a gradient (src/moe_gather_rs/ths_op/topk_scatter_reduce.cc:30-56), so these have no counterpart there.
 #include <c10/core/DeviceGuard.h>
+#include <hip/hip_runtime_api.h>
 
 #include "ths_ops.h"
 
@@ -84,6 +85,25 @@ void refuse_second_derivative(const char *who) {
   TORCH_CHECK(!at::GradMode::is_enabled(), who, ": the gradient of the gradient is not built (create_graph=True)");
 }
 
+// A backward pass that is captured hands its gradients to leaves on the stream where these were first used.  If an eager graph of a leaf is alive, that is the
+// eager stream, which would be drawn into the capture and end the process: an error is raised before it comes to that.
+void refuse_leaves_of_another_stream(const char *who) {
+  const c10::hip::HIPStream current = c10::hip::getCurrentHIPStream();
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(current.stream(), &capture) != hipSuccess) {
+    (void)hipGetLastError();
+    return;
+  }
+  const std::shared_ptr<torch::autograd::Node> node = torch::autograd::get_current_node();
+  if (capture == hipStreamCaptureStatusNone || node == nullptr) return;
+  for (const torch::autograd::Edge &edge : node->next_edges()) {
+    if (edge.function == nullptr || edge.function->name() != "torch::autograd::AccumulateGrad") continue;
+    const std::optional<c10::Stream> stream = edge.function->stream();
+    TORCH_CHECK(!stream.has_value() || stream->id() == current.id(), who,
+                ": its backward pass is captured while an eager graph of the same leaf is alive; drop that graph's outputs before the capture");
+  }
+}
+
 struct Permute : torch::autograd::Function<Permute> {
   static torch::Tensor forward(torch::autograd::AutogradContext *ctx, const torch::Tensor &input, const torch::Tensor &scatter_index) {
     ctx->save_for_backward({scatter_index});
@@ -91,6 +111,7 @@ struct Permute : torch::autograd::Function<Permute> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
     refuse_second_derivative("moe_permute");
+    refuse_leaves_of_another_stream("moe_permute");
     return {unpermute(grads[0].contiguous(), ctx->get_saved_variables()[0], {}), {}};
   }
 };
@@ -103,6 +124,7 @@ struct Sum : torch::autograd::Function<Sum> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
     refuse_second_derivative("moe_unpermute");
+    refuse_leaves_of_another_stream("moe_unpermute");
     return {permute(grads[0].contiguous(), ctx->get_saved_variables()[0]), {}};
   }
 };
@@ -117,6 +139,7 @@ struct Unpermute : torch::autograd::Function<Unpermute> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
     refuse_second_derivative("moe_unpermute");
+    refuse_leaves_of_another_stream("moe_unpermute");
     const auto saved = ctx->get_saved_variables();
     const torch::Tensor grad = grads[0].contiguous(), &scatter_index = saved[0], &weights = saved[1], &rows = saved[2];
     const bool want_rows = ctx->saved_data["rows"].toBool(), want_weights = rows.defined();

@@ -291,6 +291,34 @@ def test_graph_of_a_training_step_replays():
                 assert torch.equal(a, b)
 
 
+def test_captured_backward_pass():
+    """The recorded gradients in a graph; refused while an eager graph of the same leaves is alive, whose stream the capture would draw in."""
+    idx, x, w = leaves()
+
+    def step():
+        return torch.autograd.grad(layer(x, idx, w).sum(), [x, w])
+
+    alive = flux_amd.moe_permute(x, idx)
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph of the same leaf"):
+        with torch.cuda.graph(g):
+            flux_amd.moe_unpermute(flux_amd.moe_permute(x, idx), idx).sum().backward()
+    del alive, g
+    x.grad = w.grad = None
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    for seed in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn(x.shape, device=DEV, generator=torch.Generator(DEV).manual_seed(seed)))
+        want = step()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_refusals():
     idx, x, w = make_index(4, 2, 0.0, 1), torch.zeros(4, 16, device=DEV), torch.ones(4, 2, device=DEV)
     rows = torch.zeros(8, 16, device=DEV)
