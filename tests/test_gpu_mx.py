@@ -151,7 +151,8 @@ def operand(*shape, k, seed):
     codes = codes.view(*shape, kb * 16)
     table = torch.from_numpy(mx.values(np.arange(256, dtype=np.uint8)[:, None].repeat(16, 1), np.full((256, 1), 127, np.uint8)))[:, :2].to(DEV)
     codes, scale = codes.to(DEV), scale.to(DEV)
-    value = table[codes.long()].flatten(-2) * torch.exp2(scale.double() - 127).repeat_interleave(32, -1)
+    # (in parts: one lookup of 2^26 codes and more is past what the library's kernel launches, and what it left out would be zeros)
+    value = torch.cat([table[part.long()] for part in codes.flatten().split(1 << 22)]).view(*codes.shape[:-1], -1) * torch.exp2(scale.double() - 127).repeat_interleave(32, -1)
     return codes.view(FP4), scale.view(E8M0), value
 
 
@@ -207,6 +208,79 @@ def test_grouped_product(splits, n, k, gathered, weighted, out):
         at += r
     host = flux_amd.MxGemm(out).forward_grouped(a, sp, w, sa, sw, gather_index=gather, row_scale=factor)
     assert torch.equal(host[:rows], got[:rows])
+
+
+def grouped(splits, n, k, out, seed=3):
+    """A grouped product of random operands, checked expert by expert."""
+    rows = sum(splits)
+    a, sa, va = operand(rows, k=k, seed=seed)
+    w, sw, vw = operand(len(splits), n, k=k, seed=seed + 1)
+    factor = torch.rand(rows, generator=torch.Generator().manual_seed(seed)).to(DEV)
+    got = flux_amd.MxGemm(out).forward_grouped(a, torch.tensor(splits, dtype=torch.int32, device=DEV), w, sa, sw, row_scale=factor)
+    at = 0
+    for e, r in enumerate(splits):
+        check(got[at:at + r], va[at:at + r], vw[e], k, factor[at:at + r])
+        at += r
+
+
+def brief(v):
+    return f"{sum(v)}of{len(v)}" if isinstance(v, list) else str(v)
+
+
+# Streams of 16 and of 32 rows whose waves split K in four, in two and not at all, by the number of pieces (experts with rows times n / 32).
+@pytest.mark.parametrize("k", [512, 1024, 2560, 8192])
+@pytest.mark.parametrize("splits,n", [([1, 1], 500), ([3] * 8, 1000), ([9, 1] * 16, 1000), ([30, 17], 500), ([16, 20, 1, 33, 0, 15, 17, 28], 1000),
+                                      ([13, 0] * 15 + [40, 60], 800), ([20, 12] * 16, 1030)], ids=brief)
+def test_streams(splits, n, k):
+    for out in (BF16, F32):
+        print(f"[case] streams {splits} {n} {k} {out}", flush=True)
+        grouped(splits, n, k, out)
+
+
+# Tiles of 256 x 256: rows that end in each of a tile's four units of 64, experts without rows, columns that end in each half and quarter of a tile; as many as an
+# expert table holds and one more; results whose rows are and are not whole stores.
+@pytest.mark.parametrize("out", [BF16, F16, F32])
+@pytest.mark.parametrize("splits,n,k", [([300, 0, 1, 700], 520, 1024), ([64, 65, 128, 129, 192, 193, 256, 257], 264, 1536), ([1000, 31], 72, 2048),
+                                        ([513], 1160, 512), ([511], 136, 4096), ([2000, 1], 2048, 1024), ([40] * 128, 64, 1024), ([30] * 129, 64, 1024),
+                                        ([200, 300], 516, 1024), ([200, 300], 514, 1024), ([26] * 32, 2048, 1024), ([20] * 32, 2048, 1024)], ids=brief)
+def test_tiles(splits, n, k, out):
+    print(f"[case] tiles {splits} {n} {k} {out}", flush=True)
+    grouped(splits, n, k, out)
+
+
+@pytest.mark.parametrize("rows", [5, 100, 700])
+def test_operands_that_are_parts_of_others(rows):
+    """Scales from any byte on, codes from any row: blocks of a row are not a multiple of 16."""
+    for k in (320, 1024):
+        a, sa, va = operand(rows + 3, k=k, seed=1)
+        w, sw, vw = operand(3, 130, k=k, seed=2)
+        got = flux_amd.MxGemm(F32).forward(a[3:], w[1], sa[3:], sw[1])
+        check(got, va[3:], vw[1], k)
+        moved = sa.view(torch.uint8).new_empty(sa.numel() + 1)[1:].view(sa.shape)
+        moved.copy_(sa.view(torch.uint8))
+        assert torch.equal(flux_amd.MxGemm(F32).forward(a[3:], w[1], moved[3:].view(E8M0), sw[1]), flux_amd.MxGemm(F32).forward(a[3:], w[1].clone(), moved[3:].view(E8M0), sw[1].clone()))
+        check(flux_amd.MxGemm(F32).forward(a[3:], w[1], moved[3:].view(E8M0), sw[1]), va[3:], vw[1], k)
+
+
+def test_two_streams_at_once():
+    """Calls of every form, each on two streams that run together, and the same results as one after another."""
+    calls = []
+    for rows, n, k in ((4, 700, 2048), (40, 700, 2048), (600, 704, 2048), (600, 700, 2016), (9, 700, 2016)):
+        a, sa, _ = operand(rows, k=k, seed=rows)
+        w, sw, _ = operand(n, k=k, seed=rows + 1)
+        calls.append(lambda a=a, w=w, sa=sa, sw=sw: flux_amd.MxGemm(BF16).forward(a, w, sa, sw))
+    want = [call() for call in calls]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for which in (0, 1):
+            with torch.cuda.stream(streams[which]):
+                got[which] += [call() for call in calls]
+    torch.cuda.synchronize()
+    for results in got:
+        for i, result in enumerate(results):
+            assert torch.equal(result, want[i % len(calls)])
 
 
 def test_counts_below_zero_and_past_the_rows():
