@@ -4,8 +4,10 @@
 // values (lane l: row l & 15, block l >> 4), and the block's scale byte in a register of its own.  B's rows are the MFMA's rows, so that a lane's
 // four sums are neighbouring columns of one row of D.
 //
-// Bound by the weights' bytes with few rows per expert, by the MFMAs and what feeds them with many.  Four kernels:
-//  * streams (mx_stream_kernel): a wave, or two or four that split K, has 16 or 32 rows and 32 or 64 columns of an expert and streams through LDS on its own;
+// Bound by the weights' bytes with few rows per expert, by the MFMAs and what feeds them with many.  Five kernels:
+//  * streams (mx_stream_kernel), where there is less work than the card has room for: a wave, or two or four that split K, has 16 or 32 rows and 32 or 64 columns of
+//    an expert and streams through LDS on its own;
+//  * panels of 64 or 128 rows and 128 columns (mx_panel_kernel);
 //  * the dual tiles of 256 x 256 (grouped_gemm_dual.hip);
 //  * for K that is no multiple of 512, and whatever else those do not take, mx_few_rows_kernel, whose four waves split K in turns of 512 values and load straight into
 //    registers, and mx_tile_kernel.
@@ -387,6 +389,158 @@ __global__ __launch_bounds__(512, 2) void mx_tile_kernel(const MxParams p, int t
 #endif  // __HIP_DEVICE_COMPILE__
 }
 
+// ---- panels ----------------------------------------------------------------------------------------------------
+
+// MI x 2 blocks of 16 x 16 to a wave, 2 x 4 waves: up to 32 MI rows and 128 columns of one expert.  LDS holds S steps of 256 values of K.
+template <int MI>
+struct Panel {
+  static constexpr int S = 3;
+  static constexpr int BM = 32 * MI, BN = 128;
+  static constexpr int XF = BM / 32, WF = 4;  // fills of a step, of each of the four waves that request them
+  static constexpr int kW = S * BM * 128, kXs = kW + S * BN * 128, kWs = kXs + 2 * BM * 16, kLds = kWs + 2 * BN * 16;  // (scales: of two pairs of steps)
+  static_assert(MI % 2 == 0 && kLds <= 160 * 1024, "");
+};
+
+// A step is a line of 128 bytes of each row.  All waves read the panel's rows of A from one copy in LDS, which leaves more of it to the weights on their way than the
+// streams have, whose waves have a copy each; two workgroups of 64 rows to a compute unit.  Bound by the weights' bytes: 9 to 48 rows of 8 experts 4096 x 14336 43
+// to 47 us (5.9 to 5.5 TB/s), 32 rows of 32 experts 2048 x 7168 47, 7168 x 2048 57 (4.8).  Waves 0 to 3 request A's lines, waves 4 to 7 B's.  More steps in LDS
+// take workgroups off the compute unit (five of B: 52 and 71 us), two steps let its loads run dry (65 instead of 45 for 24 rows 4096 x 14336).
+template <int MI>
+__global__ __launch_bounds__(512, 2) void mx_panel_kernel(const MxParams p, int tiles_n) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using C = Panel<MI>;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const TileItem t = locate_tile(p, blockIdx.x, tiles_n, C::BM, C::BN);
+  if (t.rows <= 0) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)smem));
+  const int row_bytes = p.kb * 16, steps = p.kb / 8;
+  const bool of_a = wave < 4;  // whose fills this wave requests
+  const uint8_t *const codes = of_a ? p.a : p.b + static_cast<int64_t>(t.e) * p.n * row_bytes;
+  const uint8_t *const scales = of_a ? p.a_scale : p.b_scale + static_cast<int64_t>(t.e) * p.n * p.kb;
+  const int64_t rows_of = of_a ? p.a_rows : p.n;
+  const auto cr = buffer_of(codes, rows_of * row_bytes), sr = buffer_of(scales, rows_of * p.kb);
+  // ---- fills: rows of 128 bytes as in the streams; wave q of four has the fills q, q + 4 ... of 8 rows each.  (Of B: four of them.)
+  uint32_t off[C::XF > C::WF ? C::XF : C::WF], soff = kNoRow;
+  const int place = (lane & 7) ^ (lane >> 4);
+  const uint32_t chunk0 = ((place & 3) * 2 + (place >> 2)) * 16;
+#pragma unroll
+  for (int q = 0; q < (C::XF > C::WF ? C::XF : C::WF); ++q) {
+    const int R = (q * 4 + wn) * 8 + (lane >> 3);  // (fills of one wave: q * 4 + wn has the parity of wn)
+    const uint32_t chunk = chunk0 ^ ((wn & 1) * 16);
+    if (of_a) {
+      off[q] = R < t.rows ? static_cast<uint32_t>(a_row(p, t.row0 + R)) * row_bytes + chunk : kNoRow;
+    } else {
+      const int n = t.n0 + column_of(R);
+      off[q] = n < p.n ? static_cast<uint32_t>(n) * row_bytes + chunk : kNoRow;
+    }
+  }
+  const int scale_fill = of_a ? wn % (C::BM / 64) : wn & 1;  // of 64 rows each (more waves than fills: some repeat another's)
+  {
+    const int R = scale_fill * 64 + lane;
+    if (of_a) {
+      if (R < t.rows) soff = static_cast<uint32_t>(a_row(p, t.row0 + R)) * p.kb;
+    } else {
+      const int n = t.n0 + column_of(R);
+      if (n < p.n) soff = static_cast<uint32_t>(n) * p.kb;
+    }
+  }
+  // Step s, into `slot`; steps past the last are zeros.  With the first step of a pair come the scales of both.
+  auto fill_x = [&](int s, int slot) {
+    if ((s & 1) == 0) fill(lds0 + C::kXs + ((s >> 1) & 1) * (C::BM * 16) + scale_fill * 1024, s < steps ? soff : kNoRow, sr, (s >> 1) * 16);
+#pragma unroll
+    for (int q = 0; q < C::XF; ++q) fill(lds0 + slot * (C::BM * 128) + (q * 4 + wn) * 1024, s < steps ? off[q] : kNoRow, cr, s * 128);
+  };
+  auto fill_w = [&](int s, int slot) {
+    if ((s & 1) == 0) fill(lds0 + C::kWs + ((s >> 1) & 1) * (C::BN * 16) + scale_fill * 1024, s < steps ? soff : kNoRow, sr, (s >> 1) * 16);
+#pragma unroll
+    for (int q = 0; q < C::WF; ++q) fill_once(lds0 + C::kW + slot * (C::BN * 128) + (q * 4 + wn) * 1024, s < steps ? off[q] : kNoRow, cr, s * 128);
+  };
+  // ---- fragments: lane group g has chunks 2 g and 2 g + 1 of a line in two MFMAs, and bytes 2 g and 2 g + 1 of the line's 8 scales.
+  typedef const __attribute__((address_space(3))) u32x4 *LdsFrag;
+  typedef const __attribute__((address_space(3))) uint16_t *LdsPair;
+  const int g = lane >> 4, r = lane & 15;
+  const uint32_t in_rows0 = r * 128 + ((g ^ ((lane >> 1) & 7)) * 16), in_rows1 = r * 128 + (((4 + g) ^ ((lane >> 1) & 7)) * 16);
+  // Wave rows: of both halves of the panel's rows MI / 2 blocks each, so that few rows are shared out evenly.
+  auto block_row = [&](int i) { return (i / (MI / 2)) * (C::BM / 2) + wm * (MI * 8) + (i % (MI / 2)) * 16; };
+  const bool has0 = block_row(0) < t.rows, has1 = block_row(MI / 2) < t.rows;
+  f32x4 acc[MI][2] = {};
+  auto compute = [&](auto PARITY, int s, int slot) {
+    constexpr int PAR = decltype(PARITY)::value;
+    const uint32_t x_at = lds0 + slot * (C::BM * 128), w_at = lds0 + C::kW + slot * (C::BN * 128) + wn * 4096;
+    const uint32_t xs_at = lds0 + C::kXs + ((s >> 1) & 1) * (C::BM * 16) + r * 16 + PAR * 8 + g * 2;
+    const uint32_t ws_at = lds0 + C::kWs + ((s >> 1) & 1) * (C::BN * 16) + wn * 512 + r * 16 + PAR * 8 + g * 2;
+    u32x4 w[2][2];
+    uint32_t ws[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      w[j][0] = *reinterpret_cast<LdsFrag>(w_at + in_rows0 + j * 2048);
+      w[j][1] = *reinterpret_cast<LdsFrag>(w_at + in_rows1 + j * 2048);
+      ws[j] = *reinterpret_cast<LdsPair>(ws_at + j * 256);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (h == 0 ? !has0 : !has1) continue;
+#pragma unroll
+      for (int i = h * (MI / 2); i < (h + 1) * (MI / 2); ++i) {
+        const u32x4 x0 = *reinterpret_cast<LdsFrag>(x_at + in_rows0 + block_row(i) * 128), x1 = *reinterpret_cast<LdsFrag>(x_at + in_rows1 + block_row(i) * 128);
+        const uint32_t xs = *reinterpret_cast<LdsPair>(xs_at + block_row(i) * 16);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = mfma<0>(w[j][0], x0, ws[j], xs, acc[i][j]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = mfma<1>(w[j][1], x1, ws[j], xs, acc[i][j]);
+      }
+    }
+  };
+  auto sync = [&]() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // ---- the loop over K: after the barrier of step s its operands are there, and what step s - 1 had is free.  A wave requests step s + 2 then, and waits for step
+  // s + 1 at the end, when the fills of step s + 2 may be on their way, with a pair's scales if s is even.
+  auto fill_step = [&](int s, int slot) {
+    if (of_a) fill_x(s, slot);
+    else fill_w(s, slot);
+  };
+  fill_step(0, 0);
+  fill_step(1, 1);
+  if (of_a) FLUXMI_VMCNT(C::XF);
+  else FLUXMI_VMCNT(C::WF);
+  sync();
+  int slot = 0;
+  auto step = [&](auto PARITY, int s) {
+    constexpr int PAR = decltype(PARITY)::value;
+    fill_step(s + 2, slot == 0 ? 2 : slot - 1);
+    __builtin_amdgcn_sched_barrier(0);
+    compute(PARITY, s, slot);
+    FLUXMI_LGKM0();
+    if (of_a) FLUXMI_VMCNT(C::XF + 1 - PAR);
+    else FLUXMI_VMCNT(C::WF + 1 - PAR);
+    sync();
+    slot = slot == 2 ? 0 : slot + 1;
+  };
+  for (int s = 0; s < steps; s += 2) {
+    step(std::integral_constant<int, 0>{}, s);
+    step(std::integral_constant<int, 1>{}, s + 1);
+  }
+  FLUXMI_VMCNT(0);  // fills past the end write zeros: LDS is this workgroup's until they have
+
+  // ---- results: lane group g has columns 8 g .. 8 g + 7 of the wave's 32, of row r of each block
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int m = block_row(i) + r;
+    if (m >= t.rows) continue;
+    const float scale = p.row_scale ? p.row_scale[t.row0 + m] : 1.f;
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = acc[i][k / 4][k % 4] * scale;
+    store_eight(p, t.row0 + m, t.n0 + wn * 32 + g * 8, v);
+  }
+#endif  // __HIP_DEVICE_COMPILE__
+}
+
 // Scales in rows of a multiple of 16 bytes, zeros behind their end, as the tiles read them: A's rows, then those of all experts.
 __global__ __launch_bounds__(kThreads) void mx_pad_scales_kernel(const uint8_t *__restrict__ a, int64_t a_rows, const uint8_t *__restrict__ b, int64_t b_rows, int kb, int stride,
                                                                  uint8_t *__restrict__ out) {
@@ -667,6 +821,19 @@ int launch_tiles(const MxParams &p, hipStream_t s) {
   return FLUXMI_OK;
 }
 
+template <int MI>
+int launch_panel(const MxParams &p, hipStream_t s) {
+  using C = Panel<MI>;
+  static std::atomic<uint64_t> lds_done{0};
+  const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(mx_panel_kernel<MI>), C::kLds, lds_done);
+  if (rc != FLUXMI_OK) return rc;
+  const int tiles_n = (p.n + C::BN - 1) / C::BN;
+  const int64_t pieces = p.max_rows / C::BM + (p.nexperts < p.max_rows ? p.nexperts : p.max_rows), grid = (pieces * tiles_n + 7) / 8 * 8;
+  FLUXMI_REQUIRE(grid * 512 < (int64_t{1} << 32), FLUXMI_ERR_UNSUPPORTED, "grouped_gemm_mx: max_rows=%d and n=%d are more than a launch covers", p.max_rows, p.n);
+  hipLaunchKernelGGL((mx_panel_kernel<MI>), dim3(static_cast<unsigned>(grid)), dim3(512), C::kLds, s, p, tiles_n);
+  return FLUXMI_OK;
+}
+
 // The call as the dual tiles take it.
 GemmParams dual_params(const fluxmi_mx_gemm_args &a) {
   GemmParams p{};
@@ -692,38 +859,48 @@ GemmParams dual_params(const fluxmi_mx_gemm_args &a) {
 }
 
 // Which kernel computes a call.
-enum class Form { FEW_ROWS, STREAM, DUAL, TILES };
+enum class Form { FEW_ROWS, STREAM, PANEL, DUAL, TILES };
 struct Plan {
   Form form;
   int row_blocks, col_blocks, waves;  // STREAM: blocks of 16 rows and of 16 columns of an item, waves that split K
-  bool low;         // TILES: of 128 rows
+  bool low;                           // PANEL: of 64 rows; TILES: of 128 rows
   size_t workspace;
 };
 
-// The streams read an expert's weights once for every 16 or 32 of its rows, the tiles once for up to 256.  us, stream of 16 rows / of 32 rows / dual tiles, rows on
-// average and a fifth more or less: 8 experts 14336 x 4096, 9 rows 47 / 55 / 62, 24 rows 90 / 61 / 63, 48 rows - / 102 / 65; 4096 x 14336, 9 rows 50 / 49 / 71, 24
-// rows 95 / 54 / 72; 32 experts 7168 x 2048, 24 rows 86 / 62 / 67; 2048 x 7168, 9 rows 52 / 64 / 53, 24 rows 91 / 70 / 54, where the dual tiles are one
-// to a compute unit: with whole rounds of tiles they are taken from 10 rows on.
-// Few waves (one token with two experts of 4096 x 14336: 256): K is split over two or four of a workgroup, 16.3 -> 13.2 us; with 896 (14336 x 4096) 14.0 -> 15.8.
-// The dual tiles want K in multiples of 512 and N of 8 (fp32 results 4), the streams K only; what neither takes goes to the first kernel up to 16 rows (9 rows: 58,
-// tiles 61) and to the tiles of this file beyond (32 rows 2048 x 7168 of 32 experts: 81, tiles 57), of 128 rows up to 128 on average (194 rows 4096 x 14336 of
-// 8 experts 116 -> 96, 2048 rows 600 -> 750).
+// By the rows of an expert on average and by how many workgroups the card gets.  us, rows a fifth more and less on every other expert:
+//  streams / panels of 64 / of 128 / dual tiles
+//  few panels: one token of two experts 4096 x 14336 (64 panels) 13 / 33, 14336 x 4096 (224) 13.8 / 14.4 / - / 26; 4 experts 4096 x 7168 (128), 9 rows 14 / 20, 20 rows
+//  16 / 21, 40 rows 22 / 23; one expert 4096 x 4096, 60 rows 6.4 / 15 / 15 / 25, 256 rows (128) 14 / 14 / 19 / 28, 512 rows (256) 27 / 16 / 20 / 27, 1024 rows (512; 256
+//  of 128 rows) 50 / 26 / 21 / 29; 2 experts 14336 x 4096 (224), 30 rows 21 / 16 / 17 / 26; 6 experts 4096 x 7168 (192), 20 rows 23.3 / 22.4
+//  up to 48 rows: 8 experts 4096 x 14336 (256), 5 rows 49 / 42, 9 rows 49 / 43, 24 rows 54 / 45 / 48 / 69; 14336 x 4096 (896), 5 rows 46 / 46, 9 rows 47 / 47, 24 rows
+//  61 / 51 / 62 / 61, 48 rows - / 57 / 67 / 63; 32 experts 2048 x 7168 (512), 9 rows 52 / 43, 32 rows 78 / 47 / 54 / 53; 7168 x 2048, 32 rows 77 / 57 / 70 / 67
+//  more: 8 experts 4096 x 14336 (256 of 128 rows), 60 rows - / 82 / 52 / 75, 100 rows - / 84 / 60 / 79; 32 experts 2048 x 7168 (512), 60 rows - / 72 / 59 / 58, 100 rows
+//  - / 95 / 65 / 63; 14336 x 4096 (896), 60 rows - / 82 / 71 / 67; one expert 4096 x 14336, 1024 rows (256) 161 / 74 / 54 / 68, 2048 rows (512) - / 145 / 106 / 84.
+// The waves of a stream: one token of two experts 4096 x 14336 (256 streams) 16.3 / 13.0 / 13.4 of one, two and four that split K, with 896 (14336 x 4096) 13.8 / 15.7;
+// of 32 rows one expert 4096 x 4096, 128 rows (512 streams) 9.4 / 9.5 / 12.5, 1024 x 4096, 256 rows (256) 8.1 / 6.0 / 6.8, 128 rows (128) 8.0 / 5.9 / 5.6.  64 columns of
+// 32 rows: one expert 4096 x 14336, 256 rows (1024 streams) 46 -> 37, with fewer streams it is slower.
+// The dual tiles want K in multiples of 512 and N of 8 (fp32 results 4), streams and panels K only; where only N stands in the way, panels are taken up to 128 rows.  What
+// none takes goes to the first kernel up to 16 rows (9 rows: 58, tiles 61) and to the tiles of this file beyond (32 rows 2048 x 7168 of 32 experts: 81, tiles 57), of
+// 128 rows up to 128 on average (194 rows 4096 x 14336 of 8 experts 116 -> 96, 2048 rows 600 -> 750).
 Plan plan_of(const fluxmi_mx_gemm_args &a, const GemmParams &dual, int cus) {
   const int64_t rows = a.max_rows, experts = a.nexperts, active = rows < experts ? rows : experts, kb = (int64_t{a.k} + 31) / 32;
-  const bool dual_takes = dual_takes_mx(dual), streams = kb % 16 == 0 && aligned16(a.a_scale) && aligned16(a.b_scale);
-  const int64_t tiles = active * ((a.n + 255) / 256);
-  const bool whole_rounds = tiles >= cus && tiles % cus == 0;
-  if (streams && (rows <= 10 * experts || (rows <= 24 * experts && !(dual_takes && whole_rounds)))) {
-    const bool two = rows > 10 * experts;
-    const int64_t waves32 = active * ((a.n + 31) / 32);
-    const bool wide = two && waves32 >= 1024;
-    const int waves = wide || waves32 >= 768 ? 1 : waves32 >= 192 ? 2 : 4;
-    return {Form::STREAM, two ? 2 : 1, wide ? 4 : 2, waves, false, 0};
+  const int64_t each = (rows + active - 1) / active;  // rows of an expert on average
+  auto pieces = [&](int64_t high, int64_t wide) { return active * ((each + high - 1) / high) * ((a.n + wide - 1) / wide); };
+  const bool dual_takes = dual_takes_mx(dual), aligned = kb % 16 == 0 && aligned16(a.a_scale) && aligned16(a.b_scale);
+  if (aligned) {
+    const int64_t low_panels = pieces(64, 128);
+    if (low_panels < (each <= 10 ? 240 : 160)) {
+      const bool two = each > 10;
+      const int64_t streams = pieces(two ? 32 : 16, 32);
+      const bool wide = two && streams >= 1024;
+      return {Form::STREAM, two ? 2 : 1, wide ? 4 : 2, streams >= (two ? 512 : 768) ? 1 : streams >= 192 ? 2 : 4, false, 0};
+    }
+    if (each <= 48 || low_panels <= cus) return {Form::PANEL, 0, 0, 0, true, 0};
+    if (pieces(128, 128) <= cus || (!dual_takes && each <= 128)) return {Form::PANEL, 0, 0, 0, false, 0};
   }
   if (dual_takes) return {Form::DUAL, 0, 0, 0, false, 0};
   if (rows <= 16 * experts) return {Form::FEW_ROWS, 0, 0, 0, false, 0};
-  const bool padded = kb % 16 != 0 || !aligned16(a.a_scale) || !aligned16(a.b_scale);
-  return {Form::TILES, 0, 0, 0, rows <= 128 * experts, padded ? static_cast<size_t>(a.a_rows + experts * a.n) * ((kb + 15) / 16 * 16) : 0};
+  return {Form::TILES, 0, 0, 0, rows <= 128 * experts, aligned ? 0 : static_cast<size_t>(a.a_rows + experts * a.n) * ((kb + 15) / 16 * 16)};
 }
 
 }  // namespace
@@ -764,6 +941,9 @@ extern "C" int fluxmi_grouped_gemm_mx(const fluxmi_mx_gemm_args *args, void *wor
       if (plan.col_blocks == 4) rc = launch_stream<2, 4, 1>(p, s);
       else if (plan.row_blocks == 2) rc = plan.waves == 1 ? launch_stream<2, 2, 1>(p, s) : plan.waves == 2 ? launch_stream<2, 2, 2>(p, s) : launch_stream<2, 2, 4>(p, s);
       else rc = plan.waves == 1 ? launch_stream<1, 2, 1>(p, s) : plan.waves == 2 ? launch_stream<1, 2, 2>(p, s) : launch_stream<1, 2, 4>(p, s);
+      break;
+    case Form::PANEL:
+      rc = plan.low ? launch_panel<2>(p, s) : launch_panel<4>(p, s);
       break;
     case Form::DUAL: {
       // Up to four workgroups to a tile, which is cut in pieces when these still fit the card.

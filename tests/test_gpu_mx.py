@@ -152,7 +152,7 @@ def operand(*shape, k, seed):
     table = torch.from_numpy(mx.values(np.arange(256, dtype=np.uint8)[:, None].repeat(16, 1), np.full((256, 1), 127, np.uint8)))[:, :2].to(DEV)
     codes, scale = codes.to(DEV), scale.to(DEV)
     # (in parts: one lookup of 2^26 codes and more is past what the library's kernel launches, and what it left out would be zeros)
-    value = torch.cat([table[part.long()] for part in codes.flatten().split(1 << 22)]).view(*codes.shape[:-1], -1) * torch.exp2(scale.double() - 127).repeat_interleave(32, -1)
+    value = torch.cat([table[part.long()] for part in codes.flatten().split(1 << 22)]).view(*codes.shape[:-1], 2 * codes.shape[-1]) * torch.exp2(scale.double() - 127).repeat_interleave(32, -1)
     return codes.view(FP4), scale.view(E8M0), value
 
 
@@ -237,6 +237,16 @@ def test_streams(splits, n, k):
         grouped(splits, n, k, out)
 
 
+# Panels of 64 rows (experts with rows times n / 128 is 240 or more, 48 rows on average at most) and of 128: rows that end in each block of 16 and past the panel's.
+@pytest.mark.parametrize("k", [512, 1024, 2560, 7168])
+@pytest.mark.parametrize("splits,n", [([1, 0, 2] * 20, 900), ([16, 17, 31, 32, 33, 63, 64, 65, 0, 2] * 4, 1000), ([150, 1, 1, 1, 129, 2, 3, 70] * 4, 1030),
+                                      ([100, 127, 128, 129, 16, 200, 17, 90] * 2, 2000), ([97, 33, 128, 1, 130] * 8, 1001), ([700], 3001)], ids=brief)
+def test_panels(splits, n, k):
+    for out in (BF16, F16, F32):
+        print(f"[case] panels {splits} {n} {k} {out}", flush=True)
+        grouped(splits, n, k, out)
+
+
 # Tiles of 256 x 256: rows that end in each of a tile's four units of 64, experts without rows, columns that end in each half and quarter of a tile; as many as an
 # expert table holds and one more; results whose rows are and are not whole stores.
 @pytest.mark.parametrize("out", [BF16, F16, F32])
@@ -265,7 +275,7 @@ def test_operands_that_are_parts_of_others(rows):
 def test_two_streams_at_once():
     """Calls of every form, each on two streams that run together, and the same results as one after another."""
     calls = []
-    for rows, n, k in ((4, 700, 2048), (40, 700, 2048), (600, 704, 2048), (600, 700, 2016), (9, 700, 2016)):
+    for rows, n, k in ((4, 700, 2048), (40, 700, 2048), (600, 704, 2048), (600, 700, 2016), (9, 700, 2016), (600, 5000, 2048), (300, 6000, 2048)):
         a, sa, _ = operand(rows, k=k, seed=rows)
         w, sw, _ = operand(n, k=k, seed=rows + 1)
         calls.append(lambda a=a, w=w, sa=sa, sw=sw: flux_amd.MxGemm(BF16).forward(a, w, sa, sw))
