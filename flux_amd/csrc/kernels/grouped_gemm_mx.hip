@@ -7,10 +7,11 @@
 // Bound by the weights' bytes with few rows per expert, by the MFMAs and what feeds them with many.  Five kernels:
 //  * streams (mx_stream_kernel), where there is less work than the card has room for: a wave, or two or four that split K, has 16 or 32 rows and 32 or 64 columns of
 //    an expert and streams through LDS on its own;
-//  * panels of 64 or 128 rows and 128 columns (mx_panel_kernel);
+//  * panels of 64, 128 or 256 rows and 128 columns (mx_panel_kernel);
 //  * the dual tiles of 256 x 256 (grouped_gemm_dual.hip);
-//  * for K that is no multiple of 512, and whatever else those do not take, mx_few_rows_kernel, whose four waves split K in turns of 512 values and load straight into
-//    registers, and mx_tile_kernel.
+//  * for many rows and K that is no multiple of 512, or whatever else those do not take, mx_tile_kernel;
+//  * for few rows whose scales are not on whole words (K that is no multiple of 128), mx_few_rows_kernel, whose four waves split K in turns of 512 values and load
+//    straight into registers.  The others want a copy of such scales, of all experts.
 //
 // The tiles of this file: 256 x 256 on eight waves through a ring of four stages in LDS, a stage 128 values of K (64 bytes a row), filled by loads that write
 // LDS.  The waves of a SIMD take turns: while one computes a stage, the other reads its fragments and requests fills.  Scales come 16 bytes a row for four
@@ -414,20 +415,19 @@ __global__ __launch_bounds__(512, 2) void mx_panel_kernel(const MxParams p, int 
   if (t.rows <= 0) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)smem));
-  const int row_bytes = p.kb * 16, steps = p.kb / 8;
+  const int row_bytes = p.kb * 16, steps = (p.kb + 7) / 8;
   const bool of_a = wave < 4;  // whose fills this wave requests
   const uint8_t *const codes = of_a ? p.a : p.b + static_cast<int64_t>(t.e) * p.n * row_bytes;
-  const uint8_t *const scales = of_a ? p.a_scale : p.b_scale + static_cast<int64_t>(t.e) * p.n * p.kb;
+  const uint8_t *const scales = of_a ? p.a_scale : p.b_scale + static_cast<int64_t>(t.e) * p.n * p.scale_stride;
   const int64_t rows_of = of_a ? p.a_rows : p.n;
-  const auto cr = buffer_of(codes, rows_of * row_bytes), sr = buffer_of(scales, rows_of * p.kb);
+  const auto cr = buffer_of(codes, rows_of * row_bytes), sr = buffer_of(scales, rows_of * p.scale_stride);
   // ---- fills: rows of 128 bytes as in the streams; wave q of four has the fills q, q + 4 ... of 8 rows each.  (Of B: four of them.)
   uint32_t off[C::XF > C::WF ? C::XF : C::WF], soff = kNoRow;
   const int place = (lane & 7) ^ (lane >> 4);
-  const uint32_t chunk0 = ((place & 3) * 2 + (place >> 2)) * 16;
+  const uint32_t chunk = (((place & 3) * 2 + (place >> 2)) ^ (wn & 1)) * 16;  // (fill q * 4 + wn has the parity of wn)
 #pragma unroll
   for (int q = 0; q < (C::XF > C::WF ? C::XF : C::WF); ++q) {
-    const int R = (q * 4 + wn) * 8 + (lane >> 3);  // (fills of one wave: q * 4 + wn has the parity of wn)
-    const uint32_t chunk = chunk0 ^ ((wn & 1) * 16);
+    const int R = (q * 4 + wn) * 8 + (lane >> 3);
     if (of_a) {
       off[q] = R < t.rows ? static_cast<uint32_t>(a_row(p, t.row0 + R)) * row_bytes + chunk : kNoRow;
     } else {
@@ -439,22 +439,25 @@ __global__ __launch_bounds__(512, 2) void mx_panel_kernel(const MxParams p, int 
   {
     const int R = scale_fill * 64 + lane;
     if (of_a) {
-      if (R < t.rows) soff = static_cast<uint32_t>(a_row(p, t.row0 + R)) * p.kb;
+      if (R < t.rows) soff = static_cast<uint32_t>(a_row(p, t.row0 + R)) * p.scale_stride;
     } else {
       const int n = t.n0 + column_of(R);
-      if (n < p.n) soff = static_cast<uint32_t>(n) * p.kb;
+      if (n < p.n) soff = static_cast<uint32_t>(n) * p.scale_stride;
     }
   }
-  // Step s, into `slot`; steps past the last are zeros.  With the first step of a pair come the scales of both.
-  auto fill_x = [&](int s, int slot) {
-    if ((s & 1) == 0) fill(lds0 + C::kXs + ((s >> 1) & 1) * (C::BM * 16) + scale_fill * 1024, s < steps ? soff : kNoRow, sr, (s >> 1) * 16);
+  // Step s, into `slot`; blocks past the end of the rows are zero codes, and what lies there instead of their scales is masked when it is used.  With the first step of
+  // a pair come the scales of both.
+  auto fill_step = [&](int s, int slot) {
+    if ((s & 1) == 0)
+      fill(lds0 + (of_a ? C::kXs + ((s >> 1) & 1) * (C::BM * 16) : C::kWs + ((s >> 1) & 1) * (C::BN * 16)) + scale_fill * 1024, s < steps ? soff : kNoRow, sr, (s >> 1) * 16);
+    const bool in = s * 8 + static_cast<int>(chunk >> 4) < p.kb;
+    if (of_a) {
 #pragma unroll
-    for (int q = 0; q < C::XF; ++q) fill(lds0 + slot * (C::BM * 128) + (q * 4 + wn) * 1024, s < steps ? off[q] : kNoRow, cr, s * 128);
-  };
-  auto fill_w = [&](int s, int slot) {
-    if ((s & 1) == 0) fill(lds0 + C::kWs + ((s >> 1) & 1) * (C::BN * 16) + scale_fill * 1024, s < steps ? soff : kNoRow, sr, (s >> 1) * 16);
+      for (int q = 0; q < C::XF; ++q) fill(lds0 + slot * (C::BM * 128) + (q * 4 + wn) * 1024, in ? off[q] : kNoRow, cr, s * 128);
+    } else {
 #pragma unroll
-    for (int q = 0; q < C::WF; ++q) fill_once(lds0 + C::kW + slot * (C::BN * 128) + (q * 4 + wn) * 1024, s < steps ? off[q] : kNoRow, cr, s * 128);
+      for (int q = 0; q < C::WF; ++q) fill_once(lds0 + C::kW + slot * (C::BN * 128) + (q * 4 + wn) * 1024, in ? off[q] : kNoRow, cr, s * 128);
+    }
   };
   // ---- fragments: lane group g has chunks 2 g and 2 g + 1 of a line in two MFMAs, and bytes 2 g and 2 g + 1 of the line's 8 scales.
   typedef const __attribute__((address_space(3))) u32x4 *LdsFrag;
@@ -470,13 +473,15 @@ __global__ __launch_bounds__(512, 2) void mx_panel_kernel(const MxParams p, int 
     const uint32_t x_at = lds0 + slot * (C::BM * 128), w_at = lds0 + C::kW + slot * (C::BN * 128) + wn * 4096;
     const uint32_t xs_at = lds0 + C::kXs + ((s >> 1) & 1) * (C::BM * 16) + r * 16 + PAR * 8 + g * 2;
     const uint32_t ws_at = lds0 + C::kWs + ((s >> 1) & 1) * (C::BN * 16) + wn * 512 + r * 16 + PAR * 8 + g * 2;
+    const int first = s * 8 + 2 * g;  // this lane's two blocks
+    const uint32_t known = first + 1 < p.kb ? 0xffffu : first < p.kb ? 0xffu : 0u;
     u32x4 w[2][2];
     uint32_t ws[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       w[j][0] = *reinterpret_cast<LdsFrag>(w_at + in_rows0 + j * 2048);
       w[j][1] = *reinterpret_cast<LdsFrag>(w_at + in_rows1 + j * 2048);
-      ws[j] = *reinterpret_cast<LdsPair>(ws_at + j * 256);
+      ws[j] = *reinterpret_cast<LdsPair>(ws_at + j * 256) & known;
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -484,7 +489,7 @@ __global__ __launch_bounds__(512, 2) void mx_panel_kernel(const MxParams p, int 
 #pragma unroll
       for (int i = h * (MI / 2); i < (h + 1) * (MI / 2); ++i) {
         const u32x4 x0 = *reinterpret_cast<LdsFrag>(x_at + in_rows0 + block_row(i) * 128), x1 = *reinterpret_cast<LdsFrag>(x_at + in_rows1 + block_row(i) * 128);
-        const uint32_t xs = *reinterpret_cast<LdsPair>(xs_at + block_row(i) * 16);
+        const uint32_t xs = *reinterpret_cast<LdsPair>(xs_at + block_row(i) * 16) & known;
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc[i][j] = mfma<0>(w[j][0], x0, ws[j], xs, acc[i][j]);
 #pragma unroll
@@ -500,10 +505,6 @@ __global__ __launch_bounds__(512, 2) void mx_panel_kernel(const MxParams p, int 
   };
   // ---- the loop over K: after the barrier of step s its operands are there, and what step s - 1 had is free.  A wave requests step s + 2 then, and waits for step
   // s + 1 at the end, when the fills of step s + 2 may be on their way, with a pair's scales if s is even.
-  auto fill_step = [&](int s, int slot) {
-    if (of_a) fill_x(s, slot);
-    else fill_w(s, slot);
-  };
   fill_step(0, 0);
   fill_step(1, 1);
   if (of_a) FLUXMI_VMCNT(C::XF);
@@ -512,16 +513,21 @@ __global__ __launch_bounds__(512, 2) void mx_panel_kernel(const MxParams p, int 
   int slot = 0;
   auto step = [&](auto PARITY, int s) {
     constexpr int PAR = decltype(PARITY)::value;
-    fill_step(s + 2, slot == 0 ? 2 : slot - 1);
+    // (256 rows: a request stops its wave until the memory pipeline takes it, so they come after the wave's own work, 92 -> 86 us for 194 rows 4096 x 14336; fewer
+    // rows leave the pipeline room, and the earlier request is worth up to 4 %.)
+    const int next = slot == 0 ? 2 : slot - 1;
+    if constexpr (MI < 8) fill_step(s + 2, next);
     __builtin_amdgcn_sched_barrier(0);
     compute(PARITY, s, slot);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (MI >= 8) fill_step(s + 2, next);
     FLUXMI_LGKM0();
     if (of_a) FLUXMI_VMCNT(C::XF + 1 - PAR);
     else FLUXMI_VMCNT(C::WF + 1 - PAR);
     sync();
     slot = slot == 2 ? 0 : slot + 1;
   };
-  for (int s = 0; s < steps; s += 2) {
+  for (int s = 0; s < steps; s += 2) {  // (an odd last step has one of zeros behind it)
     step(std::integral_constant<int, 0>{}, s);
     step(std::integral_constant<int, 1>{}, s + 1);
   }
@@ -541,7 +547,7 @@ __global__ __launch_bounds__(512, 2) void mx_panel_kernel(const MxParams p, int 
 #endif  // __HIP_DEVICE_COMPILE__
 }
 
-// Scales in rows of a multiple of 16 bytes, zeros behind their end, as the tiles read them: A's rows, then those of all experts.
+// Scales in rows of a multiple of 16 bytes, zeros behind their end: A's rows, then those of all experts.
 __global__ __launch_bounds__(kThreads) void mx_pad_scales_kernel(const uint8_t *__restrict__ a, int64_t a_rows, const uint8_t *__restrict__ b, int64_t b_rows, int kb, int stride,
                                                                  uint8_t *__restrict__ out) {
   const int per_row = stride / 16;
@@ -578,10 +584,10 @@ __global__ __launch_bounds__(64 * P) void mx_stream_kernel(const MxParams p, int
   const Item it = locate(p, item, MT * 16);
   if (it.rows <= 0) return;
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)smem)) + wave * C::kWaveLds;
-  const int row_bytes = p.kb * 16, turns = p.kb / 16;
-  const auto xr = buffer_of(p.a, static_cast<int64_t>(p.a_rows) * row_bytes), xsr = buffer_of(p.a_scale, static_cast<int64_t>(p.a_rows) * p.kb);
+  const int row_bytes = p.kb * 16, turns = (p.kb + 15) / 16;
+  const auto xr = buffer_of(p.a, static_cast<int64_t>(p.a_rows) * row_bytes), xsr = buffer_of(p.a_scale, static_cast<int64_t>(p.a_rows) * p.scale_stride);
   const auto wr = buffer_of(p.b + static_cast<int64_t>(it.e) * p.n * row_bytes, static_cast<int64_t>(p.n) * row_bytes);
-  const auto wsr = buffer_of(p.b_scale + static_cast<int64_t>(it.e) * p.n * p.kb, static_cast<int64_t>(p.n) * p.kb);
+  const auto wsr = buffer_of(p.b_scale + static_cast<int64_t>(it.e) * p.n * p.scale_stride, static_cast<int64_t>(p.n) * p.scale_stride);
   // LDS row R of 128 bytes: its chunks of 16 bytes in the order 0, 2, 4, 6, 1, 3, 5, 7, the c-th of them at slot c ^ ((R >> 1) & 7); a fill covers 8 rows, lane l row
   // l >> 3 and slot l & 7.  (The 16 lanes that LDS serves together, of two lane groups, are so on banks of their own.)
   uint32_t xoff[2 * MT], woff[2 * NJ];
@@ -593,21 +599,31 @@ __global__ __launch_bounds__(64 * P) void mx_stream_kernel(const MxParams p, int
     woff[q] = n < p.n ? static_cast<uint32_t>(n) * row_bytes + (chunk0 ^ ((q & 1) * 16)) : kNoRow;
   }
   const int ns = n0 + column_of(lane);
-  const uint32_t wsoff = lane < NJ * 16 && ns < p.n ? static_cast<uint32_t>(ns) * p.kb : kNoRow;
+  const uint32_t wsoff = lane < NJ * 16 && ns < p.n ? static_cast<uint32_t>(ns) * p.scale_stride : kNoRow;
 #pragma unroll
   for (int q = 0; q < 2 * MT; ++q) {
     const int m = q * 8 + (lane >> 3);
     xoff[q] = m < it.rows ? static_cast<uint32_t>(a_row(p, it.row0 + m)) * row_bytes + (chunk0 ^ ((q & 1) * 16)) : kNoRow;
   }
-  const uint32_t xsoff = lane < it.rows ? static_cast<uint32_t>(a_row(p, it.row0 + lane)) * p.kb : kNoRow;  // (lanes past the rows' blocks: not read)
-  auto fill_turn = [&](int t, int slot) {
+  const uint32_t xsoff = lane < it.rows ? static_cast<uint32_t>(a_row(p, it.row0 + lane)) * p.scale_stride : kNoRow;  // (lanes past the rows' blocks: not read)
+  // Blocks past the end of the rows are zero codes; what lies there instead of their scales is masked when it is used.
+  auto fill_turn_of = [&](auto LAST, int t, int slot) {
+    constexpr bool kLast = decltype(LAST)::value;
     const uint32_t dst = lds0 + slot * C::kStage;
+    auto in_row = [&](uint32_t off, int q, int h) {
+      if constexpr (kLast) return t * 16 + h * 8 + static_cast<int>((chunk0 >> 4) ^ (q & 1)) < p.kb ? off : kNoRow;
+      else return off;
+    };
     fill_once(dst + C::kScales, wsoff, wsr, t * 16);
 #pragma unroll
-    for (int q = 0; q < 4 * NJ; ++q) fill_once(dst + q * 1024, woff[q % (2 * NJ)], wr, t * 256 + q / (2 * NJ) * 128);
+    for (int q = 0; q < 4 * NJ; ++q) fill_once(dst + q * 1024, in_row(woff[q % (2 * NJ)], q, q / (2 * NJ)), wr, t * 256 + q / (2 * NJ) * 128);
     fill(dst + C::kScales + 1024, xsoff, xsr, t * 16);
 #pragma unroll
-    for (int q = 0; q < 4 * MT; ++q) fill(dst + C::kX + q * 1024, xoff[q % (2 * MT)], xr, t * 256 + q / (2 * MT) * 128);
+    for (int q = 0; q < 4 * MT; ++q) fill(dst + C::kX + q * 1024, in_row(xoff[q % (2 * MT)], q, q / (2 * MT)), xr, t * 256 + q / (2 * MT) * 128);
+  };
+  auto fill_turn = [&](int t, int slot) {
+    if (t * 16 + 16 <= p.kb) fill_turn_of(std::false_type{}, t, slot);
+    else fill_turn_of(std::true_type{}, t, slot);
   };
   // Lane group g has chunks 2 g and 2 g + 1 of a line in two MFMAs, and their scales are bytes 2 g and 2 g + 1 of the line's 8.
   typedef const __attribute__((address_space(3))) u32x4 *LdsFrag;
@@ -626,7 +642,13 @@ __global__ __launch_bounds__(64 * P) void mx_stream_kernel(const MxParams p, int
     const uint32_t at = lds0 + slot * C::kStage;
     u32x4 w[NJ][4], x[MT][4];
     uint32_t ws[NJ], xs[MT];
-    auto scales_of = [&](uint32_t a) { return __builtin_amdgcn_perm(*reinterpret_cast<LdsWord>(a + 8), *reinterpret_cast<LdsWord>(a), pick); };
+    uint32_t known = ~0u;  // bytes of blocks that the rows have
+    if (t * 16 + 16 > p.kb) {
+      known = 0;
+#pragma unroll
+      for (int m = 0; m < 4; ++m) known |= t * 16 + (m >> 1) * 8 + 2 * g + (m & 1) < p.kb ? 0xffu << (8 * m) : 0u;
+    }
+    auto scales_of = [&](uint32_t a) { return __builtin_amdgcn_perm(*reinterpret_cast<LdsWord>(a + 8), *reinterpret_cast<LdsWord>(a), pick) & known; };
 #pragma unroll
     for (int j = 0; j < NJ; ++j) ws[j] = scales_of(at + in_scales + j * 256);
 #pragma unroll
@@ -862,9 +884,8 @@ GemmParams dual_params(const fluxmi_mx_gemm_args &a) {
 enum class Form { FEW_ROWS, STREAM, PANEL, DUAL, TILES };
 struct Plan {
   Form form;
-  int row_blocks, col_blocks, waves;  // STREAM: blocks of 16 rows and of 16 columns of an item, waves that split K
-  bool low;                           // PANEL: of 64 rows; TILES: of 128 rows
-  size_t workspace;
+  int row_blocks, col_blocks, waves;  // STREAM: blocks of 16 rows and of 16 columns of an item, waves that split K; PANEL: row blocks of 32
+  size_t workspace;                   // scales in rows of whole 16 bytes
 };
 
 // By the rows of an expert on average and by how many workgroups the card gets.  us, rows a fifth more and less on every other expert:
@@ -879,28 +900,31 @@ struct Plan {
 // The waves of a stream: one token of two experts 4096 x 14336 (256 streams) 16.3 / 13.0 / 13.4 of one, two and four that split K, with 896 (14336 x 4096) 13.8 / 15.7;
 // of 32 rows one expert 4096 x 4096, 128 rows (512 streams) 9.4 / 9.5 / 12.5, 1024 x 4096, 256 rows (256) 8.1 / 6.0 / 6.8, 128 rows (128) 8.0 / 5.9 / 5.6.  64 columns of
 // 32 rows: one expert 4096 x 14336, 256 rows (1024 streams) 46 -> 37, with fewer streams it is slower.
-// The dual tiles want K in multiples of 512 and N of 8 (fp32 results 4), streams and panels K only; where only N stands in the way, panels are taken up to 128 rows.  What
-// none takes goes to the first kernel up to 16 rows (9 rows: 58, tiles 61) and to the tiles of this file beyond (32 rows 2048 x 7168 of 32 experts: 81, tiles 57), of
-// 128 rows up to 128 on average (194 rows 4096 x 14336 of 8 experts 116 -> 96, 2048 rows 600 -> 750).
+// The dual tiles want K in multiples of 512 and N of 8 (fp32 results 4).  Without them: panels of 128 / of 256 rows / tiles of this file, 8 experts 4096 x 14208, 100 rows
+// 73 / 77 / 121, 150 rows 117 / 91 / 138, 194 rows 122 / 108 / 149, 300 rows 176 / 185 / 149; 14336 x 4224, 60 rows 89 / 101 / 83, 194 rows 160 / 149 / 111.  With them panels
+// of 256 rows would be as good at 194 rows 4096 x 14336 (86 / 91) and worse where some experts have more than 256 (4 experts of 176 and 264 rows 8192 x 4096 58 / 40).
 Plan plan_of(const fluxmi_mx_gemm_args &a, const GemmParams &dual, int cus) {
   const int64_t rows = a.max_rows, experts = a.nexperts, active = rows < experts ? rows : experts, kb = (int64_t{a.k} + 31) / 32;
   const int64_t each = (rows + active - 1) / active;  // rows of an expert on average
   auto pieces = [&](int64_t high, int64_t wide) { return active * ((each + high - 1) / high) * ((a.n + wide - 1) / wide); };
-  const bool dual_takes = dual_takes_mx(dual), aligned = kb % 16 == 0 && aligned16(a.a_scale) && aligned16(a.b_scale);
-  if (aligned) {
-    const int64_t low_panels = pieces(64, 128);
-    if (low_panels < (each <= 10 ? 240 : 160)) {
-      const bool two = each > 10;
-      const int64_t streams = pieces(two ? 32 : 16, 32);
-      const bool wide = two && streams >= 1024;
-      return {Form::STREAM, two ? 2 : 1, wide ? 4 : 2, streams >= (two ? 512 : 768) ? 1 : streams >= 192 ? 2 : 4, false, 0};
-    }
-    if (each <= 48 || low_panels <= cus) return {Form::PANEL, 0, 0, 0, true, 0};
-    if (pieces(128, 128) <= cus || (!dual_takes && each <= 128)) return {Form::PANEL, 0, 0, 0, false, 0};
+  const bool dual_takes = dual_takes_mx(dual);
+  auto scales_on = [&](int64_t bytes) {
+    return kb % bytes == 0 && (reinterpret_cast<uintptr_t>(a.a_scale) | reinterpret_cast<uintptr_t>(a.b_scale)) % static_cast<uintptr_t>(bytes) == 0;
+  };
+  const size_t padded = static_cast<size_t>(a.a_rows + experts * a.n) * ((kb + 15) / 16 * 16), unless_words = scales_on(4) ? 0 : padded;
+  if (!scales_on(4) && rows <= 16 * experts) return {Form::FEW_ROWS, 0, 0, 0, 0};
+  const int64_t low_panels = pieces(64, 128);
+  if (low_panels < (each <= 10 ? 240 : 160)) {
+    const bool two = each > 10;
+    const int64_t streams = pieces(two ? 32 : 16, 32);
+    const bool wide = two && streams >= 1024;
+    return {Form::STREAM, two ? 2 : 1, wide ? 4 : 2, streams >= (two ? 512 : 768) ? 1 : streams >= 192 ? 2 : 4, unless_words};
   }
-  if (dual_takes) return {Form::DUAL, 0, 0, 0, false, 0};
-  if (rows <= 16 * experts) return {Form::FEW_ROWS, 0, 0, 0, false, 0};
-  return {Form::TILES, 0, 0, 0, rows <= 128 * experts, aligned ? 0 : static_cast<size_t>(a.a_rows + experts * a.n) * ((kb + 15) / 16 * 16)};
+  if (each <= 48 || low_panels <= cus) return {Form::PANEL, 2, 0, 0, unless_words};
+  if (pieces(128, 128) <= cus) return {Form::PANEL, 4, 0, 0, unless_words};
+  if (!dual_takes && pieces(256, 128) <= cus) return {Form::PANEL, 8, 0, 0, unless_words};
+  if (dual_takes) return {Form::DUAL, 0, 0, 0, 0};
+  return {Form::TILES, 0, 0, 0, scales_on(16) ? 0 : padded};
 }
 
 }  // namespace
@@ -936,6 +960,15 @@ extern "C" int fluxmi_grouped_gemm_mx(const fluxmi_mx_gemm_args *args, void *wor
   p.a_rows = args->a_rows;
   p.scale_stride = p.kb;
   p.d_type = args->d_type == FLUXMI_ROWS_BF16 ? Row::BF16 : args->d_type == FLUXMI_ROWS_FP32 ? Row::F32 : Row::F16;
+  if (plan.workspace > 0) {
+    p.scale_stride = (p.kb + 15) / 16 * 16;
+    const int64_t a_rows = p.a_rows, b_rows = int64_t{p.nexperts} * p.n, groups = (a_rows + b_rows) * (p.scale_stride / 16);
+    const unsigned grid = static_cast<unsigned>(groups / kThreads < 8192 ? groups / kThreads + 1 : 8192);
+    uint8_t *const padded = static_cast<uint8_t *>(workspace);
+    hipLaunchKernelGGL(mx_pad_scales_kernel, dim3(grid), dim3(kThreads), 0, s, p.a_scale, a_rows, p.b_scale, b_rows, p.kb, p.scale_stride, padded);
+    p.a_scale = padded;
+    p.b_scale = padded + a_rows * p.scale_stride;
+  }
   switch (plan.form) {
     case Form::STREAM:
       if (plan.col_blocks == 4) rc = launch_stream<2, 4, 1>(p, s);
@@ -943,7 +976,7 @@ extern "C" int fluxmi_grouped_gemm_mx(const fluxmi_mx_gemm_args *args, void *wor
       else rc = plan.waves == 1 ? launch_stream<1, 2, 1>(p, s) : plan.waves == 2 ? launch_stream<1, 2, 2>(p, s) : launch_stream<1, 2, 4>(p, s);
       break;
     case Form::PANEL:
-      rc = plan.low ? launch_panel<2>(p, s) : launch_panel<4>(p, s);
+      rc = plan.row_blocks == 2 ? launch_panel<2>(p, s) : plan.row_blocks == 4 ? launch_panel<4>(p, s) : launch_panel<8>(p, s);
       break;
     case Form::DUAL: {
       // Up to four workgroups to a tile, which is cut in pieces when these still fit the card.
@@ -955,16 +988,7 @@ extern "C" int fluxmi_grouped_gemm_mx(const fluxmi_mx_gemm_args *args, void *wor
       rc = launch_few_rows(p, s);
       break;
     case Form::TILES:
-      if (plan.workspace > 0) {
-        p.scale_stride = (p.kb + 15) / 16 * 16;
-        const int64_t a_rows = p.a_rows, b_rows = int64_t{p.nexperts} * p.n, groups = (a_rows + b_rows) * (p.scale_stride / 16);
-        const unsigned grid = static_cast<unsigned>(groups / kThreads < 8192 ? groups / kThreads + 1 : 8192);
-        uint8_t *const padded = static_cast<uint8_t *>(workspace);
-        hipLaunchKernelGGL(mx_pad_scales_kernel, dim3(grid), dim3(kThreads), 0, s, p.a_scale, a_rows, p.b_scale, b_rows, p.kb, p.scale_stride, padded);
-        p.a_scale = padded;
-        p.b_scale = padded + a_rows * p.scale_stride;
-      }
-      rc = plan.low ? launch_tiles<4, 4, 2, 4>(p, s) : launch_tiles<8, 4, 2, 4>(p, s);
+      rc = launch_tiles<8, 4, 2, 4>(p, s);
       break;
   }
   if (rc != FLUXMI_OK) return rc;

@@ -247,6 +247,33 @@ def test_panels(splits, n, k):
         grouped(splits, n, k, out)
 
 
+@pytest.mark.parametrize("k", [32, 384, 1408, 2816, 2880, 705])
+@pytest.mark.parametrize("splits,n", [([1, 1], 500), ([30, 17], 500), ([3] * 20, 1600), ([16, 31, 33, 64, 65, 0] * 5, 1100), ([100, 129, 60, 200] * 4, 2001), ([700, 20], 512),
+                                      ([256, 150, 257, 16, 200, 180, 255, 129] * 2, 1601), ([600, 0, 33, 256, 257], 5000), ([3000], 1301)], ids=brief)
+def test_rows_that_end_inside_a_line(splits, n, k):
+    """Every form with K that is a multiple of 128 (scales on whole words) and not."""
+    for out in (BF16, F32):
+        print(f"[case] ends {splits} {n} {k} {out}", flush=True)
+        grouped(splits, n, k, out)
+
+
+@pytest.mark.parametrize("experts,rows,n", [(2, 3, 300), (2, 20, 300), (12, 9, 2600), (16, 100, 2000), (3, 600, 520), (16, 200, 1601), (4, 300, 5000)])
+@pytest.mark.parametrize("k", [384, 640, 736])
+def test_nan_blocks_beside_the_ends_of_rows(experts, rows, n, k):
+    """What lies behind a row's last scale is the next row's first: a NaN block there stays there."""
+    a, sa, va = operand(experts * rows, k=k, seed=1)
+    w, sw, vw = operand(experts, n, k=k, seed=2)
+    sa.view(torch.uint8)[1::2, 0] = 255
+    sw.view(torch.uint8)[:, 1::2, 0] = 255
+    got = flux_amd.MxGemm(F32).forward_grouped(a, torch.full((experts,), rows, dtype=torch.int32, device=DEV), w, sa, sw)
+    row, col = torch.arange(experts * rows, device=DEV) % 2 == 1, torch.arange(n, device=DEV) % 2 == 1
+    assert torch.equal(got.isnan(), row[:, None] | col[None])
+    for e in range(experts):
+        mine = torch.arange(e * rows, (e + 1) * rows, device=DEV)
+        mine = mine[mine % 2 == 0]
+        check(got[mine][:, ::2], va[mine], vw[e][::2], k)
+
+
 # Tiles of 256 x 256: rows that end in each of a tile's four units of 64, experts without rows, columns that end in each half and quarter of a tile; as many as an
 # expert table holds and one more; results whose rows are and are not whole stores.
 @pytest.mark.parametrize("out", [BF16, F16, F32])
