@@ -8,7 +8,7 @@
 // and scales at both ends of the range among them).  The maximum is taken over the patterns without sign, where infinities and NaN are largest.
 //
 // Bound by HBM: a value is read once and becomes 17 / 32 bytes.  Along the rows a lane converts one vector of 16 bytes and the four lanes (fp32: eight)
-// of a block join their maxima; rows whose length is a multiple of 32 are one flat array.  With the transposed copy a lane holds 32 rows of one vector's
+// of a block join their maxima; rows whose length is a multiple of 32 are one flat array.  With the transposed copy of many values a lane holds 32 rows of one vector's
 // columns in registers, which gives both directions from one read with no exchange but that of the maxima along the rows; eight lanes side by side and
 // eight row blocks below each other make a wave, so that its loads and its transposed stores are whole 128-byte lines.
 // Measured at 11000 x 7168 bf16: both directions 57 us (4.2 TB/s; without the stores of the row codes 47, without the transposed ones 45: two sets of
@@ -132,10 +132,13 @@ __device__ __forceinline__ void store_codes(uint8_t *to, uint32_t c) {
   else *reinterpret_cast<uint32_t *>(to) = c;
 }
 
+// One vector of the kShare of a block, in neighbouring lanes, all of which come here.
 template <Row T>
-__device__ __forceinline__ void quantise_vector(const u32x4 v, uint8_t *codes, uint8_t *scale, bool first_lane) {
+__device__ __forceinline__ void quantise_vector(const u32x4 v, uint8_t *codes, uint8_t *scale, bool first_lane, bool stores = true) {
   const uint32_t byte = scale_byte<T>(max_of_lanes<kShare<T>>(join_halves<T>(vector_max<T>(v))));
-  store_codes<T>(codes, byte == 255 ? 0u : convert_vector<T>(v, scale_value(byte)));
+  const uint32_t c = byte == 255 ? 0u : convert_vector<T>(v, scale_value(byte));
+  if (!stores) return;
+  store_codes<T>(codes, c);
   if (first_lane) *scale = static_cast<uint8_t>(byte);
 }
 
@@ -170,6 +173,36 @@ __global__ __launch_bounds__(kThreads) void quant_rows_kernel(const uint8_t *__r
 }
 
 // ---- along the rows and along the columns -----------------------------------------------------------------------------
+
+// One matrix of the batch, few values: a workgroup has 32 rows of 8 vectors, one to a thread, and reads them again from LDS by columns.  Its transposed stores are 16
+// bytes from each column.
+template <Row T>
+__global__ __launch_bounds__(kThreads) void quant_tile_kernel(const uint8_t *__restrict__ x, int rows, int cols, int col_tiles, uint8_t *__restrict__ codes,
+                                                              uint8_t *__restrict__ scale, uint8_t *__restrict__ codes_t, uint8_t *__restrict__ scale_t) {
+  constexpr int V = kVec<T>, kPitch = 8 * 16 + 16;
+  __shared__ __attribute__((aligned(16))) uint8_t tile[kBlock * kPitch];
+  const int rt = blockIdx.x / col_tiles, ct = blockIdx.x - rt * col_tiles, kb = (cols + kBlock - 1) / kBlock, rb = (rows + kBlock - 1) / kBlock;
+  const size_t matrix = static_cast<size_t>(blockIdx.y);
+  {
+    const int r = threadIdx.x >> 3, row = rt * kBlock + r, col = (ct * 8 + (threadIdx.x & 7)) * V;
+    const size_t in_batch = matrix * rows + row, block = in_batch * kb + col / kBlock;
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (row < rows && col < cols) v = load_vector<T, false>(x + (in_batch * cols + col) * kElt<T>, cols - col);
+    *reinterpret_cast<u32x4 *>(tile + r * kPitch + (threadIdx.x & 7) * 16) = v;
+    quantise_vector<T>(v, codes + block * 16 + col % kBlock / 2, scale + block, col % kBlock == 0, row < rows && col < kb * kBlock);
+  }
+  __syncthreads();
+  const int c = threadIdx.x / kShare<T>, part = threadIdx.x % kShare<T>, col = ct * 8 * V + c;
+  const uint8_t *const from = tile + part * V * kPitch + c * kElt<T>;
+  u32x4 v = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if constexpr (T == Row::F32) v[i] = *reinterpret_cast<const uint32_t *>(from + i * kPitch);
+    else v[i / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(from + i * kPitch)) << (16 * (i & 1));
+  }
+  const size_t block = (matrix * cols + col) * rb + rt;
+  quantise_vector<T>(v, codes_t + block * 16 + part * (V / 2), scale_t + block, part == 0, col < cols);
+}
 
 // One matrix of the batch.  A wave covers 8 vectors of columns x 8 blocks of 32 rows, a workgroup 4 waves side by side.
 template <Row T, bool NT>
@@ -356,6 +389,14 @@ constexpr size_t kManyVectors = size_t{1} << 19;
 // along the rows 14 and 16, 24 and 22, 59 and 53; back 15 and 13, 26 and 20, 60 and 49.  fp32 is alike.
 constexpr size_t kStreamBytes = size_t{96} << 20;
 
+// Up to so many values both directions go through LDS: many small workgroups, none of which waits for 32 loads of each lane.  Measured (us, in registers / through
+// LDS): bf16 300 x 2048 9.8 / 2.7, 2800 x 4096 12.9 / 10.3, 4096 x 4096 14.9 / 13.2, 8192 x 4096 26 / 37; fp32 9.2 / 2.8, 17.4 / 14.1, 20.6 / 20.9, 43 / 43.  Rows
+// that start inside lines: bf16 1024 x 7000 11.1 / 10.9, 4096 x 2800 12.8 / 13.0, 4100 x 5000 19 / 31; fp32 12.7 / 15.5, 17.2 / 17.0, 36 / 48.
+template <Row T>
+int64_t tile_values(int64_t cols) {
+  return int64_t{1} << (cols * kElt<T> % 128 == 0 ? 24 : 22);
+}
+
 int check_sizes(const char *who, int64_t rows, int64_t cols) {
   FLUXMI_REQUIRE(rows >= 0 && cols >= 0, FLUXMI_ERR_INVALID_ARG, "%s: negative size (rows=%lld, cols=%lld)", who, static_cast<long long>(rows),
                  static_cast<long long>(cols));
@@ -391,6 +432,17 @@ extern "C" int fluxmi_quant_mx(const void *x, int32_t row_type, int64_t batch, i
     constexpr Row T = decltype(t)::value;
     constexpr bool NT = decltype(nt)::value;
     if (codes_t != nullptr) {
+      if constexpr (!NT) {
+        if (batch * rows * cols <= tile_values<T>(cols)) {
+          const int64_t row_tiles = (rows + kBlock - 1) / kBlock, col_tiles = (cols + 8 * kVec<T> - 1) / (8 * kVec<T>);
+          fits = grid_of(row_tiles * col_tiles, 1, &grid);
+          if (!fits) return;
+          grid.y = static_cast<unsigned>(batch);
+          hipLaunchKernelGGL(quant_tile_kernel<T>, grid, dim3(kThreads), 0, s, in, static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(col_tiles), q, sc,
+                             static_cast<uint8_t *>(codes_t), static_cast<uint8_t *>(scale_t));
+          return;
+        }
+      }
       const int64_t row_tiles = (rows + 8 * kBlock - 1) / (8 * kBlock), col_tiles = (cols + 32 * kVec<T> - 1) / (32 * kVec<T>);
       fits = grid_of((row_tiles * col_tiles + 7) / 8 * 8, 1, &grid) && row_tiles * col_tiles < (int64_t{1} << 23);
       if (!fits) return;

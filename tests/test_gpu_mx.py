@@ -41,7 +41,7 @@ def hard_values(rows, cols, dtype, seed):
     return torch.from_numpy(x).clamp(-info.max, info.max).where(torch.from_numpy(~bad), torch.from_numpy(x)).to(dtype)
 
 
-SHAPES = [(1, 32), (1, 1), (3, 31), (7, 33), (128, 7168), (50, 2048), (33, 1000), (257, 96), (300, 130), (2, 16384), (1000, 64), (515, 2056)]
+SHAPES = [(1, 32), (1, 1), (3, 31), (7, 33), (128, 7168), (50, 2048), (33, 1000), (257, 96), (300, 130), (2, 16384), (1000, 64), (515, 2056), (2100, 2050), (1030, 4112), (4100, 4160)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
@@ -104,6 +104,14 @@ def test_batch_of_matrices(dtype):
         if transposed:
             want = mx.quantise(x.double().numpy().transpose(0, 2, 1))
             assert codes_t.shape == (5, 100, 48) and np.array_equal(bytes_of(codes_t), want[0]) and np.array_equal(bytes_of(scale_t), want[1])
+
+
+def test_batch_of_large_matrices():
+    x = torch.randn(3, 1211, 1250, device=DEV, generator=torch.Generator(DEV).manual_seed(1)).to(BF16)
+    whole = quantiser(BF16).quantize_mx(x, True)
+    for i in range(3):
+        for a, b in zip(whole, quantiser(BF16).quantize_mx(x[i], True)):
+            assert torch.equal(a[i].view(torch.uint8), b.view(torch.uint8))
 
 
 def test_dequantise_every_code_and_scale():
