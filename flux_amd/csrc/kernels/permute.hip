@@ -298,6 +298,20 @@ int clearer_count(int npairs) {
   return by_rows > wide ? by_rows : wide;
 }
 
+// Very many very short rows: what the clearing workgroups read, four bytes a pair for every kRowsOfClearer rows, would be more than the rows themselves.  They are all cleared
+// before the launch then.
+bool clear_first(int npairs, int64_t row_bytes) { return int64_t{npairs} * 4 / kRowsOfClearer > row_bytes; }
+
+__global__ __launch_bounds__(kThreads) void clear_kernel(uint8_t *__restrict__ rows, size_t bytes) {
+  const size_t step = static_cast<size_t>(gridDim.x) * kThreads, at = static_cast<size_t>(blockIdx.x) * kThreads + threadIdx.x;
+  for (size_t v = at; v < bytes / 16; v += step) store16(rows + v * 16, u32x4{0u, 0u, 0u, 0u});
+  if (at < bytes % 16) rows[bytes / 16 * 16 + at] = 0;
+}
+
+void clear_all(int npairs, int64_t row_bytes, void *rows, hipStream_t s) {
+  hipLaunchKernelGGL(clear_kernel, dim3(2048), dim3(kThreads), 0, s, static_cast<uint8_t *>(rows), static_cast<size_t>(npairs) * row_bytes);
+}
+
 // Workgroups of a launch, 0: more threads than a launch has.
 unsigned grid_of(int ntokens, int shift, int clearers) {
   const int64_t grid = clearers + (int64_t{ntokens} + (kThreads >> shift) - 1) / (kThreads >> shift);
@@ -343,9 +357,10 @@ extern "C" int fluxmi_moe_permute(const void *in, const int32_t *scatter_index, 
                  static_cast<long long>(row_bytes));
   if (ntokens == 0 || row_bytes == 0) return FLUXMI_OK;
   FLUXMI_REQUIRE(in != nullptr && rows != nullptr, FLUXMI_ERR_INVALID_ARG, "moe_permute: null pointer argument");
-  const int shift = lanes_shift(row_bytes / 16, ntokens, 4), clearers = clearer_count(ntokens * topk);
+  const int shift = lanes_shift(row_bytes / 16, ntokens, 4), clearers = clear_first(ntokens * topk, row_bytes) ? 0 : clearer_count(ntokens * topk);
   const unsigned grid = grid_of(ntokens, shift, clearers);
   FLUXMI_REQUIRE(grid > 0, FLUXMI_ERR_UNSUPPORTED, "moe_permute: ntokens=%d is too many for rows of %lld bytes", ntokens, static_cast<long long>(row_bytes));
+  if (clearers == 0) clear_all(ntokens * topk, row_bytes, rows, static_cast<hipStream_t>(stream));
   by_lanes(shift, static_cast<size_t>(row_bytes) * ntokens * topk, [&](auto sub, auto nt) {
     hipLaunchKernelGGL((permute_kernel<decltype(sub)::value, decltype(nt)::value>), dim3(grid), dim3(kThreads), 0, static_cast<hipStream_t>(stream),
                        static_cast<const uint8_t *>(in), scatter_index, ntokens, topk, static_cast<size_t>(row_bytes), shift, clearers,
@@ -402,9 +417,12 @@ extern "C" int fluxmi_moe_unpermute_backward(const void *grad_out, const void *r
   FLUXMI_REQUIRE(aligned_to(rows, type) && aligned_to(grad_out, type) && aligned_to(grad_rows, type) && aligned_to(weights, wtype) &&
                      aligned_to(grad_weights, wtype),
                  FLUXMI_ERR_INVALID_ARG, "moe_unpermute_backward: a pointer is not aligned to its elements");
-  const int shift = lanes_shift(n / (type == Row::F32 ? 4 : 8), ntokens, 4), clearers = grad_rows != nullptr && n > 0 ? clearer_count(ntokens * topk) : 0;
+  const int64_t row_bytes = int64_t{n} * (type == Row::F32 ? 4 : 2);
+  const bool clears = grad_rows != nullptr && n > 0;
+  const int shift = lanes_shift(n / (type == Row::F32 ? 4 : 8), ntokens, 4), clearers = clears && !clear_first(ntokens * topk, row_bytes) ? clearer_count(ntokens * topk) : 0;
   const unsigned grid = grid_of(ntokens, shift, clearers);
   FLUXMI_REQUIRE(grid > 0, FLUXMI_ERR_UNSUPPORTED, "moe_unpermute_backward: ntokens=%d is too many for n=%d", ntokens, n);
+  if (clears && clearers == 0) clear_all(ntokens * topk, row_bytes, grad_rows, static_cast<hipStream_t>(stream));
   by_type(type, [&](auto t) {
     by_topk(topk, [&](auto j) {
       by_lanes(shift, static_cast<size_t>(n) * kElt<decltype(t)::value> * ntokens * topk, [&](auto sub, auto nt) {

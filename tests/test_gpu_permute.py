@@ -184,6 +184,21 @@ def test_offsets_past_32_bits():
     assert ((grad_w[probe, 5].double() - square).abs() <= (n / 8 + 16) * 2.0**-24 * square).all()
 
 
+@pytest.mark.parametrize("dtype,n", [(BF16, 1), (F32, 1), (BF16, 3)])
+def test_very_many_short_rows(dtype, n):
+    """Four bytes a pair for every 65536 rows are more than a row: all rows are cleared before the launch."""
+    tokens, topk = 90001, 4
+    idx = make_index(tokens, topk, 0.3, 1)
+    x = torch.arange(1, tokens * n + 1, device=DEV).remainder(251).add(1).to(dtype).view(tokens, n)
+    want = torch.zeros(tokens * topk, n, dtype=dtype, device=DEV)
+    live = idx >= 0
+    want[idx[live].long()] = x.repeat_interleave(topk, 0).view(tokens, topk, n)[live]
+    assert torch.equal(flux_amd.moe_permute(x, idx), want)
+    grad_rows, grad_w = flux_amd.moe_unpermute_backward(x, want, idx, torch.full((tokens, topk), 2.0, device=DEV))
+    assert torch.equal(grad_rows, want * 2)
+    assert torch.equal(grad_w, (x.float() ** 2).sum(1, keepdim=True) * live)
+
+
 # ---- gradients through autograd ------------------------------------------------------------------------------------
 
 
