@@ -24,7 +24,7 @@
 // these read half as much again from LDS per MFMA (dense fp8 8192 x 8192 x 8192: 736 k cycles against 771 k, at 1.73 GHz against 1.95;
 // bf16 8 experts 4096 x 14336, 2048 rows each 1361 -> 1540).
 //
-// MXFP4 (K in multiples of 512): 8 experts of 2048 rows 14336 x 4096 556 us, 4096 x 14336 515 (3.5 and 3.7 PFLOP/s); dense 8192 x 8192 x 8192 269 (4.1);
+// MXFP4 (K beyond 512; a step is 256 values, steps come in pairs): 8 experts of 2048 rows 14336 x 4096 556 us, 4096 x 14336 515 (3.5 and 3.7 PFLOP/s); dense 8192 x 8192 x 8192 269 (4.1);
 // the tiles of grouped_gemm_mx.hip, of half a line of K, 650, 600 and 311.  Fills bound it, and the power limit: without the MFMAs 460, 414 and 212 us, with
 // operands of zeros, which draw less, 490, 441 and 226.  The scales' fills, 16 bytes from a line of each row, are 33 us of the first two and 2 of the last.
 // Kept: scales read once in two steps; the last two steps of a tile apart, so that the others choose no source (2 %); chunks off each other's banks
@@ -189,7 +189,8 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
   constexpr int ELT = is_fp8(T) ? 1 : 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 2, wn = wave & 3;
-  const int kbytes = MX ? p.k / 2 : p.k * ELT, steps = kbytes >> 7;
+  const int kbytes = MX ? p.k / 2 : p.k * ELT;
+  const int steps = MX ? (kbytes + 255) / 256 * 2 : kbytes >> 7;  // (MXFP4: whole pairs; the scales of what the last one has past the end are masked)
   const int tiles_n1 = (p.n + kTile - 1) / kTile, tiles_n = tiles_n1 * p.ngroups;
   const int grid = gridDim.x, bid = blockIdx.x;
   const int virt = (grid & 7) == 0 ? (bid & 7) * (grid >> 3) + (bid >> 3) : bid;
@@ -376,7 +377,7 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
       const int rs = wn * 64 + l;
       int row = t.row0 + rs;
       if (gathered) row = static_cast<int>(nxts) < 0 ? 0 : (static_cast<int>(nxts) >= a_rows ? a_rows - 1 : static_cast<int>(nxts));
-      nxts = rs < t.rows ? static_cast<uint32_t>(row) * (kbytes / 16) : kNoRow;
+      nxts = rs < t.rows ? static_cast<uint32_t>(row) * mx_scale_row(kbytes / 16) : kNoRow;
     }
   };
   __amdgpu_buffer_rsrc_t xrsrc, wrsrc;
@@ -432,16 +433,16 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
   auto start_scales = [&](const DualTile &t) {
     const KernArgs a = kernel_args();
     if constexpr (MX) {
-      const int kb = kbytes / 16, n = a->n;
+      const int scale_row = mx_scale_row(kbytes / 16), n = a->n;
       const uint8_t *const base = wm == 0 ? reinterpret_cast<const uint8_t *>(a->a_scale)
-                                          : reinterpret_cast<const uint8_t *>(a->b_scale) + static_cast<int64_t>(t.e) * n * kb;
-      srsrc = buffer_of(base, static_cast<int64_t>(wm == 0 ? a->a_rows : n) * kb);
+                                          : reinterpret_cast<const uint8_t *>(a->b_scale) + static_cast<int64_t>(t.e) * n * scale_row;
+      srsrc = buffer_of(base, static_cast<int64_t>(wm == 0 ? a->a_rows : n) * scale_row);
       soff = nxts;
       if (wm != 0) {  // the column of LDS row R of the step's W units
         const int R = wn * 64 + fresh_lane(), in_half = R & 127, q = in_half & 31;
         const int col = f32_out ? q : ((q >> 2) & 1) * 8 + (q & 3) + ((q >> 3) & 1) * 16 + (q >> 4) * 4;
         const int first = t.wide ? (in_half >> 5) * 64 + (R >> 7) * 32 : (in_half >> 5) * 32, c = t.n0 + first + col;
-        soff = t.rows > 0 && c < n && (t.wide || R < 128) ? static_cast<uint32_t>(c) * kb : kNoRow;
+        soff = t.rows > 0 && c < n && (t.wide || R < 128) ? static_cast<uint32_t>(c) * scale_row : kNoRow;
       }
       return;
     }
@@ -500,6 +501,19 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
     for (int j = 0; j < 4; ++j) ws[j] = __builtin_amdgcn_perm(raw[j][1], raw[j][0], pick);
 #pragma unroll
     for (int i = 0; i < 8; ++i) xs[i] = __builtin_amdgcn_perm(raw[4 + i][1], raw[4 + i][0], pick);
+  };
+  // Blocks past the end of K, in a tile's last pair of steps: what was read as their codes is the next row's, finite in any case, and with a scale of 2^-127 in both
+  // operands less than half of the smallest sum.
+  auto mask_mx_scales = [&](int s) {
+    const int kb = kbytes / 16;
+    if (kb % 16 == 0) return;
+    uint32_t known = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) known |= s * 8 + (b >> 1) * 8 + 2 * (lane >> 4) + (b & 1) < kb ? 0xffu << (8 * b) : 0u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ws[j] &= known;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) xs[i] &= known;
   };
   // (An opaque address: the distance of the blocks goes into the instructions.)
   auto address = [&](uint32_t at, uint32_t slot) {
@@ -649,6 +663,7 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
         read_x(slot_of(base));
         __builtin_amdgcn_sched_barrier(0);
         pick_mx_scales(raw);
+        if constexpr (ENDS) mask_mx_scales(s);
         __builtin_amdgcn_sched_barrier(0);
       } else {
         read_x(slot_of(base));
@@ -834,10 +849,11 @@ bool dual_takes(const GemmParams &p, int dtype) {
   return aligned;
 }
 
-// Whole pairs of steps of K, two at least, scale rows on 16 bytes, offsets below kNoRow; results in stores of 16 bytes.
+// Two pairs of steps of K at least, scales on whole words, offsets below kNoRow; results in stores of 16 bytes.
 bool dual_takes_mx(const GemmParams &p) {
   const int64_t kbytes = p.k / 2, span = 0x70000000ll;
-  if (p.k % 512 != 0 || p.k < 1024 || p.nexperts > kDualExperts || !aligned16(p.a) || !aligned16(p.b[0]) || !aligned16(p.a_scale) || !aligned16(p.b_scale)) return false;
+  const uintptr_t scales = reinterpret_cast<uintptr_t>(p.a_scale) | reinterpret_cast<uintptr_t>(p.b_scale);
+  if (p.k <= 512 || p.nexperts > kDualExperts || !aligned16(p.a) || !aligned16(p.b[0]) || (p.k % 128 == 0 && scales % 4 != 0)) return false;
   if (kTile * kbytes > span || p.n * kbytes > span || p.a_rows * kbytes > span) return false;
   return aligned16(p.d[0]) && p.n % (p.d_fp32 ? 4 : 8) == 0;
 }

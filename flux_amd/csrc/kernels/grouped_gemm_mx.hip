@@ -9,7 +9,7 @@
 //    an expert and streams through LDS on its own;
 //  * panels of 64, 128 or 256 rows and 128 columns (mx_panel_kernel);
 //  * the dual tiles of 256 x 256 (grouped_gemm_dual.hip);
-//  * for many rows and K that is no multiple of 512, or whatever else those do not take, mx_tile_kernel;
+//  * for many rows and what those do not take (N that is no multiple of 8, K up to 512, more than 128 experts), mx_tile_kernel;
 //  * for few rows whose scales are not on whole words (K that is no multiple of 128), mx_few_rows_kernel, whose four waves split K in turns of 512 values and load
 //    straight into registers.  The others want a copy of such scales, of all experts.
 //
@@ -900,9 +900,10 @@ struct Plan {
 // The waves of a stream: one token of two experts 4096 x 14336 (256 streams) 16.3 / 13.0 / 13.4 of one, two and four that split K, with 896 (14336 x 4096) 13.8 / 15.7;
 // of 32 rows one expert 4096 x 4096, 128 rows (512 streams) 9.4 / 9.5 / 12.5, 1024 x 4096, 256 rows (256) 8.1 / 6.0 / 6.8, 128 rows (128) 8.0 / 5.9 / 5.6.  64 columns of
 // 32 rows: one expert 4096 x 14336, 256 rows (1024 streams) 46 -> 37, with fewer streams it is slower.
-// The dual tiles want K in multiples of 512 and N of 8 (fp32 results 4).  Without them: panels of 128 / of 256 rows / tiles of this file, 8 experts 4096 x 14208, 100 rows
-// 73 / 77 / 121, 150 rows 117 / 91 / 138, 194 rows 122 / 108 / 149, 300 rows 176 / 185 / 149; 14336 x 4224, 60 rows 89 / 101 / 83, 194 rows 160 / 149 / 111.  With them panels
-// of 256 rows would be as good at 194 rows 4096 x 14336 (86 / 91) and worse where some experts have more than 256 (4 experts of 176 and 264 rows 8192 x 4096 58 / 40).
+// The dual tiles want K beyond 512 and N in multiples of 8 (fp32 results 4).  Without them: panels of 128 / of 256 rows / tiles of this file (dual tiles in brackets), 8
+// experts 4096 x 14208, 100 rows 73 / 75 / 120 (85), 194 rows 122 / 106 / 149 (101), 300 rows 176 / 187 / 148 (131), 1200 rows 586 / 513 / 400 (330); 14336 x 4224, 60 rows
+// 88 / 98 / 83 (85), 194 rows 159 / 145 / 110 (102), 1200 rows 750 / 650 / 431 (379).  Beside the dual tiles panels of 256 rows would be as good at 194 rows 4096 x 14336
+// (86 / 91) and worse where some experts have more than 256 (4 experts of 176 and 264 rows 8192 x 4096 58 / 40).
 Plan plan_of(const fluxmi_mx_gemm_args &a, const GemmParams &dual, int cus) {
   const int64_t rows = a.max_rows, experts = a.nexperts, active = rows < experts ? rows : experts, kb = (int64_t{a.k} + 31) / 32;
   const int64_t each = (rows + active - 1) / active;  // rows of an expert on average
@@ -923,7 +924,7 @@ Plan plan_of(const fluxmi_mx_gemm_args &a, const GemmParams &dual, int cus) {
   if (each <= 48 || low_panels <= cus) return {Form::PANEL, 2, 0, 0, unless_words};
   if (pieces(128, 128) <= cus) return {Form::PANEL, 4, 0, 0, unless_words};
   if (!dual_takes && pieces(256, 128) <= cus) return {Form::PANEL, 8, 0, 0, unless_words};
-  if (dual_takes) return {Form::DUAL, 0, 0, 0, 0};
+  if (dual_takes) return {Form::DUAL, 0, 0, 0, kb % 4 == 0 ? 0 : padded};
   return {Form::TILES, 0, 0, 0, scales_on(16) ? 0 : padded};
 }
 
@@ -939,7 +940,7 @@ extern "C" int fluxmi_grouped_gemm_mx(const fluxmi_mx_gemm_args *args, void *wor
   using namespace fluxmi;
   int rc = check_args(args);
   if (rc != FLUXMI_OK || args->max_rows == 0 || args->n == 0) return rc;
-  const GemmParams dual = dual_params(*args);
+  GemmParams dual = dual_params(*args);
   const Plan plan = plan_of(*args, dual, kPlanCus);
   FLUXMI_REQUIRE(plan.workspace == 0 || (workspace != nullptr && aligned16(workspace) && workspace_bytes >= plan.workspace), FLUXMI_ERR_WORKSPACE,
                  "grouped_gemm_mx: workspace of %zu bytes needed, %zu given", plan.workspace, workspace_bytes);
@@ -968,6 +969,8 @@ extern "C" int fluxmi_grouped_gemm_mx(const fluxmi_mx_gemm_args *args, void *wor
     hipLaunchKernelGGL(mx_pad_scales_kernel, dim3(grid), dim3(kThreads), 0, s, p.a_scale, a_rows, p.b_scale, b_rows, p.kb, p.scale_stride, padded);
     p.a_scale = padded;
     p.b_scale = padded + a_rows * p.scale_stride;
+    dual.a_scale = reinterpret_cast<const float *>(p.a_scale);
+    dual.b_scale = reinterpret_cast<const float *>(p.b_scale);
   }
   switch (plan.form) {
     case Form::STREAM:

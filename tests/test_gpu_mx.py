@@ -265,8 +265,16 @@ def test_rows_that_end_inside_a_line(splits, n, k):
         grouped(splits, n, k, out)
 
 
-@pytest.mark.parametrize("experts,rows,n", [(2, 3, 300), (2, 20, 300), (12, 9, 2600), (16, 100, 2000), (3, 600, 520), (16, 200, 1601), (4, 300, 5000)])
-@pytest.mark.parametrize("k", [384, 640, 736])
+@pytest.mark.parametrize("k", [544, 640, 1056, 1408, 2880, 4128])
+@pytest.mark.parametrize("splits,n", [([300, 0, 257, 700, 65], 5000), ([512] * 3, 8192), ([64, 200, 1, 129] * 8, 4104)], ids=brief)
+def test_tiles_of_rows_that_end_inside_a_line(splits, n, k):
+    for out in (BF16, F16, F32):
+        print(f"[case] tiles, ends {splits} {n} {k} {out}", flush=True)
+        grouped(splits, n, k, out)
+
+
+@pytest.mark.parametrize("experts,rows,n", [(4, 300, 5000), (2, 3, 300), (2, 20, 300), (12, 9, 2600), (16, 100, 2000), (3, 600, 520), (16, 200, 1601)])
+@pytest.mark.parametrize("k", [384, 640, 736, 1152])
 def test_nan_blocks_beside_the_ends_of_rows(experts, rows, n, k):
     """What lies behind a row's last scale is the next row's first: a NaN block there stays there."""
     a, sa, va = operand(experts * rows, k=k, seed=1)
