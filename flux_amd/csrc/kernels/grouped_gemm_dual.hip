@@ -71,6 +71,22 @@ struct DualTile {
   int e_row0, e_rows;  // the expert's rows
 };
 
+// A vector of elements of ELT bytes at any of them, or the first `count` of it.
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+template <int ELT>
+__device__ __forceinline__ void store_some(uint8_t *p, const u32x4 v, int count) {
+  if (count >= 16 / ELT) {
+    *reinterpret_cast<u32x4_any *>(p) = v;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 16 / ELT - 1; ++i) {
+    if (i >= count) continue;
+    if constexpr (ELT == 4) reinterpret_cast<uint32_t *>(p)[i] = v[i];
+    else reinterpret_cast<uint16_t *>(p)[i] = static_cast<uint16_t>(v[i / 2] >> (16 * (i & 1)));
+  }
+}
+
 template <int FIRST, class F, int... I>
 __device__ __forceinline__ void static_for_seq(F &f, std::integer_sequence<int, I...>) {
   (f(std::integral_constant<int, FIRST + I>{}), ...);
@@ -799,13 +815,18 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
             for (int j2 = 0; j2 < 2; ++j2) {
               const int j = jg * 2 + j2;
               if (cols[j] >= n) continue;
+              if constexpr (MX) {
+                store_some<4>(drow + static_cast<int64_t>(cols[j]) * 4, __builtin_bit_cast(u32x4, v[j2]), n - cols[j]);
+                continue;
+              }
               f32x4 *const dst = reinterpret_cast<f32x4 *>(drow + static_cast<int64_t>(cols[j]) * 4);
               if (nt) __builtin_nontemporal_store(v[j2], dst);
               else *dst = v[j2];
             }
           } else if (cols[jg * 2] < n) {
             const u32x4 o = {pack2<T>(v[0][0], v[0][1]), pack2<T>(v[0][2], v[0][3]), pack2<T>(v[1][0], v[1][1]), pack2<T>(v[1][2], v[1][3])};
-            *reinterpret_cast<u32x4 *>(drow + static_cast<int64_t>(cols[jg * 2]) * 2) = o;
+            if constexpr (MX) store_some<2>(drow + static_cast<int64_t>(cols[jg * 2]) * 2, o, n - cols[jg * 2]);
+            else *reinterpret_cast<u32x4 *>(drow + static_cast<int64_t>(cols[jg * 2]) * 2) = o;
           }
         }
       }
@@ -849,13 +870,13 @@ bool dual_takes(const GemmParams &p, int dtype) {
   return aligned;
 }
 
-// Two pairs of steps of K at least, scales on whole words, offsets below kNoRow; results in stores of 16 bytes.
+// Two pairs of steps of K at least, scales on whole words, offsets below kNoRow.
 bool dual_takes_mx(const GemmParams &p) {
   const int64_t kbytes = p.k / 2, span = 0x70000000ll;
   const uintptr_t scales = reinterpret_cast<uintptr_t>(p.a_scale) | reinterpret_cast<uintptr_t>(p.b_scale);
   if (p.k <= 512 || p.nexperts > kDualExperts || !aligned16(p.a) || !aligned16(p.b[0]) || (p.k % 128 == 0 && scales % 4 != 0)) return false;
   if (kTile * kbytes > span || p.n * kbytes > span || p.a_rows * kbytes > span) return false;
-  return aligned16(p.d[0]) && p.n % (p.d_fp32 ? 4 : 8) == 0;
+  return true;
 }
 
 int launch_grouped_gemm_dual_mx(const GemmParams &p, int grid, hipStream_t s) {

@@ -7,9 +7,9 @@
 // Bound by the weights' bytes with few rows per expert, by the MFMAs and what feeds them with many.  Five kernels:
 //  * streams (mx_stream_kernel), where there is less work than the card has room for: a wave, or two or four that split K, has 16 or 32 rows and 32 or 64 columns of
 //    an expert and streams through LDS on its own;
-//  * panels of 64, 128 or 256 rows and 128 columns (mx_panel_kernel);
+//  * panels of 64 or 128 rows and 128 columns (mx_panel_kernel);
 //  * the dual tiles of 256 x 256 (grouped_gemm_dual.hip);
-//  * for many rows and what those do not take (N that is no multiple of 8, K up to 512, more than 128 experts), mx_tile_kernel;
+//  * for many rows and what those do not take (K up to 512, more than 128 experts), mx_tile_kernel;
 //  * for few rows whose scales are not on whole words (K that is no multiple of 128), mx_few_rows_kernel, whose four waves split K in turns of 512 values and load
 //    straight into registers.  The others want a copy of such scales, of all experts.
 //
@@ -513,14 +513,9 @@ __global__ __launch_bounds__(512, 2) void mx_panel_kernel(const MxParams p, int 
   int slot = 0;
   auto step = [&](auto PARITY, int s) {
     constexpr int PAR = decltype(PARITY)::value;
-    // (256 rows: a request stops its wave until the memory pipeline takes it, so they come after the wave's own work, 92 -> 86 us for 194 rows 4096 x 14336; fewer
-    // rows leave the pipeline room, and the earlier request is worth up to 4 %.)
-    const int next = slot == 0 ? 2 : slot - 1;
-    if constexpr (MI < 8) fill_step(s + 2, next);
+    fill_step(s + 2, slot == 0 ? 2 : slot - 1);
     __builtin_amdgcn_sched_barrier(0);
     compute(PARITY, s, slot);
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (MI >= 8) fill_step(s + 2, next);
     FLUXMI_LGKM0();
     if (of_a) FLUXMI_VMCNT(C::XF + 1 - PAR);
     else FLUXMI_VMCNT(C::WF + 1 - PAR);
@@ -900,15 +895,13 @@ struct Plan {
 // The waves of a stream: one token of two experts 4096 x 14336 (256 streams) 16.3 / 13.0 / 13.4 of one, two and four that split K, with 896 (14336 x 4096) 13.8 / 15.7;
 // of 32 rows one expert 4096 x 4096, 128 rows (512 streams) 9.4 / 9.5 / 12.5, 1024 x 4096, 256 rows (256) 8.1 / 6.0 / 6.8, 128 rows (128) 8.0 / 5.9 / 5.6.  64 columns of
 // 32 rows: one expert 4096 x 14336, 256 rows (1024 streams) 46 -> 37, with fewer streams it is slower.
-// The dual tiles want K beyond 512 and N in multiples of 8 (fp32 results 4).  Without them: panels of 128 / of 256 rows / tiles of this file (dual tiles in brackets), 8
-// experts 4096 x 14208, 100 rows 73 / 75 / 120 (85), 194 rows 122 / 106 / 149 (101), 300 rows 176 / 187 / 148 (131), 1200 rows 586 / 513 / 400 (330); 14336 x 4224, 60 rows
-// 88 / 98 / 83 (85), 194 rows 159 / 145 / 110 (102), 1200 rows 750 / 650 / 431 (379).  Beside the dual tiles panels of 256 rows would be as good at 194 rows 4096 x 14336
-// (86 / 91) and worse where some experts have more than 256 (4 experts of 176 and 264 rows 8192 x 4096 58 / 40).
+// What keeps the dual tiles off (K up to 512, more than 128 experts) goes to the tiles of this file, which are slower (8 experts 14336 x 4224, 194 rows 102 -> 110, 1200 rows
+// 379 -> 431; 4095 x 14336, 600 rows 195 -> 245).  Panels of 256 rows would be as good as the dual tiles at 194 rows 4096 x 14336 (86 / 91) and worse where some experts have
+// more than 256 (4 experts of 176 and 264 rows 8192 x 4096 58 / 40).
 Plan plan_of(const fluxmi_mx_gemm_args &a, const GemmParams &dual, int cus) {
   const int64_t rows = a.max_rows, experts = a.nexperts, active = rows < experts ? rows : experts, kb = (int64_t{a.k} + 31) / 32;
   const int64_t each = (rows + active - 1) / active;  // rows of an expert on average
   auto pieces = [&](int64_t high, int64_t wide) { return active * ((each + high - 1) / high) * ((a.n + wide - 1) / wide); };
-  const bool dual_takes = dual_takes_mx(dual);
   auto scales_on = [&](int64_t bytes) {
     return kb % bytes == 0 && (reinterpret_cast<uintptr_t>(a.a_scale) | reinterpret_cast<uintptr_t>(a.b_scale)) % static_cast<uintptr_t>(bytes) == 0;
   };
@@ -923,8 +916,7 @@ Plan plan_of(const fluxmi_mx_gemm_args &a, const GemmParams &dual, int cus) {
   }
   if (each <= 48 || low_panels <= cus) return {Form::PANEL, 2, 0, 0, unless_words};
   if (pieces(128, 128) <= cus) return {Form::PANEL, 4, 0, 0, unless_words};
-  if (!dual_takes && pieces(256, 128) <= cus) return {Form::PANEL, 8, 0, 0, unless_words};
-  if (dual_takes) return {Form::DUAL, 0, 0, 0, kb % 4 == 0 ? 0 : padded};
+  if (dual_takes_mx(dual)) return {Form::DUAL, 0, 0, 0, kb % 4 == 0 ? 0 : padded};
   return {Form::TILES, 0, 0, 0, scales_on(16) ? 0 : padded};
 }
 
@@ -979,7 +971,7 @@ extern "C" int fluxmi_grouped_gemm_mx(const fluxmi_mx_gemm_args *args, void *wor
       else rc = plan.waves == 1 ? launch_stream<1, 2, 1>(p, s) : plan.waves == 2 ? launch_stream<1, 2, 2>(p, s) : launch_stream<1, 2, 4>(p, s);
       break;
     case Form::PANEL:
-      rc = plan.row_blocks == 2 ? launch_panel<2>(p, s) : plan.row_blocks == 4 ? launch_panel<4>(p, s) : launch_panel<8>(p, s);
+      rc = plan.row_blocks == 2 ? launch_panel<2>(p, s) : launch_panel<4>(p, s);
       break;
     case Form::DUAL: {
       // Up to four workgroups to a tile, which is cut in pieces when these still fit the card.

@@ -257,7 +257,7 @@ def test_panels(splits, n, k):
 
 @pytest.mark.parametrize("k", [32, 384, 1408, 2816, 2880, 705])
 @pytest.mark.parametrize("splits,n", [([1, 1], 500), ([30, 17], 500), ([3] * 20, 1600), ([16, 31, 33, 64, 65, 0] * 5, 1100), ([100, 129, 60, 200] * 4, 2001), ([700, 20], 512),
-                                      ([256, 150, 257, 16, 200, 180, 255, 129] * 2, 1601), ([600, 0, 33, 256, 257], 5000), ([3000], 1301)], ids=brief)
+                                      ([256, 150, 257, 16, 200, 180, 255, 129] * 2, 1601), ([600, 0, 33, 256, 257], 5000), ([3000], 1301), ([70, 52] * 65, 300)], ids=brief)
 def test_rows_that_end_inside_a_line(splits, n, k):
     """Every form with K that is a multiple of 128 (scales on whole words) and not."""
     for out in (BF16, F32):
