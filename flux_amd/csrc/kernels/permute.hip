@@ -136,8 +136,11 @@ __global__ __launch_bounds__(kThreads) void permute_kernel(const uint8_t *__rest
 template <Row T, int J, int U, bool SUB, bool NT>
 __global__ __launch_bounds__(kThreads) void unpermute_kernel(const uint8_t *__restrict__ rows, const int32_t *__restrict__ idx, const void *__restrict__ weights,
                                                              Row weight_type, int ntokens, int topk, int n, int shift, uint8_t *__restrict__ out) {
-  const Lanes me = my_token<SUB>(blockIdx.x, shift);
+  Lanes me = my_token<SUB>(blockIdx.x, shift);
   if (me.token >= ntokens) return;
+  // Few tokens: several workgroups to each.
+  me.lane += blockIdx.y * me.count;
+  me.count *= gridDim.y;
   const uint32_t npairs = static_cast<uint32_t>(ntokens) * topk;
   const size_t row_bytes = static_cast<size_t>(n) * kElt<T>, pair0 = static_cast<size_t>(me.token) * topk;
   const int nvec = n / kVec<T>;
@@ -383,14 +386,17 @@ extern "C" int fluxmi_moe_unpermute(const void *rows, int32_t row_type, const in
   FLUXMI_REQUIRE(rows != nullptr && out != nullptr, FLUXMI_ERR_INVALID_ARG, "moe_unpermute: null pointer argument");
   FLUXMI_REQUIRE(aligned_to(rows, type) && aligned_to(out, type) && aligned_to(weights, wtype), FLUXMI_ERR_INVALID_ARG,
                  "moe_unpermute: a pointer is not aligned to its elements");
-  const int shift = lanes_shift(n / (type == Row::F32 ? 4 : 8), ntokens, topk <= 2 ? 4 : 2);
+  const int nvec = n / (type == Row::F32 ? 4 : 8), shift = lanes_shift(nvec, ntokens, topk <= 2 ? 4 : 2);
+  // us with one and with several workgroups to a token: 10 tokens top-8 7168 columns bf16 9.0 / 3.5, 100 tokens 12.9 / 5.2, 1000 tokens 30 / 25; 300 tokens top-4 4096 columns
+  // 5.2 / 3.8, 1024 tokens 8.2 / 8.4.
+  const unsigned parts = ntokens > 1024 || nvec <= kThreads ? 1 : nvec > 7 * kThreads ? 8 : (nvec + kThreads - 1) / kThreads;
   const unsigned grid = grid_of(ntokens, shift, 0);
   FLUXMI_REQUIRE(grid > 0, FLUXMI_ERR_UNSUPPORTED, "moe_unpermute: ntokens=%d is too many for n=%d", ntokens, n);
   by_type(type, [&](auto t) {
     by_topk(topk, [&](auto j) {
       by_lanes(shift, static_cast<size_t>(n) * kElt<decltype(t)::value> * ntokens * topk, [&](auto sub, auto nt) {
         constexpr int J = decltype(j)::value, U = J == 1 ? 4 : J == 2 ? 2 : 1;
-        hipLaunchKernelGGL((unpermute_kernel<decltype(t)::value, J, U, decltype(sub)::value, decltype(nt)::value>), dim3(grid), dim3(kThreads), 0,
+        hipLaunchKernelGGL((unpermute_kernel<decltype(t)::value, J, U, decltype(sub)::value, decltype(nt)::value>), dim3(grid, parts), dim3(kThreads), 0,
                            static_cast<hipStream_t>(stream), static_cast<const uint8_t *>(rows), scatter_index, weights, wtype, ntokens, topk, n, shift,
                            static_cast<uint8_t *>(out));
       });
