@@ -44,6 +44,8 @@ __device__ __forceinline__ void unpack(const u32x4 v, float (&x)[kVec<T>]) {
   }
 }
 
+typedef __bf16 bf16_pair __attribute__((ext_vector_type(2)));
+
 // One rounding to the rows' type.
 template <Row T>
 __device__ __forceinline__ u32x4 pack(const float (&x)[kVec<T>]) {
@@ -52,7 +54,7 @@ __device__ __forceinline__ u32x4 pack(const float (&x)[kVec<T>]) {
   for (int i = 0; i < 4; ++i) {
     if constexpr (T == Row::F32) v[i] = __float_as_uint(x[i]);
     else if constexpr (T == Row::F16) v[i] = float_to_f16_bits(x[2 * i]) | static_cast<uint32_t>(float_to_f16_bits(x[2 * i + 1])) << 16;
-    else v[i] = float_to_bf16_bits(x[2 * i]) | static_cast<uint32_t>(float_to_bf16_bits(x[2 * i + 1])) << 16;
+    else v[i] = __builtin_bit_cast(uint32_t, bf16_pair{static_cast<__bf16>(x[2 * i]), static_cast<__bf16>(x[2 * i + 1])});  // one conversion instruction
   }
   return v;
 }
