@@ -23,9 +23,9 @@ constexpr int kRowsOfClearer = 65536;  // most rows that one clearing workgroup 
 
 // The experts' rows are moved non-temporally (NT) from this size on, twice what the L2s hold; the tokens' own rows never.  us, ordinary -> NT, three
 // sets of buffers in turn: permute 16384 tokens top-6 2048 columns 94 -> 81, 8192 top-2 4096 columns 42 -> 30; unpermute of the latter 41 -> 35,
-// 4096 top-8 7168 columns 113 -> 100, its backward pass 216 -> 202, that of the
-// former 73 -> 62.  Below, ordinary loads are the faster ones (unpermute 777 top-8 2047 columns 8.5 against 10.3, the backward pass of 1000
-// top-4 1536 fp32 columns 13.2 against 14.6).
+// 4096 top-8 7168 columns 113 -> 99, its backward pass 212 -> 197, that of the
+// former 71 -> 57.  Below, ordinary loads are the faster ones (unpermute 777 top-8 2047 columns 8.6 against 10.3, the backward pass of 1000
+// top-4 1536 fp32 columns 13.1 against 14.5).
 constexpr size_t kStreamBytes = size_t{64} << 20;
 
 __device__ __forceinline__ float load_as(const void *p, Row type, size_t i) {
