@@ -6,8 +6,9 @@
 //
 // Bound by HBM.  All three go through the tokens and not through the rows: a token's own row is then read or written once in the whole
 // launch, and the top-k rows once each, which is what the operators cannot do without; going through the rows would read x and g top-k
-// times.  Groups of 8 to 256 lanes share a token, every lane moves 16-byte vectors at whatever alignment the rows have (a width that
-// leaves a rest shorter than a vector ends with single elements), and a vector's top-k rows are requested before the first of them is used.
+// times.  Groups of 8 to 256 lanes share a token, every lane moves 16-byte vectors at whatever alignment the rows have (the last one of a
+// width that leaves a rest ends with the row and overlaps the one before it, 777 tokens top-8 2047 columns 8.5 -> 6.5 us; the backward pass, whose products would
+// count twice, and rows shorter than a vector go by elements there), and a vector's top-k rows are requested before the first of them is used.
 //
 // Rows without a pair: the first workgroups of a launch that writes rows own a range of them each, read all of idx (4 bytes a pair, beside
 // rows of kilobytes), mark in LDS which of their rows are named, and clear the others.  That needs neither a pass over the output before
@@ -24,8 +25,8 @@ constexpr int kRowsOfClearer = 65536;  // most rows that one clearing workgroup 
 // The experts' rows are moved non-temporally (NT) from this size on, twice what the L2s hold; the tokens' own rows never.  us, ordinary -> NT, three
 // sets of buffers in turn: permute 16384 tokens top-6 2048 columns 94 -> 81, 8192 top-2 4096 columns 42 -> 30; unpermute of the latter 41 -> 35,
 // 4096 top-8 7168 columns 113 -> 99, its backward pass 212 -> 197, that of the
-// former 71 -> 57.  Below, ordinary loads are the faster ones (unpermute 777 top-8 2047 columns 8.6 against 10.3, the backward pass of 1000
-// top-4 1536 fp32 columns 13.1 against 14.5).
+// former 71 -> 57.  Below, ordinary loads are the faster ones (the backward pass of 1000 top-4 1536 fp32 columns 13.1
+// against 14.5).
 constexpr size_t kStreamBytes = size_t{64} << 20;
 
 __device__ __forceinline__ float load_as(const void *p, Row type, size_t i) {
@@ -94,6 +95,10 @@ __device__ void clear_unnamed(int clearer, int clearers, const int32_t *__restri
   }
 }
 
+// Rows of `size` in vectors of `vec`: how many, and where the v-th begins.
+__device__ __forceinline__ int vectors_of(int size, int vec) { return size < vec ? 0 : (size - 1) / vec + 1; }
+__device__ __forceinline__ int vector_at(int v, int size, int vec) { return v < size / vec ? v * vec : size - vec; }
+
 template <bool SUB, bool NT>
 __global__ __launch_bounds__(kThreads) void permute_kernel(const uint8_t *__restrict__ in, const int32_t *__restrict__ idx, int ntokens, int topk,
                                                            size_t row_bytes, int shift, int clearers, uint8_t *__restrict__ rows) {
@@ -107,22 +112,27 @@ __global__ __launch_bounds__(kThreads) void permute_kernel(const uint8_t *__rest
   constexpr int U = 4;
   const uint8_t *const src = in + static_cast<size_t>(me.token) * row_bytes;
   const int32_t *const my_idx = idx + static_cast<size_t>(me.token) * topk;
-  const size_t nvec = row_bytes >> 4;
+  const size_t nvec = row_bytes < 16 ? 0 : (row_bytes + 15) >> 4;
   for (size_t v0 = me.lane; v0 < nvec; v0 += U * me.count) {
     u32x4 x[U];
+    size_t at[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (v0 + u * me.count < nvec) x[u] = load16(src + (v0 + u * me.count) * 16);
+    for (int u = 0; u < U; ++u) {
+      const size_t v = v0 + u * me.count;
+      at[u] = v * 16 + 16 <= row_bytes ? v * 16 : row_bytes - 16;
+      if (v < nvec) x[u] = load16(src + at[u]);
+    }
     for (int j = 0; j < topk; ++j) {
       const uint32_t r = my_idx[j];
       if (r >= static_cast<uint32_t>(npairs)) continue;
       uint8_t *const dst = rows + r * row_bytes;
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (v0 + u * me.count < nvec) store16<NT>(dst + (v0 + u * me.count) * 16, x[u]);
+        if (v0 + u * me.count < nvec) store16<NT>(dst + at[u], x[u]);
     }
   }
-  for (size_t b = nvec * 16 + me.lane; b < row_bytes; b += me.count) {
+  if (row_bytes >= 16) return;
+  for (size_t b = me.lane; b < row_bytes; b += me.count) {
     const uint8_t x = src[b];
     for (int j = 0; j < topk; ++j) {
       const uint32_t r = my_idx[j];
@@ -143,8 +153,9 @@ __global__ __launch_bounds__(kThreads) void unpermute_kernel(const uint8_t *__re
   me.count *= gridDim.y;
   const uint32_t npairs = static_cast<uint32_t>(ntokens) * topk;
   const size_t row_bytes = static_cast<size_t>(n) * kElt<T>, pair0 = static_cast<size_t>(me.token) * topk;
-  const int nvec = n / kVec<T>;
+  const int nvec = vectors_of(n, kVec<T>);
   uint8_t *const dst = out + static_cast<size_t>(me.token) * row_bytes;
+  auto byte_of = [&](int v) { return static_cast<size_t>(vector_at(v, n, kVec<T>)) * kElt<T>; };
   for (int v0 = me.lane; v0 < nvec; v0 += U * me.count) {
     float acc[U][kVec<T>] = {};
     for (int j0 = 0; j0 < topk; j0 += J) {
@@ -161,7 +172,7 @@ __global__ __launch_bounds__(kThreads) void unpermute_kernel(const uint8_t *__re
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           x[u][j] = u32x4{0u, 0u, 0u, 0u};
-          if (live && v0 + u * me.count < nvec) x[u][j] = load16<NT>(src + static_cast<size_t>(v0 + u * me.count) * 16);
+          if (live && v0 + u * me.count < nvec) x[u][j] = load16<NT>(src + byte_of(v0 + u * me.count));
         }
       }
 #pragma unroll
@@ -176,9 +187,10 @@ __global__ __launch_bounds__(kThreads) void unpermute_kernel(const uint8_t *__re
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (v0 + u * me.count < nvec) store16(dst + static_cast<size_t>(v0 + u * me.count) * 16, pack<T>(acc[u]));
+      if (v0 + u * me.count < nvec) store16(dst + byte_of(v0 + u * me.count), pack<T>(acc[u]));
   }
-  for (int e = nvec * kVec<T> + me.lane; e < n; e += me.count) {
+  if (nvec > 0) return;
+  for (int e = me.lane; e < n; e += me.count) {
     float acc = 0.f;
     for (int j = 0; j < topk; ++j) {
       const uint32_t r = idx[pair0 + j];
@@ -377,7 +389,7 @@ extern "C" int fluxmi_moe_permute(const void *in, const int32_t *scatter_index, 
                  static_cast<long long>(row_bytes));
   if (ntokens == 0 || row_bytes == 0) return FLUXMI_OK;
   FLUXMI_REQUIRE(in != nullptr && rows != nullptr, FLUXMI_ERR_INVALID_ARG, "moe_permute: null pointer argument");
-  const int shift = lanes_shift(row_bytes / 16, ntokens, 4), clearers = clear_first(ntokens * topk, row_bytes) ? 0 : clearer_count(ntokens * topk);
+  const int shift = lanes_shift((row_bytes + 15) / 16, ntokens, 4), clearers = clear_first(ntokens * topk, row_bytes) ? 0 : clearer_count(ntokens * topk);
   const unsigned grid = grid_of(ntokens, shift, clearers);
   FLUXMI_REQUIRE(grid > 0, FLUXMI_ERR_UNSUPPORTED, "moe_permute: ntokens=%d is too many for rows of %lld bytes", ntokens, static_cast<long long>(row_bytes));
   if (clearers == 0) clear_all(ntokens * topk, row_bytes, rows, static_cast<hipStream_t>(stream));
@@ -403,7 +415,7 @@ extern "C" int fluxmi_moe_unpermute(const void *rows, int32_t row_type, const in
   FLUXMI_REQUIRE(rows != nullptr && out != nullptr, FLUXMI_ERR_INVALID_ARG, "moe_unpermute: null pointer argument");
   FLUXMI_REQUIRE(aligned_to(rows, type) && aligned_to(out, type) && aligned_to(weights, wtype), FLUXMI_ERR_INVALID_ARG,
                  "moe_unpermute: a pointer is not aligned to its elements");
-  const int nvec = n / (type == Row::F32 ? 4 : 8), shift = lanes_shift(nvec, ntokens, topk <= 2 ? 4 : 2);
+  const int nvec = (static_cast<int64_t>(n) * (type == Row::F32 ? 4 : 2) + 15) / 16, shift = lanes_shift(nvec, ntokens, topk <= 2 ? 4 : 2);
   // us with one and with several workgroups to a token: 10 tokens top-8 7168 columns bf16 9.0 / 3.5, 100 tokens 12.9 / 5.2, 1000 tokens 30 / 25; 300 tokens top-4 4096 columns
   // 5.2 / 3.8, 1024 tokens 8.2 / 8.4.
   const unsigned parts = ntokens > 1024 || nvec <= kThreads ? 1 : nvec > 7 * kThreads ? 8 : (nvec + kThreads - 1) / kThreads;
