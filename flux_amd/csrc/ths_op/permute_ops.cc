@@ -14,7 +14,13 @@ int32_t row_type(const torch::Tensor &t, const char *name) {
   return st == at::kBFloat16 ? FLUXMI_ROWS_BF16 : st == at::kFloat ? FLUXMI_ROWS_FP32 : FLUXMI_ROWS_FP16;
 }
 
+// The kernels carry no tangents: forward mode would silently lose them.
+void refuse_tangent(const torch::Tensor &t, const char *what) {
+  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), what, ": forward-mode derivatives are not built");
+}
+
 void check_rows(const torch::Tensor &t, const char *name) {
+  refuse_tangent(t, name);
   TORCH_CHECK(t.is_cuda(), name, " must be a device tensor");
   TORCH_CHECK(t.dim() == 2, name, " must have 2 dimensions, got ", t.dim());
   TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
@@ -36,6 +42,7 @@ void check_pair_rows(const torch::Tensor &rows, const torch::Tensor &scatter_ind
 }
 
 int32_t check_weights(const torch::Tensor &weights, const torch::Tensor &scatter_index) {
+  refuse_tangent(weights, "weights");
   TORCH_CHECK(weights.is_cuda(), "weights must be a device tensor");
   TORCH_CHECK(weights.sizes() == scatter_index.sizes(), "weights shape mismatch: ", weights.sizes(), " expected ", scatter_index.sizes());
   TORCH_CHECK(weights.is_contiguous(), "weights must be contiguous");
@@ -80,8 +87,9 @@ std::tuple<torch::Tensor, torch::Tensor> unpermute_backward(const torch::Tensor 
   return {grad_rows, grad_weights};
 }
 
-// The gradients come from kernels that record nothing: a second derivative would be silently wrong, so it is refused.
-void refuse_second_derivative(const char *who) {
+// The gradients come from kernels that record nothing: a second derivative, in reverse or forward mode, would be silently wrong, so it is refused.
+void refuse_second_derivative(const char *who, const torch::Tensor &grad) {
+  refuse_tangent(grad, who);
   TORCH_CHECK(!at::GradMode::is_enabled(), who, ": the gradient of the gradient is not built (create_graph=True)");
 }
 
@@ -110,7 +118,7 @@ struct Permute : torch::autograd::Function<Permute> {
     return permute(input, scatter_index);
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
-    refuse_second_derivative("moe_permute");
+    refuse_second_derivative("moe_permute", grads[0]);
     refuse_leaves_of_another_stream("moe_permute");
     return {unpermute(grads[0].contiguous(), ctx->get_saved_variables()[0], {}), {}};
   }
@@ -123,7 +131,7 @@ struct Sum : torch::autograd::Function<Sum> {
     return unpermute(rows, scatter_index, {});
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
-    refuse_second_derivative("moe_unpermute");
+    refuse_second_derivative("moe_unpermute", grads[0]);
     refuse_leaves_of_another_stream("moe_unpermute");
     return {permute(grads[0].contiguous(), ctx->get_saved_variables()[0]), {}};
   }
@@ -138,7 +146,7 @@ struct Unpermute : torch::autograd::Function<Unpermute> {
     return unpermute(rows, scatter_index, weights);
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
-    refuse_second_derivative("moe_unpermute");
+    refuse_second_derivative("moe_unpermute", grads[0]);
     refuse_leaves_of_another_stream("moe_unpermute");
     const auto saved = ctx->get_saved_variables();
     const torch::Tensor grad = grads[0].contiguous(), &scatter_index = saved[0], &weights = saved[1], &rows = saved[2];

@@ -260,6 +260,22 @@ def test_second_derivatives_are_refused():
         torch.autograd.grad(layer(x, idx, w).sum(), [x, w], create_graph=True)
 
 
+def test_forward_mode_is_refused():
+    """A tangent of the weights, and one that comes with a gradient (forward over reverse), would be lost."""
+    ad = torch.autograd.forward_ad
+    idx, x, w = leaves()
+    rows = flux_amd.moe_permute(x.detach(), idx)
+    with ad.dual_level():
+        dual_w = ad.make_dual(w.detach(), torch.ones_like(w))
+        for call in (lambda: flux_amd.moe_unpermute(rows, idx, dual_w), lambda: flux_amd.moe_unpermute_backward(x.detach(), rows, idx, dual_w)):
+            with pytest.raises(RuntimeError, match="weights: forward-mode derivatives"):
+                call()
+        for out in (flux_amd.moe_permute(x, idx), flux_amd.moe_unpermute(rows.requires_grad_(), idx), flux_amd.moe_unpermute(rows, idx, w)):
+            up = ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+            with pytest.raises(RuntimeError, match="permute: forward-mode derivatives"):
+                out.backward(up)
+
+
 # ---- streams, graphs, refusals -------------------------------------------------------------------------------------
 
 

@@ -45,3 +45,14 @@ def test_ops_refuse_host_tensors():
                  lambda: flux_amd.moe_unpermute_backward(torch.zeros(4, 8), torch.zeros(8, 8), idx, torch.ones(4, 2))):
         with pytest.raises(RuntimeError, match="device tensor"):
             call()
+
+
+def test_tangents_are_refused():
+    """Forward mode: a dual tensor that requires no gradient would come back without its tangent."""
+    idx, x, rows, w = torch.zeros(4, 2, dtype=torch.int32), torch.ones(4, 8), torch.ones(8, 8), torch.ones(4, 2)
+    with torch.autograd.forward_ad.dual_level():
+        dx, drows = (torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, rows))
+        for call in (lambda: flux_amd.moe_permute(dx, idx), lambda: flux_amd.moe_permute_backward(drows, idx), lambda: flux_amd.moe_unpermute(drows, idx),
+                     lambda: flux_amd.moe_unpermute(drows, idx, w), lambda: flux_amd.moe_unpermute_backward(dx, rows, idx, w)):
+            with pytest.raises(RuntimeError, match="forward-mode derivatives"):
+                call()
