@@ -19,8 +19,14 @@ void refuse_tangent(const torch::Tensor &t, const char *what) {
   TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), what, ": forward-mode derivatives are not built");
 }
 
+// A conjugate or negative view stands for other values than its memory holds, which is what is moved.
+void refuse_lazy_view(const torch::Tensor &t, const char *name) {
+  TORCH_CHECK(!t.is_conj() && !t.is_neg(), name, " is a conjugate or negative view: resolve_conj() or resolve_neg() first");
+}
+
 void check_rows(const torch::Tensor &t, const char *name) {
   refuse_tangent(t, name);
+  refuse_lazy_view(t, name);
   TORCH_CHECK(t.is_cuda(), name, " must be a device tensor");
   TORCH_CHECK(t.dim() == 2, name, " must have 2 dimensions, got ", t.dim());
   TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
@@ -43,6 +49,7 @@ void check_pair_rows(const torch::Tensor &rows, const torch::Tensor &scatter_ind
 
 int32_t check_weights(const torch::Tensor &weights, const torch::Tensor &scatter_index) {
   refuse_tangent(weights, "weights");
+  refuse_lazy_view(weights, "weights");
   TORCH_CHECK(weights.is_cuda(), "weights must be a device tensor");
   TORCH_CHECK(weights.sizes() == scatter_index.sizes(), "weights shape mismatch: ", weights.sizes(), " expected ", scatter_index.sizes());
   TORCH_CHECK(weights.is_contiguous(), "weights must be contiguous");
@@ -120,7 +127,7 @@ struct Permute : torch::autograd::Function<Permute> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
     refuse_second_derivative("moe_permute", grads[0]);
     refuse_leaves_of_another_stream("moe_permute");
-    return {unpermute(grads[0].contiguous(), ctx->get_saved_variables()[0], {}), {}};
+    return {unpermute(grads[0].resolve_neg().contiguous(), ctx->get_saved_variables()[0], {}), {}};
   }
 };
 
@@ -133,7 +140,7 @@ struct Sum : torch::autograd::Function<Sum> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
     refuse_second_derivative("moe_unpermute", grads[0]);
     refuse_leaves_of_another_stream("moe_unpermute");
-    return {permute(grads[0].contiguous(), ctx->get_saved_variables()[0]), {}};
+    return {permute(grads[0].resolve_neg().contiguous(), ctx->get_saved_variables()[0]), {}};
   }
 };
 
@@ -149,7 +156,7 @@ struct Unpermute : torch::autograd::Function<Unpermute> {
     refuse_second_derivative("moe_unpermute", grads[0]);
     refuse_leaves_of_another_stream("moe_unpermute");
     const auto saved = ctx->get_saved_variables();
-    const torch::Tensor grad = grads[0].contiguous(), &scatter_index = saved[0], &weights = saved[1], &rows = saved[2];
+    const torch::Tensor grad = grads[0].resolve_neg().contiguous(), &scatter_index = saved[0], &weights = saved[1], &rows = saved[2];
     const bool want_rows = ctx->saved_data["rows"].toBool(), want_weights = rows.defined();
     const auto [grad_rows, grad_weights] = unpermute_backward(grad, rows, scatter_index, weights, want_rows, want_weights);
     return {grad_rows, {}, grad_weights};

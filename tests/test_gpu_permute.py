@@ -350,6 +350,24 @@ def test_captured_backward_pass():
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_lazy_views():
+    """What a conjugate view stands for is copied once it is resolved; a negative view of the weights is refused."""
+    idx = make_index(30, 2, 0.2, 1)
+    x = torch.view_as_complex(torch.randn(30, 17, 2, device=DEV))
+    with pytest.raises(RuntimeError, match="conjugate or negative view"):
+        flux_amd.moe_permute(x.conj(), idx)
+    got = torch.view_as_real(flux_amd.moe_permute(x.conj().resolve_conj(), idx))
+    assert torch.equal(got.reshape(60, 34).double(), want_rows(torch.view_as_real(x.conj().resolve_conj()).reshape(30, 34), idx))
+    with pytest.raises(RuntimeError, match="weights is a conjugate or negative view"):
+        flux_amd.moe_unpermute(data(60, 8, F32, 1), idx, torch._neg_view(torch.ones(30, 2, device=DEV)))
+    # a gradient that comes as one
+    rows, w = data(60, 8, F32, 1).requires_grad_(), torch.ones(30, 2, device=DEV, requires_grad=True)
+    up = torch.ones(30, 8, device=DEV)
+    for call, leaf in ((lambda: flux_amd.moe_unpermute(rows, idx), rows), (lambda: flux_amd.moe_unpermute(rows, idx, w), w)):
+        want = torch.autograd.grad(call(), leaf, -up)[0]
+        assert torch.equal(torch.autograd.grad(call(), leaf, torch._neg_view(up))[0], want)
+
+
 def test_refusals():
     idx, x, w = make_index(4, 2, 0.0, 1), torch.zeros(4, 16, device=DEV), torch.ones(4, 2, device=DEV)
     rows = torch.zeros(8, 16, device=DEV)

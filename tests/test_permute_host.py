@@ -56,3 +56,13 @@ def test_tangents_are_refused():
                      lambda: flux_amd.moe_unpermute(drows, idx, w), lambda: flux_amd.moe_unpermute_backward(dx, rows, idx, w)):
             with pytest.raises(RuntimeError, match="forward-mode derivatives"):
                 call()
+
+
+def test_conjugate_and_negative_views_are_refused():
+    """Their memory holds other values than they stand for, and rows are moved as memory."""
+    idx, w = torch.zeros(4, 2, dtype=torch.int32), torch.ones(4, 2)
+    conj, neg, neg_rows = torch.ones(4, 8, dtype=torch.complex64).conj(), torch._neg_view(torch.ones(4, 8)), torch._neg_view(torch.ones(8, 8))
+    for call in (lambda: flux_amd.moe_permute(conj, idx), lambda: flux_amd.moe_permute(neg, idx), lambda: flux_amd.moe_permute_backward(neg_rows, idx),
+                 lambda: flux_amd.moe_unpermute(neg_rows, idx, w), lambda: flux_amd.moe_unpermute_backward(neg, torch.ones(8, 8), idx, w)):
+        with pytest.raises(RuntimeError, match="conjugate or negative view"):
+            call()
