@@ -147,7 +147,9 @@ torch::Tensor MxGemm::forward_grouped(torch::Tensor input, torch::Tensor input_s
               input.device());
   const int64_t max_rows = gather_index.has_value() ? gather_index->numel() : input.size(0);
   if (!input_splits.is_cuda()) {
-    TORCH_CHECK(input_splits.sum().item<int64_t>() <= max_rows, "input_splits sum exceeds the rows of the product");
+    // Counts in pinned memory are not looked at here: a copy that the stream has yet to run may be about to write them, and the copy below, which
+    // comes after it, sees what it wrote.  (The kernels compute no rows past max_rows whatever the counts.)
+    TORCH_CHECK(input_splits.is_pinned() || input_splits.sum().item<int64_t>() <= max_rows, "input_splits sum exceeds the rows of the product");
     input_splits = input_splits.to(input.device(), /*non_blocking=*/true);
   }
   return mx_run(input, input_scale, weight, weight_scale, weight.size(0), max_rows, &input_splits, gather_index, row_scale, output, output_dtype_);

@@ -345,6 +345,27 @@ def test_counts_below_zero_and_past_the_rows():
         check(out[rows], va[rows], vw[e], 256)
 
 
+@pytest.mark.parametrize("stale", [[0, 0, 40, 0], [1000] * 4, [3, 1, 2, 0]])
+def test_row_counts_in_pinned_memory_that_the_stream_has_yet_to_write(stale):
+    """A non-blocking copy into the pinned counts is ordered before the call by the stream alone: the call must neither refuse nor use what the host sees in
+    them."""
+    fresh, n, k = [20, 8, 0, 12], 256, 512
+    a, sa, _ = operand(40, k=k, seed=1)
+    w, sw, _ = operand(4, n, k=k, seed=2)
+    gemm = flux_amd.MxGemm(F32)
+    want = gemm.forward_grouped(a, torch.tensor(fresh, dtype=torch.int32), w, sa, sw)
+    on_device = torch.tensor(fresh, dtype=torch.int32, device=DEV)
+    pinned = torch.empty(4, dtype=torch.int32, pin_memory=True)
+    pinned.copy_(torch.tensor(stale, dtype=torch.int32))
+    busy = torch.ones(8192, 8192, device=DEV)
+    torch.cuda.synchronize()
+    for _ in range(4):  # (about 40 ms on the stream)
+        torch.mm(busy, busy)
+    pinned.copy_(on_device, non_blocking=True)
+    got = gemm.forward_grouped(a, pinned, w, sa, sw)
+    assert torch.equal(got, want)
+
+
 def test_gather_entries_past_the_input_are_clamped():
     a, sa, va = operand(6, k=96, seed=1)
     w, sw, vw = operand(1, 33, k=96, seed=2)
