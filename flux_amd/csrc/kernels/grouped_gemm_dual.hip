@@ -223,13 +223,13 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
       const int ee = c * 64 + lane;
       int r = 0;
       if (ee < p.nexperts) r = few_args()->count > 0 ? few_args()->splits[ee] : p.splits[ee];
-      if (r < 0) r = 0;
+      r = r < 0 ? 0 : (r > p.max_rows ? p.max_rows : r);  // (counts past the rows do not overflow the sums)
       const int incl = wave_inclusive_scan(r);
       int begin = row_carry + incl - r, end = row_carry + incl;
       if (begin > p.max_rows) begin = p.max_rows;
       if (end > p.max_rows) end = p.max_rows;
       row_ends[ee] = end;  // (the same from every wave)
-      row_carry += __builtin_amdgcn_readlane(incl, 63);
+      row_carry = __builtin_amdgcn_readlane(end, 63);
       if (p.by_splits) {
         active += __popcll(__ballot(end > begin));
         chunks += __builtin_amdgcn_readlane(wave_inclusive_scan((end - begin + p.by_splits - 1) >> (31 - __builtin_clz(p.by_splits))), 63);

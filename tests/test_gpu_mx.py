@@ -345,6 +345,21 @@ def test_counts_below_zero_and_past_the_rows():
         check(out[rows], va[rows], vw[e], 256)
 
 
+# Streams, both heights of panels, dual tiles and the tiles for short K; counts whose sums pass 2^31, and ones that are twice the rows.
+@pytest.mark.parametrize("rows,n,k", [(40, 70, 256), (320, 3001, 512), (800, 3001, 640), (2400, 5000, 1024), (2400, 5000, 1056), (2400, 5000, 384)])
+@pytest.mark.parametrize("huge", [1 << 30, (1 << 31) - 1, 0])
+def test_counts_far_past_the_rows(rows, n, k, huge):
+    """Row counts are on the device, where no check sees them: rows past the last are in no form computed or counted, the experts before have their own."""
+    print(f"[case] counts past the rows {rows} {n} {k} {huge}", flush=True)
+    a, sa, va = operand(rows, k=k, seed=1)
+    w, sw, vw = operand(8, n, k=k, seed=2)
+    first = rows // 4 + 3
+    splits = torch.tensor([first, -7, 0, huge or rows, huge or rows, 5, huge or rows, 5], dtype=torch.int32, device=DEV)
+    got = flux_amd.MxGemm(F32).forward_grouped(a, splits, w, sa, sw)
+    check(got[:first], va[:first], vw[0], k)
+    check(got[first:], va[first:], vw[3], k)
+
+
 @pytest.mark.parametrize("stale", [[0, 0, 40, 0], [1000] * 4, [3, 1, 2, 0]])
 def test_row_counts_in_pinned_memory_that_the_stream_has_yet_to_write(stale):
     """A non-blocking copy into the pinned counts is ordered before the call by the stream alone: the call must neither refuse nor use what the host sees in
