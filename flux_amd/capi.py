@@ -35,6 +35,7 @@ EXPORTS = (
     "fluxmi_topk_gather_reduce", "fluxmi_moe_permute", "fluxmi_moe_unpermute", "fluxmi_moe_unpermute_backward", "fluxmi_quant_e4m3_rowwise", "fluxmi_quant_e4m3_square",
     "fluxmi_quant_e4m3_block128", "fluxmi_quant_e4m3_block128_filled", "fluxmi_calib_stream_sink_bytes", "fluxmi_calib_stream",
     "fluxmi_quant_mx", "fluxmi_dequant_mx", "fluxmi_grouped_gemm_mx_workspace_bytes", "fluxmi_grouped_gemm_mx",
+    "fluxmi_grouped_gemm_mx_launch_info",
 )
 
 
@@ -55,6 +56,10 @@ class GroupedGemmArgs(ctypes.Structure):
 class MxGemmArgs(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("nexperts", "max_rows", "n", "k", "a_rows", "d_type")] + [
         (n, ctypes.c_void_p) for n in ("a", "a_scale", "b", "b_scale", "d", "splits", "gather_a", "row_scale")]
+
+
+class MxLaunchInfo(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("form", "rows", "cols", "waves")]
 
 
 class GemmLaunchInfo(ctypes.Structure):
@@ -116,6 +121,7 @@ def load():
     lib.fluxmi_grouped_gemm_mx_workspace_bytes.restype = sz
     lib.fluxmi_grouped_gemm_mx_workspace_bytes.argtypes = [ctypes.POINTER(MxGemmArgs)]
     lib.fluxmi_grouped_gemm_mx.argtypes = [ctypes.POINTER(MxGemmArgs), vp, sz, vp]
+    lib.fluxmi_grouped_gemm_mx_launch_info.argtypes = [ctypes.POINTER(MxGemmArgs), ctypes.POINTER(MxLaunchInfo)]
     lib.fluxmi_calib_stream_sink_bytes.restype = sz
     lib.fluxmi_calib_stream.argtypes = [vp, vp, sz, i32, vp]
     _lib = lib
@@ -276,6 +282,20 @@ def gemm_launch_info(dtype, nexperts, max_rows, n, k, ngroups=1, block_scaled=Fa
     _check(call(ctypes.byref(args), ngroups, aligned if block_scaled else None, host, cu_count, ctypes.byref(info)),
            "fluxmi_grouped_gemm_panel_info" if panel else "fluxmi_grouped_gemm_launch_info")
     return info
+
+
+MX_NONE, MX_FEW_ROWS, MX_STREAM, MX_PANEL, MX_DUAL, MX_TILES = range(6)
+
+
+def mx_launch_info(nexperts, max_rows, n, k, a_rows=None, out_dtype=torch.bfloat16, scales_at=0):
+    """The kernel that computes an MXFP4 product with aligned operands (fluxmi_grouped_gemm_mx_launch_info) and the workspace it takes; needs no GPU.
+    a_rows: given where rows are gathered; scales_at: byte on which both scales start after a boundary of 16."""
+    aligned = 0x1000
+    args = MxGemmArgs(nexperts=nexperts, max_rows=max_rows, n=n, k=k, a_rows=max_rows if a_rows is None else a_rows, d_type=_ROW_TYPES[out_dtype], a=aligned,
+                      a_scale=aligned + scales_at, b=aligned, b_scale=aligned + scales_at, d=aligned, splits=aligned, gather_a=None if a_rows is None else aligned)
+    info, lib = MxLaunchInfo(), load()
+    _check(lib.fluxmi_grouped_gemm_mx_launch_info(ctypes.byref(args), ctypes.byref(info)), "fluxmi_grouped_gemm_mx_launch_info")
+    return info, lib.fluxmi_grouped_gemm_mx_workspace_bytes(ctypes.byref(args))
 
 
 def gemm_dual_tiles(dtype, nexperts, max_rows, n, k, ngroups=1, block_scaled=False, gathered=False, sched_flags=0, d_fp32=False):

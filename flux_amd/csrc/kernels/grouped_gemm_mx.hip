@@ -928,6 +928,33 @@ extern "C" size_t fluxmi_grouped_gemm_mx_workspace_bytes(const fluxmi_mx_gemm_ar
   return fluxmi::plan_of(*args, fluxmi::dual_params(*args), fluxmi::kPlanCus).workspace;
 }
 
+extern "C" int fluxmi_grouped_gemm_mx_launch_info(const fluxmi_mx_gemm_args *args, fluxmi_mx_launch_info *info) {
+  using namespace fluxmi;
+  FLUXMI_REQUIRE(args != nullptr && info != nullptr, FLUXMI_ERR_INVALID_ARG, "grouped_gemm_mx_launch_info: null args / info");
+  *info = fluxmi_mx_launch_info{};
+  const int rc = check_args(args);
+  if (rc != FLUXMI_OK || args->max_rows == 0 || args->n == 0) return rc;
+  const Plan plan = plan_of(*args, dual_params(*args), kPlanCus);
+  switch (plan.form) {
+    case Form::FEW_ROWS:
+      *info = {FLUXMI_MX_FEW_ROWS, 16, kCols, kThreads / 64};
+      break;
+    case Form::STREAM:
+      *info = {FLUXMI_MX_STREAM, 16 * plan.row_blocks, 16 * plan.col_blocks, plan.waves};
+      break;
+    case Form::PANEL:
+      *info = {FLUXMI_MX_PANEL, 32 * plan.row_blocks, 128, 1};
+      break;
+    case Form::DUAL:
+      *info = {FLUXMI_MX_DUAL, 256, 256, 1};
+      break;
+    case Form::TILES:
+      *info = {FLUXMI_MX_TILES, 256, 256, 1};
+      break;
+  }
+  return FLUXMI_OK;
+}
+
 extern "C" int fluxmi_grouped_gemm_mx(const fluxmi_mx_gemm_args *args, void *workspace, size_t workspace_bytes, void *stream) {
   using namespace fluxmi;
   int rc = check_args(args);

@@ -447,6 +447,21 @@ typedef struct fluxmi_mx_gemm_args {
 size_t fluxmi_grouped_gemm_mx_workspace_bytes(const fluxmi_mx_gemm_args *args);
 int fluxmi_grouped_gemm_mx(const fluxmi_mx_gemm_args *args, void *workspace, size_t workspace_bytes, void *stream);
 
+/* Which of its kernels computes a launch of fluxmi_grouped_gemm_mx.  Host only: nothing is launched, no device is needed, and pointers in `args` are only
+ * looked at for their alignment.  Returns FLUXMI_OK or the status the call itself would return. */
+#define FLUXMI_MX_NONE 0     /* no rows or no columns: nothing is launched */
+#define FLUXMI_MX_FEW_ROWS 1 /* up to 16 rows per expert, scales not on whole words */
+#define FLUXMI_MX_STREAM 2   /* a wave, or some that split K, to a piece of the result */
+#define FLUXMI_MX_PANEL 3    /* eight waves to 64 or 128 rows */
+#define FLUXMI_MX_DUAL 4     /* the dual tiles of the grouped GEMM */
+#define FLUXMI_MX_TILES 5    /* tiles for short K and many experts */
+typedef struct fluxmi_mx_launch_info {
+  int32_t form;       /* FLUXMI_MX_* */
+  int32_t rows, cols; /* most of a piece of the result */
+  int32_t waves;      /* of a workgroup that split K (FLUXMI_MX_FEW_ROWS, FLUXMI_MX_STREAM), otherwise 1 */
+} fluxmi_mx_launch_info;
+int fluxmi_grouped_gemm_mx_launch_info(const fluxmi_mx_gemm_args *args, fluxmi_mx_launch_info *info);
+
 /* ------------------------------------------------------------------------------------------------
  * Calibration streams (no counterpart in the reference; for benchmarks): what the memory system of the GPU at
  * hand gives a kernel that only streams.  copy == 0: every byte of src[0, bytes) is read once (16 bytes per lane

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import flux_amd
+from flux_amd import capi
 from oracle import mx
 
 pytestmark = pytest.mark.gpu
@@ -345,6 +346,133 @@ def test_counts_below_zero_and_past_the_rows():
         check(out[rows], va[rows], vw[e], 256)
 
 
+def form_of(splits, extra, n, k, tokens=None):
+    info, _ = capi.mx_launch_info(len(splits), sum(splits) + extra, n, k, a_rows=tokens)
+    return info.form, info.rows, info.cols, info.waves
+
+
+FEW, STREAM, PANEL, DUAL, TILES = capi.MX_FEW_ROWS, capi.MX_STREAM, capi.MX_PANEL, capi.MX_DUAL, capi.MX_TILES
+# Every kernel of the products: K that ends in each part of its steps, rows of experts that end in each unit of its pieces, columns that are not whole ones; the dual
+# tiles' table of two experts to a lane (66 and 100) and what keeps them off (K up to 512, 130 experts).
+FORMS = [([5, 0, 3], 300, 705, (FEW, 16, 64, 4)), ([16, 0, 15, 1, 16] * 3, 1001, 2880, (FEW, 16, 64, 4)),
+         ([5, 0, 3], 300, 640, (STREAM, 16, 32, 4)), ([5, 0, 3, 8] * 5, 1001, 640, (STREAM, 16, 32, 2)), ([5, 0, 3, 8] * 7, 1001, 1024, (STREAM, 16, 32, 1)),
+         ([17, 30], 300, 640, (STREAM, 32, 32, 4)), ([40, 20], 300, 705, (STREAM, 32, 32, 4)), ([17, 30, 20, 40], 4000, 640, (STREAM, 32, 32, 2)),
+         ([128], 4096, 384, (STREAM, 32, 32, 1)), ([17, 30, 20, 40, 60, 50], 3001, 1408, (STREAM, 32, 64, 1)),
+         ([40, 17, 64, 65, 0, 33, 50, 51], 3001, 640, (PANEL, 64, 128, 1)), ([260], 4095, 705, (PANEL, 64, 128, 1)),
+         ([150, 1, 250, 129, 470], 3001, 640, (PANEL, 128, 128, 1)), ([256, 300], 4000, 1056, (PANEL, 128, 128, 1)),
+         ([300, 0, 257, 700, 65, 1, 512, 130], 2305, 640, (DUAL, 256, 256, 1)), ([300, 0, 257, 700, 65, 1, 512, 130], 2305, 544, (DUAL, 256, 256, 1)),
+         ([64, 193, 600, 256, 0, 128, 449, 300], 2312, 1536, (DUAL, 256, 256, 1)), ([70, 52] * 50, 400, 640, (DUAL, 256, 256, 1)),
+         ([70, 0, 150, 5] * 16 + [3, 200], 501, 1056, (DUAL, 256, 256, 1)),
+         ([300, 0, 257, 700, 65, 1, 512, 130], 2305, 384, (TILES, 256, 256, 1)), ([300, 0, 257, 700, 65, 1, 512, 130], 2304, 512, (TILES, 256, 256, 1)),
+         ([70, 52] * 65, 300, 1408, (TILES, 256, 256, 1))]
+
+
+@pytest.mark.parametrize("gathered,weighted,out", [(False, True, F32), (True, False, BF16), (True, True, F16)])
+@pytest.mark.parametrize("splits,n,k,form", FORMS, ids=brief)
+def test_every_form(splits, n, k, form, gathered, weighted, out):
+    """Rows that are gathered from fewer (entries past them are clamped), and rows past the splits' sum that stay as they were, in every kernel."""
+    print(f"[case] form {form} {brief(splits)} {n} {k} {gathered} {weighted} {out}", flush=True)
+    rows, extra = sum(splits), 9
+    tokens = max(rows // 3, 1) if gathered else None
+    assert form_of(splits, extra, n, k, tokens) == form
+    g = torch.Generator().manual_seed(5)
+    a, sa, va = operand(tokens or rows, k=k, seed=3)
+    w, sw, vw = operand(len(splits), n, k=k, seed=4)
+    gather, source = None, torch.arange(rows, device=DEV)
+    if gathered:
+        entries = torch.randint(0, tokens, (rows + extra,), generator=g)
+        entries[1::7], entries[2::11], entries[3::13] = tokens, -5, 1 << 30
+        gather, source = entries.to(torch.int32).to(DEV), entries[:rows].clamp(0, tokens - 1).to(DEV)
+    else:
+        a, sa = (torch.cat([t.view(torch.uint8), t.view(torch.uint8).new_full((extra, t.shape[1]), 255)]).view(t.dtype) for t in (a, sa))
+    factor = torch.rand(rows + extra, generator=g).to(DEV) if weighted else None
+    got = torch.full((rows + extra, n), 77.0, dtype=out, device=DEV)
+    flux_amd.MxGemm(out).forward_grouped(a, torch.tensor(splits, dtype=torch.int32, device=DEV), w, sa, sw, gather_index=gather, row_scale=factor, output=got)
+    assert (got[rows:] == 77).all()
+    at = 0
+    for e, r in enumerate(splits):
+        mine = slice(at, at + r)
+        check(got[mine], va[source[mine]], vw[e], k, factor[mine] if weighted else None)
+        at += r
+
+
+@pytest.mark.parametrize("few", [0, 1, 40])
+def test_far_fewer_rows_than_the_bound(few):
+    """The kernel is chosen by the bound of the rows; the splits may leave most of them, or all, unused."""
+    for splits, n, k, form in FORMS:
+        print(f"[case] {few} rows in form {form} {brief(splits)} {n} {k}", flush=True)
+        rows, experts = sum(splits), len(splits)
+        few_here = min(few, rows)
+        a, sa, va = operand(rows, k=k, seed=1)
+        w, sw, vw = operand(experts, n, k=k, seed=2)
+        counts = [0] * experts  # the first and the last expert's
+        counts[-1] = few_here - few_here // 2
+        counts[0] += few_here // 2
+        got = torch.full((rows, n), 77.0, device=DEV)
+        assert form_of(splits, 0, n, k) == form
+        flux_amd.MxGemm(F32).forward_grouped(a, torch.tensor(counts, dtype=torch.int32, device=DEV), w, sa, sw, output=got)
+        check(got[:counts[0]], va[:counts[0]], vw[0], k)
+        check(got[counts[0]:few_here], va[counts[0]:few_here], vw[-1], k)
+        assert (got[few_here:] == 77).all()
+
+
+@pytest.mark.parametrize("rows,n,k,form", [(5, 300, 640, STREAM), (260, 4095, 640, PANEL), (700, 3001, 1056, PANEL), (3000, 1301, 640, DUAL), (3000, 1301, 2080, DUAL),
+                                           (777, 5000, 1024, DUAL), (3000, 1301, 384, TILES), (3000, 1400, 512, TILES)])
+def test_every_form_without_splits(rows, n, k, form):
+    print(f"[case] dense form {form} {rows} {n} {k}", flush=True)
+    assert form_of([rows], 0, n, k)[0] == form
+    a, sa, va = operand(rows, k=k, seed=1)
+    w, sw, vw = operand(n, k=k, seed=2)
+    for out in (BF16, F32):
+        check(flux_amd.MxGemm(out).forward(a, w, sa, sw), va, vw, k)
+
+
+def test_every_form_on_two_streams_at_once():
+    """Each call's workspace is its own, and nothing else is shared."""
+    calls, seen = [], set()
+    for splits, n, k, form in FORMS:
+        assert form_of(splits, 0, n, k) == form
+        seen.add(form[0])
+        a, sa, _ = operand(sum(splits), k=k, seed=1)
+        w, sw, _ = operand(len(splits), n, k=k, seed=2)
+        sp = torch.tensor(splits, dtype=torch.int32, device=DEV)
+        calls.append(lambda a=a, sp=sp, w=w, sa=sa, sw=sw: flux_amd.MxGemm(BF16).forward_grouped(a, sp, w, sa, sw))
+    assert seen == {FEW, STREAM, PANEL, DUAL, TILES}
+    want = [call() for call in calls]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(3):
+        for which in (0, 1):
+            with torch.cuda.stream(streams[which]):
+                got[which] += [call() for call in (calls if which else calls[::-1])]
+    torch.cuda.synchronize()
+    for i, result in enumerate(got[0]):
+        assert torch.equal(result, want[-1 - i % len(calls)])
+    for i, result in enumerate(got[1]):
+        assert torch.equal(result, want[i % len(calls)])
+
+
+@pytest.mark.parametrize("splits,n,k", [([9, 0, 30], 352, 544), ([300, 257, 0, 700, 65, 512], 1056, 2400)], ids=brief)
+def test_gradient_of_the_input_from_the_transposed_codes(splits, n, k):
+    """grad_x = grad_y @ W: the weights' transposed codes are the operand whose rows are K, with blocks along N."""
+    rows = sum(splits)
+    gen = torch.Generator(DEV).manual_seed(n)
+    weight = torch.randn(len(splits), n, k, device=DEV, generator=gen).to(BF16)
+    grad = torch.randn(rows, n, device=DEV, generator=gen).to(BF16)
+    q = quantiser(BF16)
+    _, _, codes_t, scale_t = q.quantize_mx(weight, return_tranpose=True)
+    gc, gs, _, _ = q.quantize_mx(grad)
+    got = flux_amd.MxGemm(F32).forward_grouped(gc, torch.tensor(splits, dtype=torch.int32, device=DEV), codes_t, gs, scale_t)
+    assert got.shape == (rows, k)
+    vg = torch.from_numpy(mx.values(*mx.quantise(grad.double().cpu().numpy()))).to(DEV)
+    at = 0
+    for e, r in enumerate(splits):
+        vw = torch.from_numpy(mx.values(*mx.quantise(weight[e].t().double().cpu().numpy()))).to(DEV)
+        check(got[at:at + r], vg[at:at + r], vw, n)
+        at += r
+
+
 # Streams, both heights of panels, dual tiles and the tiles for short K; counts whose sums pass 2^31, and ones that are twice the rows.
 @pytest.mark.parametrize("rows,n,k", [(40, 70, 256), (320, 3001, 512), (800, 3001, 640), (2400, 5000, 1024), (2400, 5000, 1056), (2400, 5000, 384)])
 @pytest.mark.parametrize("huge", [1 << 30, (1 << 31) - 1, 0])
@@ -353,7 +481,8 @@ def test_counts_far_past_the_rows(rows, n, k, huge):
     print(f"[case] counts past the rows {rows} {n} {k} {huge}", flush=True)
     a, sa, va = operand(rows, k=k, seed=1)
     w, sw, vw = operand(8, n, k=k, seed=2)
-    first = rows // 4 + 3
+    first, form = rows // 4 + 3, {40: (STREAM, 16), 320: (PANEL, 64), 800: (PANEL, 128)}.get(rows, (TILES if k < 512 else DUAL, 256))
+    assert form_of([rows] + [0] * 7, 0, n, k)[:2] == form
     splits = torch.tensor([first, -7, 0, huge or rows, huge or rows, 5, huge or rows, 5], dtype=torch.int32, device=DEV)
     got = flux_amd.MxGemm(F32).forward_grouped(a, splits, w, sa, sw)
     check(got[:first], va[:first], vw[0], k)

@@ -74,3 +74,33 @@ def test_ops_refuse():
         q.dequantize_mx(codes, scale)
     with pytest.raises(RuntimeError, match="device tensor"):
         flux_amd.MxGemm(torch.bfloat16).forward(codes, codes, scale, scale)
+
+
+def test_forms_and_workspaces():
+    """Which kernel computes a product and what it asks for: a copy of the scales where they are not on the words that the kernel reads."""
+    def of(*args, **kw):
+        info, ws = capi.mx_launch_info(*args, **kw)
+        return info.form, info.rows, ws
+
+    def padded(a_rows, b_rows, k):  # scales in rows of whole 16 bytes
+        return (a_rows + b_rows) * (((k + 31) // 32 + 15) // 16 * 16)
+
+    assert of(8, 0, 64, 64) == (capi.MX_NONE, 0, 0) and of(8, 64, 0, 64)[0] == capi.MX_NONE
+    assert of(2, 8, 300, 705) == (capi.MX_FEW_ROWS, 16, 0)
+    assert of(2, 8, 300, 640) == (capi.MX_STREAM, 16, 0) and of(2, 8, 300, 640, scales_at=4) == (capi.MX_STREAM, 16, 0)
+    assert of(2, 8, 300, 640, scales_at=1) == (capi.MX_FEW_ROWS, 16, 0)
+    assert of(2, 60, 300, 640, scales_at=1) == (capi.MX_STREAM, 32, padded(60, 600, 640)) and of(2, 60, 300, 705) == (capi.MX_STREAM, 32, padded(60, 600, 705))
+    assert of(8, 320, 3001, 640) == (capi.MX_PANEL, 64, 0) and of(8, 800, 3001, 640) == (capi.MX_PANEL, 128, 0)
+    # 128 experts and K beyond 512 for the dual tiles, which want scales on words only
+    assert of(128, 7900, 300, 1408) == (capi.MX_DUAL, 256, 0) and of(129, 7900, 300, 1408) == (capi.MX_TILES, 256, padded(7900, 129 * 300, 1408))
+    assert of(129, 7900, 300, 1536) == (capi.MX_TILES, 256, 0) and of(129, 7900, 300, 1536, scales_at=4) == (capi.MX_TILES, 256, padded(7900, 129 * 300, 1536))
+    assert of(8, 2000, 2305, 640) == (capi.MX_DUAL, 256, 0) and of(8, 2000, 2305, 512) == (capi.MX_TILES, 256, 0)
+    assert of(8, 2000, 2305, 640, a_rows=700, scales_at=2)[2] == padded(700, 8 * 2305, 640)
+    # what the call itself refuses
+    lib, info = capi.load(), capi.MxLaunchInfo()
+    refused(lib.fluxmi_grouped_gemm_mx_launch_info(None, ctypes.byref(info)), -1, "null args")
+    refused(lib.fluxmi_grouped_gemm_mx_launch_info(ctypes.byref(capi.MxGemmArgs()), None), -1, "null args")
+    with pytest.raises(RuntimeError, match="exceeds 2\\^24"):
+        capi.mx_launch_info(2, (1 << 24) + 1, 16, 32)
+    with pytest.raises(RuntimeError, match="nexperts=0"):
+        capi.mx_launch_info(0, 8, 16, 32)
