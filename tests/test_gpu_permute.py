@@ -184,6 +184,33 @@ def test_offsets_past_32_bits():
     assert ((grad_w[probe, 5].double() - square).abs() <= (n / 8 + 16) * 2.0**-24 * square).all()
 
 
+@pytest.mark.parametrize("topk", [1, 2, 4, 6, 8])
+@pytest.mark.parametrize("dtype,n", [(BF16, 2047), (F16, 1032), (F32, 1025), (BF16, 45), (F32, 3)])
+def test_rows_of_many_megabytes(dtype, n, topk):
+    """From 64 MB on the experts' rows pass the caches by: every number of pairs that is requested together, dropped pairs, widths with a rest."""
+    print(f"[case] many megabytes {topk} {n} {dtype}", flush=True)
+    tokens = (65 << 20) // (topk * n * (4 if dtype == F32 else 2)) + 1
+    g = torch.Generator(DEV).manual_seed(n + topk)
+    pairs = tokens * topk
+    idx = torch.randperm(pairs, generator=g, device=DEV).to(torch.int32).view(tokens, topk)
+    idx = torch.where(torch.rand(tokens, topk, generator=g, device=DEV) < 0.1, -1, idx)
+    x, rows = (torch.randn(r, n, generator=g, device=DEV).to(dtype) for r in (tokens, pairs))
+    w = torch.rand(tokens, topk, generator=g, device=DEV)
+    assert torch.equal(capi.moe_permute(x, idx, out=torch.full_like(rows, float("nan"))).double(), want_rows(x, idx))
+    out, magnitude = torch.zeros(tokens, n, dtype=torch.float64, device=DEV), torch.zeros(tokens, n, dtype=torch.float64, device=DEV)
+    dot, dots = torch.zeros(tokens, topk, dtype=torch.float64, device=DEV), torch.zeros(tokens, topk, dtype=torch.float64, device=DEV)
+    for j in range(topk):  # (a column of the index at a time: the terms of all together are gigabytes)
+        term = pair_rows(rows, idx[:, j])
+        out += term * w[:, j].double()[:, None]
+        magnitude += (term * w[:, j].double()[:, None]).abs()
+        dot[:, j], dots[:, j] = (term * x.double()).sum(1), (term * x.double()).abs().sum(1)
+    close(flux_amd.moe_unpermute(rows, idx, w), out, magnitude, topk + 1)
+    grad_rows, grad_w = flux_amd.moe_unpermute_backward(x, rows, idx, w)
+    want = want_rows(x, idx, w)
+    close(grad_rows, want, want.abs(), 1)
+    close(grad_w, dot, dots, n / 8 + 16)
+
+
 @pytest.mark.parametrize("dtype,n", [(BF16, 1), (F32, 1), (BF16, 3)])
 def test_very_many_short_rows(dtype, n):
     """Four bytes a pair for every 65536 rows are more than a row: all rows are cleared before the launch."""
