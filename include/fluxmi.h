@@ -326,8 +326,8 @@ int fluxmi_topk_gather_reduce(const void *const *in, int32_t ngroups, int32_t io
  *   fluxmi_moe_unpermute           out[t] = sum_j weights[t, j] * rows[scatter_index[t, j]]   (weights NULL: 1), j ascending, fp32
  *                                  multiply-adds, one rounding
  *   fluxmi_moe_unpermute_backward  grad_rows[scatter_index[t, j]] = weights[t, j] * grad_out[t]; rows that no entry names are 0
- *                                  grad_weights[t, j] = sum_n grad_out[t, n] * rows[scatter_index[t, j], n] (fp32 sums in a fixed order;
- *                                  0 for a dropped pair)
+ *                                  grad_weights[t, j] = sum_n grad_out[t, n] * rows[scatter_index[t, j], n] (fp32 sums, in an order that depends
+ *                                  on ntokens, n and row_type only; 0 for a dropped pair)
  *                                  grad_rows or grad_weights may be NULL: it is not computed (and rows not read without grad_weights).
  *
  * `row_type` is the type of rows, out, grad_out and grad_rows, `weight_type` that of weights [ntokens, topk] and grad_weights (FLUXMI_ROWS_*).

@@ -184,6 +184,22 @@ def test_offsets_past_32_bits():
     assert ((grad_w[probe, 5].double() - square).abs() <= (n / 8 + 16) * 2.0**-24 * square).all()
 
 
+@pytest.mark.parametrize("dtype,n", [(BF16, 2047), (F16, 1536), (F32, 7168)])
+def test_a_token_has_the_same_sums_in_every_batch(dtype, n):
+    """Rows and sums over a token's pairs have the bits of a small batch in a large one, where other forms of the kernels run.  (The weights' gradients need not:
+    the lanes that share a token's products are fewer where tokens are many.)"""
+    topk, few, many = 3, 40, 20000
+    g = torch.Generator(DEV).manual_seed(n)
+    idx = torch.randperm(many * topk, generator=g, device=DEV).to(torch.int32).view(many, topk)
+    x, rows = (torch.randn(r, n, generator=g, device=DEV).to(dtype) for r in (many, many * topk))
+    w = torch.rand(many, topk, generator=g, device=DEV)
+    small = torch.arange(few * topk, dtype=torch.int32, device=DEV).view(few, topk)
+    small_rows = rows[idx[:few].long().flatten()]
+    assert torch.equal(flux_amd.moe_unpermute(small_rows, small, w[:few]), flux_amd.moe_unpermute(rows, idx, w)[:few])
+    assert torch.equal(flux_amd.moe_unpermute_backward(x[:few], small_rows, small, w[:few])[0],
+                       flux_amd.moe_unpermute_backward(x, rows, idx, w)[0][idx[:few].long().flatten()])
+
+
 @pytest.mark.parametrize("topk", [1, 2, 4, 6, 8])
 @pytest.mark.parametrize("dtype,n", [(BF16, 2047), (F16, 1032), (F32, 1025), (BF16, 45), (F32, 3)])
 def test_rows_of_many_megabytes(dtype, n, topk):
