@@ -331,7 +331,8 @@ int fluxmi_topk_gather_reduce(const void *const *in, int32_t ngroups, int32_t io
  *                                  grad_rows or grad_weights may be NULL: it is not computed (and rows not read without grad_weights).
  *
  * `row_type` is the type of rows, out, grad_out and grad_rows, `weight_type` that of weights [ntokens, topk] and grad_weights (FLUXMI_ROWS_*).
- * Pointers are aligned to their elements, no more; any n; 1 <= topk <= 64; ntokens * topk <= 2^30.
+ * Pointers are aligned to their elements, no more; any n; 1 <= topk <= 64; ntokens * topk <= 2^30; row_bytes <= 2^31.  Eight lanes at least are launched for
+ * a token, and a launch has no more than 2^32 (more tokens: FLUXMI_ERR_UNSUPPORTED).
  * ---------------------------------------------------------------------------------------------- */
 #define FLUXMI_ROWS_BF16 0
 #define FLUXMI_ROWS_FP32 1
@@ -418,7 +419,9 @@ int fluxmi_quant_e4m3_block128_filled(const void *x_bf16, int64_t rows, int64_t 
  *   codes_t / scale_t (both or neither): the same of the transposed matrix, [batch, cols, 16 ceil(rows / 32)] and
  *   [batch, cols, ceil(rows / 32)], from the same read of x.
  * fluxmi_dequant_mx: codes, scale -> out [rows, cols] (FLUXMI_ROWS_*), the values they stand for (rounded where the type does not hold them: fp16).
- * Pointers are aligned to their elements, codes to 4 bytes (fluxmi_quant_mx with codes_t: that to 16); any rows and cols.
+ * Pointers are aligned to their elements, codes to 4 bytes (fluxmi_quant_mx with codes_t: that to 16).  batch <= 65535, cols <= 2^30, with codes_t rows <= 2^30.
+ * A launch has no more than 2^32 threads, of which four vectors of 16 bytes take one, and where cols is no multiple of 32 every row up to 256: what is more is
+ * FLUXMI_ERR_UNSUPPORTED.
  * ---------------------------------------------------------------------------------------------- */
 int fluxmi_quant_mx(const void *x, int32_t row_type, int64_t batch, int64_t rows, int64_t cols, void *codes, void *scale, void *codes_t,
                     void *scale_t, void *stream);
@@ -432,8 +435,11 @@ int fluxmi_dequant_mx(const void *codes, const void *scale, int64_t rows, int64_
  * A [a_rows, 16 kb] codes with scales [a_rows, kb], B [nexperts, N, 16 kb] with scales [nexperts, N, kb], kb = ceil(k / 32) (what fluxmi_quant_mx writes
  * along k).  `splits`: DEVICE int32 row counts; NULL: nexperts is 1 and all max_rows rows are its own.  Negative counts are 0.  max_rows is an upper bound
  * of their sum; rows past the sum are not touched.  Entries of gather_a are clamped into [0, a_rows).
- * Requirements: 1 <= nexperts <= 1024; a, b 16-byte aligned, d aligned to its elements; any n, k >= 1; one expert's codes and all of A below 2 GiB.
- * `workspace`: fluxmi_grouped_gemm_mx_workspace_bytes() bytes, 16-byte aligned, of any content; not shared by calls that may overlap. */
+ * Counts past max_rows are as large as what is left of it.
+ * Requirements: 1 <= nexperts <= 1024; max_rows <= 2^24; a, b 16-byte aligned, d aligned to its elements; any n, k >= 1; one expert's codes and all of A
+ * below 2 GiB.
+ * `workspace`: fluxmi_grouped_gemm_mx_workspace_bytes() bytes, 16-byte aligned, of any content; not shared by calls that may overlap.  Ask with the args of
+ * the call itself: the answer follows from the sizes and from the alignment of a_scale and b_scale (which are not read), and is 0 for many of them. */
 typedef struct fluxmi_mx_gemm_args {
   int32_t nexperts, max_rows, n, k, a_rows;
   int32_t d_type;           /* FLUXMI_ROWS_* */

@@ -96,6 +96,13 @@ def test_forms_and_workspaces():
     assert of(129, 7900, 300, 1536) == (capi.MX_TILES, 256, 0) and of(129, 7900, 300, 1536, scales_at=4) == (capi.MX_TILES, 256, padded(7900, 129 * 300, 1536))
     assert of(8, 2000, 2305, 640) == (capi.MX_DUAL, 256, 0) and of(8, 2000, 2305, 512) == (capi.MX_TILES, 256, 0)
     assert of(8, 2000, 2305, 640, a_rows=700, scales_at=2)[2] == padded(700, 8 * 2305, 640)
+    # no workspace up to 16 rows per expert, nor for K in 512s with scales on 16 bytes, whatever the sizes
+    for experts, n in ((1, 40), (3, 5000), (128, 300), (200, 2048)):
+        for k in (96, 705, 1408, 2880):
+            for at in (0, 1, 4):
+                assert of(experts, 16 * experts, n, k, scales_at=at)[2] == 0
+        for rows in (1, 50, 400, 5000, 50000):
+            assert of(experts, rows, n, 1536)[2] == 0
     # what the call itself refuses
     lib, info = capi.load(), capi.MxLaunchInfo()
     refused(lib.fluxmi_grouped_gemm_mx_launch_info(None, ctypes.byref(info)), -1, "null args")
