@@ -519,7 +519,7 @@ __global__ __launch_bounds__(kDualThreads, 2) void grouped_gemm_dual_kernel(cons
     for (int i = 0; i < 8; ++i) xs[i] = __builtin_amdgcn_perm(raw[4 + i][1], raw[4 + i][0], pick);
   };
   // Blocks past the end of K, in a tile's last pair of steps: what was read as their codes is the next row's, finite in any case, and with a scale of 2^-127 in both
-  // operands less than half of the smallest sum.
+  // operands less than half of the smallest sum.  Behind the last row there are zeros (buffer_of).
   auto mask_mx_scales = [&](int s) {
     const int kb = kbytes / 16;
     if (kb % 16 == 0) return;

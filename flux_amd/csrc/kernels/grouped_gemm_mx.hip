@@ -195,6 +195,7 @@ __device__ __forceinline__ TileItem locate_tile(const MxParams &p, int block, in
 #define FLUXMI_LGKM0() __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8))
 #define FLUXMI_VMCNT(vm) __builtin_amdgcn_s_waitcnt(((vm)&15) | (((vm) >> 4) << 14) | (7 << 4) | (15 << 8))
 
+// (Scales of a row's end are read 16 bytes at a time: words behind the last row's are zeros and not fetched, see buffer_of in grouped_gemm_rows.hpp.)
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void *base, int64_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, static_cast<int>(bytes), 0x00020000);
 }

@@ -122,6 +122,10 @@ __device__ __forceinline__ f32x4 mfma_line(const i32x4 (&w)[2], const i32x4 (&x)
   }
 }
 
+// A raw buffer.  Its bounds check is that of the instruction set's guides: out of range where the lane's offset >= bytes - the scalar offset, each word of a wide
+// load by itself; such words come as zeros and are not fetched.  So a step along K that the scalar offset takes past the last row reads nothing behind the operand.
+// (Measured with 13 pairs of sizes and scalar offsets on lane offsets around the end and from 2^31 on, in a larger allocation: the sum of both offsets counts, also
+// where the scalar one alone is past the end.)
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void *base, int64_t bytes) {
   const uint32_t n = bytes > 0xffffffffll ? 0xffffffffu : static_cast<uint32_t>(bytes < 0 ? 0 : bytes);
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, static_cast<int>(n), 0x00020000);
