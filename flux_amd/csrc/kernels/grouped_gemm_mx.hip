@@ -896,6 +896,10 @@ struct Plan {
 // The waves of a stream: one token of two experts 4096 x 14336 (256 streams) 16.3 / 13.0 / 13.4 of one, two and four that split K, with 896 (14336 x 4096) 13.8 / 15.7;
 // of 32 rows one expert 4096 x 4096, 128 rows (512 streams) 9.4 / 9.5 / 12.5, 1024 x 4096, 256 rows (256) 8.1 / 6.0 / 6.8, 128 rows (128) 8.0 / 5.9 / 5.6.  64 columns of
 // 32 rows: one expert 4096 x 14336, 256 rows (1024 streams) 46 -> 37, with fewer streams it is slower.
+// Scales that are not on words (K = 2880), few rows straight to registers / streams and panels with a copy of all scales: 32 experts of 5760 columns, 1 row each 65 / 85,
+// 16 rows 73 / 92, 20 rows 115 / 93, 48 rows 165 / 100; 128 experts of 768, 1 row 35 / 53, 16 rows 42 / 56, 20 rows 66 / 57; 8 experts of 4096, 16 rows 13.0 / 19.7, 20 to
+// 32 rows the same, 48 rows 24.1 / 21.6; only with one or two experts would 48 rows still be better off (2880 columns 11.0 / 13.0).  K = 2816, which needs neither: 32 experts of
+// 5760 columns, 1 row 51, 32 rows 60 (K = 2880: 97, of which the copy is some 20).
 // What keeps the dual tiles off (K up to 512, more than 128 experts) goes to the tiles of this file, which are slower (8 experts 14336 x 4224, 194 rows 102 -> 110, 1200 rows
 // 379 -> 431; 4095 x 14336, 600 rows 195 -> 245).  Panels of 256 rows would be as good as the dual tiles at 194 rows 4096 x 14336 (86 / 91) and worse where some experts have
 // more than 256 (4 experts of 176 and 264 rows 8192 x 4096 58 / 40).
