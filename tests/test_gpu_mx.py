@@ -585,6 +585,31 @@ def test_graph_of_a_decode_step_replays():
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("pinned", [False, True])
+def test_graph_with_row_counts_on_the_host(pinned):
+    """A replay reads the counts again from the tensor that the captured call was given."""
+    a, sa, _ = operand(40, k=256, seed=1)
+    w, sw, _ = operand(4, 70, k=256, seed=2)
+    gemm, splits = flux_amd.MxGemm(F32), torch.tensor([10, 0, 25, 5], dtype=torch.int32)
+    splits = splits.pin_memory() if pinned else splits
+    out = torch.zeros(40, 70, device=DEV)
+    gemm.forward_grouped(a, splits, w, sa, sw, output=out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        gemm.forward_grouped(a, splits, w, sa, sw, output=out)
+    for counts in ([10, 0, 25, 5], [1, 2, 3, 4], [40, 0, 0, 0], [0, 0, 0, 0]):
+        fresh = torch.tensor(counts, dtype=torch.int32)
+        want = torch.full_like(out, 9.0)
+        gemm.forward_grouped(a, fresh.to(DEV), w, sa, sw, output=want)
+        splits.copy_(fresh)
+        out.fill_(9.0)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
 def test_on_another_stream():
     a, sa, va = operand(30, k=640, seed=1)
     w, sw, vw = operand(50, k=640, seed=2)
