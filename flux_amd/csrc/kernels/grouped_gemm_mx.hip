@@ -899,7 +899,7 @@ struct Plan {
 // Scales that are not on words (K = 2880), few rows straight to registers / streams and panels with a copy of all scales: 32 experts of 5760 columns, 1 row each 65 / 85,
 // 16 rows 73 / 92, 20 rows 115 / 93, 48 rows 165 / 100; 128 experts of 768, 1 row 35 / 53, 16 rows 42 / 56, 20 rows 66 / 57; 8 experts of 4096, 16 rows 13.0 / 19.7, 20 to
 // 32 rows the same, 48 rows 24.1 / 21.6; only with one or two experts would 48 rows still be better off (2880 columns 11.0 / 13.0).  K = 2816, which needs neither: 32 experts of
-// 5760 columns, 1 row 51, 32 rows 60 (K = 2880: 97, of which the copy is some 20).
+// 5760 columns, 1 row 51, 32 rows 60 (K = 2880: 97, the copy 15 of them and the panels 80: rows of 1440 bytes do not start on lines).
 // What keeps the dual tiles off (K up to 512, more than 128 experts) goes to the tiles of this file, which are slower (8 experts 14336 x 4224, 194 rows 102 -> 110, 1200 rows
 // 379 -> 431; 4095 x 14336, 600 rows 195 -> 245).  Panels of 256 rows would be as good as the dual tiles at 194 rows 4096 x 14336 (86 / 91) and worse where some experts have
 // more than 256 (4 experts of 176 and 264 rows 8192 x 4096 58 / 40).

@@ -184,6 +184,20 @@ def test_offsets_past_32_bits():
     assert ((grad_w[probe, 5].double() - square).abs() <= (n / 8 + 16) * 2.0**-24 * square).all()
 
 
+@pytest.mark.parametrize("topk", [1, 2, 5, 8])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_unpermute_has_the_bits_of_the_gather_reduce(dtype, topk):
+    """topk_weighted_gather_reduce, whose weights lie by row: the same multiply-adds in the same order, one rounding (fp32 rows: to bf16)."""
+    tokens, n = 333, 1048
+    idx, rows = make_index(tokens, topk, 0.2, topk, shuffled=True), data(tokens * topk, n, dtype, 3)
+    w = torch.rand(tokens, topk, generator=torch.Generator().manual_seed(topk)).to(DEV)
+    by_row = torch.zeros(tokens * topk, device=DEV)
+    by_row[idx[idx >= 0].long()] = w[idx >= 0]
+    for weights, row_weight in ((w, by_row), (None, None)):
+        want = flux_amd.topk_weighted_gather_reduce([rows], idx.flatten(), topk, row_weight)
+        assert torch.equal(flux_amd.moe_unpermute(rows, idx, weights).to(want.dtype), want)
+
+
 @pytest.mark.parametrize("dtype,n", [(BF16, 2047), (F16, 1536), (F32, 7168)])
 def test_a_token_has_the_same_sums_in_every_batch(dtype, n):
     """Rows and sums over a token's pairs have the bits of a small batch in a large one, where other forms of the kernels run.  (The weights' gradients need not:
