@@ -237,7 +237,8 @@ torch::Tensor BlockScaleGemm::forward_grouped(torch::Tensor input, torch::Tensor
   TORCH_CHECK(!input_splits.is_cuda(), "input splits is not on cpu");
   TORCH_CHECK(input_splits.size(0) == weight.size(0), "splits 0-dim mismatch: ", input_splits.size(0), " != ",
               weight.size(0));
-  TORCH_CHECK(input_splits.sum().item<int64_t>() <= input.size(0), "input_splits sum exceeds the rows of input");
+  // (Counts in pinned memory, which a copy that the stream has yet to run may be about to write, are not looked at here.)
+  TORCH_CHECK(input_splits.is_pinned() || input_splits.sum().item<int64_t>() <= input.size(0), "input_splits sum exceeds the rows of input");
   TORCH_CHECK(input_scale.dim() == 3 || input_scale.dim() == 1, "input_scale must be 3-D [ceil(M/128), K/128, 128] or the "
               "reference's flat 1-D layout (per expert [K/128, M_e]); got ", input_scale.sizes());
   TORCH_CHECK(weight_scale.dim() == 3 || weight_scale.dim() == 1, "weight_scale must be 3-D [E, ceil(N/128), K/128] or the "
@@ -267,7 +268,8 @@ torch::Tensor BlockScaleGemm::forward_multistream(torch::Tensor input, torch::Te
   TORCH_CHECK(!input_splits.is_cuda(), "input splits is not on cpu");
   TORCH_CHECK(input_splits.size(0) == weight.size(0), "splits 0-dim mismatch: ", input_splits.size(0), " != ",
               weight.size(0));
-  TORCH_CHECK(input_splits.sum().item<int64_t>() <= input.size(0), "input_splits sum exceeds the rows of input");
+  // (Counts in pinned memory, which a copy that the stream has yet to run may be about to write, are not looked at here.)
+  TORCH_CHECK(input_splits.is_pinned() || input_splits.sum().item<int64_t>() <= input.size(0), "input_splits sum exceeds the rows of input");
   const int64_t m = input.size(0), kb = input.size(1) / kBlock;
   TORCH_CHECK(input_scale->is_cuda() && input_scale->scalar_type() == at::kFloat && input_scale->size(0) == m &&
                   input_scale->size(1) == kb,

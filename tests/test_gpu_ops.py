@@ -424,6 +424,33 @@ def test_row_counts_in_pinned_memory_that_the_stream_has_yet_to_write(op, stale,
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("flat", [False, True])
+def test_stale_row_counts_in_pinned_memory_are_not_refused(flat):
+    """Their sum on the host says nothing while a copy into them is pending: forward_grouped and forward_multistream take them as the stream will see them."""
+    fresh, n, k = [100, 28, 0, 72], 256, 512
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn(200, k, generator=g, device="cuda").to(torch.bfloat16)
+    q = flux_amd.Quantization(torch.bfloat16, torch.float8_e4m3fn)
+    qx, sx, _, _ = q.quantize_vector_blockwise(x, return_tranpose=False)
+    qw, sw = (torch.randn(4, n, k, generator=g, device="cuda") * 0.05).to(torch.float8_e4m3fn), torch.ones(4, n // 128, k // 128, device="cuda")
+    gemm = flux_amd.BlockScaleGemm(torch.float8_e4m3fn, torch.float8_e4m3fn, torch.bfloat16)
+    if flat:
+        rows = sx.permute(0, 2, 1).reshape(-1, k // 128)[:200].contiguous()
+        run = lambda counts: gemm.forward_multistream(qx, counts, qw, input_scale=rows, weight_scale=sw)
+    else:
+        run = lambda counts: gemm.forward_grouped(qx, counts, qw, input_scale=sx, weight_scale=sw)
+    want = run(torch.tensor(fresh, dtype=torch.int32))
+    on_device = torch.tensor(fresh, dtype=torch.int32, device="cuda")
+    pinned = torch.empty(4, dtype=torch.int32, pin_memory=True)
+    pinned.copy_(torch.tensor([1000] * 4, dtype=torch.int32))
+    busy = torch.ones(8192, 8192, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(4):  # (about 40 ms on the stream)
+        torch.mm(busy, busy)
+    pinned.copy_(on_device, non_blocking=True)
+    assert torch.equal(run(pinned), want)
+
+
 def test_blockscale_gemm_op_dense_and_grouped():
     """BlockScaleGemm.forward / forward_grouped / forward_multistream / reference (src/pybind/gemm_only.cc:77-160) fed by the Quantization op, the way
     test/python/gemm_only/test_blockwise_scale_gemm_only.py drives them: both scale layouts of forward_grouped."""
