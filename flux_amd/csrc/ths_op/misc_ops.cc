@@ -183,7 +183,7 @@ static torch::Tensor blockscale_run(const torch::Tensor &input, const torch::Ten
     out = torch::empty({m, n}, input.options().dtype(out_dtype));
   }
   if (m == 0) return out;
-  const torch::Tensor splits_host = splits_cpu.to(at::kInt).contiguous();
+  const torch::Tensor splits_host = host_counts(splits_cpu);
   fluxmi_grouped_gemm_args args{};
   args.dtype = FLUXMI_FP8_E4M3;
   args.nexperts = static_cast<int32_t>(e);
@@ -210,6 +210,12 @@ static torch::Tensor blockscale_run(const torch::Tensor &input, const torch::Ten
   return out;
 }
 
+// The row count of a product of one weight matrix.  In a graph a kernel writes it: a replay would read it from a host tensor that is gone by then.
+static torch::Tensor all_rows(const torch::Tensor &input) {
+  const at::TensorOptions counts = at::TensorOptions().dtype(at::kInt);
+  return torch::full({1}, input.size(0), stream_is_captured() ? counts.device(input.device()) : counts);
+}
+
 torch::Tensor BlockScaleGemm::forward(torch::Tensor input, torch::Tensor weight, std::optional<torch::Tensor> bias,
                                       std::optional<torch::Tensor> output, std::optional<torch::Tensor> input_scale,
                                       std::optional<torch::Tensor> weight_scale) {
@@ -219,7 +225,7 @@ torch::Tensor BlockScaleGemm::forward(torch::Tensor input, torch::Tensor weight,
   FLUX_AMD_CHECK_INPUT(weight, weight_dtype_);
   FLUX_AMD_CHECK_NDIM(input, 2);
   FLUX_AMD_CHECK_NDIM(weight, 2);
-  torch::Tensor splits = torch::full({1}, input.size(0), at::TensorOptions().dtype(at::kInt));
+  torch::Tensor splits = all_rows(input);
   TORCH_CHECK(weight_scale->dim() == 2, "weight_scale must be [ceil(N/128), K/128], got ", weight_scale->sizes());
   return blockscale_run(input, weight.unsqueeze(0), splits, output, *input_scale, FLUXMI_ASCALE_BLOCK128,
                         weight_scale->unsqueeze(0), FLUXMI_BSCALE_N_K, output_dtype_);
@@ -300,7 +306,7 @@ torch::Tensor BlockScaleGemm::reference(torch::Tensor input, torch::Tensor weigh
   FLUX_AMD_CHECK_NDIM(input, 2);
   FLUX_AMD_CHECK_NDIM(weight, 2);
   TORCH_CHECK(weight_scale->dim() == 3, "per-column weight_scale must be [ceil(N/128), K/128, 128], got ", weight_scale->sizes());
-  torch::Tensor splits = torch::full({1}, input.size(0), at::TensorOptions().dtype(at::kInt));
+  torch::Tensor splits = all_rows(input);
   return blockscale_run(input, weight.unsqueeze(0), splits, output, *input_scale, FLUXMI_ASCALE_BLOCK128,
                         weight_scale->unsqueeze(0), FLUXMI_BSCALE_COL_N_K, output_dtype_);
 }

@@ -152,11 +152,22 @@ fluxmi_grouped_gemm_args gemm_args(const torch::Tensor &a, const torch::Tensor &
 }
 }  // namespace
 
+bool stream_is_captured() {
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  return hipStreamIsCapturing(static_cast<hipStream_t>(current_stream()), &capture) != hipSuccess || capture != hipStreamCaptureStatusNone;
+}
+
+torch::Tensor host_counts(const torch::Tensor &splits) {
+  const torch::Tensor counts = splits.to(at::kInt).contiguous();
+  TORCH_CHECK(counts.is_same(splits) || !stream_is_captured(), "row counts on the host must be contiguous int32 in a captured call, got ", splits.scalar_type(),
+              " with strides ", splits.strides());
+  return counts;
+}
+
 bool run_host_splits(const fluxmi_grouped_gemm_args &args, const torch::Tensor &splits, const float *row_scale2, const float *a_scale,
                      int32_t a_layout, const float *b_scale, int32_t b_layout) {
   hipStream_t stream = static_cast<hipStream_t>(current_stream());
-  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(stream, &capture) != hipSuccess || capture != hipStreamCaptureStatusNone) return false;
+  if (stream_is_captured()) return false;
   if (splits.is_cuda() || splits.is_pinned()) return false;
   const int rc = fluxmi_grouped_gemm_host_counts(&args, splits.data_ptr<int32_t>(), row_scale2, a_scale, a_layout, b_scale, b_layout, stream);
   if (rc < 0) check_status(rc, "fluxmi_grouped_gemm_host_counts");
@@ -406,7 +417,7 @@ torch::Tensor GemmGroupedV3GatherRS::forward_impl(
   const bool f16 = st == at::ScalarType::Half;
   torch::Tensor out = torch::empty({ntokens, n_dim_}, inputs[0].options().dtype(moe_output_dtype(st)));
   if (global_m == 0) return out;
-  const torch::Tensor splits_host = splits_cpu.contiguous();
+  const torch::Tensor splits_host = host_counts(splits_cpu);
   bool splits_on_device = false;
   auto splits_to_device = [&]() {
     if (!splits_on_device) splits_dev_.copy_(splits_host, /*non_blocking=*/true);
@@ -604,7 +615,7 @@ torch::Tensor GemmGroupedV3::forward(torch::Tensor input, torch::Tensor splits_c
               weight_.size(0));
   torch::Tensor out = torch::empty({input.size(0), weight_.size(1)}, input.options().dtype(moe_output_dtype(input.scalar_type())));
   if (input.size(0) == 0) return out;
-  const torch::Tensor splits_host = splits_cpu.to(at::kInt).contiguous();
+  const torch::Tensor splits_host = host_counts(splits_cpu);
   fluxmi_grouped_gemm_args args = gemm_args(input, weight_, nullptr, out, nullptr, input.size(0), nullptr, nullptr, nullptr, nullptr, 0);
   if (run_host_splits(args, splits_host, nullptr)) return out;
   const torch::Tensor splits_dev = splits_host.to(input.device(), /*non_blocking=*/true);

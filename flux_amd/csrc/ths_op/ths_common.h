@@ -85,6 +85,12 @@ struct DistEnvTPWithEP {  // include/flux/ths_op/ths_op.h:117-130; only world si
 bool run_host_splits(const fluxmi_grouped_gemm_args &args, const torch::Tensor &splits, const float *row_scale2,
                      const float *a_scale = nullptr, int32_t a_layout = 0, const float *b_scale = nullptr, int32_t b_layout = 0);
 
+// Whether the current stream is being captured into a graph.
+bool stream_is_captured();
+
+// Row counts as the kernels take them, contiguous int32 on the host.  A replay of a captured call copies them again, so there they have to be the caller's own memory.
+torch::Tensor host_counts(const torch::Tensor &splits);
+
 // Launch tuning of a grouped GEMM: CUs to leave free (Flux's sm_margin) and the tile schedule registered
 // for the problem's shape, if any.
 void apply_launch_tuning(fluxmi_grouped_gemm_args &args, int32_t ngroups, int64_t sm_margin);

@@ -451,6 +451,53 @@ def test_stale_row_counts_in_pinned_memory_are_not_refused(flat):
     assert torch.equal(run(pinned), want)
 
 
+@pytest.mark.parametrize("m,n,k", [(5, 256, 512), (200, 256, 512), (2000, 1024, 512)])
+def test_captured_dense_block_scaled_product(m, n, k):
+    """The row count of a product of one weight matrix is the op's own: it lives as long as the graph."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x, w = torch.randn(m, k, generator=g, device="cuda").to(torch.bfloat16), (torch.randn(n, k, generator=g, device="cuda") * 0.05).to(torch.bfloat16)
+    q = flux_amd.Quantization(torch.bfloat16, torch.float8_e4m3fn)
+    qx, sx, _, _ = q.quantize_vector_blockwise(x, return_tranpose=False)
+    qw, sw, _, _ = q.quantize_square_blockwise(w, return_tranpose=False)
+    gemm, out = flux_amd.BlockScaleGemm(torch.float8_e4m3fn, torch.float8_e4m3fn, torch.bfloat16), torch.zeros(m, n, dtype=torch.bfloat16, device="cuda")
+    want = gemm.forward(qx, qw, input_scale=sx, weight_scale=sw)
+    gemm.forward(qx, qw, output=out, input_scale=sx, weight_scale=sw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gemm.forward(qx, qw, output=out, input_scale=sx, weight_scale=sw)
+    for seed in range(3):
+        kept = [torch.full((1,), v, dtype=torch.int32) for v in (0, 1, m // 2, -3) for _ in range(50)]  # host memory that was free is in use again
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and len(kept) == 200
+
+
+def test_captured_row_counts_that_would_not_last_are_refused():
+    """Counts that the op would convert or gather into a tensor of its own are read again by every replay: in a captured call they have to be as the kernels take
+    them.  Outside of one they are converted."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, w = torch.randn(60, 256, generator=g, device="cuda").to(torch.bfloat16), torch.randn(3, 128, 256, generator=g, device="cuda").to(torch.bfloat16)
+    gemm, counts = flux_amd.GemmGroupedV3(w, 3), torch.tensor([20, 0, 40])
+    want = gemm.forward(x, counts)
+    assert torch.equal(want, gemm.forward(x, counts.to(torch.int32)))
+    assert torch.equal(want, gemm.forward(x, torch.tensor([[20, 9], [0, 9], [40, 9]], dtype=torch.int32)[:, 0]))
+    torch.cuda.synchronize()
+    for bad in (counts, torch.tensor([[20, 9], [0, 9], [40, 9]], dtype=torch.int32)[:, 0]):
+        with pytest.raises(RuntimeError, match="contiguous int32 in a captured call"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                gemm.forward(x, bad)
+    graph, counts = torch.cuda.CUDAGraph(), counts.to(torch.int32)
+    with torch.cuda.graph(graph):
+        got = gemm.forward(x, counts)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
 def test_blockscale_gemm_op_dense_and_grouped():
     """BlockScaleGemm.forward / forward_grouped / forward_multistream / reference (src/pybind/gemm_only.cc:77-160) fed by the Quantization op, the way
     test/python/gemm_only/test_blockwise_scale_gemm_only.py drives them: both scale layouts of forward_grouped."""
