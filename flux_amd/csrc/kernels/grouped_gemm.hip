@@ -27,13 +27,13 @@ __global__ __launch_bounds__(256) void grouped_gemm_generic_kernel(const GemmPar
     int acc = 0;
     for (int e = 0; e < p.nexperts; ++e) {
       s_row_off[e] = acc;
-      const int v = p.splits[e];
-      acc += v > 0 ? v : 0;
+      const int v = p.splits[e], rest = p.max_rows - acc;
+      acc += v > 0 ? (v < rest ? v : rest) : 0;
     }
     s_row_off[p.nexperts] = acc;
   }
   __syncthreads();
-  const int total_rows = s_row_off[p.nexperts] < p.max_rows ? s_row_off[p.nexperts] : p.max_rows;
+  const int total_rows = s_row_off[p.nexperts];
   float scalar = p.scalar;
   if (p.scalar_dev) scalar *= p.scalar_dev[0];
   const int ncol_blocks = (p.n + 255) / 256;

@@ -1595,7 +1595,7 @@ __global__ __launch_bounds__(NTHREADS) void grouped_gemm_mfma_kernel(const GemmP
     for (int e0 = 0; e0 < p.nexperts; e0 += 64) {
       const int ee = e0 + lane;
       int rows = ee < p.nexperts ? p.splits[ee] : 0;
-      if (rows < 0) rows = 0;
+      rows = rows < 0 ? 0 : (rows > p.max_rows ? p.max_rows : rows);  // (counts past the rows do not overflow the sums)
       const int incl = wave_inclusive_scan(rows);
       int begin = row_carry + incl - rows, end = row_carry + incl;
       if (begin > p.max_rows) begin = p.max_rows;
@@ -1613,7 +1613,7 @@ __global__ __launch_bounds__(NTHREADS) void grouped_gemm_mfma_kernel(const GemmP
       }
       acc_tiles += tiles;
       acc_cand += cand;
-      row_carry += __shfl(incl, 63, 64);
+      row_carry = __shfl(end, 63, 64);
     }
     if (p.by_splits && chunks <= stream_chunks_limit(active, p.by_splits, ELT == 1, p.chunk_items, p.round_items)) return;  // the other form runs this launch
     total_tiles = __builtin_amdgcn_readfirstlane(acc_tiles);

@@ -46,14 +46,14 @@ __device__ __forceinline__ WorkItem locate(const GemmParams &p, int tiles_n, int
     const int ee = e0 + lane;
     int r = 0;
     if (ee < p.nexperts) r = args->count > 0 ? args->splits[ee] : p.splits[ee];
-    if (r < 0) r = 0;
+    r = r < 0 ? 0 : (r > p.max_rows ? p.max_rows : r);  // (counts past the rows do not overflow the sums)
     const int incl = wave_inclusive_scan(r);
     begin = row_carry + incl - r;
     int end = row_carry + incl;
     if (begin > p.max_rows) begin = p.max_rows;
     if (end > p.max_rows) end = p.max_rows;
     rows = end - begin;
-    row_carry += __builtin_amdgcn_readlane(incl, 63);
+    row_carry = __builtin_amdgcn_readlane(end, 63);
     chunks_end = chunk_carry + wave_inclusive_scan((rows + chunk_rows - 1) / chunk_rows);
     chunk_carry = __builtin_amdgcn_readlane(chunks_end, 63);
     return __popcll(__ballot(rows > 0));

@@ -105,7 +105,7 @@ int fluxmi_moe_gather_index(const int32_t *scatter_index, int32_t nrows, int32_t
  * type of `dtype` (bf16 for bf16 and fp8 operands, fp16 for fp16 operands; "bf16" below stands for that type).
  * `splits` is a DEVICE int32 array of `nexperts` row counts; the tile schedule is derived from it on
  * the device, so the host never reads it.  `max_rows` is an upper bound of sum(splits) (ntokens*topk);
- * rows beyond sum(splits) are not touched.
+ * rows beyond sum(splits) are not touched.  Negative counts are 0, and counts past max_rows as large as what is left of it.
  *
  * Limits: 1 <= nexperts <= 1024 (FLUXMI_ERR_UNSUPPORTED beyond).  Two kernels stand behind the call.  The
  * MFMA kernel takes every shape with
