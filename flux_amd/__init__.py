@@ -31,7 +31,8 @@ _THS_NAMES = (
     "MoeArguments", "DistEnvTPWithEP", "GemmGroupedV3AGScatter", "GemmGroupedV3GatherRS", "GemmGroupedV3",
     "Quantization", "BlockScaleGemm", "MxGemm", "calc_scatter_index", "topk_scatter_reduce", "bitwise_check", "init_flux_shm",
     "moe_route_sort", "topk_weighted_gather_reduce", "moe_permute", "moe_permute_backward", "moe_unpermute",
-    "moe_unpermute_backward", "uniform_initialize", "load_tuning_record",
+    "moe_unpermute_backward", "moe_linear", "moe_swiglu", "moe_mlp", "moe_dgrad", "moe_wgrad", "moe_checkpoint", "moe_swiglu_checkpoint",
+    "moe_swiglu_backward", "uniform_initialize", "load_tuning_record",
     "ProfilingContext", "TuningRecord", "load_tuning_text",
 )
 _ths = None

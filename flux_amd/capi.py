@@ -34,7 +34,8 @@ EXPORTS = (
     "fluxmi_grouped_gemm_topk_reduce", "fluxmi_grouped_gemm_blockscale",
     "fluxmi_topk_gather_reduce", "fluxmi_moe_permute", "fluxmi_moe_unpermute", "fluxmi_moe_unpermute_backward", "fluxmi_quant_e4m3_rowwise", "fluxmi_quant_e4m3_square",
     "fluxmi_quant_e4m3_block128", "fluxmi_quant_e4m3_block128_filled", "fluxmi_calib_stream_sink_bytes", "fluxmi_calib_stream",
-    "fluxmi_quant_mx", "fluxmi_dequant_mx", "fluxmi_grouped_gemm_mx_workspace_bytes", "fluxmi_grouped_gemm_mx",
+    "fluxmi_moe_dgrad", "fluxmi_moe_wgrad_workspace_bytes", "fluxmi_moe_wgrad", "fluxmi_moe_clear_rest", "fluxmi_checkpoint_e4m3", "fluxmi_swiglu",
+    "fluxmi_swiglu_backward", "fluxmi_quant_mx", "fluxmi_dequant_mx", "fluxmi_grouped_gemm_mx_workspace_bytes", "fluxmi_grouped_gemm_mx",
     "fluxmi_grouped_gemm_mx_launch_info",
 )
 
@@ -112,6 +113,14 @@ def load():
     lib.fluxmi_moe_permute.argtypes = [vp, vp, i32, i32, i64, vp, vp]
     lib.fluxmi_moe_unpermute.argtypes = [vp, i32, vp, vp, i32, i32, i32, i32, vp, vp]
     lib.fluxmi_moe_unpermute_backward.argtypes = [vp, vp, i32, vp, vp, i32, i32, i32, i32, vp, vp, vp]
+    lib.fluxmi_moe_dgrad.argtypes = [vp, vp, i32, vp, i32, i64, i64, i64, vp, vp]
+    lib.fluxmi_moe_wgrad_workspace_bytes.restype = sz
+    lib.fluxmi_moe_wgrad_workspace_bytes.argtypes = [i32, i64, i64, i64]
+    lib.fluxmi_moe_wgrad.argtypes = [vp, vp, vp, i32, vp, i32, i64, i64, i64, vp, i32, i32, vp, sz, vp]
+    lib.fluxmi_moe_clear_rest.argtypes = [vp, vp, i32, i64, i64, vp]
+    lib.fluxmi_checkpoint_e4m3.argtypes = [vp, i32, i64, i64, vp, vp, vp]
+    lib.fluxmi_swiglu.argtypes = [vp, i32, i64, i64, vp, vp, vp, vp]
+    lib.fluxmi_swiglu_backward.argtypes = [vp, vp, vp, i32, i64, i64, vp, vp, vp]
     lib.fluxmi_quant_e4m3_rowwise.argtypes = [vp, i64, i64, i32, f32, vp, vp, i32, vp]
     lib.fluxmi_quant_e4m3_square.argtypes = [vp, i64, i64, i64, f32, vp, vp, vp, vp, vp]
     lib.fluxmi_quant_e4m3_block128.argtypes = [vp, i64, i64, f32, vp, vp, vp, vp, vp]
@@ -464,6 +473,65 @@ def moe_unpermute(rows, scatter_index, weights=None):
                                     1 if weights is None else _ROW_TYPES[weights.dtype], tokens, topk, rows.shape[1], _ptr(out),
                                     _stream()), "fluxmi_moe_unpermute")
     return out
+
+
+def _splits_rows(rows, splits, name):
+    _dev_tensor(rows, rows.dtype, name)
+    _dev_tensor(splits, torch.int32, "splits")
+    if rows.dtype not in (torch.bfloat16, torch.float16) or rows.dim() != 2:
+        raise ValueError(f"{name} must be bf16 or fp16 with 2 dimensions, got {rows.dtype} {tuple(rows.shape)}")
+
+
+def moe_dgrad(grad, weight, splits):
+    """grad [rows, N], weight [E, N, K] -> grad[r] @ weight[e(r)] [rows, K] (fluxmi_moe_dgrad); rows of no expert are 0."""
+    lib = load()
+    _splits_rows(grad, splits, "grad")
+    _dev_tensor(weight, grad.dtype, "weight")
+    if weight.dim() != 3 or weight.shape[:2] != (splits.numel(), grad.shape[1]):
+        raise ValueError(f"weight {tuple(weight.shape)} is not [{splits.numel()}, {grad.shape[1]}, K]")
+    out = torch.empty(grad.shape[0], weight.shape[2], dtype=grad.dtype, device=grad.device)
+    _check(lib.fluxmi_moe_dgrad(_ptr(grad), _ptr(weight), _ROW_TYPES[grad.dtype], _ptr(splits), splits.numel(), grad.shape[0], grad.shape[1], weight.shape[2],
+                                _ptr(out), _stream()), "fluxmi_moe_dgrad")
+    return out
+
+
+def moe_wgrad(grad, x, splits, x_scale=None, out_dtype=None, out=None, accumulate=False):
+    """grad [rows, N], x [rows, K] (with x_scale: codes of checkpoint_e4m3) -> grad[rows of e].T @ x[rows of e] [E, N, K] (fluxmi_moe_wgrad)."""
+    lib = load()
+    _splits_rows(grad, splits, "grad")
+    _dev_tensor(x, grad.dtype if x_scale is None else torch.float8_e4m3fn, "x")
+    rows, n, k, e = grad.shape[0], grad.shape[1], x.shape[1], splits.numel()
+    if x.dim() != 2 or x.shape[0] != rows:
+        raise ValueError(f"x {tuple(x.shape)} is not [{rows}, K]")
+    if x_scale is not None:
+        _dev_tensor(x_scale, torch.float8_e8m0fnu, "x_scale")
+        if x_scale.shape != (rows, -(-k // 32)):
+            raise ValueError(f"x_scale {tuple(x_scale.shape)} is not [{rows}, {-(-k // 32)}]")
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate needs an output")
+        out = torch.empty(e, n, k, dtype=out_dtype or grad.dtype, device=grad.device)
+    _dev_tensor(out, out.dtype, "out")
+    if out.dtype not in (grad.dtype, torch.float32) or out.shape != (e, n, k):
+        raise ValueError(f"out must be {grad.dtype} or fp32 [{e}, {n}, {k}], got {out.dtype} {tuple(out.shape)}")
+    ws_bytes = lib.fluxmi_moe_wgrad_workspace_bytes(e, rows, n, k)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=grad.device) if ws_bytes else None
+    _check(lib.fluxmi_moe_wgrad(_ptr(grad), _ptr(x), _ptr(x_scale), _ROW_TYPES[grad.dtype], _ptr(splits), e, rows, n, k, _ptr(out), _ROW_TYPES[out.dtype],
+                                int(accumulate), _ptr(ws), ws_bytes, _stream()), "fluxmi_moe_wgrad")
+    return out
+
+
+def checkpoint_e4m3(x):
+    """x [rows, K] bf16 or fp16 -> codes e4m3 [rows, K], scale e8m0 [rows, ceil(K / 32)] (fluxmi_checkpoint_e4m3)."""
+    lib = load()
+    _dev_tensor(x, x.dtype, "x")
+    if x.dtype not in (torch.bfloat16, torch.float16) or x.dim() != 2:
+        raise ValueError(f"x must be bf16 or fp16 with 2 dimensions, got {x.dtype} {tuple(x.shape)}")
+    rows, cols = x.shape
+    codes = torch.empty(rows, cols, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty(rows, -(-cols // 32), dtype=torch.float8_e8m0fnu, device=x.device)
+    _check(lib.fluxmi_checkpoint_e4m3(_ptr(x), _ROW_TYPES[x.dtype], rows, cols, _ptr(codes), _ptr(scale), _stream()), "fluxmi_checkpoint_e4m3")
+    return codes, scale
 
 
 def quant_e4m3(x, block_cols=0, eps=0.0, permute_scale=False, out=None):

@@ -1,0 +1,338 @@
+// Activation checkpoints in 8 bits, and the gated activation between an expert's two products.
+//
+//   block of 32 values of a row, m its largest magnitude, f the biased fp32 exponent of m:
+//     b = 255 and codes 0 where the block holds an infinity or a NaN, else max(f - 8 + (m > 1.75 * 2^(f - 127)), 0): the least scale
+//         2^(b - 127) with m <= 448 times the scale, so that no code saturates
+//     code = e4m3(x / 2^(b - 127)), ties to even; x beyond 15/8 times the type's largest power of two counts as that much, because the next code
+//         up stands for a value that the type does not hold
+//   out = silu(g) u, silu(g) = g s, s = 1 / (1 + exp(-g))
+//   backwards, d the gradient of out: dg = d u s (1 + g (1 - s)), du = d g s
+//
+// All of it is fp32 inside, with one rounding to 16 bits at the end; values of a checkpoint are exact in fp32, scales and codes are exact up to the
+// code's own rounding.
+#include "rows.hpp"
+
+namespace fluxmi {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBlock = 32;
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(1)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// Largest magnitude that a code may stand for: 15/8 times the type's largest power of two, as a pattern of the type.
+template <Row T>
+constexpr uint32_t kLargest = T == Row::BF16 ? 0x7f70u : 0x7b80u;
+
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  return __uint_as_float(byte == 0 ? 0x00400000u : (byte == 255 ? 0x7fc00000u : byte << 23));
+}
+
+// The maximum of 4 neighbouring lanes, in each of them.
+__device__ __forceinline__ uint32_t max_of_4_lanes(uint32_t m) {
+  auto with = [&](uint32_t o) { return m > o ? m : o; };
+  m = with(__builtin_amdgcn_mov_dpp(m, 0xb1, 0xf, 0xf, false));  // quad_perm [1,0,3,2]
+  m = with(__builtin_amdgcn_mov_dpp(m, 0x4e, 0xf, 0xf, false));  // quad_perm [2,3,0,1]
+  return m;
+}
+
+// The largest pattern without sign of a vector's eight values.
+template <Row T>
+__device__ __forceinline__ uint32_t vector_max(const u32x4 v) {
+  u16x2 m = __builtin_bit_cast(u16x2, v[0] & 0x7fff7fffu);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu));
+  return m[0] > m[1] ? m[0] : m[1];
+}
+
+template <Row T>
+__device__ __forceinline__ uint32_t scale_byte(uint32_t largest) {
+  const uint32_t bits = T == Row::BF16 ? largest << 16 : __float_as_uint(f16_bits_to_float(static_cast<uint16_t>(largest)));
+  const uint32_t f = bits >> 23, b = f + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return f == 255 ? 255 : (b > 8 ? b - 8 : 0);
+}
+
+// Eight codes.
+template <Row T>
+__device__ __forceinline__ u32x2 codes_of(const u32x4 v, uint32_t byte) {
+  u32x2 c;
+  const float scale = __uint_as_float(byte == 0 ? 0x00400000u : byte << 23);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t pair[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t w = v[2 * i + j], a = w & 0x7fff7fffu;
+      const u16x2 most = {static_cast<uint16_t>(kLargest<T>), static_cast<uint16_t>(kLargest<T>)};
+      pair[j] = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, a), most)) | (w & 0x80008000u);
+    }
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    s16x2 two = {0, 0};
+    if constexpr (T == Row::BF16) {
+      two = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(two, __builtin_bit_cast(bf16x2, pair[0]), scale, false);
+      two = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(two, __builtin_bit_cast(bf16x2, pair[1]), scale, true);
+    } else {
+      two = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(two, __builtin_bit_cast(f16x2, pair[0]), scale, false);
+      two = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(two, __builtin_bit_cast(f16x2, pair[1]), scale, true);
+    }
+    c[i] = byte == 255 ? 0u : __builtin_bit_cast(uint32_t, two);
+  }
+  return c;
+}
+
+// `count` of a vector's eight values, zeros behind them; all of them where count >= 8.
+template <Row T>
+__device__ __forceinline__ u32x4 load_some(const uint8_t *p, int count) {
+  if (count >= 8) return load16(p);
+  u32x4 v = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < count) v[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(p)[i]) << (16 * (i & 1));
+  return v;
+}
+__device__ __forceinline__ void store_some(uint8_t *p, const u32x4 v, int count) {
+  if (count >= 8) {
+    store16(p, v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 7; ++i)
+    if (i < count) reinterpret_cast<uint16_t *>(p)[i] = static_cast<uint16_t>(v[i / 2] >> (16 * (i & 1)));
+}
+__device__ __forceinline__ u32x2 load_codes(const uint8_t *p, int count) {
+  if (count >= 8) return *reinterpret_cast<const u32x2_any *>(p);
+  u32x2 v = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < count) v[i / 4] |= static_cast<uint32_t>(p[i]) << (8 * (i & 3));
+  return v;
+}
+__device__ __forceinline__ void store_codes(uint8_t *p, const u32x2 c, int count) {
+  if (count >= 8) {
+    *reinterpret_cast<u32x2_any *>(p) = c;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 7; ++i)
+    if (i < count) p[i] = static_cast<uint8_t>(c[i / 4] >> (8 * (i & 3)));
+}
+
+// Eight codes' values.
+__device__ __forceinline__ void values_of(const u32x2 c, uint32_t byte, float (&x)[8]) {
+  const float scale = scale_value(byte);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(c[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(c[i], true);
+    x[4 * i] = lo[0] * scale;
+    x[4 * i + 1] = lo[1] * scale;
+    x[4 * i + 2] = hi[0] * scale;
+    x[4 * i + 3] = hi[1] * scale;
+  }
+}
+
+__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __expf(-g)); }
+
+// ---- a row's vectors -----------------------------------------------------------------------------------------
+// A group of 2^lanes_log lanes has a row, or a piece of one where a row has more vectors than a workgroup has lanes.  Lane l of the group has the
+// vectors l, l + lanes, .. of the piece; four neighbouring lanes have a block.
+struct RowsArgs {
+  const uint8_t *x, *grad;
+  const uint8_t *in_scale;
+  uint8_t *out, *grad_x;
+  uint8_t *codes, *scale;
+  int64_t rows;
+  int32_t cols;    // of one half
+  int32_t blocks;  // of one half: ceil(cols / 32)
+  int32_t lanes_log, pieces, pad;
+};
+
+struct Place {
+  int64_t row;
+  int col;  // first of a vector's columns
+  bool any;
+};
+__device__ __forceinline__ Place place_of(const RowsArgs &a) {
+  const int group = threadIdx.x >> a.lanes_log, lane = threadIdx.x & ((1 << a.lanes_log) - 1);
+  const int64_t item = static_cast<int64_t>(blockIdx.x) / a.pieces;
+  const int piece = static_cast<int>(blockIdx.x - item * a.pieces);
+  Place p;
+  p.row = item * (kThreads >> a.lanes_log) + group;
+  p.col = ((piece << a.lanes_log) + lane) * 8;
+  p.any = p.row < a.rows && p.col < a.blocks * kBlock;
+  return p;
+}
+
+template <Row T, bool GATED, bool KEEP>
+__global__ __launch_bounds__(kThreads) void checkpoint_kernel(const RowsArgs a) {
+  const Place p = place_of(a);
+  if (!p.any) return;  // (whole blocks of four lanes)
+  const int count = a.cols - p.col;
+  constexpr int halves = GATED ? 2 : 1;
+  const uint8_t *x = a.x + (p.row * halves * a.cols + p.col) * 2;
+  u32x4 v[halves];
+#pragma unroll
+  for (int h = 0; h < halves; ++h) v[h] = count > 0 ? load_some<T>(x + static_cast<int64_t>(h) * a.cols * 2, count) : u32x4{0u, 0u, 0u, 0u};
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int h = 0; h < halves; ++h) {
+      const uint32_t byte = scale_byte<T>(max_of_4_lanes(vector_max<T>(v[h])));
+      if (count > 0) store_codes(a.codes + (p.row * halves + h) * a.cols + p.col, codes_of<T>(v[h], byte), count);
+      if ((p.col & (kBlock - 1)) == 0) a.scale[(p.row * halves + h) * a.blocks + (p.col >> 5)] = static_cast<uint8_t>(byte);
+    }
+  }
+  if constexpr (GATED) {
+    if (count <= 0) return;
+    float g[8], u[8], o[8];
+    unpack<T>(v[0], g);
+    unpack<T>(v[1], u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = g[i] * sigmoid(g[i]) * u[i];
+    store_some(a.out + (p.row * a.cols + p.col) * 2, pack<T>(o), count);
+  }
+}
+
+// KEPT: from codes and scales, otherwise from 16 bits.
+template <Row T, bool KEPT>
+__global__ __launch_bounds__(kThreads) void swiglu_backward_kernel(const RowsArgs a) {
+  const Place p = place_of(a);
+  const int count = a.cols - p.col;
+  if (!p.any || count <= 0) return;
+  float g[8], u[8], d[8], dg[8], du[8], o[8];
+  if constexpr (KEPT) {
+    const uint8_t *c = a.x + p.row * 2 * a.cols + p.col, *s = a.in_scale + p.row * 2 * a.blocks + (p.col >> 5);
+    const u32x2 cg = load_codes(c, count), cu = load_codes(c + a.cols, count);
+    values_of(cg, s[0], g);
+    values_of(cu, s[a.blocks], u);
+  } else {
+    const uint8_t *x = a.x + (p.row * 2 * a.cols + p.col) * 2;
+    unpack<T>(load_some<T>(x, count), g);
+    unpack<T>(load_some<T>(x + static_cast<int64_t>(a.cols) * 2, count), u);
+  }
+  const int64_t at = (p.row * a.cols + p.col) * 2;
+  unpack<T>(load_some<T>(a.grad + at, count), d);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float s = sigmoid(g[i]), silu = g[i] * s;
+    o[i] = silu * u[i];
+    du[i] = d[i] * silu;
+    dg[i] = d[i] * u[i] * s * (1.f + g[i] * (1.f - s));
+  }
+  uint8_t *gx = a.grad_x + (p.row * 2 * a.cols + p.col) * 2;
+  store_some(gx, pack<T>(dg), count);
+  store_some(gx + static_cast<int64_t>(a.cols) * 2, pack<T>(du), count);
+  if (a.out != nullptr) store_some(a.out + at, pack<T>(o), count);
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------
+int check_rows(const char *who, int32_t type, int64_t rows, int64_t cols, Row *row) {
+  FLUXMI_REQUIRE(type == FLUXMI_ROWS_BF16 || type == FLUXMI_ROWS_FP16, FLUXMI_ERR_INVALID_ARG, "%s: type %d (bf16 and fp16 are built)", who, type);
+  FLUXMI_REQUIRE(rows >= 0 && cols >= 0, FLUXMI_ERR_INVALID_ARG, "%s: negative rows or columns", who);
+  FLUXMI_REQUIRE(cols <= (1 << 30), FLUXMI_ERR_UNSUPPORTED, "%s: more than 2^30 columns", who);
+  *row = type == FLUXMI_ROWS_BF16 ? Row::BF16 : Row::F16;
+  return FLUXMI_OK;
+}
+
+bool even(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
+
+// Lanes and workgroups; *blocks = 0: nothing to do.
+int plan_rows(const char *who, RowsArgs *a, uint32_t *grid) {
+  *grid = 0;
+  if (a->rows == 0 || a->cols == 0) return FLUXMI_OK;
+  a->blocks = (a->cols + kBlock - 1) / kBlock;
+  const int vectors = a->blocks * 4;
+  a->lanes_log = 2;
+  while (a->lanes_log < 8 && (1 << a->lanes_log) < vectors) ++a->lanes_log;
+  a->pieces = (vectors + (1 << a->lanes_log) - 1) >> a->lanes_log;
+  const int per = kThreads >> a->lanes_log;
+  const int64_t groups = (a->rows + per - 1) / per;
+  FLUXMI_REQUIRE(groups <= ((int64_t{1} << 32) / kThreads - 1) / a->pieces, FLUXMI_ERR_UNSUPPORTED, "%s: too many rows for one launch", who);
+  *grid = static_cast<uint32_t>(groups * a->pieces);
+  return FLUXMI_OK;
+}
+
+template <class F>
+void by_half(Row t, F &&f) {
+  if (t == Row::BF16) f(std::integral_constant<Row, Row::BF16>{});
+  else f(std::integral_constant<Row, Row::F16>{});
+}
+
+}  // namespace
+}  // namespace fluxmi
+
+using namespace fluxmi;
+
+extern "C" int fluxmi_checkpoint_e4m3(const void *x, int32_t row_type, int64_t rows, int64_t cols, void *codes, void *scale, void *stream) {
+  Row type;
+  if (const int rc = check_rows("checkpoint_e4m3", row_type, rows, cols, &type)) return rc;
+  RowsArgs a{};
+  a.rows = rows;
+  a.cols = static_cast<int32_t>(cols);
+  uint32_t grid;
+  if (const int rc = plan_rows("checkpoint_e4m3", &a, &grid)) return rc;
+  if (grid == 0) return FLUXMI_OK;
+  FLUXMI_REQUIRE(x && codes && scale, FLUXMI_ERR_INVALID_ARG, "checkpoint_e4m3: null pointer");
+  FLUXMI_REQUIRE(even(x), FLUXMI_ERR_INVALID_ARG, "checkpoint_e4m3: x is not aligned to its elements");
+  a.x = static_cast<const uint8_t *>(x);
+  a.codes = static_cast<uint8_t *>(codes);
+  a.scale = static_cast<uint8_t *>(scale);
+  by_half(type, [&](auto T) {
+    checkpoint_kernel<decltype(T)::value, false, true><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+  });
+  FLUXMI_HIP_CHECK(hipGetLastError());
+  return FLUXMI_OK;
+}
+
+extern "C" int fluxmi_swiglu(const void *x, int32_t row_type, int64_t rows, int64_t cols, void *out, void *codes, void *scale, void *stream) {
+  Row type;
+  if (const int rc = check_rows("swiglu", row_type, rows, cols, &type)) return rc;
+  RowsArgs a{};
+  a.rows = rows;
+  a.cols = static_cast<int32_t>(cols);
+  uint32_t grid;
+  if (const int rc = plan_rows("swiglu", &a, &grid)) return rc;
+  if (grid == 0) return FLUXMI_OK;
+  FLUXMI_REQUIRE(x && out, FLUXMI_ERR_INVALID_ARG, "swiglu: null pointer");
+  FLUXMI_REQUIRE((codes == nullptr) == (scale == nullptr), FLUXMI_ERR_INVALID_ARG, "swiglu: codes and scale come together");
+  FLUXMI_REQUIRE(even(x) && even(out), FLUXMI_ERR_INVALID_ARG, "swiglu: a pointer is not aligned to its elements");
+  a.x = static_cast<const uint8_t *>(x);
+  a.out = static_cast<uint8_t *>(out);
+  a.codes = static_cast<uint8_t *>(codes);
+  a.scale = static_cast<uint8_t *>(scale);
+  by_half(type, [&](auto T) {
+    if (codes != nullptr) checkpoint_kernel<decltype(T)::value, true, true><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+    else checkpoint_kernel<decltype(T)::value, true, false><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+  });
+  FLUXMI_HIP_CHECK(hipGetLastError());
+  return FLUXMI_OK;
+}
+
+extern "C" int fluxmi_swiglu_backward(const void *grad, const void *x, const void *x_scale, int32_t row_type, int64_t rows, int64_t cols, void *grad_x,
+                                      void *out, void *stream) {
+  Row type;
+  if (const int rc = check_rows("swiglu_backward", row_type, rows, cols, &type)) return rc;
+  RowsArgs a{};
+  a.rows = rows;
+  a.cols = static_cast<int32_t>(cols);
+  uint32_t grid;
+  if (const int rc = plan_rows("swiglu_backward", &a, &grid)) return rc;
+  if (grid == 0) return FLUXMI_OK;
+  FLUXMI_REQUIRE(grad && x && grad_x, FLUXMI_ERR_INVALID_ARG, "swiglu_backward: null pointer");
+  FLUXMI_REQUIRE(even(grad) && (x_scale != nullptr || even(x)) && even(grad_x) && even(out), FLUXMI_ERR_INVALID_ARG,
+                 "swiglu_backward: a pointer is not aligned to its elements");
+  a.grad = static_cast<const uint8_t *>(grad);
+  a.x = static_cast<const uint8_t *>(x);
+  a.in_scale = static_cast<const uint8_t *>(x_scale);
+  a.grad_x = static_cast<uint8_t *>(grad_x);
+  a.out = static_cast<uint8_t *>(out);
+  by_half(type, [&](auto T) {
+    if (x_scale != nullptr) swiglu_backward_kernel<decltype(T)::value, true><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+    else swiglu_backward_kernel<decltype(T)::value, false><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+  });
+  FLUXMI_HIP_CHECK(hipGetLastError());
+  return FLUXMI_OK;
+}

@@ -1,8 +1,8 @@
 // Tokens sorted by expert and back, with gradients: moe_permute, moe_unpermute and their backward passes.  The reference gathers inside its GEMM
 // and reduces without a gradient (src/moe_gather_rs/ths_op/topk_scatter_reduce.cc:30-56), so these have no counterpart there.
 #include <c10/core/DeviceGuard.h>
-#include <hip/hip_runtime_api.h>
 
+#include "autograd_checks.h"
 #include "ths_ops.h"
 
 namespace flux_amd {
@@ -12,16 +12,6 @@ int32_t row_type(const torch::Tensor &t, const char *name) {
   const at::ScalarType st = t.scalar_type();
   TORCH_CHECK(st == at::kBFloat16 || st == at::kHalf || st == at::kFloat, name, " must be bfloat16, float16 or float32, got ", st);
   return st == at::kBFloat16 ? FLUXMI_ROWS_BF16 : st == at::kFloat ? FLUXMI_ROWS_FP32 : FLUXMI_ROWS_FP16;
-}
-
-// The kernels carry no tangents: forward mode would silently lose them.
-void refuse_tangent(const torch::Tensor &t, const char *what) {
-  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), what, ": forward-mode derivatives are not built");
-}
-
-// A conjugate or negative view stands for other values than its memory holds, which is what is moved.
-void refuse_lazy_view(const torch::Tensor &t, const char *name) {
-  TORCH_CHECK(!t.is_conj() && !t.is_neg(), name, " is a conjugate or negative view: resolve_conj() or resolve_neg() first");
 }
 
 void check_rows(const torch::Tensor &t, const char *name) {
@@ -92,31 +82,6 @@ std::tuple<torch::Tensor, torch::Tensor> unpermute_backward(const torch::Tensor 
                                              want_weights ? grad_weights.data_ptr() : nullptr, current_stream()),
                "fluxmi_moe_unpermute_backward");
   return {grad_rows, grad_weights};
-}
-
-// The gradients come from kernels that record nothing: a second derivative, in reverse or forward mode, would be silently wrong, so it is refused.
-void refuse_second_derivative(const char *who, const torch::Tensor &grad) {
-  refuse_tangent(grad, who);
-  TORCH_CHECK(!at::GradMode::is_enabled(), who, ": the gradient of the gradient is not built (create_graph=True)");
-}
-
-// A backward pass that is captured hands its gradients to leaves on the stream where these were first used.  If an eager graph of a leaf is alive, that is the
-// eager stream, which would be drawn into the capture and end the process: an error is raised before it comes to that.
-void refuse_leaves_of_another_stream(const char *who) {
-  const c10::hip::HIPStream current = c10::hip::getCurrentHIPStream();
-  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(current.stream(), &capture) != hipSuccess) {
-    (void)hipGetLastError();
-    return;
-  }
-  const std::shared_ptr<torch::autograd::Node> node = torch::autograd::get_current_node();
-  if (capture == hipStreamCaptureStatusNone || node == nullptr) return;
-  for (const torch::autograd::Edge &edge : node->next_edges()) {
-    if (edge.function == nullptr || edge.function->name() != "torch::autograd::AccumulateGrad") continue;
-    const std::optional<c10::Stream> stream = edge.function->stream();
-    TORCH_CHECK(!stream.has_value() || stream->id() == current.id(), who,
-                ": its backward pass is captured while an eager graph of the same leaf is alive; drop that graph's outputs before the capture");
-  }
 }
 
 struct Permute : torch::autograd::Function<Permute> {

@@ -190,6 +190,18 @@ PYBIND11_MODULE(flux_ths_pybind, m) {
   m.def("moe_unpermute", &moe_unpermute, py::arg("rows"), py::arg("scatter_index"), py::arg("weights") = py::none());
   m.def("moe_unpermute_backward", &moe_unpermute_backward, py::arg("grad_out"), py::arg("rows"), py::arg("scatter_index"),
         py::arg("weights"));
+  m.def("moe_linear", &moe_linear, py::arg("input"), py::arg("weight"), py::arg("splits"), py::arg("checkpoint") = false);
+  m.def("moe_swiglu", &moe_swiglu, py::arg("input"), py::arg("checkpoint") = false);
+  m.def("moe_mlp", &moe_mlp, py::arg("input"), py::arg("weight1"), py::arg("weight2"), py::arg("splits"), py::arg("checkpoint") = false);
+  m.def("moe_dgrad", &moe_dgrad, py::arg("grad"), py::arg("weight"), py::arg("splits"));
+  m.def("moe_wgrad", [](torch::Tensor grad, torch::Tensor input, torch::Tensor splits, std::optional<torch::Tensor> input_scale,
+                        std::optional<torch::Tensor> output, bool accumulate, py::object output_dtype) {
+    return moe_wgrad(grad, input, splits, input_scale, output, accumulate, output_dtype.is_none() ? std::nullopt : std::make_optional(to_dtype(output_dtype)));
+  }, py::arg("grad"), py::arg("input"), py::arg("splits"), py::arg("input_scale") = py::none(), py::arg("output") = py::none(),
+        py::arg("accumulate") = false, py::arg("output_dtype") = py::none());
+  m.def("moe_checkpoint", &moe_checkpoint, py::arg("input"));
+  m.def("moe_swiglu_checkpoint", &moe_swiglu_checkpoint, py::arg("input"));
+  m.def("moe_swiglu_backward", &moe_swiglu_backward, py::arg("grad"), py::arg("input"), py::arg("input_scale") = py::none());
   m.def("bitwise_check", &bitwise_check);
   m.def("init_flux_shm", [](py::object) {}, py::arg("group") = py::none());  // nothing to set up on one GPU
   // Test helper of the reference (src/ths_op/helper_ops.cc:33-44, src/cuda/random_initialize.cu:27-51): fills a

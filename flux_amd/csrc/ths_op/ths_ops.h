@@ -182,6 +182,20 @@ torch::Tensor moe_permute_backward(torch::Tensor grad_rows, torch::Tensor scatte
 torch::Tensor moe_unpermute(torch::Tensor rows, torch::Tensor scatter_index, std::optional<torch::Tensor> weights);
 std::tuple<torch::Tensor, torch::Tensor> moe_unpermute_backward(torch::Tensor grad_out, torch::Tensor rows, torch::Tensor scatter_index,
                                                                 torch::Tensor weights);
+
+// Experts that learn (expert_grad_ops.cc).  Rows are sorted by expert, weight is [experts, n, k], splits int32 [experts] on the rows' device or the host; rows past
+// their sum belong to no expert and are 0 in what is computed of them.  moe_linear, moe_swiglu and moe_mlp are differentiable once; checkpoint: what their
+// backward pass reads of activations is kept in 8 bits.
+torch::Tensor moe_linear(torch::Tensor input, torch::Tensor weight, torch::Tensor splits, bool checkpoint);
+torch::Tensor moe_swiglu(torch::Tensor input, bool checkpoint);
+torch::Tensor moe_mlp(torch::Tensor input, torch::Tensor weight1, torch::Tensor weight2, torch::Tensor splits, bool checkpoint);
+// The gradients, for callers without autograd, and the 8 bits: e4m3 codes and a float8_e8m0fnu scale for every 32 values of a row.
+torch::Tensor moe_dgrad(torch::Tensor grad, torch::Tensor weight, torch::Tensor splits);
+torch::Tensor moe_wgrad(torch::Tensor grad, torch::Tensor input, torch::Tensor splits, std::optional<torch::Tensor> input_scale,
+                        std::optional<torch::Tensor> output, bool accumulate, std::optional<at::ScalarType> output_dtype);
+std::tuple<torch::Tensor, torch::Tensor> moe_checkpoint(torch::Tensor input);
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_swiglu_checkpoint(torch::Tensor input);
+std::tuple<torch::Tensor, torch::Tensor> moe_swiglu_backward(torch::Tensor grad, torch::Tensor input, std::optional<torch::Tensor> input_scale);
 bool bitwise_check(torch::Tensor a, torch::Tensor b);
 
 }  // namespace flux_amd

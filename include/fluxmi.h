@@ -469,6 +469,53 @@ typedef struct fluxmi_mx_launch_info {
 int fluxmi_grouped_gemm_mx_launch_info(const fluxmi_mx_gemm_args *args, fluxmi_mx_launch_info *info);
 
 /* ------------------------------------------------------------------------------------------------
+ * Gradients of the grouped product D[r, :] = X[r, :] W[e(r)]^T, W [nexperts, n, k], whose rows are sorted by expert.  The reference has no gradient of its
+ * MoE operators; its block-scaled GEMM has wgrad methods for fp8 operands (src/pybind/gemm_only.cc:77-160).
+ *
+ *   fluxmi_moe_dgrad   grad_input[r, k] = sum_n grad[r, n] * weight[e(r), n, k]; rows that belong to no expert are 0
+ *   fluxmi_moe_wgrad   grad_weight[e, n, k] = sum_{r of e} grad[r, n] * input[r, k]; 0 for an expert without rows.  accumulate != 0: added to what
+ *                      grad_weight holds.  input_scale: `input` is a checkpoint (below) with these scales, and its values are rounded to the rows' type
+ *                      (those that fluxmi_checkpoint_e4m3 made from that type are values of it)
+ *
+ * `row_type` (FLUXMI_ROWS_BF16 or FLUXMI_ROWS_FP16) is the type of grad [rows, n], weight, input [rows, k] and grad_input [rows, k]; grad_weight is of
+ * `out_type`: that or FLUXMI_ROWS_FP32.  Sums are fp32, in an order that follows from the sizes and the alignment alone, and are rounded once.
+ * `splits`: DEVICE int32 row counts.  Negative ones are 0; what they have past `rows` does not exist.  Rows past the sum are not read by fluxmi_moe_wgrad.
+ * Requirements: nexperts <= 1024; rows, n, k <= 2^24; operands aligned to their elements, grad_input to 8 bytes, grad_weight and workspace to 16.  Operands
+ * that start on 16 bytes with n and k multiples of 8 are fast.
+ * `workspace`: fluxmi_moe_wgrad_workspace_bytes() bytes (0 for many sizes) of any content; not shared by calls that may overlap.
+ * ---------------------------------------------------------------------------------------------- */
+int fluxmi_moe_dgrad(const void *grad, const void *weight, int32_t row_type, const int32_t *splits, int32_t nexperts, int64_t rows, int64_t n,
+                     int64_t k, void *grad_input, void *stream);
+size_t fluxmi_moe_wgrad_workspace_bytes(int32_t nexperts, int64_t rows, int64_t n, int64_t k);
+int fluxmi_moe_wgrad(const void *grad, const void *input, const void *input_scale, int32_t row_type, const int32_t *splits, int32_t nexperts,
+                     int64_t rows, int64_t n, int64_t k, void *grad_weight, int32_t out_type, int32_t accumulate, void *workspace,
+                     size_t workspace_bytes, void *stream);
+
+/* Rows past the sum of the splits are set to 0 (`rows` rows of `row_bytes` bytes; the grouped products leave them as they were). */
+int fluxmi_moe_clear_rest(void *data, const int32_t *splits, int32_t nexperts, int64_t rows, int64_t row_bytes, void *stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Activation checkpoints in 8 bits, and the gated activation between an expert's two products.  No counterpart in the reference.
+ *
+ * 32 values of a row (of either half of a gated row; a last block may be shorter) share a scale byte b that stands for 2^(b - 127).  With m a block's largest
+ * magnitude and f its biased fp32 exponent: b = 255 and zero codes if the block holds an infinity or a NaN, else b = max(f - 8 + (m > 1.75 * 2^(f - 127)), 0),
+ * so that m is at most 448 times the scale; a code is the e4m3 value nearest to x / 2^(b - 127), ties to the even one.  x beyond 15/8 times the largest power of
+ * two of its type counts as that much: the value of the code above is not one of the type.
+ *
+ *   fluxmi_checkpoint_e4m3   x [rows, cols] -> codes [rows, cols], scale [rows, ceil(cols / 32)]
+ *   fluxmi_swiglu            x [rows, 2 cols], gate and up halves -> out [rows, cols] = gate / (1 + exp(-gate)) * up; with codes and scale (both or
+ *                            neither) also the checkpoint of x: codes [rows, 2 cols], scale [rows, 2 ceil(cols / 32)], each half in blocks of its own
+ *   fluxmi_swiglu_backward   grad [rows, cols], x as above, or codes with x_scale -> grad_x [rows, 2 cols], and out again unless NULL
+ *
+ * `row_type` is FLUXMI_ROWS_BF16 or FLUXMI_ROWS_FP16, of x, out, grad and grad_x; what is between is fp32, rounded once.  Pointers are aligned to their
+ * elements; cols <= 2^30; a launch has no more than 2^32 threads, of which eight columns take one (more rows: FLUXMI_ERR_UNSUPPORTED).
+ * ---------------------------------------------------------------------------------------------- */
+int fluxmi_checkpoint_e4m3(const void *x, int32_t row_type, int64_t rows, int64_t cols, void *codes, void *scale, void *stream);
+int fluxmi_swiglu(const void *x, int32_t row_type, int64_t rows, int64_t cols, void *out, void *codes, void *scale, void *stream);
+int fluxmi_swiglu_backward(const void *grad, const void *x, const void *x_scale, int32_t row_type, int64_t rows, int64_t cols, void *grad_x,
+                           void *out, void *stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Calibration streams (no counterpart in the reference; for benchmarks): what the memory system of the GPU at
  * hand gives a kernel that only streams.  copy == 0: every byte of src[0, bytes) is read once (16 bytes per lane
  * and load, eight loads in flight per lane) and fluxmi_calib_stream_sink_bytes() bytes of dst are written;
