@@ -8,7 +8,7 @@
 // What is summed over lies across the rows of W, X and, for the weights, G: a lane of the MFMA needs eight values of one column, from eight rows.  The
 // rows go to LDS as they lie in memory and come back through the transposing LDS read: 16 lanes together read four rows of 16 columns, and each of
 // them gets the four values of one column.
-#include "grouped_gemm_grad.hpp"
+#include "grouped_gemm_grad_tiles.hpp"
 
 namespace fluxmi {
 namespace {
@@ -288,6 +288,7 @@ extern "C" int fluxmi_moe_dgrad(const void *grad, const void *weight, int32_t ro
   a.n = static_cast<int32_t>(n);
   a.k = static_cast<int32_t>(k);
   a.parts = 1;
+  if (grad_tiles_take(Grad::INPUT, a) && grad_tiles_are_faster(Grad::INPUT, a)) return launch_grad_tiles(Grad::INPUT, row_type == FLUXMI_ROWS_FP16, a, stream);
   // Every expert and the rows of none end with a tile that may be partial.
   const int64_t row_tiles = rows / kPiece + (rows < nexperts ? rows : nexperts) + 1, items = row_tiles * tiles_of(k);
   FLUXMI_REQUIRE(items <= kMostItems, FLUXMI_ERR_UNSUPPORTED, "moe_dgrad: too many rows and columns for one launch");
@@ -329,6 +330,8 @@ extern "C" int fluxmi_moe_wgrad(const void *grad, const void *input, const void 
   FLUXMI_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && on(workspace, 16)), FLUXMI_ERR_WORKSPACE,
                  "moe_wgrad: workspace of %zu bytes, 16-byte aligned, expected, got %zu", need, workspace_bytes);
   a.partial = static_cast<float *>(workspace);
+  const Grad kind = input_scale != nullptr ? Grad::WEIGHT_8BIT : Grad::WEIGHT;
+  if (grad_tiles_take(kind, a) && grad_tiles_are_faster(kind, a)) return launch_grad_tiles(kind, row_type == FLUXMI_ROWS_FP16, a, stream);
   const int64_t pieces = nexperts * tiles_of(n) * tiles_of(k), items = pieces * a.parts;
   FLUXMI_REQUIRE(items <= kMostItems, FLUXMI_ERR_UNSUPPORTED, "moe_wgrad: too many experts, rows and columns for one launch");
   const bool f16 = row_type == FLUXMI_ROWS_FP16;

@@ -3,7 +3,6 @@
 #include "common.hpp"
 
 namespace fluxmi {
-namespace {
 
 constexpr int kGradMaxRows = 1 << 24;  // 64 counts of it still fit 32 bits
 
@@ -20,6 +19,8 @@ struct GradArgs {
   int32_t out_f32, accumulate;
   int32_t parts;           // an expert's rows are summed in so many parts
 };
+
+namespace {
 
 #if defined(__HIP_DEVICE_COMPILE__)
 
@@ -90,38 +91,41 @@ __device__ __forceinline__ RowTile row_tile(const GradArgs &a, int tile) {
   return {a.nexperts, static_cast<int>(row0), a.rows - static_cast<int>(row0) < HEIGHT ? a.rows - static_cast<int>(row0) : HEIGHT};
 }
 
-// Four neighbouring sums of a row to out[at ..]; `count` of them exist.  aligned: they start on a multiple of four elements of `out`.
+// Four neighbouring sums of a row to out[at ..], which starts on a multiple of four elements.
 template <bool F16>
-__device__ __forceinline__ void store4(const GradArgs &a, int64_t at, f32x4 v, int count, bool aligned) {
-  if (count <= 0) return;
+__device__ __forceinline__ void store4_whole(const GradArgs &a, int64_t at, f32x4 v) {
   if (a.out_f32) {
     float *p = reinterpret_cast<float *>(a.out) + at;
-    if (count >= 4 && aligned) {
-      if (a.accumulate) v += *reinterpret_cast<const f32x4 *>(p);
-      *reinterpret_cast<f32x4 *>(p) = v;
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < count) p[i] = a.accumulate ? p[i] + v[i] : v[i];
+    if (a.accumulate) v += *reinterpret_cast<const f32x4 *>(p);
+    *reinterpret_cast<f32x4 *>(p) = v;
     return;
   }
   uint16_t *p = reinterpret_cast<uint16_t *>(a.out) + at;
-  if (count >= 4 && aligned) {
-    if (a.accumulate) {
-      const u32x2 old = *reinterpret_cast<const u32x2 *>(p);
+  if (a.accumulate) {
+    const u32x2 old = *reinterpret_cast<const u32x2 *>(p);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += unpack1<F16>(static_cast<uint16_t>(old[i / 2] >> (16 * (i & 1))));
-    }
-    *reinterpret_cast<u32x2 *>(p) = u32x2{pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3])};
+    for (int i = 0; i < 4; ++i) v[i] += unpack1<F16>(static_cast<uint16_t>(old[i / 2] >> (16 * (i & 1))));
+  }
+  *reinterpret_cast<u32x2 *>(p) = u32x2{pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3])};
+}
+// The same for the first `count` of them, at any element unless `aligned`.
+template <bool F16>
+__device__ __forceinline__ void store4(const GradArgs &a, int64_t at, f32x4 v, int count, bool aligned) {
+  if (count >= 4 && aligned) {
+    store4_whole<F16>(a, at, v);
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < count) {
-      const float s = a.accumulate ? v[i] + unpack1<F16>(p[i]) : v[i];
-      p[i] = static_cast<uint16_t>(pack2<F16>(s, 0.f));
+  for (int i = 0; i < 4; ++i) {
+    if (i >= count) continue;
+    if (a.out_f32) {
+      float *p = reinterpret_cast<float *>(a.out) + at + i;
+      *p = a.accumulate ? *p + v[i] : v[i];
+    } else {
+      uint16_t *p = reinterpret_cast<uint16_t *>(a.out) + at + i;
+      *p = static_cast<uint16_t>(pack2<F16>(a.accumulate ? v[i] + unpack1<F16>(*p) : v[i], 0.f));
     }
+  }
 }
 
 #endif  // __HIP_DEVICE_COMPILE__

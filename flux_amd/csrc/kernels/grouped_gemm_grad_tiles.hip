@@ -1,0 +1,404 @@
+// Gradients of the grouped product (grouped_gemm_grad.hip has the formulas) by tiles of 256 x 256 of the result.
+//
+//  * Four waves, one to a SIMD, 128 x 128 to each: 256 sums in accumulation registers, two sets of fragments of 16 x 32 in vector registers.  A step
+//    sums over 32 values: 64 MFMAs of 16 x 16 x 32 on one set, while the other is read from LDS for the next step and the step four further on is
+//    requested.
+//  * LDS holds four steps of both operands, 16 KiB each, filled by loads that go there directly.  An operand whose rows are what is summed over ("across": W,
+//    X, and G for the weights' gradient) lies in rows of 256 columns, 512 bytes; 16 columns of a row (32 bytes) are at place s ^ f(row), f = row % 4 + 4 (row / 8 % 2), so
+//    that the eight rows which half a wave reads together are on different banks.  G for the input's gradient lies in rows of 32 values, 64 bytes.
+//  * A fragment of an "across" operand comes back through the transposing read, twice four rows of 16 columns.
+//  * What is past the end of the sum is zeros, fetched from a page of them; rows and columns past the end of the result are others' values, which reach
+//    no result that is stored.
+#include "grouped_gemm_grad_tiles.hpp"
+
+#include <type_traits>
+#include <utility>
+
+namespace fluxmi {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kTile = 256;
+constexpr int kStep = 32;
+constexpr int kSlot = 16384;           // bytes of one operand's step
+constexpr int kSlots = 4;
+constexpr int kCodeSlot = 8192, kScaleSlot = 1024;  // WEIGHT_8BIT: a step's codes, and its scales in words
+// The columns' operand in kSlots slots (WEIGHT_8BIT: two, of converted values), the rows' operand in kSlots, then codes and scales.
+constexpr int rows_at(Grad g) { return (g == Grad::WEIGHT_8BIT ? 2 : kSlots) * kSlot; }
+constexpr int codes_at() { return rows_at(Grad::WEIGHT_8BIT) + kSlots * kSlot; }
+constexpr int scales_at() { return codes_at() + kSlots * kCodeSlot; }
+constexpr int lds_bytes(Grad g) { return g == Grad::WEIGHT_8BIT ? scales_at() + kSlots * kScaleSlot : rows_at(g) + kSlots * kSlot; }
+
+__device__ uint4 g_zeros[64];  // 16 bytes of zeros for each lane
+
+#if defined(__HIP_DEVICE_COMPILE__)
+
+#define FLUXMI_VMCNT(vm) __builtin_amdgcn_s_waitcnt(((vm)&15) | (((vm) >> 4) << 14) | (7 << 4) | (15 << 8))
+#define FLUXMI_LGKM0() __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8))
+
+typedef __attribute__((address_space(3))) uint32_t *LdsPtr;
+typedef const __attribute__((address_space(1))) void *GlobalPtr;
+typedef const __attribute__((address_space(3))) u32x4 *LdsFrag;
+
+template <class F, int... I>
+__device__ __forceinline__ void static_for_seq(F &f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int END, class F>
+__device__ __forceinline__ void static_for(F &&f) {
+  static_for_seq(f, std::make_integer_sequence<int, END>{});
+}
+
+// Pinned to the accumulation registers: given the builtin, the compiler spreads the sums over both files and moves them about.
+template <bool F16>
+__device__ __forceinline__ void mfma(f32x4 &acc, const u32x4 &a, const u32x4 &b) {
+  if constexpr (F16) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+  else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+}
+
+// Sixteen codes of one block to values of 16 bits.
+template <bool F16>
+__device__ __forceinline__ void convert16(const u32x4 codes, uint32_t byte, u32x4 (&v)[2]) {
+  const float scale = __uint_as_float(byte == 0 ? 0x00400000u : (byte == 255 ? 0x7fc00000u : byte << 23));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (F16) {
+      v[i >> 1][(i & 1) * 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[i], scale, false));
+      v[i >> 1][(i & 1) * 2 + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[i], scale, true));
+    } else {
+      v[i >> 1][(i & 1) * 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i], scale, false));
+      v[i >> 1][(i & 1) * 2 + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i], scale, true));
+    }
+  }
+}
+
+#endif  // __HIP_DEVICE_COMPILE__
+
+template <bool F16, Grad G>
+__global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const GradArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr bool INPUT = G == Grad::INPUT, EIGHT = G == Grad::WEIGHT_8BIT;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)smem));
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wave >> 1, wc = wave & 1;
+
+  // ---- which tile: workgroups are dealt to the eight XCDs in turn; 32 in a row on one XCD take neighbouring tiles ----
+  const int tiles_k = (a.k + kTile - 1) / kTile;
+  const int grid = gridDim.x;
+  int item = blockIdx.x;
+  if (item < grid / 256 * 256) item = (item >> 8) * 256 + (item & 7) * 32 + ((item & 255) >> 3);
+  int e, out_rows, sum_over, row0, col0;
+  int64_t out_row0;
+  const uint8_t *rbase, *cbase, *sbase = nullptr;
+  const int blocks = (a.k + 31) / 32;
+  int64_t rpitch = static_cast<int64_t>(a.n) * 2, cpitch = static_cast<int64_t>(a.k) * (EIGHT ? 1 : 2);
+  if constexpr (INPUT) {
+    // (row tiles in groups of eight, walked column by column)
+    const int row_tiles = grid / tiles_k;
+    const int group = item / (8 * tiles_k), in_group = item - group * 8 * tiles_k;
+    const int height = row_tiles - group * 8 < 8 ? row_tiles - group * 8 : 8;
+    const int kt = in_group / height;
+    const RowTile t = row_tile<kTile>(a, group * 8 + in_group - kt * height);
+    if (t.rows <= 0) return;
+    e = t.e;
+    col0 = kt * kTile;
+    row0 = 0;
+    out_rows = t.rows;
+    out_row0 = t.row0;
+    sum_over = e < a.nexperts ? a.n : 0;
+    rbase = a.grad + t.row0 * rpitch;
+    cbase = a.other + static_cast<int64_t>(e < a.nexperts ? e : 0) * a.n * cpitch;
+  } else {
+    const int tiles_n = (a.n + kTile - 1) / kTile, per = tiles_n * tiles_k;
+    e = item / per;
+    const int local = item - e * per;
+    const int group = local / (8 * tiles_k), in_group = local - group * 8 * tiles_k;
+    const int height = tiles_n - group * 8 < 8 ? tiles_n - group * 8 : 8;
+    const int kt = in_group / height, nt = group * 8 + in_group - kt * height;
+    row0 = nt * kTile;
+    col0 = kt * kTile;
+    out_rows = a.n - row0 < kTile ? a.n - row0 : kTile;
+    out_row0 = static_cast<int64_t>(e) * a.n + row0;
+    const ExpertRows x = rows_of_expert(a, e);
+    sum_over = x.end - x.begin;
+    rbase = a.grad + x.begin * rpitch;
+    cbase = a.other + x.begin * cpitch;
+    if constexpr (EIGHT) sbase = a.scale + static_cast<int64_t>(x.begin) * blocks;
+  }
+  const int out_cols = a.k - col0 < kTile ? a.k - col0 : kTile;
+  const int steps = (sum_over + kStep - 1) / kStep, whole = sum_over / kStep;
+
+  // ---- fills: four instructions of a wave to either operand's step ------------------------------------------------
+  // Across: an instruction fills two rows, lane l place l % 32 (of 16 bytes) of row l / 32; along: 16 rows, lane l place l % 4 of row l / 4.
+  // Codes: four rows, lane l chunk l % 16 (of 16 columns) of row l / 16; scales: the eight rows whose codes this wave fetches, a word to each byte.
+  constexpr int kColFills = EIGHT ? 3 : 4, kFills = kColFills + 4;
+  uint32_t coff[4], roff[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = wave * 8 + i * 2 + (lane >> 5), f = (t & 3) | ((t >> 1) & 4);
+    const int col = (((lane & 31) >> 1) ^ f) * 16 + (lane & 1) * 8;
+    if constexpr (EIGHT) {
+      const int c = (lane & 15) * 16, b = lane & 7;
+      if (i < 2) coff[i] = static_cast<uint32_t>((wave * 8 + i * 4 + (lane >> 4)) * cpitch) + col0 + (c < out_cols ? c : 0);
+      else if (i == 2) coff[i] = static_cast<uint32_t>((wave * 8 + (lane >> 3)) * blocks) + col0 / 32 + (b * 32 < out_cols ? b : 0);
+    } else {
+      coff[i] = static_cast<uint32_t>(t * cpitch) + (col0 + (col < out_cols ? col : 0)) * 2u;
+    }
+    if constexpr (INPUT) {
+      const int r = wave * 64 + i * 16 + (lane >> 2), c = (lane & 3) ^ ((r >> 1) & 3);
+      roff[i] = static_cast<uint32_t>((r < out_rows ? r : out_rows - 1) * rpitch) + c * 16u;
+    } else {
+      roff[i] = static_cast<uint32_t>(t * rpitch) + (row0 + (col < out_rows ? col : 0)) * 2u;
+    }
+  }
+  const int64_t cstep = kStep * cpitch, rstep = INPUT ? kStep * 2 : kStep * rpitch;
+  auto buffer_of = [](const uint8_t *p) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p), 0, -1, 0x00020000); };
+  const uint32_t cdst = lds0 + wave * 4096, rdst = cdst + rows_at(G), codes = lds0 + codes_at() + wave * 2048, scales = lds0 + scales_at() + wave * 256;
+  // Where fill q of a step goes.
+  auto target = [&](int slot, int q) {
+    if (q >= kColFills) return rdst + slot * kSlot + (q - kColFills) * 1024;
+    if (!EIGHT) return cdst + slot * kSlot + q * 1024;
+    return q < 2 ? codes + slot * kCodeSlot + q * 1024 : scales + slot * kScaleSlot;
+  };
+
+  f32x4 acc[8][8];  // [row block][column block]
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // ---- fragment addresses -------------------------------------------------------------------------------------------
+  uint32_t cfrag[8], rfrag[8];
+  {
+    const int g = lane >> 4, i = lane & 15, t = 8 * g + (i >> 2), f = (t & 3) | ((t >> 1) & 4);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      cfrag[j] = lds0 + t * 512 + ((wc * 8 + j) ^ f) * 32 + (i & 3) * 8;
+      if constexpr (INPUT) rfrag[j] = lds0 + rows_at(G) + (wr * 128 + i) * 64 + (g ^ ((i >> 1) & 3)) * 16;
+      else rfrag[j] = lds0 + rows_at(G) + t * 512 + ((wr * 8 + j) ^ f) * 32 + (i & 3) * 8;
+    }
+  }
+  u32x4 ca[8], ra[8], cb[8], rb[8];
+  // Read R of the 32 (INPUT: 24) that a step's fragments take, from slot SLOT.
+  constexpr int kReads = INPUT ? 24 : 32;
+  auto read_one = [&](auto SLOT, auto R, u32x4(&cf)[8], u32x4(&rf)[8]) {
+    constexpr int slot = decltype(SLOT)::value, r = decltype(R)::value;
+    if constexpr (r < 16) {
+      const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr)(uintptr_t)(cfrag[r / 2] + (EIGHT ? slot % 2 : slot) * kSlot + (r & 1) * 2048)));
+      cf[r / 2][(r & 1) * 2] = v[0];
+      cf[r / 2][(r & 1) * 2 + 1] = v[1];
+    } else if constexpr (INPUT) {
+      rf[r - 16] = *(LdsFrag)(uintptr_t)(rfrag[0] + slot * kSlot + (r - 16) * 1024);
+    } else {
+      constexpr int q = r - 16;
+      const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr)(uintptr_t)(rfrag[q / 2] + slot * kSlot + (q & 1) * 2048)));
+      rf[q / 2][(q & 1) * 2] = v[0];
+      rf[q / 2][(q & 1) * 2 + 1] = v[1];
+    }
+  };
+
+  // WEIGHT_8BIT: what this wave fetched of a step becomes values in the slot of its parity.  In three parts: read, convert, write.
+  u32x4 code[2], value[2][2];
+  uint32_t scale_byte[2];
+  const uint32_t scale_at = scales + ((lane >> 4) * 8 + ((lane & 15) >> 1)) * 4;
+  uint32_t value_at[2];
+  if constexpr (EIGHT) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t = wave * 8 + i * 4 + (lane >> 4), f = (t & 3) | ((t >> 1) & 4);
+      value_at[i] = lds0 + t * 512 + ((lane & 15) ^ f) * 32;
+    }
+  }
+  auto read_codes = [&](auto SLOT) {
+    constexpr int slot = decltype(SLOT)::value;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      code[i] = *(LdsFrag)(uintptr_t)(codes + lane * 16 + slot * kCodeSlot + i * 1024);
+      scale_byte[i] = *(const __attribute__((address_space(3))) uint32_t *)(uintptr_t)(scale_at + slot * kScaleSlot + i * 128);
+    }
+  };
+  auto write_values = [&](auto SLOT, int i) {
+    constexpr int slot = decltype(SLOT)::value;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(value_at[i] + (slot % 2) * kSlot + h * 16) = value[i][h];
+  };
+
+  // Fill Q of a step (the columns' operand first) that may be the partial last one: `valid` of its 32 values exist.
+  auto fill_guarded = [&](int slot, auto Q, const uint8_t *cat, const uint8_t *rat, const uint8_t *sat, int valid) {
+    constexpr int q = decltype(Q)::value, r = q - kColFills;
+    const uint8_t *zeros = reinterpret_cast<const uint8_t *>(g_zeros) + lane * 16;
+    const uint8_t *src;
+    if constexpr (r >= 0 && INPUT) src = ((lane & 3) ^ (((wave * 64 + r * 16 + (lane >> 2)) >> 1) & 3)) * 8 < valid ? rat + roff[r] : zeros;
+    else if constexpr (r >= 0) src = wave * 8 + r * 2 + (lane >> 5) < valid ? rat + roff[r] : zeros;
+    else if constexpr (!EIGHT) src = wave * 8 + q * 2 + (lane >> 5) < valid ? cat + coff[q] : zeros;
+    else if constexpr (q < 2) src = wave * 8 + q * 4 + (lane >> 4) < valid ? cat + coff[q] : zeros;
+    else src = wave * 8 + (lane >> 3) < valid ? sat + coff[q] : zeros;
+    const LdsPtr dst = (LdsPtr)(uintptr_t)__builtin_amdgcn_readfirstlane(target(slot, q));
+    if constexpr (EIGHT && q == 2) __builtin_amdgcn_global_load_lds((GlobalPtr)src, dst, 1, 0, 0);
+    else __builtin_amdgcn_global_load_lds((GlobalPtr)src, dst, 16, 0, 0);
+  };
+  auto valid_of = [&](int s) { return s < whole ? kStep : sum_over - s * kStep; };
+
+  // ---- the first four steps -------------------------------------------------------------------------------------
+  const int64_t sstep = static_cast<int64_t>(kStep) * blocks;
+  using std::integral_constant;
+#pragma unroll
+  for (int s = 0; s < kSlots; ++s)
+    static_for<kFills>([&](auto Q) { fill_guarded(s, Q, cbase + s * cstep, rbase + s * rstep, EIGHT ? sbase + s * sstep : nullptr, valid_of(s)); });
+  if constexpr (EIGHT) {
+    FLUXMI_VMCNT(2 * kFills);
+    static_for<2>([&](auto S) {
+      read_codes(S);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) convert16<F16>(code[i], scale_byte[i], value[i]), write_values(S, i);
+    });
+    FLUXMI_LGKM0();
+  } else {
+    FLUXMI_VMCNT(3 * kFills);
+  }
+  __builtin_amdgcn_s_barrier();
+  static_for<kReads>([&](auto R) { read_one(integral_constant<int, 0>{}, R, ca, ra); });
+  FLUXMI_LGKM0();
+
+  // What a step waits for: the next one's rows and columns; WEIGHT_8BIT: that one's rows and the codes of the one after it.
+  constexpr int kOpen = EIGHT ? kFills + 4 : 2 * kFills;
+  // Step U of a trip of four: its fragments are in (cf, rf), those of the next go to (cn, rn), and its slot is filled with the step four further on,
+  // `at` bytes behind the buffers' start.
+  const int cstep32 = static_cast<int>(cstep), rstep32 = static_cast<int>(rstep), sstep32 = static_cast<int>(sstep);
+  __amdgpu_buffer_rsrc_t crsrc, rrsrc, srsrc;
+  // The part of a step's conversion that stands beside MFMA t of 64.
+  auto conversion = [&](auto U, auto T) {
+    constexpr int u = decltype(U)::value, t = decltype(T)::value;
+    constexpr integral_constant<int, (u + 2) % kSlots> slot{};
+    if constexpr (!EIGHT) return;
+    else if constexpr (t == 0) read_codes(slot);
+    else if constexpr (t == 16 || t == 32) convert16<F16>(code[t / 32], scale_byte[t / 32], value[t / 32]);
+    else if constexpr (t == 24 || t == 40) write_values(slot, t / 40);
+  };
+  auto step = [&](auto U, u32x4(&cf)[8], u32x4(&rf)[8], u32x4(&cn)[8], u32x4(&rn)[8]) {
+    constexpr int u = decltype(U)::value;
+    FLUXMI_VMCNT(kOpen);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    static_for<64>([&](auto T) {
+      constexpr int t = decltype(T)::value;
+      conversion(U, T);
+      if constexpr (t < 2 * kReads && t % 2 == 0) read_one(integral_constant<int, (u + 1) % kSlots>{}, integral_constant<int, t / 2>{}, cn, rn);
+      constexpr int q = t / 8, r = q - kColFills;
+      if constexpr (t % 8 == 3 && q < kFills) {
+        const uint32_t dst = target(u, q);
+        asm volatile("s_mov_b32 m0, %0" : : "s"(dst) : "memory");
+      }
+      if constexpr (t % 8 == 4 && q < kFills) {
+        if constexpr (r >= 0) asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds" : : "v"(roff[r]), "s"(rrsrc), "s"(u * rstep32) : "memory");
+        else if constexpr (EIGHT && q == 2) asm volatile("buffer_load_ubyte %0, %1, %2 offen lds" : : "v"(coff[q]), "s"(srsrc), "s"(u * sstep32) : "memory");
+        else asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds" : : "v"(coff[q]), "s"(crsrc), "s"(u * cstep32) : "memory");
+      }
+      mfma<F16>(acc[t / 8][t % 8], cf[t % 8], rf[t / 8]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    FLUXMI_LGKM0();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // The same near the end of the sum: s is the step's number.  What lies past the end is filled as well, with zeros, so that the waits count the same.
+  auto last_step = [&](auto U, int s, u32x4(&cf)[8], u32x4(&rf)[8], u32x4(&cn)[8], u32x4(&rn)[8]) {
+    constexpr int u = decltype(U)::value;
+    FLUXMI_VMCNT(kOpen);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    const uint8_t *const cat = cbase + (s + 4) * cstep, *const rat = rbase + (s + 4) * rstep, *const sat = EIGHT ? sbase + (s + 4) * sstep : nullptr;
+    const int valid = valid_of(s + 4);
+    static_for<8>([&](auto I) {
+      constexpr int i = decltype(I)::value;
+      conversion(U, integral_constant<int, i * 8>{});
+      static_for<kReads / 8>([&](auto R) {
+        read_one(integral_constant<int, (u + 1) % kSlots>{}, integral_constant<int, i * (kReads / 8) + decltype(R)::value>{}, cn, rn);
+      });
+      if constexpr (i < kFills) fill_guarded(u, I, cat, rat, sat, valid);
+      __builtin_amdgcn_sched_barrier(0);
+      static_for<8>([&](auto J) { mfma<F16>(acc[i][decltype(J)::value], cf[decltype(J)::value], rf[i]); });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    FLUXMI_LGKM0();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  int s = 0;
+  for (; s + 8 <= whole; s += 4) {
+    crsrc = buffer_of(cbase + (s + 4) * cstep);
+    rrsrc = buffer_of(rbase + (s + 4) * rstep);
+    if constexpr (EIGHT) srsrc = buffer_of(sbase + (s + 4) * sstep);
+    step(integral_constant<int, 0>{}, ca, ra, cb, rb);
+    step(integral_constant<int, 1>{}, cb, rb, ca, ra);
+    step(integral_constant<int, 2>{}, ca, ra, cb, rb);
+    step(integral_constant<int, 3>{}, cb, rb, ca, ra);
+  }
+  while (s < steps) {
+    last_step(integral_constant<int, 0>{}, s, ca, ra, cb, rb);
+    if (++s >= steps) break;
+    last_step(integral_constant<int, 1>{}, s, cb, rb, ca, ra);
+    if (++s >= steps) break;
+    last_step(integral_constant<int, 2>{}, s, ca, ra, cb, rb);
+    if (++s >= steps) break;
+    last_step(integral_constant<int, 3>{}, s, cb, rb, ca, ra);
+    ++s;
+  }
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // the last sums are in their registers
+  FLUXMI_VMCNT(0);  // no fill may come after the workgroup's end
+
+  // ---- lane l has columns 4 (l / 16) .. + 3 of row l % 16 of a block -----------------------------------------------
+  const int g = lane >> 4;
+  static_for<8>([&](auto I) {
+    constexpr int i = decltype(I)::value;
+    const int r = wr * 128 + i * 16 + (lane & 15);
+    if (a.out_f32 || a.accumulate) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int c = wc * 128 + j * 16 + g * 4;
+        if (r < out_rows && c < out_cols) store4_whole<F16>(a, (out_row0 + r) * a.k + col0 + c, acc[i][j]);
+      }
+    } else {
+      // Two blocks' sums change lanes, so that each has eight neighbouring columns: of the first block in lane groups 0 and 2, of the second in 1 and 3.
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        uint32_t x0 = pack2<F16>(acc[i][j][0], acc[i][j][1]), x1 = pack2<F16>(acc[i][j][2], acc[i][j][3]);
+        uint32_t y0 = pack2<F16>(acc[i][j + 1][0], acc[i][j + 1][1]), y1 = pack2<F16>(acc[i][j + 1][2], acc[i][j + 1][3]);
+        const auto p = __builtin_amdgcn_permlane16_swap(x0, y0, false, false);
+        const auto q = __builtin_amdgcn_permlane16_swap(x1, y1, false, false);
+        const int c = wc * 128 + (j + (g & 1)) * 16 + (g >> 1) * 8;
+        if (r < out_rows && c < out_cols)
+          *reinterpret_cast<u32x4 *>(a.out + ((out_row0 + r) * a.k + col0 + c) * 2) = u32x4{p[0], q[0], p[1], q[1]};
+      }
+    }
+  });
+#endif
+}
+
+}  // namespace
+
+bool grad_tiles_take(Grad g, const GradArgs &a) {
+  const auto on16 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  if (a.n % 8 != 0 || a.k % (g == Grad::WEIGHT_8BIT ? 16 : 8) != 0 || !on16(a.grad) || !on16(a.other) || !on16(a.out)) return false;
+  // Offsets: 256 rows of G along, or 32 rows and seven more steps of 32 across.
+  return static_cast<int64_t>(a.n) * 2 * kTile < (int64_t{1} << 31) && static_cast<int64_t>(a.k) * 2 * kTile < (int64_t{1} << 31);
+}
+
+bool grad_tiles_are_faster(Grad, const GradArgs &) { return true; }
+
+int launch_grad_tiles(Grad g, bool f16, const GradArgs &a, void *stream) {
+  const int64_t tiles_k = (a.k + kTile - 1) / kTile, tiles_n = (a.n + kTile - 1) / kTile;
+  const int64_t items = g == Grad::INPUT ? (a.rows / kTile + (a.rows < a.nexperts ? a.rows : a.nexperts) + 1) * tiles_k : a.nexperts * tiles_n * tiles_k;
+  FLUXMI_REQUIRE(items < (1 << 24), FLUXMI_ERR_UNSUPPORTED, "gradients of the grouped product: too many rows and columns for one launch");
+  auto launch = [&](auto kernel, std::atomic<uint64_t> &done) -> int {
+    if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds_bytes(g), done)) return rc;
+    kernel<<<static_cast<uint32_t>(items), kThreads, lds_bytes(g), static_cast<hipStream_t>(stream)>>>(a);
+    FLUXMI_HIP_CHECK(hipGetLastError());
+    return FLUXMI_OK;
+  };
+  static std::atomic<uint64_t> done[6];
+  if (g == Grad::WEIGHT_8BIT) return f16 ? launch(grad_tile_kernel<true, Grad::WEIGHT_8BIT>, done[4]) : launch(grad_tile_kernel<false, Grad::WEIGHT_8BIT>, done[5]);
+  if (g == Grad::INPUT) return f16 ? launch(grad_tile_kernel<true, Grad::INPUT>, done[0]) : launch(grad_tile_kernel<false, Grad::INPUT>, done[1]);
+  return f16 ? launch(grad_tile_kernel<true, Grad::WEIGHT>, done[2]) : launch(grad_tile_kernel<false, Grad::WEIGHT>, done[3]);
+}
+
+}  // namespace fluxmi
