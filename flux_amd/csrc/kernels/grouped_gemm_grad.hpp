@@ -4,6 +4,7 @@
 
 namespace fluxmi {
 
+constexpr int kMaxExperts = 1024;
 constexpr int kGradMaxRows = 1 << 24;  // 64 counts of it still fit 32 bits
 
 enum class Grad { INPUT, WEIGHT, WEIGHT_8BIT };  // WEIGHT_8BIT: the product's input is a checkpoint in 8 bits

@@ -27,7 +27,15 @@ constexpr int kCodeSlot = 8192, kScaleSlot = 1024;  // WEIGHT_8BIT: a step's cod
 constexpr int rows_at(Grad g) { return (g == Grad::WEIGHT_8BIT ? 2 : kSlots) * kSlot; }
 constexpr int codes_at() { return rows_at(Grad::WEIGHT_8BIT) + kSlots * kSlot; }
 constexpr int scales_at() { return codes_at() + kSlots * kCodeSlot; }
-constexpr int lds_bytes(Grad g) { return g == Grad::WEIGHT_8BIT ? scales_at() + kSlots * kScaleSlot : rows_at(g) + kSlots * kSlot; }
+// Behind them the experts' tables: where their rows end, and (INPUT) their tiles.
+constexpr int tables_at(Grad g) { return g == Grad::WEIGHT_8BIT ? scales_at() + kSlots * kScaleSlot : rows_at(g) + kSlots * kSlot; }
+constexpr int lds_bytes(Grad g) { return tables_at(g) + (g == Grad::INPUT ? 2 : 1) * 4 * kMaxExperts; }
+
+struct TileArgs {
+  GradArgs a;
+  int32_t items;  // tiles of the result (INPUT: as many as there can be)
+  int32_t turns;  // tiles that a workgroup computes
+};
 
 __device__ uint4 g_zeros[64];  // 16 bytes of zeros for each lane
 
@@ -36,8 +44,6 @@ __device__ uint4 g_zeros[64];  // 16 bytes of zeros for each lane
 #define FLUXMI_VMCNT(vm) __builtin_amdgcn_s_waitcnt(((vm)&15) | (((vm) >> 4) << 14) | (7 << 4) | (15 << 8))
 #define FLUXMI_LGKM0() __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8))
 
-typedef __attribute__((address_space(3))) uint32_t *LdsPtr;
-typedef const __attribute__((address_space(1))) void *GlobalPtr;
 typedef const __attribute__((address_space(3))) u32x4 *LdsFrag;
 
 template <class F, int... I>
@@ -56,6 +62,18 @@ __device__ __forceinline__ void mfma(f32x4 &acc, const u32x4 &a, const u32x4 &b)
   else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
 
+// A sum's block, read where it is used: the compiler would copy all of them to vector registers ahead of the branches of the stores.
+__device__ __forceinline__ f32x4 sums_of(const f32x4 &acc) {
+  f32x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float x;
+    asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(x) : "a"(acc[i]));
+    v[i] = x;
+  }
+  return v;
+}
+
 // Sixteen codes of one block to values of 16 bits.
 template <bool F16>
 __device__ __forceinline__ void convert16(const u32x4 codes, uint32_t byte, u32x4 (&v)[2]) {
@@ -72,101 +90,157 @@ __device__ __forceinline__ void convert16(const u32x4 codes, uint32_t byte, u32x
   }
 }
 
+
+// A tile of the result and where its operands begin.
+struct Tile {
+  int e, row0, rows, col0, cols;  // row0: column of grad for weights, otherwise 0; rows = 0: there is no such tile
+  int sum_over;
+  int64_t out_row0;
+  int64_t first;  // of the rows that it sums over (INPUT: reads)
+};
+
+// The lane, opaque to the compiler: what is computed from it is not kept in registers through the loops.
+__device__ __forceinline__ int fresh_lane() {
+  int l = lane_id();
+  asm volatile("" : "+v"(l));
+  return l;
+}
+
+// Direct-to-LDS loads of 16 bytes (BYTE: one, to a word) by address; M0 holds the LDS address.  Not the builtins: with these the compiler lets every LDS read wait for
+// all loads.
+template <bool BYTE>
+__device__ __forceinline__ void fill_from(const uint8_t *src) {
+  asm volatile("s_nop 0" : : : "memory");
+  if constexpr (BYTE) asm volatile("global_load_lds_ubyte %0, off" : : "v"(src) : "memory");
+  else asm volatile("global_load_lds_dwordx4 %0, off" : : "v"(src) : "memory");
+}
+
 #endif  // __HIP_DEVICE_COMPILE__
 
 template <bool F16, Grad G>
-__global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const GradArgs a) {
+__global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs args) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr bool INPUT = G == Grad::INPUT, EIGHT = G == Grad::WEIGHT_8BIT;
+  const GradArgs &a = args.a;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)smem));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wave >> 1, wc = wave & 1;
-
-  // ---- which tile: workgroups are dealt to the eight XCDs in turn; 32 in a row on one XCD take neighbouring tiles ----
-  const int tiles_k = (a.k + kTile - 1) / kTile;
-  const int grid = gridDim.x;
-  int item = blockIdx.x;
-  if (item < grid / 256 * 256) item = (item >> 8) * 256 + (item & 7) * 32 + ((item & 255) >> 3);
-  int e, out_rows, sum_over, row0, col0;
-  int64_t out_row0;
-  const uint8_t *rbase, *cbase, *sbase = nullptr;
+  const int tiles_k = (a.k + kTile - 1) / kTile, tiles_n = (a.n + kTile - 1) / kTile;
+  const int64_t rpitch = static_cast<int64_t>(a.n) * 2, cpitch = static_cast<int64_t>(a.k) * (EIGHT ? 1 : 2);
   const int blocks = (a.k + 31) / 32;
-  int64_t rpitch = static_cast<int64_t>(a.n) * 2, cpitch = static_cast<int64_t>(a.k) * (EIGHT ? 1 : 2);
-  if constexpr (INPUT) {
-    // (row tiles in groups of eight, walked column by column)
-    const int row_tiles = grid / tiles_k;
-    const int group = item / (8 * tiles_k), in_group = item - group * 8 * tiles_k;
-    const int height = row_tiles - group * 8 < 8 ? row_tiles - group * 8 : 8;
-    const int kt = in_group / height;
-    const RowTile t = row_tile<kTile>(a, group * 8 + in_group - kt * height);
-    if (t.rows <= 0) return;
-    e = t.e;
-    col0 = kt * kTile;
-    row0 = 0;
-    out_rows = t.rows;
-    out_row0 = t.row0;
-    sum_over = e < a.nexperts ? a.n : 0;
-    rbase = a.grad + t.row0 * rpitch;
-    cbase = a.other + static_cast<int64_t>(e < a.nexperts ? e : 0) * a.n * cpitch;
-  } else {
-    const int tiles_n = (a.n + kTile - 1) / kTile, per = tiles_n * tiles_k;
-    e = item / per;
-    const int local = item - e * per;
-    const int group = local / (8 * tiles_k), in_group = local - group * 8 * tiles_k;
-    const int height = tiles_n - group * 8 < 8 ? tiles_n - group * 8 : 8;
-    const int kt = in_group / height, nt = group * 8 + in_group - kt * height;
-    row0 = nt * kTile;
-    col0 = kt * kTile;
-    out_rows = a.n - row0 < kTile ? a.n - row0 : kTile;
-    out_row0 = static_cast<int64_t>(e) * a.n + row0;
-    const ExpertRows x = rows_of_expert(a, e);
-    sum_over = x.end - x.begin;
-    rbase = a.grad + x.begin * rpitch;
-    cbase = a.other + x.begin * cpitch;
-    if constexpr (EIGHT) sbase = a.scale + static_cast<int64_t>(x.begin) * blocks;
+
+  // ---- the experts' rows and tiles, in LDS ------------------------------------------------------------------------
+  typedef __attribute__((address_space(3))) int *LdsInt;
+  const LdsInt row_ends = (LdsInt)(uintptr_t)(lds0 + tables_at(G)), tile_ends = row_ends + kMaxExperts;
+  int all_rows = 0, row_tiles = 0;
+  for (int e0 = 0; e0 < a.nexperts; e0 += 64) {  // (the same from every wave)
+    const ExpertRows x = rows_of_lane(a, e0, all_rows);
+    row_ends[e0 + lane] = x.end;
+    if constexpr (INPUT) {
+      const int end = row_tiles + wave_inclusive_scan((x.end - x.begin + kTile - 1) / kTile);
+      tile_ends[e0 + lane] = end;
+      row_tiles = __builtin_amdgcn_readlane(end, 63);
+    }
   }
-  const int out_cols = a.k - col0 < kTile ? a.k - col0 : kTile;
-  const int steps = (sum_over + kStep - 1) / kStep, whole = sum_over / kStep;
+  __syncthreads();
+  const int expert_tiles = row_tiles;
+  if constexpr (INPUT) row_tiles += (a.rows - all_rows + kTile - 1) / kTile;  // the rows that belong to no expert
+  const int items = INPUT ? row_tiles * tiles_k : args.items;
+
+  // Tile number `turn` of this workgroup.  Workgroups are dealt to the eight XCDs in turn; 32 in a row on one XCD take neighbouring tiles: an expert's (INPUT: all) tiles in
+  // groups of eight along the result's rows, walked column by column.
+  auto describe = [&](int turn) {
+    Tile t{};
+    int item = blockIdx.x + turn * static_cast<int>(gridDim.x);
+    if (item < args.items / 256 * 256) item = (item & ~255) + (item & 7) * 32 + ((item & 255) >> 3);
+    if (item >= items) return t;
+    const int per = tiles_n * tiles_k, e = INPUT ? 0 : item / per, local = INPUT ? item : item - e * per;
+    const int group = local / (8 * tiles_k), in_group = local - group * 8 * tiles_k;
+    const int high = (INPUT ? row_tiles : tiles_n) - group * 8, height = high < 8 ? high : 8;
+    const int kt = in_group / height, rt = group * 8 + in_group - kt * height;
+    t.col0 = kt * kTile;
+    t.cols = a.k - t.col0 < kTile ? a.k - t.col0 : kTile;
+    if constexpr (INPUT) {
+      t.e = a.nexperts;
+      int begin = all_rows + (rt - expert_tiles) * kTile, end = a.rows;
+      if (rt < expert_tiles) {
+        for (int e0 = 0;; e0 += 64) {
+          const int ends = tile_ends[e0 + lane];
+          const uint64_t hit = __ballot(e0 + lane < a.nexperts && rt < ends);
+          if (hit == 0) continue;
+          const int src = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+          t.e = e0 + src;
+          const int first = t.e > 0 ? __builtin_amdgcn_readfirstlane(row_ends[t.e - 1]) : 0;
+          end = __builtin_amdgcn_readfirstlane(row_ends[t.e]);
+          begin = first + (rt - (__builtin_amdgcn_readlane(ends, src) - (end - first + kTile - 1) / kTile)) * kTile;
+          break;
+        }
+      }
+      t.rows = end - begin < kTile ? end - begin : kTile;
+      t.out_row0 = t.first = begin;
+      t.sum_over = t.e < a.nexperts ? a.n : 0;
+    } else {
+      t.e = e;
+      t.row0 = rt * kTile;
+      t.rows = a.n - t.row0 < kTile ? a.n - t.row0 : kTile;
+      t.out_row0 = static_cast<int64_t>(e) * a.n + t.row0;
+      t.first = e > 0 ? __builtin_amdgcn_readfirstlane(row_ends[e - 1]) : 0;
+      t.sum_over = __builtin_amdgcn_readfirstlane(row_ends[e]) - static_cast<int>(t.first);
+    }
+    return t;
+  };
 
   // ---- fills: four instructions of a wave to either operand's step ------------------------------------------------
   // Across: an instruction fills two rows, lane l place l % 32 (of 16 bytes) of row l / 32; along: 16 rows, lane l place l % 4 of row l / 4.
   // Codes: four rows, lane l chunk l % 16 (of 16 columns) of row l / 16; scales: the eight rows whose codes this wave fetches, a word to each byte.
   constexpr int kColFills = EIGHT ? 3 : 4, kFills = kColFills + 4;
   uint32_t coff[4], roff[4];
+  const uint8_t *rbase = nullptr, *cbase = nullptr, *sbase = nullptr;
+  int steps = 0, whole = 0, sum_over = 0;
+  auto begin_tile = [&](const Tile &t) {
+    const int lane = fresh_lane();
+    sum_over = t.sum_over;
+    steps = (sum_over + kStep - 1) / kStep;
+    whole = sum_over / kStep;
+    rbase = a.grad + t.first * rpitch;
+    if constexpr (INPUT) cbase = a.other + static_cast<int64_t>(t.e < a.nexperts ? t.e : 0) * a.n * cpitch;
+    else cbase = a.other + t.first * cpitch;
+    if constexpr (EIGHT) sbase = a.scale + t.first * blocks;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int t = wave * 8 + i * 2 + (lane >> 5), f = (t & 3) | ((t >> 1) & 4);
-    const int col = (((lane & 31) >> 1) ^ f) * 16 + (lane & 1) * 8;
-    if constexpr (EIGHT) {
-      const int c = (lane & 15) * 16, b = lane & 7;
-      if (i < 2) coff[i] = static_cast<uint32_t>((wave * 8 + i * 4 + (lane >> 4)) * cpitch) + col0 + (c < out_cols ? c : 0);
-      else if (i == 2) coff[i] = static_cast<uint32_t>((wave * 8 + (lane >> 3)) * blocks) + col0 / 32 + (b * 32 < out_cols ? b : 0);
-    } else {
-      coff[i] = static_cast<uint32_t>(t * cpitch) + (col0 + (col < out_cols ? col : 0)) * 2u;
+    for (int i = 0; i < 4; ++i) {
+      const int row = wave * 8 + i * 2 + (lane >> 5), f = (row & 3) | ((row >> 1) & 4);
+      const int col = (((lane & 31) >> 1) ^ f) * 16 + (lane & 1) * 8;
+      if constexpr (EIGHT) {
+        const int c = (lane & 15) * 16, b = lane & 7;
+        if (i < 2) coff[i] = static_cast<uint32_t>((wave * 8 + i * 4 + (lane >> 4)) * cpitch) + t.col0 + (c < t.cols ? c : 0);
+        else if (i == 2) coff[i] = static_cast<uint32_t>((wave * 8 + (lane >> 3)) * blocks) + t.col0 / 32 + (b * 32 < t.cols ? b : 0);
+      } else {
+        coff[i] = static_cast<uint32_t>(row * cpitch) + (t.col0 + (col < t.cols ? col : 0)) * 2u;
+      }
+      if constexpr (INPUT) {
+        const int r = wave * 64 + i * 16 + (lane >> 2), c = (lane & 3) ^ ((r >> 1) & 3);
+        roff[i] = static_cast<uint32_t>((r < t.rows ? r : t.rows - 1) * rpitch) + c * 16u;
+      } else {
+        roff[i] = static_cast<uint32_t>(row * rpitch) + (t.row0 + (col < t.rows ? col : 0)) * 2u;
+      }
     }
-    if constexpr (INPUT) {
-      const int r = wave * 64 + i * 16 + (lane >> 2), c = (lane & 3) ^ ((r >> 1) & 3);
-      roff[i] = static_cast<uint32_t>((r < out_rows ? r : out_rows - 1) * rpitch) + c * 16u;
-    } else {
-      roff[i] = static_cast<uint32_t>(t * rpitch) + (row0 + (col < out_rows ? col : 0)) * 2u;
-    }
-  }
-  const int64_t cstep = kStep * cpitch, rstep = INPUT ? kStep * 2 : kStep * rpitch;
+  };
+  const int64_t cstep = kStep * cpitch, rstep = INPUT ? kStep * 2 : kStep * rpitch, sstep = static_cast<int64_t>(kStep) * blocks;
   auto buffer_of = [](const uint8_t *p) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p), 0, -1, 0x00020000); };
   const uint32_t cdst = lds0 + wave * 4096, rdst = cdst + rows_at(G), codes = lds0 + codes_at() + wave * 2048, scales = lds0 + scales_at() + wave * 256;
-  // Where fill q of a step goes.
-  auto target = [&](int slot, int q) {
-    if (q >= kColFills) return rdst + slot * kSlot + (q - kColFills) * 1024;
-    if (!EIGHT) return cdst + slot * kSlot + q * 1024;
-    return q < 2 ? codes + slot * kCodeSlot + q * 1024 : scales + slot * kScaleSlot;
+  using std::integral_constant;
+  // M0 for fill Q of the step in slot SLOT: where it goes.  (Base and constant apart: 28 addresses would take as many registers, and what the compiler brings back
+  // from a vector register's lanes right before a load comes too late for it.)
+  auto set_target = [&](auto SLOT, auto Q) {
+    constexpr int slot = decltype(SLOT)::value, q = decltype(Q)::value;
+    constexpr bool row = q >= kColFills, code = !row && EIGHT && q < 2, scale = !row && EIGHT && q == 2;
+    constexpr int at = row ? slot * kSlot + (q - kColFills) * 1024 : (code ? slot * kCodeSlot + q * 1024 : (scale ? slot * kScaleSlot : slot * kSlot + q * 1024));
+    const uint32_t base = row ? rdst : (code ? codes : (scale ? scales : cdst));
+    asm volatile("s_add_u32 m0, %0, %1" : : "s"(base), "i"(at) : "memory", "scc");
   };
 
   f32x4 acc[8][8];  // [row block][column block]
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   // ---- fragment addresses -------------------------------------------------------------------------------------------
   uint32_t cfrag[8], rfrag[8];
@@ -225,8 +299,9 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const GradArgs a
   };
 
   // Fill Q of a step (the columns' operand first) that may be the partial last one: `valid` of its 32 values exist.
-  auto fill_guarded = [&](int slot, auto Q, const uint8_t *cat, const uint8_t *rat, const uint8_t *sat, int valid) {
+  auto fill_guarded = [&](auto SLOT, auto Q, const uint8_t *cat, const uint8_t *rat, const uint8_t *sat, int valid) {
     constexpr int q = decltype(Q)::value, r = q - kColFills;
+    const int lane = fresh_lane();
     const uint8_t *zeros = reinterpret_cast<const uint8_t *>(g_zeros) + lane * 16;
     const uint8_t *src;
     if constexpr (r >= 0 && INPUT) src = ((lane & 3) ^ (((wave * 64 + r * 16 + (lane >> 2)) >> 1) & 3)) * 8 < valid ? rat + roff[r] : zeros;
@@ -234,35 +309,33 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const GradArgs a
     else if constexpr (!EIGHT) src = wave * 8 + q * 2 + (lane >> 5) < valid ? cat + coff[q] : zeros;
     else if constexpr (q < 2) src = wave * 8 + q * 4 + (lane >> 4) < valid ? cat + coff[q] : zeros;
     else src = wave * 8 + (lane >> 3) < valid ? sat + coff[q] : zeros;
-    const LdsPtr dst = (LdsPtr)(uintptr_t)__builtin_amdgcn_readfirstlane(target(slot, q));
-    if constexpr (EIGHT && q == 2) __builtin_amdgcn_global_load_lds((GlobalPtr)src, dst, 1, 0, 0);
-    else __builtin_amdgcn_global_load_lds((GlobalPtr)src, dst, 16, 0, 0);
+    set_target(SLOT, Q);
+    fill_from<EIGHT && q == 2>(src);
   };
   auto valid_of = [&](int s) { return s < whole ? kStep : sum_over - s * kStep; };
 
-  // ---- the first four steps -------------------------------------------------------------------------------------
-  const int64_t sstep = static_cast<int64_t>(kStep) * blocks;
-  using std::integral_constant;
-#pragma unroll
-  for (int s = 0; s < kSlots; ++s)
-    static_for<kFills>([&](auto Q) { fill_guarded(s, Q, cbase + s * cstep, rbase + s * rstep, EIGHT ? sbase + s * sstep : nullptr, valid_of(s)); });
-  if constexpr (EIGHT) {
-    FLUXMI_VMCNT(2 * kFills);
-    static_for<2>([&](auto S) {
-      read_codes(S);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) convert16<F16>(code[i], scale_byte[i], value[i]), write_values(S, i);
+  auto first_fills = [&]() {
+    static_for<kSlots>([&](auto S) {
+      constexpr int s = decltype(S)::value;
+      static_for<kFills>([&](auto Q) { fill_guarded(S, Q, cbase + s * cstep, rbase + s * rstep, EIGHT ? sbase + s * sstep : nullptr, valid_of(s)); });
     });
-    FLUXMI_LGKM0();
-  } else {
-    FLUXMI_VMCNT(3 * kFills);
-  }
-  __builtin_amdgcn_s_barrier();
-  static_for<kReads>([&](auto R) { read_one(integral_constant<int, 0>{}, R, ca, ra); });
-  FLUXMI_LGKM0();
+  };
 
   // What a step waits for: the next one's rows and columns; WEIGHT_8BIT: that one's rows and the codes of the one after it.
   constexpr int kOpen = EIGHT ? kFills + 4 : 2 * kFills;
+  // Loads and stores leave the counter in their order.  A tile's first fills are requested before the stores of the tile before it, so that the first kFresh steps
+  // need not wait for those: kStores of them for 16 bits; those of 32 bits are more than the counter holds, which has then seen all fills in.
+  constexpr int kFresh = EIGHT ? 2 : 3, kStores = 32;
+  int behind = 0;  // stores behind the first fills: 0 none, 1 kStores, 2 as many as the counter holds
+  auto wait_step = [&](auto U, int s) {
+    if constexpr (decltype(U)::value < kFresh) {
+      if (s == decltype(U)::value && behind != 0) {
+        if (behind == 1) FLUXMI_VMCNT(kOpen + kStores);
+        return;
+      }
+    }
+    FLUXMI_VMCNT(kOpen);
+  };
   // Step U of a trip of four: its fragments are in (cf, rf), those of the next go to (cn, rn), and its slot is filled with the step four further on,
   // `at` bytes behind the buffers' start.
   const int cstep32 = static_cast<int>(cstep), rstep32 = static_cast<int>(rstep), sstep32 = static_cast<int>(sstep);
@@ -276,9 +349,9 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const GradArgs a
     else if constexpr (t == 16 || t == 32) convert16<F16>(code[t / 32], scale_byte[t / 32], value[t / 32]);
     else if constexpr (t == 24 || t == 40) write_values(slot, t / 40);
   };
-  auto step = [&](auto U, u32x4(&cf)[8], u32x4(&rf)[8], u32x4(&cn)[8], u32x4(&rn)[8]) {
+  auto step = [&](auto U, int s, u32x4(&cf)[8], u32x4(&rf)[8], u32x4(&cn)[8], u32x4(&rn)[8]) {
     constexpr int u = decltype(U)::value;
-    FLUXMI_VMCNT(kOpen);
+    wait_step(U, s);
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     static_for<64>([&](auto T) {
@@ -287,8 +360,7 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const GradArgs a
       if constexpr (t < 2 * kReads && t % 2 == 0) read_one(integral_constant<int, (u + 1) % kSlots>{}, integral_constant<int, t / 2>{}, cn, rn);
       constexpr int q = t / 8, r = q - kColFills;
       if constexpr (t % 8 == 3 && q < kFills) {
-        const uint32_t dst = target(u, q);
-        asm volatile("s_mov_b32 m0, %0" : : "s"(dst) : "memory");
+        set_target(U, integral_constant<int, q>{});
       }
       if constexpr (t % 8 == 4 && q < kFills) {
         if constexpr (r >= 0) asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds" : : "v"(roff[r]), "s"(rrsrc), "s"(u * rstep32) : "memory");
@@ -304,7 +376,7 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const GradArgs a
   // The same near the end of the sum: s is the step's number.  What lies past the end is filled as well, with zeros, so that the waits count the same.
   auto last_step = [&](auto U, int s, u32x4(&cf)[8], u32x4(&rf)[8], u32x4(&cn)[8], u32x4(&rn)[8]) {
     constexpr int u = decltype(U)::value;
-    FLUXMI_VMCNT(kOpen);
+    wait_step(U, s);
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     const uint8_t *const cat = cbase + (s + 4) * cstep, *const rat = rbase + (s + 4) * rstep, *const sat = EIGHT ? sbase + (s + 4) * sstep : nullptr;
@@ -315,7 +387,7 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const GradArgs a
       static_for<kReads / 8>([&](auto R) {
         read_one(integral_constant<int, (u + 1) % kSlots>{}, integral_constant<int, i * (kReads / 8) + decltype(R)::value>{}, cn, rn);
       });
-      if constexpr (i < kFills) fill_guarded(u, I, cat, rat, sat, valid);
+      if constexpr (i < kFills) fill_guarded(U, I, cat, rat, sat, valid);
       __builtin_amdgcn_sched_barrier(0);
       static_for<8>([&](auto J) { mfma<F16>(acc[i][decltype(J)::value], cf[decltype(J)::value], rf[i]); });
       __builtin_amdgcn_sched_barrier(0);
@@ -323,54 +395,119 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const GradArgs a
     FLUXMI_LGKM0();
     __builtin_amdgcn_sched_barrier(0);
   };
-  int s = 0;
-  for (; s + 8 <= whole; s += 4) {
-    crsrc = buffer_of(cbase + (s + 4) * cstep);
-    rrsrc = buffer_of(rbase + (s + 4) * rstep);
-    if constexpr (EIGHT) srsrc = buffer_of(sbase + (s + 4) * sstep);
-    step(integral_constant<int, 0>{}, ca, ra, cb, rb);
-    step(integral_constant<int, 1>{}, cb, rb, ca, ra);
-    step(integral_constant<int, 2>{}, ca, ra, cb, rb);
-    step(integral_constant<int, 3>{}, cb, rb, ca, ra);
-  }
-  while (s < steps) {
-    last_step(integral_constant<int, 0>{}, s, ca, ra, cb, rb);
-    if (++s >= steps) break;
-    last_step(integral_constant<int, 1>{}, s, cb, rb, ca, ra);
-    if (++s >= steps) break;
-    last_step(integral_constant<int, 2>{}, s, ca, ra, cb, rb);
-    if (++s >= steps) break;
-    last_step(integral_constant<int, 3>{}, s, cb, rb, ca, ra);
-    ++s;
-  }
-  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // the last sums are in their registers
-  FLUXMI_VMCNT(0);  // no fill may come after the workgroup's end
 
-  // ---- lane l has columns 4 (l / 16) .. + 3 of row l % 16 of a block -----------------------------------------------
-  const int g = lane >> 4;
-  static_for<8>([&](auto I) {
-    constexpr int i = decltype(I)::value;
-    const int r = wr * 128 + i * 16 + (lane & 15);
-    if (a.out_f32 || a.accumulate) {
+  Tile tile{};
+  int turn = 0;
+  auto next_tile = [&]() {
+    Tile t{};
+    while (turn < args.turns && t.rows == 0) t = describe(turn++);
+    return t;
+  };
+  tile = next_tile();
+  if (tile.rows == 0) return;
+  begin_tile(tile);
+  first_fills();
+  for (;;) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int c = wc * 128 + j * 16 + g * 4;
-        if (r < out_rows && c < out_cols) store4_whole<F16>(a, (out_row0 + r) * a.k + col0 + c, acc[i][j]);
-      }
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if constexpr (EIGHT) {
+      if (behind == 0) FLUXMI_VMCNT(2 * kFills);
+      else if (behind == 1) FLUXMI_VMCNT(2 * kFills + kStores);
+      static_for<2>([&](auto S) {
+        read_codes(S);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) convert16<F16>(code[i], scale_byte[i], value[i]), write_values(S, i);
+      });
+      FLUXMI_LGKM0();
     } else {
-      // Two blocks' sums change lanes, so that each has eight neighbouring columns: of the first block in lane groups 0 and 2, of the second in 1 and 3.
+      if (behind == 0) FLUXMI_VMCNT(3 * kFills);
+      else if (behind == 1) FLUXMI_VMCNT(3 * kFills + kStores);
+    }
+    __builtin_amdgcn_s_barrier();
+    static_for<kReads>([&](auto R) { read_one(integral_constant<int, 0>{}, R, ca, ra); });
+    FLUXMI_LGKM0();
+    int s = 0;
+    for (; s + 8 <= whole; s += 4) {
+      crsrc = buffer_of(cbase + (s + 4) * cstep);
+      rrsrc = buffer_of(rbase + (s + 4) * rstep);
+      if constexpr (EIGHT) srsrc = buffer_of(sbase + (s + 4) * sstep);
+      step(integral_constant<int, 0>{}, s, ca, ra, cb, rb);
+      step(integral_constant<int, 1>{}, s + 1, cb, rb, ca, ra);
+      step(integral_constant<int, 2>{}, s + 2, ca, ra, cb, rb);
+      step(integral_constant<int, 3>{}, s + 3, cb, rb, ca, ra);
+    }
+    while (s < steps) {
+      last_step(integral_constant<int, 0>{}, s, ca, ra, cb, rb);
+      if (++s >= steps) break;
+      last_step(integral_constant<int, 1>{}, s, cb, rb, ca, ra);
+      if (++s >= steps) break;
+      last_step(integral_constant<int, 2>{}, s, ca, ra, cb, rb);
+      if (++s >= steps) break;
+      last_step(integral_constant<int, 3>{}, s, cb, rb, ca, ra);
+      ++s;
+    }
+    const Tile next = next_tile();
+    __builtin_amdgcn_s_barrier();  // nobody reads the slots any more
+    if (next.rows > 0) {
+      begin_tile(next);
+      first_fills();
+    }
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // the last sums are in their registers
+
+    // ---- lane l has columns 4 (l / 16) .. + 3 of row l % 16 of a block --------------------------------------------
+    const int out_lane = fresh_lane(), g = out_lane >> 4;
+    if (a.accumulate) {
+      static_for<8>([&](auto I) {
+        const int r = wr * 128 + decltype(I)::value * 16 + (out_lane & 15);
 #pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        uint32_t x0 = pack2<F16>(acc[i][j][0], acc[i][j][1]), x1 = pack2<F16>(acc[i][j][2], acc[i][j][3]);
-        uint32_t y0 = pack2<F16>(acc[i][j + 1][0], acc[i][j + 1][1]), y1 = pack2<F16>(acc[i][j + 1][2], acc[i][j + 1][3]);
-        const auto p = __builtin_amdgcn_permlane16_swap(x0, y0, false, false);
-        const auto q = __builtin_amdgcn_permlane16_swap(x1, y1, false, false);
-        const int c = wc * 128 + (j + (g & 1)) * 16 + (g >> 1) * 8;
-        if (r < out_rows && c < out_cols)
-          *reinterpret_cast<u32x4 *>(a.out + ((out_row0 + r) * a.k + col0 + c) * 2) = u32x4{p[0], q[0], p[1], q[1]};
+        for (int j = 0; j < 8; ++j) {
+          const int c = wc * 128 + j * 16 + g * 4;
+          if (r < tile.rows && c < tile.cols) store4_whole<F16>(a, (tile.out_row0 + r) * a.k + tile.col0 + c, sums_of(acc[decltype(I)::value][j]));
+        }
+      });
+      FLUXMI_VMCNT(0);
+      behind = 0;
+    } else {
+      // The buffer ends with the tile's rows; columns past its end are sent past the buffer's.  Every store is issued, so that they can be counted.
+      const int out_size = a.out_f32 ? 4 : 2;
+      const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(a.out + tile.out_row0 * a.k * out_size, 0,
+                                                                           static_cast<int>(static_cast<uint32_t>(tile.rows) * a.k * out_size), 0x00020000);
+      const uint32_t row_at = static_cast<uint32_t>(wr * 128 + (out_lane & 15)) * a.k + tile.col0;
+      if (a.out_f32) {
+        static_for<8>([&](auto I) {
+          constexpr int i = decltype(I)::value;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int c = wc * 128 + j * 16 + g * 4;
+            const uint32_t at = c < tile.cols ? (row_at + i * 16 * a.k + c) * 4 : 0xfffffff0u;
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sums_of(acc[i][j])), out, at, 0, 0);
+          }
+        });
+        behind = 2;
+      } else {
+        // Two blocks' sums change lanes, so that each has eight neighbouring columns: of the first block in lane groups 0 and 2, of the second in 1 and 3.
+        static_for<8>([&](auto I) {
+          constexpr int i = decltype(I)::value;
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            const f32x4 x = sums_of(acc[i][j]), y = sums_of(acc[i][j + 1]);
+            const uint32_t x0 = pack2<F16>(x[0], x[1]), x1 = pack2<F16>(x[2], x[3]), y0 = pack2<F16>(y[0], y[1]), y1 = pack2<F16>(y[2], y[3]);
+            const auto p = __builtin_amdgcn_permlane16_swap(x0, y0, false, false);
+            const auto q = __builtin_amdgcn_permlane16_swap(x1, y1, false, false);
+            const int c = wc * 128 + (j + (g & 1)) * 16 + (g >> 1) * 8;
+            const uint32_t at = c < tile.cols ? (row_at + i * 16 * a.k + c) * 2 : 0xfffffff0u;
+            __builtin_amdgcn_raw_buffer_store_b128(u32x4{p[0], q[0], p[1], q[1]}, out, at, 0, 0);
+          }
+        });
+        behind = 1;
       }
     }
-  });
+    if (next.rows == 0) break;
+    tile = next;
+  }
+  FLUXMI_VMCNT(0);  // no fill may come after the workgroup's end
 #endif
 }
 
@@ -389,9 +526,14 @@ int launch_grad_tiles(Grad g, bool f16, const GradArgs &a, void *stream) {
   const int64_t tiles_k = (a.k + kTile - 1) / kTile, tiles_n = (a.n + kTile - 1) / kTile;
   const int64_t items = g == Grad::INPUT ? (a.rows / kTile + (a.rows < a.nexperts ? a.rows : a.nexperts) + 1) * tiles_k : a.nexperts * tiles_n * tiles_k;
   FLUXMI_REQUIRE(items < (1 << 24), FLUXMI_ERR_UNSUPPORTED, "gradients of the grouped product: too many rows and columns for one launch");
+  // A workgroup's tiles follow each other without a gap; several workgroups to a compute unit even out experts of different sizes.
+  int64_t turns = items / (3 * 256);
+  if (turns < 1) turns = 1;
+  TileArgs t{a, static_cast<int32_t>(items), static_cast<int32_t>(turns)};
+  const uint32_t grid = static_cast<uint32_t>(((items + turns - 1) / turns + 7) / 8 * 8);
   auto launch = [&](auto kernel, std::atomic<uint64_t> &done) -> int {
     if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds_bytes(g), done)) return rc;
-    kernel<<<static_cast<uint32_t>(items), kThreads, lds_bytes(g), static_cast<hipStream_t>(stream)>>>(a);
+    kernel<<<grid, kThreads, lds_bytes(g), static_cast<hipStream_t>(stream)>>>(t);
     FLUXMI_HIP_CHECK(hipGetLastError());
     return FLUXMI_OK;
   };

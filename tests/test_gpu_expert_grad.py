@@ -115,6 +115,47 @@ def test_wgrad(splits, rest, n, k, dtype, out, kept):
     assert torch.equal(total, got)
 
 
+# Sums of every length around the steps of the tiles, widths that end anywhere in them, and several tiles to a workgroup.
+TILES = [([s for s in range(0, 40)], 3, 264, 272), ([224, 255, 256, 257, 287, 288, 289, 320, 33], 1, 96, 48), ([1000, 31, 513], 0, 776, 528), ([640, 0, 2100], 40, 256, 256),
+         ([96, 500], 7, 2056, 2064)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("splits,rest,n,k", TILES)
+def test_tiles(splits, rest, n, k, dtype):
+    print(f"[case] tiles {splits[:6]} {rest} {n} {k} {dtype}", flush=True)
+    rows = sum(splits) + rest
+    grad, x, weight = data((rows, n), dtype, 3), data((rows, k), dtype, 4), data((len(splits), n, k), dtype, 5)
+    close(flux_amd.moe_dgrad(grad, weight, counts(splits)), want_dgrad(grad, weight, splits), n * 2.0**-23 * want_dgrad(grad.abs(), weight.abs(), splits))
+    codes, scale = flux_amd.moe_checkpoint(x)
+    for given, its_scale, x64 in ((x, None, x.double()), (codes, scale, values(codes, scale))):
+        want, slack = want_wgrad(grad, x64, splits), max(splits) * 2.0**-23 * want_wgrad(grad.abs(), x64.abs(), splits)
+        for out in (dtype, F32):
+            got = flux_amd.moe_wgrad(grad, given, counts(splits), its_scale, output_dtype=out)
+            close(got, want, slack)
+            total = torch.ones_like(got)
+            flux_amd.moe_wgrad(grad, given, counts(splits), its_scale, output=total, accumulate=True)
+            close(total, want + 1, slack + 2.0**-23 * (1 + want.abs()))
+
+
+@pytest.mark.parametrize("experts", [60, 150])
+def test_many_tiles_to_a_workgroup(experts):
+    """Thousands of tiles, of which neighbours differ in length, each against the tile's own call."""
+    n, k = 1024, 1040
+    g = torch.Generator().manual_seed(experts)
+    splits = torch.randint(0, 90, (experts,), generator=g).tolist()
+    rows = sum(splits) + 11
+    grad, x, w = data((rows, n), BF16, 1), data((rows, k), BF16, 2), data((experts, n, k), BF16, 3)
+    codes, scale = flux_amd.moe_checkpoint(x)
+    for given, its_scale, x64 in ((x, None, x.double()), (codes, scale, values(codes, scale))):
+        want, slack = want_wgrad(grad, x64, splits), 90 * 2.0**-23 * want_wgrad(grad.abs(), x64.abs(), splits)
+        for out in (BF16, F32):
+            close(flux_amd.moe_wgrad(grad, given, counts(splits), its_scale, output_dtype=out), want, slack)
+    big = [s * 9 for s in splits]
+    grad = data((sum(big) + 5, n), BF16, 4)
+    close(flux_amd.moe_dgrad(grad, w, counts(big)), want_dgrad(grad, w, big), n * 2.0**-23 * want_dgrad(grad.abs(), w.abs(), big))
+
+
 def test_counts_past_the_rows():
     """What the counts have past the rows does not exist; sums of them overflow nothing."""
     grad, x, w = data((50, 64), BF16, 1), data((50, 40), BF16, 2), data((3, 64, 40), BF16, 3)
