@@ -7,8 +7,8 @@
 //    X, and G for the weights' gradient) lies in rows of 256 columns, 512 bytes; 16 columns of a row (32 bytes) are at place s ^ f(row), f = row % 4 + 4 (row / 8 % 2), so
 //    that the eight rows which half a wave reads together are on different banks.  G for the input's gradient lies in rows of 32 values, 64 bytes.
 //  * A fragment of an "across" operand comes back through the transposing read, twice four rows of 16 columns.
-//  * What is past the end of the sum is zeros, fetched from a page of them; rows and columns past the end of the result are others' values, which reach
-//    no result that is stored.
+//  * A step that is not whole is fetched as far as the sum goes, and the rest of it is cleared in LDS; rows and columns past the end of the result are others'
+//    values, which reach no result that is stored.
 #include "grouped_gemm_grad_tiles.hpp"
 
 #include <type_traits>
@@ -27,17 +27,17 @@ constexpr int kCodeSlot = 8192, kScaleSlot = 1024;  // WEIGHT_8BIT: a step's cod
 constexpr int rows_at(Grad g) { return (g == Grad::WEIGHT_8BIT ? 2 : kSlots) * kSlot; }
 constexpr int codes_at() { return rows_at(Grad::WEIGHT_8BIT) + kSlots * kSlot; }
 constexpr int scales_at() { return codes_at() + kSlots * kCodeSlot; }
-// Behind them the experts' tables: where their rows end, and (INPUT) their tiles.
-constexpr int tables_at(Grad g) { return g == Grad::WEIGHT_8BIT ? scales_at() + kSlots * kScaleSlot : rows_at(g) + kSlots * kSlot; }
-constexpr int lds_bytes(Grad g) { return tables_at(g) + (g == Grad::INPUT ? 2 : 1) * 4 * kMaxExperts; }
+// Behind them a window of each wave, through which results go out, and the experts' tables: where their rows end, and (INPUT) their tiles.
+constexpr int kWindow = 2048;
+constexpr int windows_at(Grad g) { return g == Grad::WEIGHT_8BIT ? scales_at() + kSlots * kScaleSlot : rows_at(g) + kSlots * kSlot; }
+constexpr int tables_at(Grad g) { return windows_at(g) + kThreads / 64 * kWindow; }
+constexpr int lds_bytes(Grad g) { return tables_at(g) + (g == Grad::INPUT ? 2 : 1) * 4 * kMaxExperts + 16; }
 
 struct TileArgs {
   GradArgs a;
   int32_t items;  // tiles of the result (INPUT: as many as there can be)
   int32_t turns;  // tiles that a workgroup computes
 };
-
-__device__ uint4 g_zeros[64];  // 16 bytes of zeros for each lane
 
 #if defined(__HIP_DEVICE_COMPILE__)
 
@@ -55,11 +55,16 @@ __device__ __forceinline__ void static_for(F &&f) {
   static_for_seq(f, std::make_integer_sequence<int, END>{});
 }
 
-// Pinned to the accumulation registers: given the builtin, the compiler spreads the sums over both files and moves them about.
-template <bool F16>
+// Pinned to the accumulation registers: given the builtin, the compiler spreads the sums over both files and moves them about.  FIRST: a sum begins.
+template <bool F16, bool FIRST>
 __device__ __forceinline__ void mfma(f32x4 &acc, const u32x4 &a, const u32x4 &b) {
-  if constexpr (F16) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
-  else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+  if constexpr (F16) {
+    if constexpr (FIRST) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, 0" : "=a"(acc) : "v"(a), "v"(b));
+    else asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+  } else {
+    if constexpr (FIRST) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=a"(acc) : "v"(a), "v"(b));
+    else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+  }
 }
 
 // A sum's block, read where it is used: the compiler would copy all of them to vector registers ahead of the branches of the stores.
@@ -74,6 +79,12 @@ __device__ __forceinline__ f32x4 sums_of(const f32x4 &acc) {
   return v;
 }
 
+// Sixteen bytes (BYTE: one, to a word) of each lane to LDS, from M0 on.  Not the builtin: with it the compiler lets every LDS read wait for all loads.
+template <bool BYTE>
+__device__ __forceinline__ void load_to_lds(uint32_t off, __amdgpu_buffer_rsrc_t rsrc) {
+  if constexpr (BYTE) asm volatile("buffer_load_ubyte %0, %1, 0 offen lds" : : "v"(off), "s"(rsrc) : "memory");
+  else asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(off), "s"(rsrc) : "memory");
+}
 // Sixteen codes of one block to values of 16 bits.
 template <bool F16>
 __device__ __forceinline__ void convert16(const u32x4 codes, uint32_t byte, u32x4 (&v)[2]) {
@@ -95,8 +106,8 @@ __device__ __forceinline__ void convert16(const u32x4 codes, uint32_t byte, u32x
 struct Tile {
   int e, row0, rows, col0, cols;  // row0: column of grad for weights, otherwise 0; rows = 0: there is no such tile
   int sum_over;
+  int first;  // of the rows that it sums over (INPUT: reads)
   int64_t out_row0;
-  int64_t first;  // of the rows that it sums over (INPUT: reads)
 };
 
 // The lane, opaque to the compiler: what is computed from it is not kept in registers through the loops.
@@ -104,15 +115,6 @@ __device__ __forceinline__ int fresh_lane() {
   int l = lane_id();
   asm volatile("" : "+v"(l));
   return l;
-}
-
-// Direct-to-LDS loads of 16 bytes (BYTE: one, to a word) by address; M0 holds the LDS address.  Not the builtins: with these the compiler lets every LDS read wait for
-// all loads.
-template <bool BYTE>
-__device__ __forceinline__ void fill_from(const uint8_t *src) {
-  asm volatile("s_nop 0" : : : "memory");
-  if constexpr (BYTE) asm volatile("global_load_lds_ubyte %0, off" : : "v"(src) : "memory");
-  else asm volatile("global_load_lds_dwordx4 %0, off" : : "v"(src) : "memory");
 }
 
 #endif  // __HIP_DEVICE_COMPILE__
@@ -186,7 +188,7 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
       t.rows = a.n - t.row0 < kTile ? a.n - t.row0 : kTile;
       t.out_row0 = static_cast<int64_t>(e) * a.n + t.row0;
       t.first = e > 0 ? __builtin_amdgcn_readfirstlane(row_ends[e - 1]) : 0;
-      t.sum_over = __builtin_amdgcn_readfirstlane(row_ends[e]) - static_cast<int>(t.first);
+      t.sum_over = __builtin_amdgcn_readfirstlane(row_ends[e]) - t.first;
     }
     return t;
   };
@@ -196,17 +198,25 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
   // Codes: four rows, lane l chunk l % 16 (of 16 columns) of row l / 16; scales: the eight rows whose codes this wave fetches, a word to each byte.
   constexpr int kColFills = EIGHT ? 3 : 4, kFills = kColFills + 4;
   uint32_t coff[4], roff[4];
-  const uint8_t *rbase = nullptr, *cbase = nullptr, *sbase = nullptr;
-  int steps = 0, whole = 0, sum_over = 0;
+  // The step that is requested next: where it begins, and how much of the sum (INPUT: of the tile's rows of G, in bytes) is left there.
+  const uint8_t *rnext = nullptr, *cnext = nullptr, *snext = nullptr;
+  int left = 0, rbytes = 0;
+  int steps = 0, rest = 0;  // rest: values of the last step
   auto begin_tile = [&](const Tile &t) {
     const int lane = fresh_lane();
-    sum_over = t.sum_over;
-    steps = (sum_over + kStep - 1) / kStep;
-    whole = sum_over / kStep;
-    rbase = a.grad + t.first * rpitch;
-    if constexpr (INPUT) cbase = a.other + static_cast<int64_t>(t.e < a.nexperts ? t.e : 0) * a.n * cpitch;
-    else cbase = a.other + t.first * cpitch;
-    if constexpr (EIGHT) sbase = a.scale + t.first * blocks;
+    left = __builtin_amdgcn_readfirstlane(t.sum_over);
+    steps = left > 0 ? (left + kStep - 1) / kStep : 1;  // (a sum of nothing is a step that is cleared)
+    rest = left - (steps - 1) * kStep;
+    const int64_t first = __builtin_amdgcn_readfirstlane(t.first);
+    rnext = a.grad + first * rpitch;
+    if constexpr (INPUT) {
+      const int e = __builtin_amdgcn_readfirstlane(t.e);
+      cnext = a.other + static_cast<int64_t>(e < a.nexperts ? e : 0) * a.n * cpitch;
+      rbytes = __builtin_amdgcn_readfirstlane(t.rows) * static_cast<int>(rpitch);
+    } else {
+      cnext = a.other + first * cpitch;
+    }
+    if constexpr (EIGHT) snext = a.scale + first * blocks;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = wave * 8 + i * 2 + (lane >> 5), f = (row & 3) | ((row >> 1) & 4);
@@ -227,7 +237,24 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
     }
   };
   const int64_t cstep = kStep * cpitch, rstep = INPUT ? kStep * 2 : kStep * rpitch, sstep = static_cast<int64_t>(kStep) * blocks;
-  auto buffer_of = [](const uint8_t *p) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p), 0, -1, 0x00020000); };
+  __amdgpu_buffer_rsrc_t crsrc, rrsrc, srsrc;
+  // The buffers of the step that is requested next; what lies behind their end is not fetched.
+  auto next_buffers = [&]() {
+    auto buffer = [](const uint8_t *p, int bytes) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p), 0, bytes, 0x00020000); };
+    int rows = left < kStep ? left : kStep;
+    asm("" : "+s"(rows));  // (as one clamp it would be computed in vector registers)
+    rows = rows < 0 ? 0 : rows;
+    crsrc = buffer(cnext, rows * static_cast<int>(cpitch));
+    cnext += cstep;
+    if constexpr (EIGHT) {
+      srsrc = buffer(snext, rows * blocks);
+      snext += sstep;
+    }
+    rrsrc = buffer(rnext, INPUT ? (rbytes < 0 || rows == 0 ? 0 : rbytes) : rows * static_cast<int>(rpitch));
+    rnext += rstep;
+    if constexpr (INPUT) rbytes -= kStep * 2;
+    left -= kStep;
+  };
   const uint32_t cdst = lds0 + wave * 4096, rdst = cdst + rows_at(G), codes = lds0 + codes_at() + wave * 2048, scales = lds0 + scales_at() + wave * 256;
   using std::integral_constant;
   // M0 for fill Q of the step in slot SLOT: where it goes.  (Base and constant apart: 28 addresses would take as many registers, and what the compiler brings back
@@ -298,27 +325,43 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
     for (int h = 0; h < 2; ++h) *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(value_at[i] + (slot % 2) * kSlot + h * 16) = value[i][h];
   };
 
-  // Fill Q of a step (the columns' operand first) that may be the partial last one: `valid` of its 32 values exist.
-  auto fill_guarded = [&](auto SLOT, auto Q, const uint8_t *cat, const uint8_t *rat, const uint8_t *sat, int valid) {
+  auto fill = [&](auto Q) {
     constexpr int q = decltype(Q)::value, r = q - kColFills;
-    const int lane = fresh_lane();
-    const uint8_t *zeros = reinterpret_cast<const uint8_t *>(g_zeros) + lane * 16;
-    const uint8_t *src;
-    if constexpr (r >= 0 && INPUT) src = ((lane & 3) ^ (((wave * 64 + r * 16 + (lane >> 2)) >> 1) & 3)) * 8 < valid ? rat + roff[r] : zeros;
-    else if constexpr (r >= 0) src = wave * 8 + r * 2 + (lane >> 5) < valid ? rat + roff[r] : zeros;
-    else if constexpr (!EIGHT) src = wave * 8 + q * 2 + (lane >> 5) < valid ? cat + coff[q] : zeros;
-    else if constexpr (q < 2) src = wave * 8 + q * 4 + (lane >> 4) < valid ? cat + coff[q] : zeros;
-    else src = wave * 8 + (lane >> 3) < valid ? sat + coff[q] : zeros;
-    set_target(SLOT, Q);
-    fill_from<EIGHT && q == 2>(src);
+    if constexpr (r >= 0) load_to_lds<false>(roff[r < 0 ? 0 : r], rrsrc);
+    else if constexpr (EIGHT && q == 2) load_to_lds<true>(coff[2], srsrc);
+    else load_to_lds<false>(coff[q < 4 ? q : 0], crsrc);
   };
-  auto valid_of = [&](int s) { return s < whole ? kStep : sum_over - s * kStep; };
-
   auto first_fills = [&]() {
     static_for<kSlots>([&](auto S) {
-      constexpr int s = decltype(S)::value;
-      static_for<kFills>([&](auto Q) { fill_guarded(S, Q, cbase + s * cstep, rbase + s * rstep, EIGHT ? sbase + s * sstep : nullptr, valid_of(s)); });
+      next_buffers();
+      static_for<kFills>([&](auto Q) {
+        set_target(S, Q);
+        asm volatile("s_nop 0" : : : "memory");
+        fill(Q);
+      });
     });
+    next_buffers();
+  };
+
+  // Clears what this wave fetched of a step that is not whole, behind its `rest` values.  (Lanes with nothing to clear write to a place of no use: a branch among the
+  // lanes would cost the sums their registers.)
+  const uint32_t nowhere = lds0 + lds_bytes(G) - 16;
+  auto clear = [&](uint32_t at, bool there) { *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(there ? nowhere : at) = u32x4{0u, 0u, 0u, 0u}; };
+  auto clear_columns = [&](int s) {
+    const int lane = fresh_lane(), slot = s & (kSlots - 1);
+    if constexpr (EIGHT) {
+      for (int i = 0; i < 2; ++i) clear(codes + slot * kCodeSlot + i * 1024 + lane * 16, wave * 8 + i * 4 + (lane >> 4) < rest);
+      *(__attribute__((address_space(3))) uint32_t *)(uintptr_t)(wave * 8 + (lane >> 3) < rest ? nowhere : scales + slot * kScaleSlot + lane * 4) = 0;
+    } else {
+      for (int i = 0; i < 4; ++i) clear(cdst + slot * kSlot + i * 1024 + lane * 16, wave * 8 + i * 2 + (lane >> 5) < rest);
+    }
+  };
+  auto clear_rows = [&](int s) {
+    const int lane = fresh_lane(), slot = s & (kSlots - 1);
+    for (int i = 0; i < 4; ++i) {
+      const int r = wave * 64 + i * 16 + (lane >> 2);
+      clear(rdst + slot * kSlot + i * 1024 + lane * 16, INPUT ? ((lane & 3) ^ ((r >> 1) & 3)) * 8 < rest : wave * 8 + i * 2 + (lane >> 5) < rest);
+    }
   };
 
   // What a step waits for: the next one's rows and columns; WEIGHT_8BIT: that one's rows and the codes of the one after it.
@@ -328,18 +371,25 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
   constexpr int kFresh = EIGHT ? 2 : 3, kStores = 32;
   int behind = 0;  // stores behind the first fills: 0 none, 1 kStores, 2 as many as the counter holds
   auto wait_step = [&](auto U, int s) {
+    bool waited = false;
     if constexpr (decltype(U)::value < kFresh) {
       if (s == decltype(U)::value && behind != 0) {
         if (behind == 1) FLUXMI_VMCNT(kOpen + kStores);
-        return;
+        waited = true;
       }
     }
-    FLUXMI_VMCNT(kOpen);
+    if (!waited) FLUXMI_VMCNT(kOpen);
+    if (s + 3 >= steps && rest < kStep) {
+      if (s + 2 == steps) {
+        clear_rows(s + 1);
+        if (!EIGHT) clear_columns(s + 1);
+      } else if (EIGHT && s + 3 == steps) {
+        clear_columns(s + 2);
+      }
+      FLUXMI_LGKM0();
+    }
   };
-  // Step U of a trip of four: its fragments are in (cf, rf), those of the next go to (cn, rn), and its slot is filled with the step four further on,
-  // `at` bytes behind the buffers' start.
-  const int cstep32 = static_cast<int>(cstep), rstep32 = static_cast<int>(rstep), sstep32 = static_cast<int>(sstep);
-  __amdgpu_buffer_rsrc_t crsrc, rrsrc, srsrc;
+
   // The part of a step's conversion that stands beside MFMA t of 64.
   auto conversion = [&](auto U, auto T) {
     constexpr int u = decltype(U)::value, t = decltype(T)::value;
@@ -349,47 +399,20 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
     else if constexpr (t == 16 || t == 32) convert16<F16>(code[t / 32], scale_byte[t / 32], value[t / 32]);
     else if constexpr (t == 24 || t == 40) write_values(slot, t / 40);
   };
-  auto step = [&](auto U, int s, u32x4(&cf)[8], u32x4(&rf)[8], u32x4(&cn)[8], u32x4(&rn)[8]) {
+  // Step s, in slot U = s % 4: its fragments are in (cf, rf), those of the next go to (cn, rn), and its slot is filled with the step four further on.
+  auto step = [&](auto U, auto FIRST, int s, u32x4(&cf)[8], u32x4(&rf)[8], u32x4(&cn)[8], u32x4(&rn)[8]) {
     constexpr int u = decltype(U)::value;
     wait_step(U, s);
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     static_for<64>([&](auto T) {
-      constexpr int t = decltype(T)::value;
+      constexpr int t = decltype(T)::value, q = t / 8;
       conversion(U, T);
       if constexpr (t < 2 * kReads && t % 2 == 0) read_one(integral_constant<int, (u + 1) % kSlots>{}, integral_constant<int, t / 2>{}, cn, rn);
-      constexpr int q = t / 8, r = q - kColFills;
-      if constexpr (t % 8 == 3 && q < kFills) {
-        set_target(U, integral_constant<int, q>{});
-      }
-      if constexpr (t % 8 == 4 && q < kFills) {
-        if constexpr (r >= 0) asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds" : : "v"(roff[r]), "s"(rrsrc), "s"(u * rstep32) : "memory");
-        else if constexpr (EIGHT && q == 2) asm volatile("buffer_load_ubyte %0, %1, %2 offen lds" : : "v"(coff[q]), "s"(srsrc), "s"(u * sstep32) : "memory");
-        else asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds" : : "v"(coff[q]), "s"(crsrc), "s"(u * cstep32) : "memory");
-      }
-      mfma<F16>(acc[t / 8][t % 8], cf[t % 8], rf[t / 8]);
-      __builtin_amdgcn_sched_barrier(0);
-    });
-    FLUXMI_LGKM0();
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  // The same near the end of the sum: s is the step's number.  What lies past the end is filled as well, with zeros, so that the waits count the same.
-  auto last_step = [&](auto U, int s, u32x4(&cf)[8], u32x4(&rf)[8], u32x4(&cn)[8], u32x4(&rn)[8]) {
-    constexpr int u = decltype(U)::value;
-    wait_step(U, s);
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    const uint8_t *const cat = cbase + (s + 4) * cstep, *const rat = rbase + (s + 4) * rstep, *const sat = EIGHT ? sbase + (s + 4) * sstep : nullptr;
-    const int valid = valid_of(s + 4);
-    static_for<8>([&](auto I) {
-      constexpr int i = decltype(I)::value;
-      conversion(U, integral_constant<int, i * 8>{});
-      static_for<kReads / 8>([&](auto R) {
-        read_one(integral_constant<int, (u + 1) % kSlots>{}, integral_constant<int, i * (kReads / 8) + decltype(R)::value>{}, cn, rn);
-      });
-      if constexpr (i < kFills) fill_guarded(U, I, cat, rat, sat, valid);
-      __builtin_amdgcn_sched_barrier(0);
-      static_for<8>([&](auto J) { mfma<F16>(acc[i][decltype(J)::value], cf[decltype(J)::value], rf[i]); });
+      if constexpr (t % 8 == 3 && q < kFills) set_target(U, integral_constant<int, q>{});
+      if constexpr (t % 8 == 4 && q < kFills) fill(integral_constant<int, q>{});
+      if constexpr (t == 62) next_buffers();
+      mfma<F16, decltype(FIRST)::value>(acc[t / 8][t % 8], cf[t % 8], rf[t / 8]);
       __builtin_amdgcn_sched_barrier(0);
     });
     FLUXMI_LGKM0();
@@ -408,45 +431,39 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
   begin_tile(tile);
   first_fills();
   for (;;) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     if constexpr (EIGHT) {
       if (behind == 0) FLUXMI_VMCNT(2 * kFills);
       else if (behind == 1) FLUXMI_VMCNT(2 * kFills + kStores);
+      if (rest < kStep && steps <= 2) clear_columns(steps - 1), FLUXMI_LGKM0();
       static_for<2>([&](auto S) {
         read_codes(S);
 #pragma unroll
         for (int i = 0; i < 2; ++i) convert16<F16>(code[i], scale_byte[i], value[i]), write_values(S, i);
       });
-      FLUXMI_LGKM0();
     } else {
       if (behind == 0) FLUXMI_VMCNT(3 * kFills);
       else if (behind == 1) FLUXMI_VMCNT(3 * kFills + kStores);
+      if (rest < kStep && steps == 1) clear_columns(0);
     }
+    if (rest < kStep && steps == 1) clear_rows(0);
+    FLUXMI_LGKM0();
     __builtin_amdgcn_s_barrier();
     static_for<kReads>([&](auto R) { read_one(integral_constant<int, 0>{}, R, ca, ra); });
     FLUXMI_LGKM0();
-    int s = 0;
-    for (; s + 8 <= whole; s += 4) {
-      crsrc = buffer_of(cbase + (s + 4) * cstep);
-      rrsrc = buffer_of(rbase + (s + 4) * rstep);
-      if constexpr (EIGHT) srsrc = buffer_of(sbase + (s + 4) * sstep);
-      step(integral_constant<int, 0>{}, s, ca, ra, cb, rb);
-      step(integral_constant<int, 1>{}, s + 1, cb, rb, ca, ra);
-      step(integral_constant<int, 2>{}, s + 2, ca, ra, cb, rb);
-      step(integral_constant<int, 3>{}, s + 3, cb, rb, ca, ra);
+    step(integral_constant<int, 0>{}, std::true_type{}, 0, ca, ra, cb, rb);
+    int s = 1;
+    for (; s + 4 <= steps; s += 4) {
+      step(integral_constant<int, 1>{}, std::false_type{}, s, cb, rb, ca, ra);
+      step(integral_constant<int, 2>{}, std::false_type{}, s + 1, ca, ra, cb, rb);
+      step(integral_constant<int, 3>{}, std::false_type{}, s + 2, cb, rb, ca, ra);
+      step(integral_constant<int, 0>{}, std::false_type{}, s + 3, ca, ra, cb, rb);
     }
-    while (s < steps) {
-      last_step(integral_constant<int, 0>{}, s, ca, ra, cb, rb);
-      if (++s >= steps) break;
-      last_step(integral_constant<int, 1>{}, s, cb, rb, ca, ra);
-      if (++s >= steps) break;
-      last_step(integral_constant<int, 2>{}, s, ca, ra, cb, rb);
-      if (++s >= steps) break;
-      last_step(integral_constant<int, 3>{}, s, cb, rb, ca, ra);
-      ++s;
+    if (s < steps) {
+      step(integral_constant<int, 1>{}, std::false_type{}, s, cb, rb, ca, ra);
+      if (s + 1 < steps) {
+        step(integral_constant<int, 2>{}, std::false_type{}, s + 1, ca, ra, cb, rb);
+        if (s + 2 < steps) step(integral_constant<int, 3>{}, std::false_type{}, s + 2, cb, rb, ca, ra);
+      }
     }
     const Tile next = next_tile();
     __builtin_amdgcn_s_barrier();  // nobody reads the slots any more
@@ -456,49 +473,61 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
     }
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // the last sums are in their registers
 
-    // ---- lane l has columns 4 (l / 16) .. + 3 of row l % 16 of a block --------------------------------------------
-    const int out_lane = fresh_lane(), g = out_lane >> 4;
-    if (a.accumulate) {
-      static_for<8>([&](auto I) {
-        const int r = wr * 128 + decltype(I)::value * 16 + (out_lane & 15);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int c = wc * 128 + j * 16 + g * 4;
-          if (r < tile.rows && c < tile.cols) store4_whole<F16>(a, (tile.out_row0 + r) * a.k + tile.col0 + c, sums_of(acc[decltype(I)::value][j]));
-        }
-      });
-      FLUXMI_VMCNT(0);
-      behind = 0;
-    } else {
-      // The buffer ends with the tile's rows; columns past its end are sent past the buffer's.  Every store is issued, so that they can be counted.
+    // ---- results: lane l has columns 4 (l / 16) .. + 3 of row l % 16 of a block.  Sixteen rows of 128 bytes at a time change lanes in the wave's window (chunk c of 16
+    // bytes of row r at place c ^ (r / 2 % 8), off the other lanes' banks either way), so that eight neighbouring lanes store a whole line: stored from where
+    // they are, neighbouring lanes' pieces lie in different rows, and a compute unit brings out a quarter as much. ----
+    {
+      const int l = fresh_lane(), r = l & 15, g = l >> 4;
+      const uint32_t window = lds0 + windows_at(G) + wave * kWindow;
+      const uint32_t from = window + (l >> 3) * 128 + ((l & 7) ^ ((l >> 4) & 7)) * 16;  // rows l / 8 and l / 8 + 8: the latter's place is another, 64 bytes from it
       const int out_size = a.out_f32 ? 4 : 2;
+      // The buffer ends with the tile's rows; columns past its end are sent past the buffer's.  Every store is issued, so that they can be counted.
       const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(a.out + tile.out_row0 * a.k * out_size, 0,
                                                                            static_cast<int>(static_cast<uint32_t>(tile.rows) * a.k * out_size), 0x00020000);
-      const uint32_t row_at = static_cast<uint32_t>(wr * 128 + (out_lane & 15)) * a.k + tile.col0;
-      if (a.out_f32) {
-        static_for<8>([&](auto I) {
-          constexpr int i = decltype(I)::value;
+      const uint32_t row_at = static_cast<uint32_t>(wr * 128 + (l >> 3)) * a.k + tile.col0;
+      if (a.out_f32 || a.accumulate) {
+        static_for<32>([&](auto N) {
+          constexpr int i = decltype(N)::value / 4, j = decltype(N)::value % 4 * 2;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int c = wc * 128 + j * 16 + g * 4;
-            const uint32_t at = c < tile.cols ? (row_at + i * 16 * a.k + c) * 4 : 0xfffffff0u;
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sums_of(acc[i][j])), out, at, 0, 0);
+          for (int h = 0; h < 2; ++h)
+            *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(window + r * 128 + ((h * 4 + g) ^ (r >> 1)) * 16) = __builtin_bit_cast(u32x4, sums_of(acc[i][j + h]));
+          const int c = wc * 128 + j * 16 + (l & 7) * 4;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            f32x4 v = __builtin_bit_cast(f32x4, *(LdsFrag)(uintptr_t)((from ^ (h * 64)) + h * 1024));
+            const uint32_t at = c < tile.cols ? (row_at + (i * 16 + h * 8) * a.k + c) * out_size : 0xfffffff0u;
+            if (!a.accumulate) {
+              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), out, at, 0, 0);
+            } else if (a.out_f32) {
+              v += __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(out, at, 0, 0));
+              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), out, at, 0, 0);
+            } else {
+              const u32x2 old = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(out, at, 0, 0));
+#pragma unroll
+              for (int q = 0; q < 4; ++q) v[q] += unpack1<F16>(static_cast<uint16_t>(old[q / 2] >> (16 * (q & 1))));
+              __builtin_amdgcn_raw_buffer_store_b64(u32x2{pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3])}, out, at, 0, 0);
+            }
           }
         });
         behind = 2;
+        if (a.accumulate) {
+          FLUXMI_VMCNT(0);
+          behind = 0;
+        }
       } else {
-        // Two blocks' sums change lanes, so that each has eight neighbouring columns: of the first block in lane groups 0 and 2, of the second in 1 and 3.
-        static_for<8>([&](auto I) {
-          constexpr int i = decltype(I)::value;
+        static_for<16>([&](auto N) {
+          constexpr int i = decltype(N)::value / 2, j = decltype(N)::value % 2 * 4;
 #pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            const f32x4 x = sums_of(acc[i][j]), y = sums_of(acc[i][j + 1]);
-            const uint32_t x0 = pack2<F16>(x[0], x[1]), x1 = pack2<F16>(x[2], x[3]), y0 = pack2<F16>(y[0], y[1]), y1 = pack2<F16>(y[2], y[3]);
-            const auto p = __builtin_amdgcn_permlane16_swap(x0, y0, false, false);
-            const auto q = __builtin_amdgcn_permlane16_swap(x1, y1, false, false);
-            const int c = wc * 128 + (j + (g & 1)) * 16 + (g >> 1) * 8;
-            const uint32_t at = c < tile.cols ? (row_at + i * 16 * a.k + c) * 2 : 0xfffffff0u;
-            __builtin_amdgcn_raw_buffer_store_b128(u32x4{p[0], q[0], p[1], q[1]}, out, at, 0, 0);
+          for (int h = 0; h < 4; ++h) {
+            const f32x4 x = sums_of(acc[i][j + h]);
+            *(__attribute__((address_space(3))) u32x2 *)(uintptr_t)(window + r * 128 + ((h * 2 + (g >> 1)) ^ (r >> 1)) * 16 + (g & 1) * 8) =
+                u32x2{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3])};
+          }
+          const int c = wc * 128 + j * 16 + (l & 7) * 8;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const u32x4 v = *(LdsFrag)(uintptr_t)((from ^ (h * 64)) + h * 1024);
+            __builtin_amdgcn_raw_buffer_store_b128(v, out, c < tile.cols ? (row_at + (i * 16 + h * 8) * a.k + c) * 2 : 0xfffffff0u, 0, 0);
           }
         });
         behind = 1;
@@ -526,14 +555,14 @@ int launch_grad_tiles(Grad g, bool f16, const GradArgs &a, void *stream) {
   const int64_t tiles_k = (a.k + kTile - 1) / kTile, tiles_n = (a.n + kTile - 1) / kTile;
   const int64_t items = g == Grad::INPUT ? (a.rows / kTile + (a.rows < a.nexperts ? a.rows : a.nexperts) + 1) * tiles_k : a.nexperts * tiles_n * tiles_k;
   FLUXMI_REQUIRE(items < (1 << 24), FLUXMI_ERR_UNSUPPORTED, "gradients of the grouped product: too many rows and columns for one launch");
-  // A workgroup's tiles follow each other without a gap; several workgroups to a compute unit even out experts of different sizes.
-  int64_t turns = items / (3 * 256);
-  if (turns < 1) turns = 1;
-  TileArgs t{a, static_cast<int32_t>(items), static_cast<int32_t>(turns)};
-  const uint32_t grid = static_cast<uint32_t>(((items + turns - 1) / turns + 7) / 8 * 8);
+  // One workgroup to a compute unit: its tiles follow each other without a gap.
+  const int cus = fluxmi_device_cu_count();
+  FLUXMI_REQUIRE(cus > 0, FLUXMI_ERR_HIP, "gradients of the grouped product: no device");
+  const int64_t grid = items < cus ? (items + 7) / 8 * 8 : cus;
+  TileArgs t{a, static_cast<int32_t>(items), static_cast<int32_t>((items + grid - 1) / grid)};
   auto launch = [&](auto kernel, std::atomic<uint64_t> &done) -> int {
     if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds_bytes(g), done)) return rc;
-    kernel<<<grid, kThreads, lds_bytes(g), static_cast<hipStream_t>(stream)>>>(t);
+    kernel<<<static_cast<uint32_t>(grid), kThreads, lds_bytes(g), static_cast<hipStream_t>(stream)>>>(t);
     FLUXMI_HIP_CHECK(hipGetLastError());
     return FLUXMI_OK;
   };
