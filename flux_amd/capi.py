@@ -34,7 +34,7 @@ EXPORTS = (
     "fluxmi_grouped_gemm_topk_reduce", "fluxmi_grouped_gemm_blockscale",
     "fluxmi_topk_gather_reduce", "fluxmi_moe_permute", "fluxmi_moe_unpermute", "fluxmi_moe_unpermute_backward", "fluxmi_quant_e4m3_rowwise", "fluxmi_quant_e4m3_square",
     "fluxmi_quant_e4m3_block128", "fluxmi_quant_e4m3_block128_filled", "fluxmi_calib_stream_sink_bytes", "fluxmi_calib_stream",
-    "fluxmi_moe_dgrad", "fluxmi_moe_wgrad_workspace_bytes", "fluxmi_moe_wgrad", "fluxmi_moe_clear_rest", "fluxmi_checkpoint_e4m3", "fluxmi_swiglu",
+    "fluxmi_moe_dgrad", "fluxmi_moe_dgrad_workspace_bytes", "fluxmi_moe_wgrad_workspace_bytes", "fluxmi_moe_wgrad", "fluxmi_moe_clear_rest", "fluxmi_checkpoint_e4m3", "fluxmi_swiglu",
     "fluxmi_swiglu_backward", "fluxmi_quant_mx", "fluxmi_dequant_mx", "fluxmi_grouped_gemm_mx_workspace_bytes", "fluxmi_grouped_gemm_mx",
     "fluxmi_grouped_gemm_mx_launch_info",
 )
@@ -113,7 +113,9 @@ def load():
     lib.fluxmi_moe_permute.argtypes = [vp, vp, i32, i32, i64, vp, vp]
     lib.fluxmi_moe_unpermute.argtypes = [vp, i32, vp, vp, i32, i32, i32, i32, vp, vp]
     lib.fluxmi_moe_unpermute_backward.argtypes = [vp, vp, i32, vp, vp, i32, i32, i32, i32, vp, vp, vp]
-    lib.fluxmi_moe_dgrad.argtypes = [vp, vp, i32, vp, i32, i64, i64, i64, vp, vp]
+    lib.fluxmi_moe_dgrad.argtypes = [vp, vp, i32, vp, i32, i64, i64, i64, vp, vp, sz, vp]
+    lib.fluxmi_moe_dgrad_workspace_bytes.restype = sz
+    lib.fluxmi_moe_dgrad_workspace_bytes.argtypes = [i32, i64, i64, i64]
     lib.fluxmi_moe_wgrad_workspace_bytes.restype = sz
     lib.fluxmi_moe_wgrad_workspace_bytes.argtypes = [i32, i64, i64, i64]
     lib.fluxmi_moe_wgrad.argtypes = [vp, vp, vp, i32, vp, i32, i64, i64, i64, vp, i32, i32, vp, sz, vp]
@@ -490,8 +492,10 @@ def moe_dgrad(grad, weight, splits):
     if weight.dim() != 3 or weight.shape[:2] != (splits.numel(), grad.shape[1]):
         raise ValueError(f"weight {tuple(weight.shape)} is not [{splits.numel()}, {grad.shape[1]}, K]")
     out = torch.empty(grad.shape[0], weight.shape[2], dtype=grad.dtype, device=grad.device)
+    ws_bytes = lib.fluxmi_moe_dgrad_workspace_bytes(splits.numel(), grad.shape[0], grad.shape[1], weight.shape[2])
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=grad.device) if ws_bytes else None
     _check(lib.fluxmi_moe_dgrad(_ptr(grad), _ptr(weight), _ROW_TYPES[grad.dtype], _ptr(splits), splits.numel(), grad.shape[0], grad.shape[1], weight.shape[2],
-                                _ptr(out), _stream()), "fluxmi_moe_dgrad")
+                                _ptr(out), _ptr(ws), ws_bytes, _stream()), "fluxmi_moe_dgrad")
     return out
 
 

@@ -270,8 +270,13 @@ void launch_pieces(const GradArgs &a, bool f16, bool vec, uint32_t grid, hipStre
 
 using namespace fluxmi;
 
+extern "C" size_t fluxmi_moe_dgrad_workspace_bytes(int32_t nexperts, int64_t rows, int64_t n, int64_t k) {
+  if (check_product("moe_dgrad", FLUXMI_ROWS_BF16, nexperts, rows, n, k) != FLUXMI_OK) return 0;
+  return grad_tiles_workspace_bytes(Grad::INPUT, nexperts, rows, n, k);
+}
+
 extern "C" int fluxmi_moe_dgrad(const void *grad, const void *weight, int32_t row_type, const int32_t *splits, int32_t nexperts, int64_t rows, int64_t n,
-                                int64_t k, void *grad_input, void *stream) {
+                                int64_t k, void *grad_input, void *workspace, size_t workspace_bytes, void *stream) {
   if (const int rc = check_product("moe_dgrad", row_type, nexperts, rows, n, k)) return rc;
   if (rows == 0 || k == 0) return FLUXMI_OK;
   FLUXMI_REQUIRE(grad_input && (n == 0 || grad) && (n == 0 || nexperts == 0 || weight) && (nexperts == 0 || splits), FLUXMI_ERR_INVALID_ARG,
@@ -288,6 +293,10 @@ extern "C" int fluxmi_moe_dgrad(const void *grad, const void *weight, int32_t ro
   a.n = static_cast<int32_t>(n);
   a.k = static_cast<int32_t>(k);
   a.parts = 1;
+  a.partial = static_cast<float *>(workspace);
+  const size_t need = fluxmi_moe_dgrad_workspace_bytes(nexperts, rows, n, k);
+  FLUXMI_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && on(workspace, 16)), FLUXMI_ERR_WORKSPACE,
+                 "moe_dgrad: workspace of %zu bytes, 16-byte aligned, expected, got %zu", need, workspace_bytes);
   if (grad_tiles_take(Grad::INPUT, a) && grad_tiles_are_faster(Grad::INPUT, a)) return launch_grad_tiles(Grad::INPUT, row_type == FLUXMI_ROWS_FP16, a, stream);
   // Every expert and the rows of none end with a tile that may be partial.
   const int64_t row_tiles = rows / kPiece + (rows < nexperts ? rows : nexperts) + 1, items = row_tiles * tiles_of(k);
@@ -301,7 +310,9 @@ extern "C" int fluxmi_moe_dgrad(const void *grad, const void *weight, int32_t ro
 extern "C" size_t fluxmi_moe_wgrad_workspace_bytes(int32_t nexperts, int64_t rows, int64_t n, int64_t k) {
   if (check_product("moe_wgrad", FLUXMI_ROWS_BF16, nexperts, rows, n, k) != FLUXMI_OK) return 0;
   const int parts = parts_of(nexperts, rows, n, k);
-  return parts > 1 ? static_cast<size_t>(nexperts * tiles_of(n) * tiles_of(k)) * parts * kPiece * kPiece * sizeof(float) : 0;
+  const size_t pieces = parts > 1 ? static_cast<size_t>(nexperts * tiles_of(n) * tiles_of(k)) * parts * kPiece * kPiece * sizeof(float) : 0;
+  const size_t tiles = grad_tiles_workspace_bytes(Grad::WEIGHT, nexperts, rows, n, k);
+  return pieces > tiles ? pieces : tiles;  // (which of them computes a call also depends on alignment)
 }
 
 extern "C" int fluxmi_moe_wgrad(const void *grad, const void *input, const void *input_scale, int32_t row_type, const int32_t *splits, int32_t nexperts,

@@ -33,11 +33,41 @@ constexpr int windows_at(Grad g) { return g == Grad::WEIGHT_8BIT ? scales_at() +
 constexpr int tables_at(Grad g) { return windows_at(g) + kThreads / 64 * kWindow; }
 constexpr int lds_bytes(Grad g) { return tables_at(g) + (g == Grad::INPUT ? 2 : 1) * 4 * kMaxExperts + 16; }
 
-struct TileArgs {
-  GradArgs a;
-  int32_t items;  // tiles of the result (INPUT: as many as there can be)
-  int32_t turns;  // tiles that a workgroup computes
+// Division of numbers below 2^24 by one that the host knows.
+struct Divisor {
+  uint32_t by, factor, shift;
 };
+Divisor divisor(int64_t by) {
+  Divisor d{static_cast<uint32_t>(by), 0, 24};
+  while ((int64_t{1} << (d.shift - 24)) < by) ++d.shift;
+  d.factor = static_cast<uint32_t>(((uint64_t{1} << d.shift) + by - 1) / by);
+  return d;
+}
+__device__ __forceinline__ int divide(int x, Divisor d) { return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(x)) * d.factor) >> d.shift); }
+
+struct TileArgs {
+  GradArgs a;             // a.parts: parts that a tile's sum may be cut into
+  int32_t grid;           // workgroups, a multiple of 8
+  int32_t turns;          // tiles that a workgroup computes at most
+  Divisor per_expert, per_group;  // an expert's tiles; those of eight along the result's rows
+};
+
+constexpr int kLeastSteps = 8;   // of a part
+constexpr int kMostParts = 16;
+
+// Every workgroup computes one tile in a turn.  Where the last turn's tiles are at most half as many as workgroups, their sums are cut into parts, which a second
+// kernel joins: tiles [0, whole), then `parts` of each of `cut` tiles.
+struct Turns {
+  int whole, cut, parts;
+};
+__host__ __device__ inline Turns turns_of(int tiles, int grid, int most_parts) {
+  const int whole = tiles / grid * grid, cut = tiles - whole;
+  if (cut == 0) return {whole, 0, 1};
+  int parts = grid / cut;
+  if (parts > most_parts) parts = most_parts;
+  if (parts < 2) return {tiles, 0, 1};
+  return {whole, cut, parts};
+}
 
 #if defined(__HIP_DEVICE_COMPILE__)
 
@@ -85,26 +115,28 @@ __device__ __forceinline__ void load_to_lds(uint32_t off, __amdgpu_buffer_rsrc_t
   if constexpr (BYTE) asm volatile("buffer_load_ubyte %0, %1, 0 offen lds" : : "v"(off), "s"(rsrc) : "memory");
   else asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(off), "s"(rsrc) : "memory");
 }
-// Sixteen codes of one block to values of 16 bits.
-template <bool F16>
-__device__ __forceinline__ void convert16(const u32x4 codes, uint32_t byte, u32x4 (&v)[2]) {
-  const float scale = __uint_as_float(byte == 0 ? 0x00400000u : (byte == 255 ? 0x7fc00000u : byte << 23));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (F16) {
-      v[i >> 1][(i & 1) * 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[i], scale, false));
-      v[i >> 1][(i & 1) * 2 + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[i], scale, true));
-    } else {
-      v[i >> 1][(i & 1) * 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i], scale, false));
-      v[i >> 1][(i & 1) * 2 + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i], scale, true));
-    }
-  }
-}
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte == 0 ? 0x00400000u : (byte == 255 ? 0x7fc00000u : byte << 23)); }
 
+// Two of sixteen codes of one block to values of 16 bits.
+template <bool F16>
+__device__ __forceinline__ void convert_pair(const u32x4 codes, float scale, u32x4 (&v)[2], int pair) {
+  const int w = pair >> 1;
+  uint32_t x;
+  if constexpr (F16) {
+    x = pair & 1 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[w], scale, true))
+                 : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[w], scale, false));
+  } else {
+    x = pair & 1 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[w], scale, true))
+                 : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[w], scale, false));
+  }
+  v[pair >> 2][pair & 3] = x;
+}
 
 // A tile of the result and where its operands begin.
 struct Tile {
   int e, row0, rows, col0, cols;  // row0: column of grad for weights, otherwise 0; rows = 0: there is no such tile
+  int part, slot;  // part < 0: the whole sum; otherwise its sums go to place `slot` of the parts'
+  int begin;    // INPUT: first of the columns of G that it sums over
   int sum_over;
   int first;  // of the rows that it sums over (INPUT: reads)
   int64_t out_row0;
@@ -148,19 +180,25 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
   __syncthreads();
   const int expert_tiles = row_tiles;
   if constexpr (INPUT) row_tiles += (a.rows - all_rows + kTile - 1) / kTile;  // the rows that belong to no expert
-  const int items = INPUT ? row_tiles * tiles_k : args.items;
+  const Turns turns = turns_of((INPUT ? row_tiles : a.nexperts * tiles_n) * tiles_k, args.grid, a.parts);
 
-  // Tile number `turn` of this workgroup.  Workgroups are dealt to the eight XCDs in turn; 32 in a row on one XCD take neighbouring tiles: an expert's (INPUT: all) tiles in
+  // This workgroup's tile of a turn.  Workgroups are dealt to the eight XCDs in turn; those on one XCD take neighbouring tiles: an expert's (INPUT: all) tiles in
   // groups of eight along the result's rows, walked column by column.
   auto describe = [&](int turn) {
     Tile t{};
-    int item = blockIdx.x + turn * static_cast<int>(gridDim.x);
-    if (item < args.items / 256 * 256) item = (item & ~255) + (item & 7) * 32 + ((item & 255) >> 3);
-    if (item >= items) return t;
-    const int per = tiles_n * tiles_k, e = INPUT ? 0 : item / per, local = INPUT ? item : item - e * per;
-    const int group = local / (8 * tiles_k), in_group = local - group * 8 * tiles_k;
+    int item = turn * args.grid + (blockIdx.x & 7) * (args.grid >> 3) + (blockIdx.x >> 3);
+    t.part = -1;
+    if (item >= turns.whole) {
+      item -= turns.whole;
+      if (item >= turns.cut * turns.parts) return t;
+      t.part = item / turns.cut;
+      t.slot = item;
+      item += turns.whole - t.part * turns.cut;
+    }
+    const int e = INPUT ? 0 : divide(item, args.per_expert), local = INPUT ? item : item - e * static_cast<int>(args.per_expert.by);
+    const int group = divide(local, args.per_group), in_group = local - group * static_cast<int>(args.per_group.by);
     const int high = (INPUT ? row_tiles : tiles_n) - group * 8, height = high < 8 ? high : 8;
-    const int kt = in_group / height, rt = group * 8 + in_group - kt * height;
+    const int kt = height == 8 ? in_group >> 3 : in_group / height, rt = group * 8 + in_group - kt * height;
     t.col0 = kt * kTile;
     t.cols = a.k - t.col0 < kTile ? a.k - t.col0 : kTile;
     if constexpr (INPUT) {
@@ -190,6 +228,12 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
       t.first = e > 0 ? __builtin_amdgcn_readfirstlane(row_ends[e - 1]) : 0;
       t.sum_over = __builtin_amdgcn_readfirstlane(row_ends[e]) - t.first;
     }
+    if (t.part >= 0) {
+      const int all = (t.sum_over + kStep - 1) / kStep, from = all * t.part / turns.parts * kStep, to = all * (t.part + 1) / turns.parts * kStep;
+      t.sum_over = (to < t.sum_over ? to : t.sum_over) - from;
+      if constexpr (INPUT) t.begin = from;
+      else t.first += from;
+    }
     return t;
   };
 
@@ -210,9 +254,10 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
     const int64_t first = __builtin_amdgcn_readfirstlane(t.first);
     rnext = a.grad + first * rpitch;
     if constexpr (INPUT) {
-      const int e = __builtin_amdgcn_readfirstlane(t.e);
-      cnext = a.other + static_cast<int64_t>(e < a.nexperts ? e : 0) * a.n * cpitch;
-      rbytes = __builtin_amdgcn_readfirstlane(t.rows) * static_cast<int>(rpitch);
+      const int e = __builtin_amdgcn_readfirstlane(t.e), begin = __builtin_amdgcn_readfirstlane(t.begin);
+      cnext = a.other + (static_cast<int64_t>(e < a.nexperts ? e : 0) * a.n + begin) * cpitch;
+      rnext += begin * 2;
+      rbytes = __builtin_amdgcn_readfirstlane(t.rows) * static_cast<int>(rpitch) - begin * 2;
     } else {
       cnext = a.other + first * cpitch;
     }
@@ -311,18 +356,15 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
       value_at[i] = lds0 + t * 512 + ((lane & 15) ^ f) * 32;
     }
   }
-  auto read_codes = [&](auto SLOT) {
+  float scale_bits[2];
+  auto read_codes = [&](auto SLOT, int i) {
     constexpr int slot = decltype(SLOT)::value;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      code[i] = *(LdsFrag)(uintptr_t)(codes + lane * 16 + slot * kCodeSlot + i * 1024);
-      scale_byte[i] = *(const __attribute__((address_space(3))) uint32_t *)(uintptr_t)(scale_at + slot * kScaleSlot + i * 128);
-    }
+    code[i] = *(LdsFrag)(uintptr_t)(codes + lane * 16 + slot * kCodeSlot + i * 1024);
+    scale_byte[i] = *(const __attribute__((address_space(3))) uint32_t *)(uintptr_t)(scale_at + slot * kScaleSlot + i * 128);
   };
-  auto write_values = [&](auto SLOT, int i) {
+  auto write_values = [&](auto SLOT, int i, int h) {
     constexpr int slot = decltype(SLOT)::value;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(value_at[i] + (slot % 2) * kSlot + h * 16) = value[i][h];
+    *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(value_at[i] + (slot % 2) * kSlot + h * 16) = value[i][h];
   };
 
   auto fill = [&](auto Q) {
@@ -395,9 +437,12 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
     constexpr int u = decltype(U)::value, t = decltype(T)::value;
     constexpr integral_constant<int, (u + 2) % kSlots> slot{};
     if constexpr (!EIGHT) return;
-    else if constexpr (t == 0) read_codes(slot);
-    else if constexpr (t == 16 || t == 32) convert16<F16>(code[t / 32], scale_byte[t / 32], value[t / 32]);
-    else if constexpr (t == 24 || t == 40) write_values(slot, t / 40);
+    else if constexpr (t == 1 || t == 3) read_codes(slot, t / 2);
+    else if constexpr (t == 15 || t == 37) scale_bits[t / 37] = scale_of(scale_byte[t / 37]);
+    else if constexpr (t >= 17 && t < 33 && t % 2 == 1) convert_pair<F16>(code[0], scale_bits[0], value[0], (t - 17) / 2);
+    else if constexpr (t >= 39 && t < 55 && t % 2 == 1) convert_pair<F16>(code[1], scale_bits[1], value[1], (t - 39) / 2);
+    else if constexpr (t == 33 || t == 35) write_values(slot, 0, (t - 33) / 2);
+    else if constexpr (t == 55 || t == 57) write_values(slot, 1, (t - 55) / 2);
   };
   // Step s, in slot U = s % 4: its fragments are in (cf, rf), those of the next go to (cn, rn), and its slot is filled with the step four further on.
   auto step = [&](auto U, auto FIRST, int s, u32x4(&cf)[8], u32x4(&rf)[8], u32x4(&cn)[8], u32x4(&rn)[8]) {
@@ -436,9 +481,14 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
       else if (behind == 1) FLUXMI_VMCNT(2 * kFills + kStores);
       if (rest < kStep && steps <= 2) clear_columns(steps - 1), FLUXMI_LGKM0();
       static_for<2>([&](auto S) {
-        read_codes(S);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) convert16<F16>(code[i], scale_byte[i], value[i]), write_values(S, i);
+        for (int i = 0; i < 2; ++i) {
+          read_codes(S, i);
+          const float scale = scale_of(scale_byte[i]);
+#pragma unroll
+          for (int pair = 0; pair < 8; ++pair) convert_pair<F16>(code[i], scale, value[i], pair);
+          write_values(S, i, 0), write_values(S, i, 1);
+        }
       });
     } else {
       if (behind == 0) FLUXMI_VMCNT(3 * kFills);
@@ -480,58 +530,85 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
       const int l = fresh_lane(), r = l & 15, g = l >> 4;
       const uint32_t window = lds0 + windows_at(G) + wave * kWindow;
       const uint32_t from = window + (l >> 3) * 128 + ((l & 7) ^ ((l >> 4) & 7)) * 16;  // rows l / 8 and l / 8 + 8: the latter's place is another, 64 bytes from it
-      const int out_size = a.out_f32 ? 4 : 2;
       // The buffer ends with the tile's rows; columns past its end are sent past the buffer's.  Every store is issued, so that they can be counted.
-      const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(a.out + tile.out_row0 * a.k * out_size, 0,
-                                                                           static_cast<int>(static_cast<uint32_t>(tile.rows) * a.k * out_size), 0x00020000);
-      const uint32_t row_at = static_cast<uint32_t>(wr * 128 + (l >> 3)) * a.k + tile.col0;
-      if (a.out_f32 || a.accumulate) {
-        static_for<32>([&](auto N) {
-          constexpr int i = decltype(N)::value / 4, j = decltype(N)::value % 4 * 2;
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(window + r * 128 + ((h * 4 + g) ^ (r >> 1)) * 16) = __builtin_bit_cast(u32x4, sums_of(acc[i][j + h]));
-          const int c = wc * 128 + j * 16 + (l & 7) * 4;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            f32x4 v = __builtin_bit_cast(f32x4, *(LdsFrag)(uintptr_t)((from ^ (h * 64)) + h * 1024));
-            const uint32_t at = c < tile.cols ? (row_at + (i * 16 + h * 8) * a.k + c) * out_size : 0xfffffff0u;
-            if (!a.accumulate) {
-              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), out, at, 0, 0);
-            } else if (a.out_f32) {
-              v += __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(out, at, 0, 0));
-              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), out, at, 0, 0);
-            } else {
-              const u32x2 old = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(out, at, 0, 0));
-#pragma unroll
-              for (int q = 0; q < 4; ++q) v[q] += unpack1<F16>(static_cast<uint16_t>(old[q / 2] >> (16 * (q & 1))));
-              __builtin_amdgcn_raw_buffer_store_b64(u32x2{pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3])}, out, at, 0, 0);
+      const bool part = tile.part >= 0, f32 = part || a.out_f32, add = !part && a.accumulate;
+      const int out_size = f32 ? 4 : 2;
+      const uint32_t pitch = part ? kTile : a.k;
+      uint8_t *const base = part ? reinterpret_cast<uint8_t *>(a.partial + static_cast<int64_t>(tile.slot) * kTile * kTile) : a.out + tile.out_row0 * a.k * out_size;
+      const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(base, 0, static_cast<int>(static_cast<uint32_t>(tile.rows) * pitch * out_size), 0x00020000);
+      const uint32_t row_at = static_cast<uint32_t>(wr * 128 + (l >> 3)) * pitch + (part ? 0 : tile.col0);
+      // Results of group N are read before those of the one before it are stored.
+      u32x4 v[2][2];
+      auto read_back = [&](auto N) {
+        constexpr int b = decltype(N)::value & 1;
+        v[b][0] = *(LdsFrag)(uintptr_t)from;
+        v[b][1] = *(LdsFrag)(uintptr_t)((from ^ 64) + 1024);
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      auto store_results = [&](auto LINES) {
+        constexpr int policy = decltype(LINES)::value ? 2 : 0;  // non-temporal
+        if (f32 || add) {
+          auto put = [&](auto N) {
+            constexpr int i = decltype(N)::value / 4, j = decltype(N)::value % 4 * 2;
+  #pragma unroll
+            for (int h = 0; h < 2; ++h)
+              *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(window + r * 128 + ((h * 4 + g) ^ (r >> 1)) * 16) = __builtin_bit_cast(u32x4, sums_of(acc[i][j + h]));
+            read_back(N);
+          };
+          put(integral_constant<int, 0>{});
+          static_for<32>([&](auto N) {
+            constexpr int n = decltype(N)::value, i = n / 4, j = n % 4 * 2;
+            if constexpr (n < 31) put(integral_constant<int, (n < 31 ? n + 1 : 0)>{});
+            const int c = wc * 128 + j * 16 + (l & 7) * 4;
+  #pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t at = c < tile.cols ? (row_at + (i * 16 + h * 8) * pitch + c) * out_size : 0xfffffff0u;
+              f32x4 x = __builtin_bit_cast(f32x4, v[n & 1][h]);
+              if (!add) {
+                __builtin_amdgcn_raw_buffer_store_b128(v[n & 1][h], out, at, 0, policy);
+              } else if (f32) {
+                x += __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(out, at, 0, 0));
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), out, at, 0, 0);
+              } else {
+                const u32x2 old = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(out, at, 0, 0));
+  #pragma unroll
+                for (int q = 0; q < 4; ++q) x[q] += unpack1<F16>(static_cast<uint16_t>(old[q / 2] >> (16 * (q & 1))));
+                __builtin_amdgcn_raw_buffer_store_b64(u32x2{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3])}, out, at, 0, 0);
+              }
             }
+            __builtin_amdgcn_sched_barrier(0);
+          });
+          behind = 2;
+          if (add) {
+            FLUXMI_VMCNT(0);
+            behind = 0;
           }
-        });
-        behind = 2;
-        if (a.accumulate) {
-          FLUXMI_VMCNT(0);
-          behind = 0;
+        } else {
+          auto put = [&](auto N) {
+            constexpr int i = decltype(N)::value / 2, j = decltype(N)::value % 2 * 4;
+  #pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              const f32x4 x = sums_of(acc[i][j + h]);
+              *(__attribute__((address_space(3))) u32x2 *)(uintptr_t)(window + r * 128 + ((h * 2 + (g >> 1)) ^ (r >> 1)) * 16 + (g & 1) * 8) =
+                  u32x2{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3])};
+            }
+            read_back(N);
+          };
+          put(integral_constant<int, 0>{});
+          static_for<16>([&](auto N) {
+            constexpr int n = decltype(N)::value, i = n / 2, j = n % 2 * 4;
+            if constexpr (n < 15) put(integral_constant<int, (n < 15 ? n + 1 : 0)>{});
+            const int c = wc * 128 + j * 16 + (l & 7) * 8;
+  #pragma unroll
+            for (int h = 0; h < 2; ++h) __builtin_amdgcn_raw_buffer_store_b128(v[n & 1][h], out, c < tile.cols ? (row_at + (i * 16 + h * 8) * pitch + c) * 2 : 0xfffffff0u, 0, policy);
+            __builtin_amdgcn_sched_barrier(0);
+          });
+          behind = 1;
         }
-      } else {
-        static_for<16>([&](auto N) {
-          constexpr int i = decltype(N)::value / 2, j = decltype(N)::value % 2 * 4;
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            const f32x4 x = sums_of(acc[i][j + h]);
-            *(__attribute__((address_space(3))) u32x2 *)(uintptr_t)(window + r * 128 + ((h * 2 + (g >> 1)) ^ (r >> 1)) * 16 + (g & 1) * 8) =
-                u32x2{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3])};
-          }
-          const int c = wc * 128 + j * 16 + (l & 7) * 8;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const u32x4 v = *(LdsFrag)(uintptr_t)((from ^ (h * 64)) + h * 1024);
-            __builtin_amdgcn_raw_buffer_store_b128(v, out, c < tile.cols ? (row_at + (i * 16 + h * 8) * a.k + c) * 2 : 0xfffffff0u, 0, 0);
-          }
-        });
-        behind = 1;
-      }
+      };
+      // Whole lines pass the caches by; parts of lines would come from memory again.
+      if (!part && (a.k * out_size & 127) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 127) == 0) store_results(std::true_type{});
+      else store_results(std::false_type{});
     }
     if (next.rows == 0) break;
     tile = next;
@@ -540,36 +617,119 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
 #endif
 }
 
+// The parts of the last turn's tiles, added in their order: a workgroup has sixteen rows of a tile.
+template <bool F16, Grad G>
+__global__ __launch_bounds__(kThreads) void grad_tile_join_kernel(const TileArgs args) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr bool INPUT = G == Grad::INPUT;
+  const GradArgs &a = args.a;
+  const int tiles_k = (a.k + kTile - 1) / kTile, tiles_n = (a.n + kTile - 1) / kTile;
+  int row_tiles = a.nexperts * tiles_n, all_rows = 0;
+  if constexpr (INPUT) {
+    row_tiles = 0;
+    for (int e0 = 0; e0 < a.nexperts; e0 += 64) {
+      const ExpertRows x = rows_of_lane(a, e0, all_rows);
+      row_tiles += __builtin_amdgcn_readlane(wave_inclusive_scan((x.end - x.begin + kTile - 1) / kTile), 63);
+    }
+    row_tiles += (a.rows - all_rows + kTile - 1) / kTile;
+  }
+  const Turns turns = turns_of(row_tiles * tiles_k, args.grid, a.parts);
+  const int cut = blockIdx.x >> 4;
+  if (cut >= turns.cut) return;
+  const int item = turns.whole + cut, e = INPUT ? 0 : item / (tiles_n * tiles_k), local = INPUT ? item : item - e * tiles_n * tiles_k;
+  const int group = local / (8 * tiles_k), in_group = local - group * 8 * tiles_k;
+  const int high = (INPUT ? row_tiles : tiles_n) - group * 8, height = high < 8 ? high : 8;
+  const int kt = in_group / height, rt = group * 8 + in_group - kt * height;
+  int rows;
+  int64_t out_row0;
+  if constexpr (INPUT) {
+    const RowTile t = row_tile<kTile>(a, rt);
+    rows = t.rows;
+    out_row0 = t.row0;
+  } else {
+    rows = a.n - rt * kTile;
+    out_row0 = static_cast<int64_t>(e) * a.n + rt * kTile;
+  }
+  const int c = (threadIdx.x & 63) * 4, col = kt * kTile + c;
+  if (col >= a.k) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = (blockIdx.x & 15) * 16 + i * 4 + (threadIdx.x >> 6);
+    if (r >= rows) return;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int part = 0; part < turns.parts; ++part)
+      v += *reinterpret_cast<const f32x4 *>(a.partial + (static_cast<int64_t>(part * turns.cut + cut) * kTile + r) * kTile + c);
+    store4_whole<F16>(a, (out_row0 + r) * a.k + col, v);
+  }
+#endif
+}
+
+// Tiles of the result (INPUT: as many as there can be).
+int64_t most_tiles(Grad g, int64_t nexperts, int64_t rows, int64_t n, int64_t k) {
+  const int64_t tiles_k = (k + kTile - 1) / kTile, tiles_n = (n + kTile - 1) / kTile;
+  return g == Grad::INPUT ? (rows / kTile + (rows < nexperts ? rows : nexperts) + 1) * tiles_k : nexperts * tiles_n * tiles_k;
+}
+
+// Parts that a sum may be cut into: kLeastSteps to each (of the weights' gradient on average).
+int most_parts(Grad g, int64_t nexperts, int64_t rows, int64_t n) {
+  const int64_t steps = (g == Grad::INPUT ? n : rows / (nexperts > 0 ? nexperts : 1)) / kStep, parts = steps / kLeastSteps;
+  return parts < 1 ? 1 : (parts > kMostParts ? kMostParts : static_cast<int>(parts));
+}
+
+// One workgroup to a compute unit: its tiles follow each other without a gap.
+int grid_of(int64_t tiles, int parts) {
+  const int cus = fluxmi_device_cu_count(), all = cus > 8 ? cus / 8 * 8 : 256;
+  const int64_t want = (tiles * parts + 7) / 8 * 8;
+  return want < all ? static_cast<int>(want) : all;
+}
+
 }  // namespace
 
 bool grad_tiles_take(Grad g, const GradArgs &a) {
   const auto on16 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   if (a.n % 8 != 0 || a.k % (g == Grad::WEIGHT_8BIT ? 16 : 8) != 0 || !on16(a.grad) || !on16(a.other) || !on16(a.out)) return false;
-  // Offsets: 256 rows of G along, or 32 rows and seven more steps of 32 across.
-  return static_cast<int64_t>(a.n) * 2 * kTile < (int64_t{1} << 31) && static_cast<int64_t>(a.k) * 2 * kTile < (int64_t{1} << 31);
+  if (most_tiles(g, a.nexperts, a.rows, a.n, a.k) >= 1 << 24) return false;
+  // Offsets: 256 rows of G along, 32 rows across, 256 rows of the result.
+  return a.n < 1 << 22 && a.k < 1 << 22;
 }
 
 bool grad_tiles_are_faster(Grad, const GradArgs &) { return true; }
 
-int launch_grad_tiles(Grad g, bool f16, const GradArgs &a, void *stream) {
-  const int64_t tiles_k = (a.k + kTile - 1) / kTile, tiles_n = (a.n + kTile - 1) / kTile;
-  const int64_t items = g == Grad::INPUT ? (a.rows / kTile + (a.rows < a.nexperts ? a.rows : a.nexperts) + 1) * tiles_k : a.nexperts * tiles_n * tiles_k;
-  FLUXMI_REQUIRE(items < (1 << 24), FLUXMI_ERR_UNSUPPORTED, "gradients of the grouped product: too many rows and columns for one launch");
-  // One workgroup to a compute unit: its tiles follow each other without a gap.
-  const int cus = fluxmi_device_cu_count();
-  FLUXMI_REQUIRE(cus > 0, FLUXMI_ERR_HIP, "gradients of the grouped product: no device");
-  const int64_t grid = items < cus ? (items + 7) / 8 * 8 : cus;
-  TileArgs t{a, static_cast<int32_t>(items), static_cast<int32_t>((items + grid - 1) / grid)};
-  auto launch = [&](auto kernel, std::atomic<uint64_t> &done) -> int {
-    if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds_bytes(g), done)) return rc;
-    kernel<<<static_cast<uint32_t>(grid), kThreads, lds_bytes(g), static_cast<hipStream_t>(stream)>>>(t);
+size_t grad_tiles_workspace_bytes(Grad g, int32_t nexperts, int64_t rows, int64_t n, int64_t k) {
+  const int parts = most_parts(g, nexperts, rows, n);
+  const int64_t tiles = most_tiles(g, nexperts, rows, n, k);
+  if (parts < 2 || tiles == 0) return 0;
+  const int grid = grid_of(tiles, parts);
+  if (g != Grad::INPUT && (tiles >= 1 << 24 || turns_of(static_cast<int>(tiles), grid, parts).cut == 0)) return 0;
+  return static_cast<size_t>(grid) * kTile * kTile * sizeof(float);  // (a part to each workgroup at most)
+}
+
+int launch_grad_tiles(Grad g, bool f16, const GradArgs &args, void *stream) {
+  GradArgs a = args;
+  const int64_t tiles_k = (a.k + kTile - 1) / kTile, tiles_n = (a.n + kTile - 1) / kTile, tiles = most_tiles(g, a.nexperts, a.rows, a.n, a.k);
+  a.parts = most_parts(g, a.nexperts, a.rows, a.n);
+  const int grid = grid_of(tiles, a.parts);
+  const TileArgs t{a, grid, static_cast<int32_t>(tiles / grid + 1), divisor(tiles_n * tiles_k), divisor(8 * tiles_k)};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool join = grad_tiles_workspace_bytes(g, a.nexperts, a.rows, a.n, a.k) > 0;
+  auto launch = [&](auto F, auto K, std::atomic<uint64_t> &done) -> int {
+    constexpr bool f = decltype(F)::value;
+    constexpr Grad k = decltype(K)::value;
+    if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(grad_tile_kernel<f, k>), lds_bytes(k), done)) return rc;
+    grad_tile_kernel<f, k><<<grid, kThreads, lds_bytes(k), s>>>(t);
     FLUXMI_HIP_CHECK(hipGetLastError());
+    if (join) {
+      // (at most half the workgroups have a tile that is cut)
+      grad_tile_join_kernel<f, k == Grad::INPUT ? Grad::INPUT : Grad::WEIGHT><<<grid / 2 * 16, kThreads, 0, s>>>(t);
+      FLUXMI_HIP_CHECK(hipGetLastError());
+    }
     return FLUXMI_OK;
   };
   static std::atomic<uint64_t> done[6];
-  if (g == Grad::WEIGHT_8BIT) return f16 ? launch(grad_tile_kernel<true, Grad::WEIGHT_8BIT>, done[4]) : launch(grad_tile_kernel<false, Grad::WEIGHT_8BIT>, done[5]);
-  if (g == Grad::INPUT) return f16 ? launch(grad_tile_kernel<true, Grad::INPUT>, done[0]) : launch(grad_tile_kernel<false, Grad::INPUT>, done[1]);
-  return f16 ? launch(grad_tile_kernel<true, Grad::WEIGHT>, done[2]) : launch(grad_tile_kernel<false, Grad::WEIGHT>, done[3]);
+  const auto by_type = [&](auto K, int at) { return f16 ? launch(std::true_type{}, K, done[at]) : launch(std::false_type{}, K, done[at + 1]); };
+  if (g == Grad::INPUT) return by_type(std::integral_constant<Grad, Grad::INPUT>{}, 0);
+  if (g == Grad::WEIGHT) return by_type(std::integral_constant<Grad, Grad::WEIGHT>{}, 2);
+  return by_type(std::integral_constant<Grad, Grad::WEIGHT_8BIT>{}, 4);
 }
 
 }  // namespace fluxmi

@@ -86,8 +86,11 @@ torch::Tensor product(const torch::Tensor &input, const torch::Tensor &weight, c
 torch::Tensor input_gradient(const torch::Tensor &grad, const torch::Tensor &weight, const torch::Tensor &splits) {
   const c10::DeviceGuard guard(grad.device());
   torch::Tensor out = empty_on(grad, {grad.size(0), weight.size(2)}, grad.scalar_type());
+  const size_t ws_bytes = fluxmi_moe_dgrad_workspace_bytes(static_cast<int32_t>(weight.size(0)), grad.size(0), grad.size(1), weight.size(2));
+  torch::Tensor ws;
+  if (ws_bytes > 0) ws = empty_on(grad, {static_cast<int64_t>(ws_bytes)}, at::kByte);
   check_status(fluxmi_moe_dgrad(grad.data_ptr(), weight.data_ptr(), row_type(grad), splits.data_ptr<int32_t>(), static_cast<int32_t>(weight.size(0)),
-                                grad.size(0), grad.size(1), weight.size(2), out.data_ptr(), current_stream()),
+                                grad.size(0), grad.size(1), weight.size(2), out.data_ptr(), ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, current_stream()),
                "fluxmi_moe_dgrad");
   return out;
 }

@@ -478,14 +478,15 @@ int fluxmi_grouped_gemm_mx_launch_info(const fluxmi_mx_gemm_args *args, fluxmi_m
  *                      (those that fluxmi_checkpoint_e4m3 made from that type are values of it)
  *
  * `row_type` (FLUXMI_ROWS_BF16 or FLUXMI_ROWS_FP16) is the type of grad [rows, n], weight, input [rows, k] and grad_input [rows, k]; grad_weight is of
- * `out_type`: that or FLUXMI_ROWS_FP32.  Sums are fp32, in an order that follows from the sizes and the alignment alone, and are rounded once.
+ * `out_type`: that or FLUXMI_ROWS_FP32.  Sums are fp32, in an order that follows from the sizes, the row counts and the alignment alone, and are rounded once.
  * `splits`: DEVICE int32 row counts.  Negative ones are 0; what they have past `rows` does not exist.  Rows past the sum are not read by fluxmi_moe_wgrad.
  * Requirements: nexperts <= 1024; rows, n, k <= 2^24; operands aligned to their elements, grad_input to 8 bytes, grad_weight and workspace to 16.  Operands
  * that start on 16 bytes with n and k multiples of 8 are fast.
- * `workspace`: fluxmi_moe_wgrad_workspace_bytes() bytes (0 for many sizes) of any content; not shared by calls that may overlap.
+ * `workspace`: fluxmi_moe_dgrad_workspace_bytes() or fluxmi_moe_wgrad_workspace_bytes() bytes (0 for many sizes, 64 MiB for most others) of any content; not shared by calls that may overlap.
  * ---------------------------------------------------------------------------------------------- */
 int fluxmi_moe_dgrad(const void *grad, const void *weight, int32_t row_type, const int32_t *splits, int32_t nexperts, int64_t rows, int64_t n,
-                     int64_t k, void *grad_input, void *stream);
+                     int64_t k, void *grad_input, void *workspace, size_t workspace_bytes, void *stream);
+size_t fluxmi_moe_dgrad_workspace_bytes(int32_t nexperts, int64_t rows, int64_t n, int64_t k);
 size_t fluxmi_moe_wgrad_workspace_bytes(int32_t nexperts, int64_t rows, int64_t n, int64_t k);
 int fluxmi_moe_wgrad(const void *grad, const void *input, const void *input_scale, int32_t row_type, const int32_t *splits, int32_t nexperts,
                      int64_t rows, int64_t n, int64_t k, void *grad_weight, int32_t out_type, int32_t accumulate, void *workspace,

@@ -17,7 +17,7 @@ def refused(rc, status, text):
 
 def test_c_entry_points_refuse():
     lib = capi.load()
-    dgrad = lambda grad=P, weight=P, t=0, splits=P, e=2, rows=4, n=64, k=64, out=Q: lib.fluxmi_moe_dgrad(grad, weight, t, splits, e, rows, n, k, out, None)  # noqa: E731
+    dgrad = lambda grad=P, weight=P, t=0, splits=P, e=2, rows=4, n=64, k=64, out=Q, ws=None, ws_bytes=0: lib.fluxmi_moe_dgrad(grad, weight, t, splits, e, rows, n, k, out, ws, ws_bytes, None)  # noqa: E731
     refused(dgrad(t=1), -1, "type 1")
     refused(dgrad(e=-1), -1, "negative")
     refused(dgrad(rows=-4), -1, "negative")
@@ -29,6 +29,11 @@ def test_c_entry_points_refuse():
     refused(dgrad(splits=None), -1, "null pointer")
     refused(dgrad(grad=ODD), -1, "aligned")
     refused(dgrad(out=ctypes.c_void_p(0x1002)), -1, "aligned")
+    need = lib.fluxmi_moe_dgrad_workspace_bytes(2, 4, 4096, 64)
+    assert need > 0
+    refused(dgrad(n=4096, ws=P, ws_bytes=need - 1), -3, "workspace")
+    refused(dgrad(n=4096, ws=ctypes.c_void_p(0x1004), ws_bytes=need), -3, "workspace")
+    assert lib.fluxmi_moe_dgrad_workspace_bytes(-1, 4, 4096, 64) == 0 and lib.fluxmi_moe_dgrad_workspace_bytes(0, 0, 0, 0) == 0
     assert dgrad(rows=0, grad=None, out=None) == 0 and dgrad(k=0, out=None) == 0
 
     wgrad = lambda grad=P, x=P, scale=None, t=0, splits=P, e=2, rows=4, n=64, k=64, out=Q, out_t=0, ws=None, ws_bytes=0: lib.fluxmi_moe_wgrad(  # noqa: E731
