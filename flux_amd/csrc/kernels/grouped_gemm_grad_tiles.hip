@@ -97,6 +97,28 @@ __device__ __forceinline__ void mfma(f32x4 &acc, const u32x4 &a, const u32x4 &b)
   }
 }
 
+// Block `block` of a wave's rows, unless the tile has no more than `blocks` of them.  One statement with its branch: as a branch that the compiler sees, the sums' registers
+// would be moved about.
+template <bool F16, bool FIRST>
+__device__ __forceinline__ void row_block(f32x4 (&acc)[8], const u32x4 (&c)[8], const u32x4 &r, int block, int blocks) {
+#define FLUXMI_ROW_BLOCK(MFMA, D)                                                                                                                   \
+  asm volatile("s_cmp_gt_i32 %17, %18\n\ts_cbranch_scc0 .Lrow_block%=\n\t" MFMA " %0, %8, %16, " D("%0") "\n\t" MFMA " %1, %9, %16, " D("%1") "\n\t"      \
+               MFMA " %2, %10, %16, " D("%2") "\n\t" MFMA " %3, %11, %16, " D("%3") "\n\t" MFMA " %4, %12, %16, " D("%4") "\n\t"                       \
+               MFMA " %5, %13, %16, " D("%5") "\n\t" MFMA " %6, %14, %16, " D("%6") "\n\t" MFMA " %7, %15, %16, " D("%7") "\n.Lrow_block%=:"          \
+               : "+a"(acc[0]), "+a"(acc[1]), "+a"(acc[2]), "+a"(acc[3]), "+a"(acc[4]), "+a"(acc[5]), "+a"(acc[6]), "+a"(acc[7])                       \
+               : "v"(c[0]), "v"(c[1]), "v"(c[2]), "v"(c[3]), "v"(c[4]), "v"(c[5]), "v"(c[6]), "v"(c[7]), "v"(r), "s"(blocks), "i"(block)              \
+               : "scc")
+#define FLUXMI_SAME(x) x
+#define FLUXMI_ZERO(x) "0"
+  if constexpr (F16 && FIRST) FLUXMI_ROW_BLOCK("v_mfma_f32_16x16x32_f16", FLUXMI_ZERO);
+  else if constexpr (F16) FLUXMI_ROW_BLOCK("v_mfma_f32_16x16x32_f16", FLUXMI_SAME);
+  else if constexpr (FIRST) FLUXMI_ROW_BLOCK("v_mfma_f32_16x16x32_bf16", FLUXMI_ZERO);
+  else FLUXMI_ROW_BLOCK("v_mfma_f32_16x16x32_bf16", FLUXMI_SAME);
+#undef FLUXMI_ROW_BLOCK
+#undef FLUXMI_SAME
+#undef FLUXMI_ZERO
+}
+
 // A sum's block, read where it is used: the compiler would copy all of them to vector registers ahead of the branches of the stores.
 __device__ __forceinline__ f32x4 sums_of(const f32x4 &acc) {
   f32x4 v;
@@ -151,7 +173,8 @@ __device__ __forceinline__ int fresh_lane() {
 
 #endif  // __HIP_DEVICE_COMPILE__
 
-template <bool F16, Grad G>
+// FEW: most tiles have far fewer rows than 256 (INPUT).
+template <bool F16, Grad G, bool FEW>
 __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs args) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr bool INPUT = G == Grad::INPUT, EIGHT = G == Grad::WEIGHT_8BIT;
@@ -245,12 +268,14 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
   // The step that is requested next: where it begins, and how much of the sum (INPUT: of the tile's rows of G, in bytes) is left there.
   const uint8_t *rnext = nullptr, *cnext = nullptr, *snext = nullptr;
   int left = 0, rbytes = 0;
+  int row_blocks = 0;
   int steps = 0, rest = 0;  // rest: values of the last step
   auto begin_tile = [&](const Tile &t) {
     const int lane = fresh_lane();
     left = __builtin_amdgcn_readfirstlane(t.sum_over);
     steps = left > 0 ? (left + kStep - 1) / kStep : 1;  // (a sum of nothing is a step that is cleared)
     rest = left - (steps - 1) * kStep;
+    row_blocks = (__builtin_amdgcn_readfirstlane(t.rows) - wr * 16 + 31) / 32;
     const int64_t first = __builtin_amdgcn_readfirstlane(t.first);
     rnext = a.grad + first * rpitch;
     if constexpr (INPUT) {
@@ -321,8 +346,8 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       cfrag[j] = lds0 + t * 512 + ((wc * 8 + j) ^ f) * 32 + (i & 3) * 8;
-      if constexpr (INPUT) rfrag[j] = lds0 + rows_at(G) + (wr * 128 + i) * 64 + (g ^ ((i >> 1) & 3)) * 16;
-      else rfrag[j] = lds0 + rows_at(G) + t * 512 + ((wr * 8 + j) ^ f) * 32 + (i & 3) * 8;
+      if constexpr (INPUT) rfrag[j] = lds0 + rows_at(G) + (wr * 16 + i) * 64 + (g ^ ((i >> 1) & 3)) * 16;
+      else rfrag[j] = lds0 + rows_at(G) + t * 512 + ((2 * j + wr) ^ f) * 32 + (i & 3) * 8;
     }
   }
   u32x4 ca[8], ra[8], cb[8], rb[8];
@@ -335,7 +360,7 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
       cf[r / 2][(r & 1) * 2] = v[0];
       cf[r / 2][(r & 1) * 2 + 1] = v[1];
     } else if constexpr (INPUT) {
-      rf[r - 16] = *(LdsFrag)(uintptr_t)(rfrag[0] + slot * kSlot + (r - 16) * 1024);
+      rf[r - 16] = *(LdsFrag)(uintptr_t)(rfrag[0] + slot * kSlot + (r - 16) * 2048);
     } else {
       constexpr int q = r - 16;
       const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr)(uintptr_t)(rfrag[q / 2] + slot * kSlot + (q & 1) * 2048)));
@@ -450,7 +475,22 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
     wait_step(U, s);
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    static_for<64>([&](auto T) {
+    if constexpr (FEW) {
+      // (the reads and fills of eight MFMAs stand together before them, which costs whole tiles 7 to 10 %)
+      static_for<8>([&](auto I) {
+        constexpr int i = decltype(I)::value;
+        static_for<kReads / 8>([&](auto R) { read_one(integral_constant<int, (u + 1) % kSlots>{}, integral_constant<int, i * (kReads / 8) + decltype(R)::value>{}, cn, rn); });
+        if constexpr (i < kFills) {
+          set_target(U, I);
+          asm volatile("s_nop 0" : : : "memory");
+          fill(I);
+        }
+        if constexpr (i == 7) next_buffers();
+        __builtin_amdgcn_sched_barrier(0);
+        row_block<F16, decltype(FIRST)::value>(acc[i], cf, rf[i], i, row_blocks);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    } else static_for<64>([&](auto T) {
       constexpr int t = decltype(T)::value, q = t / 8;
       conversion(U, T);
       if constexpr (t < 2 * kReads && t % 2 == 0) read_one(integral_constant<int, (u + 1) % kSlots>{}, integral_constant<int, t / 2>{}, cn, rn);
@@ -536,7 +576,7 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
       const uint32_t pitch = part ? kTile : a.k;
       uint8_t *const base = part ? reinterpret_cast<uint8_t *>(a.partial + static_cast<int64_t>(tile.slot) * kTile * kTile) : a.out + tile.out_row0 * a.k * out_size;
       const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(base, 0, static_cast<int>(static_cast<uint32_t>(tile.rows) * pitch * out_size), 0x00020000);
-      const uint32_t row_at = static_cast<uint32_t>(wr * 128 + (l >> 3)) * pitch + (part ? 0 : tile.col0);
+      const uint32_t row_at = static_cast<uint32_t>(wr * 16 + (l >> 3)) * pitch + (part ? 0 : tile.col0);
       // Results of group N are read before those of the one before it are stored.
       u32x4 v[2][2];
       auto read_back = [&](auto N) {
@@ -562,7 +602,7 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
             const int c = wc * 128 + j * 16 + (l & 7) * 4;
   #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint32_t at = c < tile.cols ? (row_at + (i * 16 + h * 8) * pitch + c) * out_size : 0xfffffff0u;
+              const uint32_t at = c < tile.cols ? (row_at + (i * 32 + h * 8) * pitch + c) * out_size : 0xfffffff0u;
               f32x4 x = __builtin_bit_cast(f32x4, v[n & 1][h]);
               if (!add) {
                 __builtin_amdgcn_raw_buffer_store_b128(v[n & 1][h], out, at, 0, policy);
@@ -600,7 +640,7 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
             if constexpr (n < 15) put(integral_constant<int, (n < 15 ? n + 1 : 0)>{});
             const int c = wc * 128 + j * 16 + (l & 7) * 8;
   #pragma unroll
-            for (int h = 0; h < 2; ++h) __builtin_amdgcn_raw_buffer_store_b128(v[n & 1][h], out, c < tile.cols ? (row_at + (i * 16 + h * 8) * pitch + c) * 2 : 0xfffffff0u, 0, policy);
+            for (int h = 0; h < 2; ++h) __builtin_amdgcn_raw_buffer_store_b128(v[n & 1][h], out, c < tile.cols ? (row_at + (i * 32 + h * 8) * pitch + c) * 2 : 0xfffffff0u, 0, policy);
             __builtin_amdgcn_sched_barrier(0);
           });
           behind = 1;
@@ -712,11 +752,11 @@ int launch_grad_tiles(Grad g, bool f16, const GradArgs &args, void *stream) {
   const TileArgs t{a, grid, static_cast<int32_t>(tiles / grid + 1), divisor(tiles_n * tiles_k), divisor(8 * tiles_k)};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const bool join = grad_tiles_workspace_bytes(g, a.nexperts, a.rows, a.n, a.k) > 0;
-  auto launch = [&](auto F, auto K, std::atomic<uint64_t> &done) -> int {
-    constexpr bool f = decltype(F)::value;
+  auto launch = [&](auto F, auto K, auto FEW, std::atomic<uint64_t> &done) -> int {
+    constexpr bool f = decltype(F)::value, few = decltype(FEW)::value;
     constexpr Grad k = decltype(K)::value;
-    if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(grad_tile_kernel<f, k>), lds_bytes(k), done)) return rc;
-    grad_tile_kernel<f, k><<<grid, kThreads, lds_bytes(k), s>>>(t);
+    if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(grad_tile_kernel<f, k, few>), lds_bytes(k), done)) return rc;
+    grad_tile_kernel<f, k, few><<<grid, kThreads, lds_bytes(k), s>>>(t);
     FLUXMI_HIP_CHECK(hipGetLastError());
     if (join) {
       // (at most half the workgroups have a tile that is cut)
@@ -725,11 +765,15 @@ int launch_grad_tiles(Grad g, bool f16, const GradArgs &args, void *stream) {
     }
     return FLUXMI_OK;
   };
-  static std::atomic<uint64_t> done[6];
-  const auto by_type = [&](auto K, int at) { return f16 ? launch(std::true_type{}, K, done[at]) : launch(std::false_type{}, K, done[at + 1]); };
-  if (g == Grad::INPUT) return by_type(std::integral_constant<Grad, Grad::INPUT>{}, 0);
-  if (g == Grad::WEIGHT) return by_type(std::integral_constant<Grad, Grad::WEIGHT>{}, 2);
-  return by_type(std::integral_constant<Grad, Grad::WEIGHT_8BIT>{}, 4);
+  static std::atomic<uint64_t> done[8];
+  const auto by_type = [&](auto K, auto FEW, int at) { return f16 ? launch(std::true_type{}, K, FEW, done[at]) : launch(std::false_type{}, K, FEW, done[at + 1]); };
+  using std::integral_constant;
+  // us, all row blocks -> those that there are: 8 experts 14336 x 4096, 74 rows in all 190 -> 176, 512 rows 195 -> 186, 4096 x 14336, 512 rows 210 -> 196, 32 experts 2048 x 7168,
+  // 1024 rows 207 -> 191; 8 experts 4096 x 4096, 2048 rows 106 -> 109, 16384 rows 411 -> 454; 64 experts 1408 x 2048, 98304 rows 531 -> 570.
+  if (g == Grad::INPUT && a.rows < static_cast<int64_t>(a.nexperts) * 160) return by_type(integral_constant<Grad, Grad::INPUT>{}, std::true_type{}, 0);
+  if (g == Grad::INPUT) return by_type(integral_constant<Grad, Grad::INPUT>{}, std::false_type{}, 2);
+  if (g == Grad::WEIGHT) return by_type(integral_constant<Grad, Grad::WEIGHT>{}, std::false_type{}, 4);
+  return by_type(integral_constant<Grad, Grad::WEIGHT_8BIT>{}, std::false_type{}, 6);
 }
 
 }  // namespace fluxmi
