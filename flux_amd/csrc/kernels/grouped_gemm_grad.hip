@@ -337,14 +337,15 @@ extern "C" int fluxmi_moe_wgrad(const void *grad, const void *input, const void 
   a.out_f32 = out_type == FLUXMI_ROWS_FP32;
   a.accumulate = accumulate != 0;
   a.parts = parts_of(nexperts, rows, n, k);
+  const Grad kind = input_scale != nullptr ? Grad::WEIGHT_8BIT : Grad::WEIGHT;
+  const bool tiles = grad_tiles_take(kind, a) && grad_tiles_are_faster(kind, a);
+  const int64_t pieces = nexperts * tiles_of(n) * tiles_of(k), items = pieces * a.parts;
+  FLUXMI_REQUIRE(tiles || items <= kMostItems, FLUXMI_ERR_UNSUPPORTED, "moe_wgrad: too many experts, rows and columns for one launch");
   const size_t need = fluxmi_moe_wgrad_workspace_bytes(nexperts, rows, n, k);
   FLUXMI_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && on(workspace, 16)), FLUXMI_ERR_WORKSPACE,
                  "moe_wgrad: workspace of %zu bytes, 16-byte aligned, expected, got %zu", need, workspace_bytes);
   a.partial = static_cast<float *>(workspace);
-  const Grad kind = input_scale != nullptr ? Grad::WEIGHT_8BIT : Grad::WEIGHT;
-  if (grad_tiles_take(kind, a) && grad_tiles_are_faster(kind, a)) return launch_grad_tiles(kind, row_type == FLUXMI_ROWS_FP16, a, stream);
-  const int64_t pieces = nexperts * tiles_of(n) * tiles_of(k), items = pieces * a.parts;
-  FLUXMI_REQUIRE(items <= kMostItems, FLUXMI_ERR_UNSUPPORTED, "moe_wgrad: too many experts, rows and columns for one launch");
+  if (tiles) return launch_grad_tiles(kind, row_type == FLUXMI_ROWS_FP16, a, stream);
   const bool f16 = row_type == FLUXMI_ROWS_FP16;
   const bool vec = n % 8 == 0 && k % 8 == 0 && on(grad, 16) && on(input, input_scale != nullptr ? 8 : 16);
   const hipStream_t s = static_cast<hipStream_t>(stream);

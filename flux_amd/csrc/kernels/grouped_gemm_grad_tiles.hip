@@ -27,11 +27,12 @@ constexpr int kCodeSlot = 8192, kScaleSlot = 1024;  // WEIGHT_8BIT: a step's cod
 constexpr int rows_at(Grad g) { return (g == Grad::WEIGHT_8BIT ? 2 : kSlots) * kSlot; }
 constexpr int codes_at() { return rows_at(Grad::WEIGHT_8BIT) + kSlots * kSlot; }
 constexpr int scales_at() { return codes_at() + kSlots * kCodeSlot; }
-// Behind them a window of each wave, through which results go out, and the experts' tables: where their rows end, and (INPUT) their tiles.
+// Behind them a window of each wave, through which results go out, and the experts' tables: where their rows end, and (INPUT) their tiles or (otherwise) the order
+// they are taken in.
 constexpr int kWindow = 2048;
 constexpr int windows_at(Grad g) { return g == Grad::WEIGHT_8BIT ? scales_at() + kSlots * kScaleSlot : rows_at(g) + kSlots * kSlot; }
 constexpr int tables_at(Grad g) { return windows_at(g) + kThreads / 64 * kWindow; }
-constexpr int lds_bytes(Grad g) { return tables_at(g) + (g == Grad::INPUT ? 2 : 1) * 4 * kMaxExperts + 16; }
+constexpr int lds_bytes(Grad g) { return tables_at(g) + 2 * 4 * kMaxExperts + 32; }
 
 // Division of numbers below 2^24 by one that the host knows.
 struct Divisor {
@@ -50,7 +51,13 @@ struct TileArgs {
   int32_t grid;           // workgroups, a multiple of 8
   int32_t turns;          // tiles that a workgroup computes at most
   Divisor per_expert, per_group;  // an expert's tiles; those of eight along the result's rows
+  int32_t *queue;         // NULL: tiles are dealt in turns; otherwise workgroups fetch them: counters, then the experts by their rows
 };
+
+// Queues: eight of them, one to an XCD, a counter each (a line apart) of the tiles that were fetched from it beyond every workgroup's first; then the experts, those with most
+// rows first.
+constexpr int kQueueLine = 32, kQueueExperts = 8 * kQueueLine;
+constexpr size_t kQueueBytes = (kQueueExperts + kMaxExperts) * sizeof(int32_t);
 
 constexpr int kLeastSteps = 8;   // of a part
 constexpr int kMostParts = 16;
@@ -189,11 +196,12 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
 
   // ---- the experts' rows and tiles, in LDS ------------------------------------------------------------------------
   typedef __attribute__((address_space(3))) int *LdsInt;
-  const LdsInt row_ends = (LdsInt)(uintptr_t)(lds0 + tables_at(G)), tile_ends = row_ends + kMaxExperts;
+  const LdsInt row_ends = (LdsInt)(uintptr_t)(lds0 + tables_at(G)), tile_ends = row_ends + kMaxExperts, order = tile_ends, mail = tile_ends + kMaxExperts;
   int all_rows = 0, row_tiles = 0;
   for (int e0 = 0; e0 < a.nexperts; e0 += 64) {  // (the same from every wave)
     const ExpertRows x = rows_of_lane(a, e0, all_rows);
     row_ends[e0 + lane] = x.end;
+    if (!INPUT && args.queue != nullptr) order[e0 + lane] = e0 + lane < a.nexperts ? args.queue[kQueueExperts + e0 + lane] : 0;
     if constexpr (INPUT) {
       const int end = row_tiles + wave_inclusive_scan((x.end - x.begin + kTile - 1) / kTile);
       tile_ends[e0 + lane] = end;
@@ -205,19 +213,10 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
   if constexpr (INPUT) row_tiles += (a.rows - all_rows + kTile - 1) / kTile;  // the rows that belong to no expert
   const Turns turns = turns_of((INPUT ? row_tiles : a.nexperts * tiles_n) * tiles_k, args.grid, a.parts);
 
-  // This workgroup's tile of a turn.  Workgroups are dealt to the eight XCDs in turn; those on one XCD take neighbouring tiles: an expert's (INPUT: all) tiles in
-  // groups of eight along the result's rows, walked column by column.
-  auto describe = [&](int turn) {
+  // Tile number `item`.  An expert's (INPUT: all) tiles lie in groups of eight along the result's rows, walked column by column.
+  auto describe = [&](int item, int part) {
     Tile t{};
-    int item = turn * args.grid + (blockIdx.x & 7) * (args.grid >> 3) + (blockIdx.x >> 3);
-    t.part = -1;
-    if (item >= turns.whole) {
-      item -= turns.whole;
-      if (item >= turns.cut * turns.parts) return t;
-      t.part = item / turns.cut;
-      t.slot = item;
-      item += turns.whole - t.part * turns.cut;
-    }
+    t.part = part;
     const int e = INPUT ? 0 : divide(item, args.per_expert), local = INPUT ? item : item - e * static_cast<int>(args.per_expert.by);
     const int group = divide(local, args.per_group), in_group = local - group * static_cast<int>(args.per_group.by);
     const int high = (INPUT ? row_tiles : tiles_n) - group * 8, height = high < 8 ? high : 8;
@@ -244,12 +243,12 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
       t.out_row0 = t.first = begin;
       t.sum_over = t.e < a.nexperts ? a.n : 0;
     } else {
-      t.e = e;
+      t.e = args.queue != nullptr ? __builtin_amdgcn_readfirstlane(order[e]) : e;
       t.row0 = rt * kTile;
       t.rows = a.n - t.row0 < kTile ? a.n - t.row0 : kTile;
-      t.out_row0 = static_cast<int64_t>(e) * a.n + t.row0;
-      t.first = e > 0 ? __builtin_amdgcn_readfirstlane(row_ends[e - 1]) : 0;
-      t.sum_over = __builtin_amdgcn_readfirstlane(row_ends[e]) - t.first;
+      t.out_row0 = static_cast<int64_t>(t.e) * a.n + t.row0;
+      t.first = t.e > 0 ? __builtin_amdgcn_readfirstlane(row_ends[t.e - 1]) : 0;
+      t.sum_over = __builtin_amdgcn_readfirstlane(row_ends[t.e]) - t.first;
     }
     if (t.part >= 0) {
       const int all = (t.sum_over + kStep - 1) / kStep, from = all * t.part / turns.parts * kStep, to = all * (t.part + 1) / turns.parts * kStep;
@@ -258,6 +257,23 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
       else t.first += from;
     }
     return t;
+  };
+  // This workgroup's tile of a turn.  Workgroups are dealt to the eight XCDs in turn; those on one XCD take neighbouring tiles.
+  const int home = blockIdx.x & 7, place = blockIdx.x >> 3;
+  auto tile_of_turn = [&](int turn) {
+    int item = turn * args.grid + home * (args.grid >> 3) + place;
+    if (item < turns.whole) return describe(item, -1);
+    item -= turns.whole;
+    if (item >= turns.cut * turns.parts) return Tile{};
+    const int part = item / turns.cut;
+    Tile t = describe(turns.whole + item - part * turns.cut, part);
+    t.slot = item;
+    return t;
+  };
+  // Tile at a place of a queue: groups of eight tiles are dealt to the queues in turn, so that those that an XCD has at a time share their rows of G or X.
+  auto tile_of_queue = [&](int queue, int at) {
+    const int item = ((at & ~7) + queue) * 8 + (at & 7);
+    return item < a.nexperts * tiles_n * tiles_k ? describe(item, -1) : Tile{};
   };
 
   // ---- fills: four instructions of a wave to either operand's step ------------------------------------------------
@@ -504,14 +520,8 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  Tile tile{};
-  int turn = 0;
-  auto next_tile = [&]() {
-    Tile t{};
-    while (turn < args.turns && t.rows == 0) t = describe(turn++);
-    return t;
-  };
-  tile = next_tile();
+  Tile tile = !INPUT && args.queue != nullptr ? tile_of_queue(home, place) : tile_of_turn(0);
+  int turn = 1;
   if (tile.rows == 0) return;
   begin_tile(tile);
   first_fills();
@@ -538,6 +548,9 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
     if (rest < kStep && steps == 1) clear_rows(0);
     FLUXMI_LGKM0();
     __builtin_amdgcn_s_barrier();
+    // The next tile's number, asked for now and looked at when this one's sums are done.
+    int fetched = 0;
+    if (!INPUT && args.queue != nullptr && threadIdx.x == 0) fetched = atomicAdd(args.queue + home * kQueueLine, 1);
     static_for<kReads>([&](auto R) { read_one(integral_constant<int, 0>{}, R, ca, ra); });
     FLUXMI_LGKM0();
     step(integral_constant<int, 0>{}, std::true_type{}, 0, ca, ra, cb, rb);
@@ -555,8 +568,24 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
         if (s + 2 < steps) step(integral_constant<int, 3>{}, std::false_type{}, s + 2, cb, rb, ca, ra);
       }
     }
-    const Tile next = next_tile();
-    __builtin_amdgcn_s_barrier();  // nobody reads the slots any more
+    Tile next{};
+    if (!INPUT && args.queue != nullptr) {
+      if (threadIdx.x == 0) *mail = fetched;
+      FLUXMI_LGKM0();
+      __builtin_amdgcn_s_barrier();  // nobody reads the slots any more
+      next = tile_of_queue(home, (args.grid >> 3) + __builtin_amdgcn_readfirstlane(*mail));
+      // The own queue is empty: the others'.
+      for (int q = 1; q < 8 && next.rows == 0; ++q) {
+        const int other = (home + q) & 7;
+        __syncthreads();
+        if (threadIdx.x == 0) *mail = atomicAdd(args.queue + other * kQueueLine, 1);
+        __syncthreads();
+        next = tile_of_queue(other, (args.grid >> 3) + __builtin_amdgcn_readfirstlane(*mail));
+      }
+    } else {
+      if (turn < args.turns) next = tile_of_turn(turn++);
+      __builtin_amdgcn_s_barrier();  // nobody reads the slots any more
+    }
     if (next.rows > 0) {
       begin_tile(next);
       first_fills();
@@ -657,6 +686,28 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
 #endif
 }
 
+// Empties the queues, and puts the experts in order.
+__global__ __launch_bounds__(kMaxExperts) void grad_queue_kernel(const GradArgs a, int32_t *queue) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __shared__ int rows[kMaxExperts];
+  if (threadIdx.x < 64) {
+    int carry = 0;
+    for (int e0 = 0; e0 < a.nexperts; e0 += 64) {
+      const ExpertRows x = rows_of_lane(a, e0, carry);
+      rows[e0 + threadIdx.x] = x.end - x.begin;
+    }
+  }
+  if (threadIdx.x < 8) queue[threadIdx.x * kQueueLine] = 0;
+  __syncthreads();
+  const int e = threadIdx.x;
+  if (e >= a.nexperts) return;
+  const int mine = rows[e];
+  int before = 0;
+  for (int i = 0; i < a.nexperts; ++i) before += rows[i] > mine || (rows[i] == mine && i < e) ? 1 : 0;
+  queue[kQueueExperts + before] = e;
+#endif
+}
+
 // The parts of the last turn's tiles, added in their order: a workgroup has sixteen rows of a tile.
 template <bool F16, Grad G>
 __global__ __launch_bounds__(kThreads) void grad_tile_join_kernel(const TileArgs args) {
@@ -735,11 +786,17 @@ bool grad_tiles_take(Grad g, const GradArgs &a) {
 
 bool grad_tiles_are_faster(Grad, const GradArgs &) { return true; }
 
+// Experts of different sizes in several turns: a workgroup fetches its next tile when it has done with one.  The result has the same bits: a tile's sum is the same wherever
+// it is computed.
+static bool by_queue(Grad g, int64_t nexperts, int64_t tiles, int grid) { return g != Grad::INPUT && nexperts > 1 && tiles >= 4 * static_cast<int64_t>(grid); }
+
 size_t grad_tiles_workspace_bytes(Grad g, int32_t nexperts, int64_t rows, int64_t n, int64_t k) {
   const int parts = most_parts(g, nexperts, rows, n);
   const int64_t tiles = most_tiles(g, nexperts, rows, n, k);
-  if (parts < 2 || tiles == 0) return 0;
+  if (tiles == 0) return 0;
   const int grid = grid_of(tiles, parts);
+  if (by_queue(g, nexperts, tiles, grid)) return kQueueBytes;
+  if (parts < 2) return 0;
   if (g != Grad::INPUT && (tiles >= 1 << 24 || turns_of(static_cast<int>(tiles), grid, parts).cut == 0)) return 0;
   return static_cast<size_t>(grid) * kTile * kTile * sizeof(float);  // (a part to each workgroup at most)
 }
@@ -749,9 +806,14 @@ int launch_grad_tiles(Grad g, bool f16, const GradArgs &args, void *stream) {
   const int64_t tiles_k = (a.k + kTile - 1) / kTile, tiles_n = (a.n + kTile - 1) / kTile, tiles = most_tiles(g, a.nexperts, a.rows, a.n, a.k);
   a.parts = most_parts(g, a.nexperts, a.rows, a.n);
   const int grid = grid_of(tiles, a.parts);
-  const TileArgs t{a, grid, static_cast<int32_t>(tiles / grid + 1), divisor(tiles_n * tiles_k), divisor(8 * tiles_k)};
+  const bool queue = by_queue(g, a.nexperts, tiles, grid);
+  const TileArgs t{a, grid, static_cast<int32_t>(tiles / grid + 1), divisor(tiles_n * tiles_k), divisor(8 * tiles_k), queue ? reinterpret_cast<int32_t *>(a.partial) : nullptr};
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool join = grad_tiles_workspace_bytes(g, a.nexperts, a.rows, a.n, a.k) > 0;
+  if (queue) {
+    grad_queue_kernel<<<1, kMaxExperts, 0, s>>>(a, t.queue);
+    FLUXMI_HIP_CHECK(hipGetLastError());
+  }
+  const bool join = !queue && grad_tiles_workspace_bytes(g, a.nexperts, a.rows, a.n, a.k) > 0;
   auto launch = [&](auto F, auto K, auto FEW, std::atomic<uint64_t> &done) -> int {
     constexpr bool f = decltype(F)::value, few = decltype(FEW)::value;
     constexpr Grad k = decltype(K)::value;
