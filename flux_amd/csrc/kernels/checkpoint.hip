@@ -10,6 +10,11 @@
 //
 // All of it is fp32 inside, with one rounding to 16 bits at the end; values of a checkpoint are exact in fp32, scales and codes are exact up to the
 // code's own rounding.
+//
+// Memory bounds all of it: every byte is read and written once.  A lane has eight values of a row (16 bytes in, 8 out), four lanes a block, whose maximum they find among
+// themselves; rows of any length and start, whole vectors wherever eight values are left.  Of MI355X's 8 TB/s (a copy reaches 5.6, reading alone 6.9): swiglu with a checkpoint of
+// 16384 x 2 x 14336 bf16 303 us, 6.2 TB/s; its gradient from 8 bits 385 us, 6.1 TB/s; a checkpoint of 16384 x 4096 39 us, 5.3 TB/s; calls below 10 MB take 5 to 6 us, which is the
+// way through the call and not the memory.
 #include "rows.hpp"
 
 namespace fluxmi {
@@ -23,7 +28,6 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef u32x2 u32x2_any __attribute__((aligned(1)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // Largest magnitude that a code may stand for: 15/8 times the type's largest power of two, as a pattern of the type.
 template <Row T>
@@ -86,35 +90,42 @@ __device__ __forceinline__ u32x2 codes_of(const u32x4 v, uint32_t byte) {
 }
 
 // `count` of a vector's eight values, zeros behind them; all of them where count >= 8.
-template <Row T>
+template <Row T, bool NT>
 __device__ __forceinline__ u32x4 load_some(const uint8_t *p, int count) {
-  if (count >= 8) return load16(p);
+  if (count >= 8) return load16<NT>(p);
   u32x4 v = {0u, 0u, 0u, 0u};
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     if (i < count) v[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(p)[i]) << (16 * (i & 1));
   return v;
 }
+template <bool NT>
 __device__ __forceinline__ void store_some(uint8_t *p, const u32x4 v, int count) {
   if (count >= 8) {
-    store16(p, v);
+    store16<NT>(p, v);
     return;
   }
 #pragma unroll
   for (int i = 0; i < 7; ++i)
     if (i < count) reinterpret_cast<uint16_t *>(p)[i] = static_cast<uint16_t>(v[i / 2] >> (16 * (i & 1)));
 }
+template <bool NT>
 __device__ __forceinline__ u32x2 load_codes(const uint8_t *p, int count) {
-  if (count >= 8) return *reinterpret_cast<const u32x2_any *>(p);
+  if (count >= 8) {
+    if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const u32x2_any *>(p));
+    else return *reinterpret_cast<const u32x2_any *>(p);
+  }
   u32x2 v = {0u, 0u};
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     if (i < count) v[i / 4] |= static_cast<uint32_t>(p[i]) << (8 * (i & 3));
   return v;
 }
+template <bool NT>
 __device__ __forceinline__ void store_codes(uint8_t *p, const u32x2 c, int count) {
   if (count >= 8) {
-    *reinterpret_cast<u32x2_any *>(p) = c;
+    if constexpr (NT) __builtin_nontemporal_store(c, reinterpret_cast<u32x2_any *>(p));
+    else *reinterpret_cast<u32x2_any *>(p) = c;
     return;
   }
 #pragma unroll
@@ -167,7 +178,7 @@ __device__ __forceinline__ Place place_of(const RowsArgs &a) {
   return p;
 }
 
-template <Row T, bool GATED, bool KEEP>
+template <Row T, bool GATED, bool KEEP, int PASS>
 __global__ __launch_bounds__(kThreads) void checkpoint_kernel(const RowsArgs a) {
   const Place p = place_of(a);
   if (!p.any) return;  // (whole blocks of four lanes)
@@ -176,12 +187,12 @@ __global__ __launch_bounds__(kThreads) void checkpoint_kernel(const RowsArgs a) 
   const uint8_t *x = a.x + (p.row * halves * a.cols + p.col) * 2;
   u32x4 v[halves];
 #pragma unroll
-  for (int h = 0; h < halves; ++h) v[h] = count > 0 ? load_some<T>(x + static_cast<int64_t>(h) * a.cols * 2, count) : u32x4{0u, 0u, 0u, 0u};
+  for (int h = 0; h < halves; ++h) v[h] = count > 0 ? load_some<T, PASS == 2>(x + static_cast<int64_t>(h) * a.cols * 2, count) : u32x4{0u, 0u, 0u, 0u};
   if constexpr (KEEP) {
 #pragma unroll
     for (int h = 0; h < halves; ++h) {
       const uint32_t byte = scale_byte<T>(max_of_4_lanes(vector_max<T>(v[h])));
-      if (count > 0) store_codes(a.codes + (p.row * halves + h) * a.cols + p.col, codes_of<T>(v[h], byte), count);
+      if (count > 0) store_codes<PASS != 0>(a.codes + (p.row * halves + h) * a.cols + p.col, codes_of<T>(v[h], byte), count);
       if ((p.col & (kBlock - 1)) == 0) a.scale[(p.row * halves + h) * a.blocks + (p.col >> 5)] = static_cast<uint8_t>(byte);
     }
   }
@@ -192,12 +203,12 @@ __global__ __launch_bounds__(kThreads) void checkpoint_kernel(const RowsArgs a) 
     unpack<T>(v[1], u);
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] = g[i] * sigmoid(g[i]) * u[i];
-    store_some(a.out + (p.row * a.cols + p.col) * 2, pack<T>(o), count);
+    store_some<PASS != 0>(a.out + (p.row * a.cols + p.col) * 2, pack<T>(o), count);
   }
 }
 
 // KEPT: from codes and scales, otherwise from 16 bits.
-template <Row T, bool KEPT>
+template <Row T, bool KEPT, int PASS>
 __global__ __launch_bounds__(kThreads) void swiglu_backward_kernel(const RowsArgs a) {
   const Place p = place_of(a);
   const int count = a.cols - p.col;
@@ -205,16 +216,16 @@ __global__ __launch_bounds__(kThreads) void swiglu_backward_kernel(const RowsArg
   float g[8], u[8], d[8], dg[8], du[8], o[8];
   if constexpr (KEPT) {
     const uint8_t *c = a.x + p.row * 2 * a.cols + p.col, *s = a.in_scale + p.row * 2 * a.blocks + (p.col >> 5);
-    const u32x2 cg = load_codes(c, count), cu = load_codes(c + a.cols, count);
+    const u32x2 cg = load_codes<PASS == 2>(c, count), cu = load_codes<PASS == 2>(c + a.cols, count);
     values_of(cg, s[0], g);
     values_of(cu, s[a.blocks], u);
   } else {
     const uint8_t *x = a.x + (p.row * 2 * a.cols + p.col) * 2;
-    unpack<T>(load_some<T>(x, count), g);
-    unpack<T>(load_some<T>(x + static_cast<int64_t>(a.cols) * 2, count), u);
+    unpack<T>(load_some<T, PASS == 2>(x, count), g);
+    unpack<T>(load_some<T, PASS == 2>(x + static_cast<int64_t>(a.cols) * 2, count), u);
   }
   const int64_t at = (p.row * a.cols + p.col) * 2;
-  unpack<T>(load_some<T>(a.grad + at, count), d);
+  unpack<T>(load_some<T, PASS == 2>(a.grad + at, count), d);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float s = sigmoid(g[i]), silu = g[i] * s;
@@ -223,9 +234,9 @@ __global__ __launch_bounds__(kThreads) void swiglu_backward_kernel(const RowsArg
     dg[i] = d[i] * u[i] * s * (1.f + g[i] * (1.f - s));
   }
   uint8_t *gx = a.grad_x + (p.row * 2 * a.cols + p.col) * 2;
-  store_some(gx, pack<T>(dg), count);
-  store_some(gx + static_cast<int64_t>(a.cols) * 2, pack<T>(du), count);
-  if (a.out != nullptr) store_some(a.out + at, pack<T>(o), count);
+  store_some<PASS != 0>(gx, pack<T>(dg), count);
+  store_some<PASS != 0>(gx + static_cast<int64_t>(a.cols) * 2, pack<T>(du), count);
+  if (a.out != nullptr) store_some<PASS != 0>(a.out + at, pack<T>(o), count);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------
@@ -255,10 +266,19 @@ int plan_rows(const char *who, RowsArgs *a, uint32_t *grid) {
   return FLUXMI_OK;
 }
 
+// f(type, PASS): 0, or results pass the caches by (1), or inputs as well (2).  A call of `bytes` in all; us with 0 / 1 / 2: swiglu with a checkpoint 16384 x 14336 339 / 326 / 304, 16384 x 4096
+// 94 / 78 / 87, 20000 x 1407 41 / 42 / 60; its gradient from 8 bits 414 / 392 / 386, 115 / 98 / 108, 89 / 56 / 86.  Inputs of a few hundred MB are still cached where they
+// were just made, and rows that do not start on lines would be fetched twice.
 template <class F>
-void by_half(Row t, F &&f) {
-  if (t == Row::BF16) f(std::integral_constant<Row, Row::BF16>{});
-  else f(std::integral_constant<Row, Row::F16>{});
+void by_half(Row t, int64_t bytes, int32_t cols, F &&f) {
+  const int pass = bytes < (int64_t{96} << 20) ? 0 : (bytes < (int64_t{1} << 30) || cols % 64 != 0 ? 1 : 2);
+  auto with = [&](auto T) {
+    if (pass == 0) f(T, std::integral_constant<int, 0>{});
+    else if (pass == 1) f(T, std::integral_constant<int, 1>{});
+    else f(T, std::integral_constant<int, 2>{});
+  };
+  if (t == Row::BF16) with(std::integral_constant<Row, Row::BF16>{});
+  else with(std::integral_constant<Row, Row::F16>{});
 }
 
 }  // namespace
@@ -280,8 +300,8 @@ extern "C" int fluxmi_checkpoint_e4m3(const void *x, int32_t row_type, int64_t r
   a.x = static_cast<const uint8_t *>(x);
   a.codes = static_cast<uint8_t *>(codes);
   a.scale = static_cast<uint8_t *>(scale);
-  by_half(type, [&](auto T) {
-    checkpoint_kernel<decltype(T)::value, false, true><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+  by_half(type, rows * cols * 3, a.cols, [&](auto T, auto PASS) {
+    checkpoint_kernel<decltype(T)::value, false, true, decltype(PASS)::value><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
   });
   FLUXMI_HIP_CHECK(hipGetLastError());
   return FLUXMI_OK;
@@ -303,9 +323,9 @@ extern "C" int fluxmi_swiglu(const void *x, int32_t row_type, int64_t rows, int6
   a.out = static_cast<uint8_t *>(out);
   a.codes = static_cast<uint8_t *>(codes);
   a.scale = static_cast<uint8_t *>(scale);
-  by_half(type, [&](auto T) {
-    if (codes != nullptr) checkpoint_kernel<decltype(T)::value, true, true><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
-    else checkpoint_kernel<decltype(T)::value, true, false><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+  by_half(type, rows * cols * (codes != nullptr ? 8 : 6), a.cols, [&](auto T, auto PASS) {
+    if (codes != nullptr) checkpoint_kernel<decltype(T)::value, true, true, decltype(PASS)::value><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+    else checkpoint_kernel<decltype(T)::value, true, false, decltype(PASS)::value><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
   });
   FLUXMI_HIP_CHECK(hipGetLastError());
   return FLUXMI_OK;
@@ -329,9 +349,9 @@ extern "C" int fluxmi_swiglu_backward(const void *grad, const void *x, const voi
   a.in_scale = static_cast<const uint8_t *>(x_scale);
   a.grad_x = static_cast<uint8_t *>(grad_x);
   a.out = static_cast<uint8_t *>(out);
-  by_half(type, [&](auto T) {
-    if (x_scale != nullptr) swiglu_backward_kernel<decltype(T)::value, true><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
-    else swiglu_backward_kernel<decltype(T)::value, false><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+  by_half(type, rows * cols * (x_scale != nullptr ? 10 : 12), a.cols, [&](auto T, auto PASS) {
+    if (x_scale != nullptr) swiglu_backward_kernel<decltype(T)::value, true, decltype(PASS)::value><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+    else swiglu_backward_kernel<decltype(T)::value, false, decltype(PASS)::value><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
   });
   FLUXMI_HIP_CHECK(hipGetLastError());
   return FLUXMI_OK;
