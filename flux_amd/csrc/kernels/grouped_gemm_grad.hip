@@ -21,6 +21,9 @@ constexpr int kAlong = 80;      // 32 columns, and 16 bytes
 
 #if defined(__HIP_DEVICE_COMPILE__)
 
+typedef u32x4 u32x4_any __attribute__((aligned(1)));  // at any address: one instruction on this hardware
+typedef u32x2 u32x2_any __attribute__((aligned(1)));
+
 // `count` of eight elements of 16 bits, zeros behind them.  VEC: all eight or none, on 16 bytes.
 template <bool VEC>
 __device__ __forceinline__ u32x4 load8(const uint8_t *p, int count) {
@@ -28,8 +31,9 @@ __device__ __forceinline__ u32x4 load8(const uint8_t *p, int count) {
   if constexpr (VEC) {
     if (count > 0) v = *reinterpret_cast<const u32x4 *>(p);
   } else {
+    if (count >= 8) return *reinterpret_cast<const u32x4_any *>(p);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 7; ++i)
       if (i < count) v[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(p)[i]) << (16 * (i & 1));
   }
   return v;
@@ -42,9 +46,11 @@ __device__ __forceinline__ u32x4 load8_codes(const uint8_t *p, int count, const 
   u32x2 c = {0u, 0u};
   if constexpr (VEC) {
     c = *reinterpret_cast<const u32x2 *>(p);
+  } else if (count >= 8) {
+    c = *reinterpret_cast<const u32x2_any *>(p);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 7; ++i)
       if (i < count) c[i / 4] |= static_cast<uint32_t>(p[i]) << (8 * (i & 3));
   }
   const uint32_t byte = *scale;

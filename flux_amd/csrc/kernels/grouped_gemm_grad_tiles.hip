@@ -46,35 +46,48 @@ Divisor divisor(int64_t by) {
 }
 __device__ __forceinline__ int divide(int x, Divisor d) { return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(x)) * d.factor) >> d.shift); }
 
-struct TileArgs {
-  GradArgs a;             // a.parts: parts that a tile's sum may be cut into
-  int32_t grid;           // workgroups, a multiple of 8
-  int32_t turns;          // tiles that a workgroup computes at most
-  Divisor per_expert, per_group;  // an expert's tiles; those of eight along the result's rows
-  int32_t *queue;         // NULL: tiles are dealt in turns; otherwise workgroups fetch them: counters, then the experts by their rows
-};
-
 // Queues: eight of them, one to an XCD, a counter each (a line apart) of the tiles that were fetched from it beyond every workgroup's first; then the experts, those with most
 // rows first.
 constexpr int kQueueLine = 32, kQueueExperts = 8 * kQueueLine;
 constexpr size_t kQueueBytes = (kQueueExperts + kMaxExperts) * sizeof(int32_t);
 
-constexpr int kLeastSteps = 8;   // of a part
+// Every workgroup computes one tile in a turn.  Where the last turn's tiles are at most half as many as workgroups, their sums may be cut into parts, which a second
+// kernel joins: tiles [0, whole), then `parts` of each of `cut` tiles.  In 1/128 us, a step takes 64, and parts cost their way through memory (15 for a tile of 256 rows,
+// written and read) and the second kernel (512): the cheapest number of them is taken.  us, 8 experts, none / cut as here: input 14336 x 4096, 16384 rows 1564 / 1470, 74 rows 240 / 202.
 constexpr int kMostParts = 16;
-
-// Every workgroup computes one tile in a turn.  Where the last turn's tiles are at most half as many as workgroups, their sums are cut into parts, which a second
-// kernel joins: tiles [0, whole), then `parts` of each of `cut` tiles.
 struct Turns {
   int whole, cut, parts;
 };
-__host__ __device__ inline Turns turns_of(int tiles, int grid, int most_parts) {
-  const int whole = tiles / grid * grid, cut = tiles - whole;
-  if (cut == 0) return {whole, 0, 1};
-  int parts = grid / cut;
-  if (parts > most_parts) parts = most_parts;
-  if (parts < 2) return {tiles, 0, 1};
+struct Cutting {
+  int32_t steps, height;  // of a tile's sum, and its rows, on average
+};
+__host__ __device__ inline Turns turns_of(int tiles, int grid, Cutting c) {
+  const int whole = tiles / grid * grid, cut = tiles - whole, each = cut * (c.height * 15) / kTile;
+  int parts = 1, best = c.steps * 64 - 512;
+  auto consider = [&](auto P) {
+    constexpr int p = decltype(P)::value;
+    const int cost = c.steps * 64 / p + each * p;
+    if (cut * p <= grid && cost < best) best = cost, parts = p;
+  };
+  consider(std::integral_constant<int, 2>{});
+  consider(std::integral_constant<int, 3>{});
+  consider(std::integral_constant<int, 4>{});
+  consider(std::integral_constant<int, 6>{});
+  consider(std::integral_constant<int, 8>{});
+  consider(std::integral_constant<int, 12>{});
+  consider(std::integral_constant<int, kMostParts>{});
+  if (cut == 0 || parts == 1) return {tiles, 0, 1};
   return {whole, cut, parts};
 }
+
+struct TileArgs {
+  GradArgs a;
+  Cutting cutting;
+  int32_t grid;           // workgroups, a multiple of 8
+  int32_t turns;          // tiles that a workgroup computes at most
+  Divisor per_expert, per_group;  // an expert's tiles; those of eight along the result's rows
+  int32_t *queue;         // NULL: tiles are dealt in turns; otherwise workgroups fetch them: counters, then the experts by their rows
+};
 
 #if defined(__HIP_DEVICE_COMPILE__)
 
@@ -211,7 +224,7 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
   __syncthreads();
   const int expert_tiles = row_tiles;
   if constexpr (INPUT) row_tiles += (a.rows - all_rows + kTile - 1) / kTile;  // the rows that belong to no expert
-  const Turns turns = turns_of((INPUT ? row_tiles : a.nexperts * tiles_n) * tiles_k, args.grid, a.parts);
+  const Turns turns = turns_of((INPUT ? row_tiles : a.nexperts * tiles_n) * tiles_k, args.grid, args.cutting);
 
   // Tile number `item`.  An expert's (INPUT: all) tiles lie in groups of eight along the result's rows, walked column by column.
   auto describe = [&](int item, int part) {
@@ -724,7 +737,7 @@ __global__ __launch_bounds__(kThreads) void grad_tile_join_kernel(const TileArgs
     }
     row_tiles += (a.rows - all_rows + kTile - 1) / kTile;
   }
-  const Turns turns = turns_of(row_tiles * tiles_k, args.grid, a.parts);
+  const Turns turns = turns_of(row_tiles * tiles_k, args.grid, args.cutting);
   const int cut = blockIdx.x >> 4;
   if (cut >= turns.cut) return;
   const int item = turns.whole + cut, e = INPUT ? 0 : item / (tiles_n * tiles_k), local = INPUT ? item : item - e * tiles_n * tiles_k;
@@ -761,16 +774,16 @@ int64_t most_tiles(Grad g, int64_t nexperts, int64_t rows, int64_t n, int64_t k)
   return g == Grad::INPUT ? (rows / kTile + (rows < nexperts ? rows : nexperts) + 1) * tiles_k : nexperts * tiles_n * tiles_k;
 }
 
-// Parts that a sum may be cut into: kLeastSteps to each (of the weights' gradient on average).
-int most_parts(Grad g, int64_t nexperts, int64_t rows, int64_t n) {
-  const int64_t steps = (g == Grad::INPUT ? n : rows / (nexperts > 0 ? nexperts : 1)) / kStep, parts = steps / kLeastSteps;
-  return parts < 1 ? 1 : (parts > kMostParts ? kMostParts : static_cast<int>(parts));
+Cutting cutting_of(Grad g, int64_t nexperts, int64_t rows, int64_t n) {
+  const int64_t each = rows / (nexperts > 0 ? nexperts : 1), height = g == Grad::INPUT ? each : n;
+  const int64_t steps = (g == Grad::INPUT ? n : each) / kStep;
+  return {static_cast<int32_t>(steps < 1 << 20 ? steps : 1 << 20), static_cast<int32_t>(height < 16 ? 16 : (height > kTile ? kTile : height))};
 }
 
 // One workgroup to a compute unit: its tiles follow each other without a gap.
-int grid_of(int64_t tiles, int parts) {
+int grid_of(int64_t tiles) {
   const int cus = fluxmi_device_cu_count(), all = cus > 8 ? cus / 8 * 8 : 256;
-  const int64_t want = (tiles * parts + 7) / 8 * 8;
+  const int64_t want = (tiles * kMostParts + 7) / 8 * 8;
   return want < all ? static_cast<int>(want) : all;
 }
 
@@ -778,36 +791,42 @@ int grid_of(int64_t tiles, int parts) {
 
 bool grad_tiles_take(Grad g, const GradArgs &a) {
   const auto on16 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-  if (a.n % 8 != 0 || a.k % (g == Grad::WEIGHT_8BIT ? 16 : 8) != 0 || !on16(a.grad) || !on16(a.other) || !on16(a.out)) return false;
+  if (a.n == 0 || a.nexperts == 0 || a.n % 8 != 0 || a.k % (g == Grad::WEIGHT_8BIT ? 16 : 8) != 0 || !on16(a.grad) || !on16(a.other) || !on16(a.out)) return false;
   if (most_tiles(g, a.nexperts, a.rows, a.n, a.k) >= 1 << 24) return false;
   // Offsets: 256 rows of G along, 32 rows across, 256 rows of the result.
   return a.n < 1 << 22 && a.k < 1 << 22;
 }
 
-bool grad_tiles_are_faster(Grad, const GradArgs &) { return true; }
+// us, pieces of 128 x 128 / tiles.  Weights (experts, n x k, rows in all): 1, 1024 x 1024, 8192 41 / 55, 16384 62 / 59; 8, 512 x 512, 32768 41 / 52; 8, 1024 x 1024, 2048 15 / 15, 16384 56 / 51; 1, 1408 x 2048,
+// 2048 39 / 45, 8192 92 / 67; 32, 1024 x 1024, 4096 34 / 22.  Input: 1, 512 x 512, 8192 16 / 25, 32768 38 / 26; 8, 1024 x 1024, 2048 26 / 33, 16384 63 / 36; 8, 1408 x 2048, 2048 34 / 45, 8192 73 / 45;
+// 8, 2048 x 4096, 64 41 / 37; 8, 2048 x 128, 64 37 / 20; 32, 2048 x 4096, 64 123 / 96.
+bool grad_tiles_are_faster(Grad g, const GradArgs &a) {
+  const double weights = static_cast<double>(a.nexperts) * a.n * a.k, flops = 2.0 * a.rows * a.n * a.k;
+  if (g == Grad::INPUT) return flops >= 1.6e10 || weights >= 6e7 || a.n >= 2048;
+  return flops >= 2.4e10 || most_tiles(g, a.nexperts, a.rows, a.n, a.k) >= 64;
+}
 
 // Experts of different sizes in several turns: a workgroup fetches its next tile when it has done with one.  The result has the same bits: a tile's sum is the same wherever
 // it is computed.
 static bool by_queue(Grad g, int64_t nexperts, int64_t tiles, int grid) { return g != Grad::INPUT && nexperts > 1 && tiles >= 4 * static_cast<int64_t>(grid); }
 
 size_t grad_tiles_workspace_bytes(Grad g, int32_t nexperts, int64_t rows, int64_t n, int64_t k) {
-  const int parts = most_parts(g, nexperts, rows, n);
   const int64_t tiles = most_tiles(g, nexperts, rows, n, k);
-  if (tiles == 0) return 0;
-  const int grid = grid_of(tiles, parts);
+  if (tiles == 0 || tiles >= 1 << 24) return 0;
+  const int grid = grid_of(tiles);
   if (by_queue(g, nexperts, tiles, grid)) return kQueueBytes;
-  if (parts < 2) return 0;
-  if (g != Grad::INPUT && (tiles >= 1 << 24 || turns_of(static_cast<int>(tiles), grid, parts).cut == 0)) return 0;
+  const Cutting c = cutting_of(g, nexperts, rows, n);
+  // (the input's gradient has as many tiles as the row counts make, which are not known here: one may be all that is cut)
+  if (turns_of(g == Grad::INPUT ? 1 : static_cast<int>(tiles), grid, c).cut == 0) return 0;
   return static_cast<size_t>(grid) * kTile * kTile * sizeof(float);  // (a part to each workgroup at most)
 }
 
 int launch_grad_tiles(Grad g, bool f16, const GradArgs &args, void *stream) {
-  GradArgs a = args;
+  const GradArgs &a = args;
   const int64_t tiles_k = (a.k + kTile - 1) / kTile, tiles_n = (a.n + kTile - 1) / kTile, tiles = most_tiles(g, a.nexperts, a.rows, a.n, a.k);
-  a.parts = most_parts(g, a.nexperts, a.rows, a.n);
-  const int grid = grid_of(tiles, a.parts);
+  const int grid = grid_of(tiles);
   const bool queue = by_queue(g, a.nexperts, tiles, grid);
-  const TileArgs t{a, grid, static_cast<int32_t>(tiles / grid + 1), divisor(tiles_n * tiles_k), divisor(8 * tiles_k), queue ? reinterpret_cast<int32_t *>(a.partial) : nullptr};
+  const TileArgs t{a, cutting_of(g, a.nexperts, a.rows, a.n), grid, static_cast<int32_t>(tiles / grid + 1), divisor(tiles_n * tiles_k), divisor(8 * tiles_k), queue ? reinterpret_cast<int32_t *>(a.partial) : nullptr};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (queue) {
     grad_queue_kernel<<<1, kMaxExperts, 0, s>>>(a, t.queue);

@@ -1,5 +1,6 @@
 // Experts that learn: the gradients of the grouped product, activation checkpoints in 8 bits, and both joined to layers with autograd.  The reference has no
 // gradients of its MoE operators; moe_linear's forward pass is the product of GemmGroupedV3 (src/comm_none/ths_op/gemm_grouped_v3.cc:43-171).
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 
 #include "autograd_checks.h"
@@ -30,6 +31,7 @@ void check_like(const torch::Tensor &t, const char *name, const torch::Tensor &l
 }
 
 void check_splits(const torch::Tensor &splits, const torch::Tensor &like, int64_t experts) {
+  refuse_lazy_view(splits, "splits");
   FLUX_AMD_CHECK_NDIM(splits, 1);
   TORCH_CHECK(splits.scalar_type() == at::kInt, "splits must be int32, got ", splits.scalar_type());
   TORCH_CHECK(splits.is_contiguous(), "splits must be contiguous");
@@ -37,7 +39,8 @@ void check_splits(const torch::Tensor &splits, const torch::Tensor &like, int64_
   TORCH_CHECK(splits.is_cuda() ? splits.device() == like.device() : splits.device().is_cpu(), "splits must be on the host or on ", like.device());
 }
 
-// Counts on the host are copied in the stream's order; what they have past the rows does not exist for the kernels.
+// Counts on the host are copied in the stream's order (a replay of a captured call reads them again, so that they have to live as long as the graph); what they have past
+// the rows does not exist for the kernels.
 torch::Tensor on_device(const torch::Tensor &splits, const torch::Tensor &like) {
   return splits.is_cuda() ? splits : splits.to(like.device(), /*non_blocking=*/true);
 }
@@ -50,6 +53,8 @@ void check_weight(const torch::Tensor &weight, const char *name, const torch::Te
 
 // Codes [rows, cols] and scales [rows, halves * blocks] of a checkpoint.
 void check_kept(const torch::Tensor &codes, const torch::Tensor &scale, const torch::Tensor &like, int64_t halves) {
+  refuse_lazy_view(codes, "input");
+  refuse_lazy_view(scale, "input_scale");
   TORCH_CHECK(codes.is_cuda() && scale.is_cuda(), "input and input_scale must be device tensors");
   TORCH_CHECK(codes.scalar_type() == kCodes, "an input with a scale must be float8_e4m3fn, got ", codes.scalar_type());
   TORCH_CHECK(scale.scalar_type() == kScales, "input_scale must be float8_e8m0fnu, got ", scale.scalar_type());
@@ -290,10 +295,13 @@ torch::Tensor moe_wgrad(torch::Tensor grad, torch::Tensor input, torch::Tensor s
   if (output.has_value()) {
     out = *output;
     refuse_tangent(out, "output");
+    refuse_lazy_view(out, "output");
     FLUX_AMD_CHECK_INPUT(out, out_type);
     FLUX_AMD_CHECK_3D(out, splits.size(0), grad.size(1), input.size(1));
     TORCH_CHECK(out.device() == grad.device(), "output is on ", out.device(), ", grad is on ", grad.device());
     TORCH_CHECK(!at::GradMode::is_enabled() || !out.requires_grad(), "output requires a gradient: write it under no_grad()");
+    for (const torch::Tensor &t : {grad, input, splits, input_scale.value_or(splits)})
+      TORCH_CHECK(at::get_overlap_status(out, t) == at::MemOverlapStatus::No, "output lies in the memory of an operand");
   } else {
     out = empty_on(grad, {splits.size(0), grad.size(1), input.size(1)}, out_type);
   }

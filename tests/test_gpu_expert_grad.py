@@ -115,9 +115,11 @@ def test_wgrad(splits, rest, n, k, dtype, out, kept):
     assert torch.equal(total, got)
 
 
-# Sums of every length around the steps of the tiles, widths that end anywhere in them, and several tiles to a workgroup.
-TILES = [([s for s in range(0, 40)], 3, 264, 272), ([224, 255, 256, 257, 287, 288, 289, 320, 33], 1, 96, 48), ([1000, 31, 513], 0, 776, 528), ([640, 0, 2100], 40, 256, 256),
-         ([96, 500], 7, 2056, 2064)]
+# Sums of every length around the steps of the tiles, widths that end anywhere in them, one and several tiles to a workgroup, and few tiles with long sums, which are
+# cut.  The first of them are small for the weights' gradient (pieces of 128 x 128), and those with n below 2048 for the input's.
+TILES = [([224, 255, 256, 257, 287, 288, 289, 320, 33], 1, 96, 48), ([1000, 31, 513], 0, 776, 528), ([s for s in range(0, 40)], 3, 264, 272),
+         ([224, 255, 256, 257, 287, 288, 289, 320, 33, 0, 1] * 7, 1, 96, 48), ([40, 31, 70] * 14, 0, 776, 528), ([96, 500], 7, 2056, 2064), ([3000, 2001], 5, 1544, 1288),
+         ([640, 0, 700], 40, 2048, 264), ([5, 0, 40, 129, 1], 2, 2056, 136), ([300, 250, 0, 600], 0, 2072, 72), ([257, 1, 255], 9, 4104, 256), ([9, 9], 300, 2064, 512)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
@@ -550,6 +552,89 @@ def test_two_streams_at_once():
     assert all(torch.equal(g, want[i % 2]) for i, g in enumerate(got))
 
 
+# Weights' gradients whose tiles are fetched from queues, and both gradients with tiles that are cut: (rows, experts, n, k)
+WORKSPACES = [("wgrad", 2600, 64, 1024, 1024), ("wgrad", 5001, 2, 1544, 1288), ("dgrad", 90, 3, 4104, 264), ("dgrad", 700, 2, 4096, 520)]
+
+
+def workspace_call(kind, rows, experts, n, k, seed):
+    grad, other = data((rows, n), BF16, seed), data((rows, k) if kind == "wgrad" else (experts, n, k), BF16, seed + 1)
+    size = getattr(capi.load(), f"fluxmi_moe_{kind}_workspace_bytes")(experts, rows, n, k)
+    assert size > 0
+    call = flux_amd.moe_wgrad if kind == "wgrad" else flux_amd.moe_dgrad
+    return grad, lambda splits: call(grad, other, splits)
+
+
+def some_counts(rows, experts, seed):
+    g = torch.Generator().manual_seed(seed)
+    cuts = torch.randint(0, rows + 1, (experts,), generator=g).sort().values
+    return counts(torch.diff(cuts, prepend=torch.tensor([0])).tolist())
+
+
+@pytest.mark.parametrize("kind,rows,experts,n,k", WORKSPACES)
+def test_workspaces_on_two_streams_at_once(kind, rows, experts, n, k):
+    splits = some_counts(rows, experts, 1)
+    both = [workspace_call(kind, rows, experts, n, k, seed) for seed in (1, 3)]
+    want = [call(splits) for _, call in both]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(6):
+        for s, (_, call) in zip(streams, both):
+            with torch.cuda.stream(s):
+                got.append(call(splits))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i % 2]) for i, g in enumerate(got))
+
+
+@pytest.mark.parametrize("kind,rows,experts,n,k", WORKSPACES)
+def test_workspaces_in_two_graphs(kind, rows, experts, n, k):
+    """Two graphs out of one pool of memory, replayed in turn, with other operands and row counts and eager work between."""
+    splits = some_counts(rows, experts, 1)
+    both = [workspace_call(kind, rows, experts, n, k, seed) for seed in (1, 3)]
+    for _, call in both:
+        call(splits)
+    torch.cuda.synchronize()
+    graphs, pool = [], torch.cuda.graph_pool_handle()
+    for _, call in both:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            got = call(splits)
+        graphs.append((g, got))
+    for seed in (1, 5, 7):
+        splits.copy_(some_counts(rows, experts, seed))
+        for (grad, call), (g, got) in zip(both, graphs):
+            grad.copy_(data(grad.shape, BF16, 20 + seed))
+            want = call(splits)
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("pinned", [False, True])
+def test_graph_with_row_counts_on_the_host(pinned):
+    """A replay reads the counts again from the tensor that the captured call was given."""
+    x, w = data((40, 64), BF16, 1), data((4, 72, 64), BF16, 2)
+    splits = torch.tensor([10, 0, 25, 5], dtype=torch.int32)
+    splits = splits.pin_memory() if pinned else splits
+
+    def run(splits):
+        y = flux_amd.moe_linear(x, w, splits)
+        return y, flux_amd.moe_dgrad(y, w, splits), flux_amd.moe_wgrad(y, x, splits)
+
+    run(splits)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = run(splits)
+    for new in ([10, 0, 25, 5], [1, 2, 3, 4], [40, 0, 0, 0], [0, 0, 0, 0]):
+        want = run(counts(new))
+        splits.copy_(torch.tensor(new, dtype=torch.int32))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 @pytest.mark.parametrize("ckpt", [False, True])
 def test_graph_of_a_training_step_replays(ckpt):
     """Forward and backward in two graphs, with eager work between the replays and other row counts each time; weights' gradients in parts among it."""
@@ -621,6 +706,7 @@ def test_captured_backward_pass():
 def test_refusals():
     x, w, splits = data((10, 64), BF16, 1), data((2, 32, 64), BF16, 2), counts([4, 6])
     codes, scale = flux_amd.moe_checkpoint(x)
+    both = torch.zeros(200, 64, dtype=BF16, device=DEV)
     bad = [
         (lambda: flux_amd.moe_linear(x.float(), w, splits), "bfloat16 or float16"),
         (lambda: flux_amd.moe_linear(x, w.half(), splits), "weight is Half"),
@@ -641,6 +727,8 @@ def test_refusals():
         (lambda: flux_amd.moe_wgrad(x, x, splits, output=torch.zeros(2, 64, 64, device=DEV), output_dtype=BF16), "output is"),
         (lambda: flux_amd.moe_wgrad(x, x, splits, output=torch.zeros(2, 64, 64, device=DEV, requires_grad=True)), "no_grad"),
         (lambda: flux_amd.moe_wgrad(x, x, splits, output=torch.zeros(2 * 64 * 64 + 1, device=DEV)[1:].view(2, 64, 64)), "aligned"),
+        (lambda: flux_amd.moe_wgrad(both[:10], x, splits, output=both[9:].view(-1)[:2 * 64 * 64].view(2, 64, 64)), "memory of an operand"),
+        (lambda: flux_amd.moe_wgrad(x, codes, splits, scale, output=torch.zeros(2, 64, 64, device=DEV)._neg_view()), "negative view"),
         (lambda: flux_amd.moe_swiglu(x[:, :63].contiguous()), "gate and up"),
         (lambda: flux_amd.moe_swiglu_backward(x, x), "shape mismatch"),
         (lambda: flux_amd.moe_swiglu_backward(x[:, :32].contiguous(), codes, scale[:, :1].contiguous()), "shape mismatch"),
