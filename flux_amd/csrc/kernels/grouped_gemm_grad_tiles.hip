@@ -294,6 +294,7 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
   // Codes: four rows, lane l chunk l % 16 (of 16 columns) of row l / 16; scales: the eight rows whose codes this wave fetches, a word to each byte.
   constexpr int kColFills = EIGHT ? 3 : 4, kFills = kColFills + 4;
   uint32_t coff[4], roff[4];
+  constexpr uint32_t kNowhere = 0xfffffff0u;  // past every buffer's end: rows and columns that the tile does not have are not fetched
   // The step that is requested next: where it begins, and how much of the sum (INPUT: of the tile's rows of G, in bytes) is left there.
   const uint8_t *rnext = nullptr, *cnext = nullptr, *snext = nullptr;
   int left = 0, rbytes = 0;
@@ -322,16 +323,16 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
       const int col = (((lane & 31) >> 1) ^ f) * 16 + (lane & 1) * 8;
       if constexpr (EIGHT) {
         const int c = (lane & 15) * 16, b = lane & 7;
-        if (i < 2) coff[i] = static_cast<uint32_t>((wave * 8 + i * 4 + (lane >> 4)) * cpitch) + t.col0 + (c < t.cols ? c : 0);
+        if (i < 2) coff[i] = c < t.cols ? static_cast<uint32_t>((wave * 8 + i * 4 + (lane >> 4)) * cpitch) + t.col0 + c : kNowhere;
         else if (i == 2) coff[i] = static_cast<uint32_t>((wave * 8 + (lane >> 3)) * blocks) + t.col0 / 32 + (b * 32 < t.cols ? b : 0);
       } else {
-        coff[i] = static_cast<uint32_t>(row * cpitch) + (t.col0 + (col < t.cols ? col : 0)) * 2u;
+        coff[i] = col < t.cols ? static_cast<uint32_t>(row * cpitch) + (t.col0 + col) * 2u : kNowhere;
       }
       if constexpr (INPUT) {
         const int r = wave * 64 + i * 16 + (lane >> 2), c = (lane & 3) ^ ((r >> 1) & 3);
-        roff[i] = static_cast<uint32_t>((r < t.rows ? r : t.rows - 1) * rpitch) + c * 16u;
+        roff[i] = r < t.rows ? static_cast<uint32_t>(r * rpitch) + c * 16u : kNowhere;
       } else {
-        roff[i] = static_cast<uint32_t>(row * rpitch) + (t.row0 + (col < t.rows ? col : 0)) * 2u;
+        roff[i] = col < t.rows ? static_cast<uint32_t>(row * rpitch) + (t.row0 + col) * 2u : kNowhere;
       }
     }
   };
