@@ -463,10 +463,12 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
 
   // What a step waits for: the next one's rows and columns; WEIGHT_8BIT: that one's rows and the codes of the one after it.
   constexpr int kOpen = EIGHT ? kFills + 4 : 2 * kFills;
-  // Loads and stores leave the counter in their order.  A tile's first fills are requested before the stores of the tile before it, so that the first kFresh steps
-  // need not wait for those: kStores of them for 16 bits; those of 32 bits are more than the counter holds, which has then seen all fills in.
-  constexpr int kFresh = EIGHT ? 2 : 3, kStores = 32;
-  int behind = 0;  // stores behind the first fills: 0 none, 1 kStores, 2 as many as the counter holds
+  // Loads and stores leave the counter in their order, also when the loads go to LDS from cold memory and a single store to the caches comes after them (measured: 3 G
+  // words behind 1 to 96 stores, none missing).  A tile's first fills are requested before the stores of the tile before it, so that the first kFresh steps need not wait
+  // for those: kStores of them for 16 bits; twice as many for 32 bits, which with the fills are more than the counter holds: all fills are in before the first step.
+  constexpr int kFresh = EIGHT ? 2 : 3, kStores = 32, kMostCounted = 62;
+  static_assert(kOpen + kFills + kStores <= kMostCounted && 2 * kStores >= kMostCounted, "waits that the counter holds");
+  int behind = 0;  // stores behind the first fills, times kStores
   auto wait_step = [&](auto U, int s) {
     bool waited = false;
     if constexpr (decltype(U)::value < kFresh) {
@@ -543,6 +545,7 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
     if constexpr (EIGHT) {
       if (behind == 0) FLUXMI_VMCNT(2 * kFills);
       else if (behind == 1) FLUXMI_VMCNT(2 * kFills + kStores);
+      else FLUXMI_VMCNT(kMostCounted);
       if (rest < kStep && steps <= 2) clear_columns(steps - 1), FLUXMI_LGKM0();
       static_for<2>([&](auto S) {
 #pragma unroll
@@ -557,6 +560,7 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
     } else {
       if (behind == 0) FLUXMI_VMCNT(3 * kFills);
       else if (behind == 1) FLUXMI_VMCNT(3 * kFills + kStores);
+      else FLUXMI_VMCNT(kMostCounted);
       if (rest < kStep && steps == 1) clear_columns(0);
     }
     if (rest < kStep && steps == 1) clear_rows(0);
