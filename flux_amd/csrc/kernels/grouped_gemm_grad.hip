@@ -8,6 +8,10 @@
 // What is summed over lies across the rows of W, X and, for the weights, G: a lane of the MFMA needs eight values of one column, from eight rows.  The
 // rows go to LDS as they lie in memory and come back through the transposing LDS read: 16 lanes together read four rows of 16 columns, and each of
 // them gets the four values of one column.
+//
+// Here: pieces of 128 x 128 on four waves, one step in LDS and the next in registers, for operands of any width and start and for small products; the weights' sums are cut into parts
+// of 256 rows or more where pieces are few, so that the card is full.  Latency and barriers bound them: 8 experts 1024 x 1024, 2048 rows 15 us (weights), 26 (input); at the large
+// sizes of grouped_gemm_grad_tiles.hip, which computes what is larger, they take 2360 and 2460 where its tiles take 1430 and 1470.
 #include "grouped_gemm_grad_tiles.hpp"
 
 namespace fluxmi {
@@ -303,7 +307,7 @@ extern "C" int fluxmi_moe_dgrad(const void *grad, const void *weight, int32_t ro
   const size_t need = fluxmi_moe_dgrad_workspace_bytes(nexperts, rows, n, k);
   FLUXMI_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && on(workspace, 16)), FLUXMI_ERR_WORKSPACE,
                  "moe_dgrad: workspace of %zu bytes, 16-byte aligned, expected, got %zu", need, workspace_bytes);
-  if (grad_tiles_take(Grad::INPUT, a) && grad_tiles_are_faster(Grad::INPUT, a)) return launch_grad_tiles(Grad::INPUT, row_type == FLUXMI_ROWS_FP16, a, stream);
+  if (grad_tiles_take(Grad::INPUT, a) && grad_tiles_are_faster(Grad::INPUT, nexperts, rows, n, k)) return launch_grad_tiles(Grad::INPUT, row_type == FLUXMI_ROWS_FP16, a, stream);
   // Every expert and the rows of none end with a tile that may be partial.
   const int64_t row_tiles = rows / kPiece + (rows < nexperts ? rows : nexperts) + 1, items = row_tiles * tiles_of(k);
   FLUXMI_REQUIRE(items <= kMostItems, FLUXMI_ERR_UNSUPPORTED, "moe_dgrad: too many rows and columns for one launch");
@@ -344,7 +348,7 @@ extern "C" int fluxmi_moe_wgrad(const void *grad, const void *input, const void 
   a.accumulate = accumulate != 0;
   a.parts = parts_of(nexperts, rows, n, k);
   const Grad kind = input_scale != nullptr ? Grad::WEIGHT_8BIT : Grad::WEIGHT;
-  const bool tiles = grad_tiles_take(kind, a) && grad_tiles_are_faster(kind, a);
+  const bool tiles = grad_tiles_take(kind, a) && grad_tiles_are_faster(kind, nexperts, rows, n, k);
   const int64_t pieces = nexperts * tiles_of(n) * tiles_of(k), items = pieces * a.parts;
   FLUXMI_REQUIRE(tiles || items <= kMostItems, FLUXMI_ERR_UNSUPPORTED, "moe_wgrad: too many experts, rows and columns for one launch");
   const size_t need = fluxmi_moe_wgrad_workspace_bytes(nexperts, rows, n, k);

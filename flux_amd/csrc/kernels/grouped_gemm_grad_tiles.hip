@@ -7,8 +7,20 @@
 //    X, and G for the weights' gradient) lies in rows of 256 columns, 512 bytes; 16 columns of a row (32 bytes) are at place s ^ f(row), f = row % 4 + 4 (row / 8 % 2), so
 //    that the eight rows which half a wave reads together are on different banks.  G for the input's gradient lies in rows of 32 values, 64 bytes.
 //  * A fragment of an "across" operand comes back through the transposing read, twice four rows of 16 columns.
-//  * A step that is not whole is fetched as far as the sum goes, and the rest of it is cleared in LDS; rows and columns past the end of the result are others'
-//    values, which reach no result that is stored.
+//  * A step that is not whole is fetched as far as the sum goes, and the rest of it is cleared in LDS; rows and columns past the end of the result are not fetched: what
+//    LDS held there reaches no result that is stored.
+//  * A checkpoint's codes and scale bytes (WEIGHT_8BIT) are fetched like the rest, and each wave turns what it fetched to values of 16 bits two steps ahead, in LDS, beside the
+//    MFMAs; the values are exact in the rows' type.
+//  * One workgroup to a compute unit computes several tiles, in turns or (weights, experts of different sizes) from a queue to each XCD.  The next tile's first four steps are
+//    requested before a tile's results go out, through a window in LDS and in whole lines.  The last turn's tiles are cut along the sum where that is cheaper, and joined in
+//    the parts' order: results have the same bits in every launch.
+//
+// What bounds it on MI355X (us): large products the board's power, 8 experts 14336 x 4096, 16384 rows: input 1470, weights 1430, 1.31 to 1.34 PFLOP/s, MFMA 70 to 79 % busy at 1.5 to 1.9 GHz
+// (zero operands reach 1.75 PFLOP/s).  Many small experts what lies between two tiles' sums, about 6 to each of 25 to 45: 64 experts, 93000 rows, input 1408 x 2048 525, weights
+// 1400 x 2040 to fp32 630 (1408 x 2048, whose rows begin on lines, 560).  Weights from 8 bits, 32 experts 2048 x 7168 to fp32, 32768 rows: 1050, the conversion a tenth of it.  Few rows
+// the read of W: 74 rows on 8 experts 14336 x 4096 166, 5.7 TB/s.
+// Also built: without the window 1594 for weights (neighbouring lanes store to different rows); row blocks left out one by one in tiles of any height + 7 to 10 %; small and large
+// experts in turn from the queues 668 where the largest come first 631.
 #include "grouped_gemm_grad_tiles.hpp"
 
 #include <type_traits>
@@ -805,10 +817,10 @@ bool grad_tiles_take(Grad g, const GradArgs &a) {
 // us, pieces of 128 x 128 / tiles.  Weights (experts, n x k, rows in all): 1, 1024 x 1024, 8192 41 / 55, 16384 62 / 59; 8, 512 x 512, 32768 41 / 52; 8, 1024 x 1024, 2048 15 / 15, 16384 56 / 51; 1, 1408 x 2048,
 // 2048 39 / 45, 8192 92 / 67; 32, 1024 x 1024, 4096 34 / 22.  Input: 1, 512 x 512, 8192 16 / 25, 32768 38 / 26; 8, 1024 x 1024, 2048 26 / 33, 16384 63 / 36; 8, 1408 x 2048, 2048 34 / 45, 8192 73 / 45;
 // 8, 2048 x 4096, 64 41 / 37; 8, 2048 x 128, 64 37 / 20; 32, 2048 x 4096, 64 123 / 96.
-bool grad_tiles_are_faster(Grad g, const GradArgs &a) {
-  const double weights = static_cast<double>(a.nexperts) * a.n * a.k, flops = 2.0 * a.rows * a.n * a.k;
-  if (g == Grad::INPUT) return flops >= 1.6e10 || weights >= 6e7 || a.n >= 2048;
-  return flops >= 2.4e10 || most_tiles(g, a.nexperts, a.rows, a.n, a.k) >= 64;
+bool grad_tiles_are_faster(Grad g, int32_t nexperts, int64_t rows, int64_t n, int64_t k) {
+  const double weights = static_cast<double>(nexperts) * n * k, flops = 2.0 * rows * n * k;
+  if (g == Grad::INPUT) return flops >= 1.6e10 || weights >= 6e7 || n >= 2048;
+  return flops >= 2.4e10 || most_tiles(g, nexperts, rows, n, k) >= 64;
 }
 
 // Experts of different sizes in several turns: a workgroup fetches its next tile when it has done with one.  The result has the same bits: a tile's sum is the same wherever
@@ -817,7 +829,7 @@ static bool by_queue(Grad g, int64_t nexperts, int64_t tiles, int grid) { return
 
 size_t grad_tiles_workspace_bytes(Grad g, int32_t nexperts, int64_t rows, int64_t n, int64_t k) {
   const int64_t tiles = most_tiles(g, nexperts, rows, n, k);
-  if (tiles == 0 || tiles >= 1 << 24) return 0;
+  if (tiles == 0 || tiles >= 1 << 24 || !grad_tiles_are_faster(g, nexperts, rows, n, k)) return 0;
   const int grid = grid_of(tiles);
   if (by_queue(g, nexperts, tiles, grid)) return kQueueBytes;
   const Cutting c = cutting_of(g, nexperts, rows, n);

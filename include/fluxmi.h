@@ -482,7 +482,7 @@ int fluxmi_grouped_gemm_mx_launch_info(const fluxmi_mx_gemm_args *args, fluxmi_m
  * `splits`: DEVICE int32 row counts.  Negative ones are 0; what they have past `rows` does not exist.  Rows past the sum are not read by fluxmi_moe_wgrad.
  * Requirements: nexperts <= 1024; rows, n, k <= 2^24; operands aligned to their elements, grad_input to 8 bytes, grad_weight and workspace to 16.  Operands
  * that start on 16 bytes with n and k multiples of 8 are fast.
- * `workspace`: fluxmi_moe_dgrad_workspace_bytes() or fluxmi_moe_wgrad_workspace_bytes() bytes (0 for many sizes, 64 MiB for most others) of any content; not shared by calls that may overlap.
+ * `workspace`: fluxmi_moe_dgrad_workspace_bytes() or fluxmi_moe_wgrad_workspace_bytes() bytes (at most 64 MiB; 0 for many sizes) of any content; not shared by calls that may overlap.
  * ---------------------------------------------------------------------------------------------- */
 int fluxmi_moe_dgrad(const void *grad, const void *weight, int32_t row_type, const int32_t *splits, int32_t nexperts, int64_t rows, int64_t n,
                      int64_t k, void *grad_input, void *workspace, size_t workspace_bytes, void *stream);
