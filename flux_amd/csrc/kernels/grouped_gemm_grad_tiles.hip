@@ -16,8 +16,8 @@
 //    the parts' order: results have the same bits in every launch.
 //
 // What bounds it on MI355X (us): large products the board's power, 8 experts 14336 x 4096, 16384 rows: input 1470, weights 1430, 1.31 to 1.34 PFLOP/s, MFMA 70 to 79 % busy at 1.5 to 1.9 GHz
-// (zero operands reach 1.75 PFLOP/s).  Many small experts what lies between two tiles' sums, about 6 to each of 25 to 45: 64 experts, 93000 rows, input 1408 x 2048 525, weights
-// 1400 x 2040 to fp32 630 (1408 x 2048, whose rows begin on lines, 560).  Weights from 8 bits, 32 experts 2048 x 7168 to fp32, 32768 rows: 1050, the conversion a tenth of it.  Few rows
+// (zero operands reach 1.75 PFLOP/s).  Many small experts what lies between two tiles' sums, about 7 to each of 25 to 45: 64 skewed experts, 93000 rows, input 1408 x 2048 530, weights
+// 1400 x 2040 to fp32 607 (1408 x 2048, whose rows begin on lines, 560).  Weights from 8 bits, 32 experts 2048 x 7168 to fp32, 32768 rows: 1050, the conversion a tenth of it.  Few rows
 // the read of W: 74 rows on 8 experts 14336 x 4096 166, 5.7 TB/s.
 // Also built: without the window 1594 for weights (neighbouring lanes store to different rows); row blocks left out one by one in tiles of any height + 7 to 10 %; small and large
 // experts in turn from the queues 668 where the largest come first 631.
