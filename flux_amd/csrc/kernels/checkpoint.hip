@@ -231,7 +231,7 @@ __global__ __launch_bounds__(kThreads) void swiglu_backward_kernel(const RowsArg
     const float s = sigmoid(g[i]), silu = g[i] * s;
     o[i] = silu * u[i];
     du[i] = d[i] * silu;
-    dg[i] = d[i] * u[i] * s * (1.f + g[i] * (1.f - s));
+    dg[i] = d[i] * (s * (1.f + g[i] * (1.f - s))) * u[i];  // (d u may be beyond fp32 where s is 0)
   }
   uint8_t *gx = a.grad_x + (p.row * 2 * a.cols + p.col) * 2;
   store_some<PASS != 0>(gx, pack<T>(dg), count);

@@ -35,6 +35,7 @@ void check_splits(const torch::Tensor &splits, const torch::Tensor &like, int64_
   FLUX_AMD_CHECK_NDIM(splits, 1);
   TORCH_CHECK(splits.scalar_type() == at::kInt, "splits must be int32, got ", splits.scalar_type());
   TORCH_CHECK(splits.is_contiguous(), "splits must be contiguous");
+  TORCH_CHECK(splits.size(0) <= 1024, "at most 1024 experts, got ", splits.size(0));
   TORCH_CHECK(experts < 0 || splits.size(0) == experts, "splits 0-dim mismatch: ", splits.size(0), " != ", experts);
   TORCH_CHECK(splits.is_cuda() ? splits.device() == like.device() : splits.device().is_cpu(), "splits must be on the host or on ", like.device());
 }
@@ -68,6 +69,9 @@ void check_kept(const torch::Tensor &codes, const torch::Tensor &scale, const to
 // ---- the calls ------------------------------------------------------------------------------------------------
 
 torch::Tensor product(const torch::Tensor &input, const torch::Tensor &weight, const torch::Tensor &splits) {
+  constexpr int64_t kMost = 1 << 24;  // the gradients' limits
+  TORCH_CHECK(input.size(0) <= kMost && weight.size(1) <= kMost && weight.size(2) <= kMost, "at most 2^24 rows and weights of 2^24 x 2^24, got ", input.size(0), " rows, ",
+              weight.size(1), " x ", weight.size(2));
   const c10::DeviceGuard guard(input.device());
   torch::Tensor out = empty_on(input, {input.size(0), weight.size(1)}, input.scalar_type());
   if (out.numel() == 0) return out;

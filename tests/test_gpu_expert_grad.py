@@ -128,6 +128,7 @@ def test_tiles(splits, rest, n, k, dtype):
     print(f"[case] tiles {splits[:6]} {rest} {n} {k} {dtype}", flush=True)
     rows = sum(splits) + rest
     grad, x, weight = data((rows, n), dtype, 3), data((rows, k), dtype, 4), data((len(splits), n, k), dtype, 5)
+    grad[rows - rest:] = x[rows - rest:] = float("nan")  # rows of no expert are not used
     close(flux_amd.moe_dgrad(grad, weight, counts(splits)), want_dgrad(grad, weight, splits), n * 2.0**-23 * want_dgrad(grad.abs(), weight.abs(), splits))
     codes, scale = flux_amd.moe_checkpoint(x)
     for given, its_scale, x64 in ((x, None, x.double()), (codes, scale, values(codes, scale))):
@@ -209,6 +210,29 @@ def test_infinities_stay_in_their_rows_and_experts():
     codes, scale = flux_amd.moe_checkpoint(x)  # a block of them is NaN
     dw = flux_amd.moe_wgrad(torch.ones_like(grad), codes, counts(splits), scale)
     assert torch.isnan(dw[1, :, :32]).all() and torch.isfinite(dw[0]).all() and torch.isfinite(dw[1, :, 32:]).all()
+
+
+def test_infinities_in_the_steps_of_tiles():
+    """The same by tiles: steps of which the next expert's rows and W's are no part, rows and columns that a tile does not have."""
+    splits, n, k = [40, 33, 0, 70] * 8, 2056, 264
+    grad, w = data((sum(splits) + 3, n), BF16, 1), data((len(splits), n, k), BF16, 2)
+    grad[40], w[3, 5, 6], grad[-3:] = float("inf"), float("-inf"), float("nan")
+    bad = ~torch.isfinite(flux_amd.moe_dgrad(grad, w, counts(splits)))
+    assert bad[40].all() and bad[73:143, 6].all()
+    bad[40] = bad[73:143, 6] = False
+    assert not bad.any()
+    n, k = 1032, 528
+    grad, x = data((sum(splits) + 3, n), BF16, 3), data((sum(splits) + 3, k), BF16, 4)
+    grad[40, 1031], x[72, 527], grad[-3:], x[-3:] = float("inf"), float("nan"), float("nan"), float("inf")
+    bad = ~torch.isfinite(flux_amd.moe_wgrad(grad, x, counts(splits)))
+    assert bad[1, 1031].all() and bad[1, :, 527].all()
+    bad[1, 1031] = bad[1, :, 527] = False
+    assert not bad.any()
+    codes, scale = flux_amd.moe_checkpoint(x)
+    bad = ~torch.isfinite(flux_amd.moe_wgrad(grad, codes, counts(splits), scale))
+    assert bad[1, 1031].all() and bad[1, :, 512:].all()
+    bad[1, 1031] = bad[1, :, 512:] = False
+    assert not bad.any()
 
 
 def test_offsets_past_32_bits():
@@ -327,6 +351,13 @@ def test_swiglu_backward(rows, cols, dtype, kept):
     want, slack, want_out, out_slack = want_swiglu_backward(grad.double(), g, u)
     close(grad_input, want, slack)
     close(out, want_out, out_slack)
+
+
+def test_gradient_of_a_closed_gate():
+    """The gate's slope is 0 before the product of gradient and value, which alone is beyond fp32."""
+    gated = torch.tensor([[-200.0] * 8 + [1e30] * 8], dtype=BF16, device=DEV)
+    grad_input, out = flux_amd.moe_swiglu_backward(torch.full((1, 8), 1e30, dtype=BF16, device=DEV), gated)
+    assert not grad_input[:, :8].any() and not grad_input[:, 8:].any() and not out.any()
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
@@ -735,6 +766,8 @@ def test_refusals():
         (lambda: flux_amd.moe_mlp(x, w, data((2, 64, 15), BF16, 3), splits), "gate and up"),
         (lambda: flux_amd.moe_mlp(x, w, data((3, 64, 16), BF16, 3), splits), "experts"),
         (lambda: flux_amd.moe_checkpoint(x.view(-1)), "2 dimensions"),
+        (lambda: flux_amd.moe_linear(x, torch.zeros(1025, 8, 64, dtype=BF16, device=DEV), counts([0] * 1025)), "1024 experts"),
+        (lambda: flux_amd.moe_linear(torch.empty((1 << 24) + 1, 8, dtype=BF16, device=DEV), torch.zeros(1, 8, 8, dtype=BF16, device=DEV), counts([1])), "2\\^24 rows"),
     ]
     for call, text in bad:
         with pytest.raises(RuntimeError, match=text):
@@ -747,6 +780,10 @@ def test_empty_sizes():
     assert flux_amd.moe_linear(x, w, splits).shape == (0, 32) and flux_amd.moe_dgrad(data((0, 32), BF16, 1), w, splits).shape == (0, 64)
     dw = flux_amd.moe_wgrad(data((0, 32), BF16, 1), x, splits)
     assert dw.shape == (2, 32, 64) and not dw.any()
+    for kept in (None, torch.empty(0, 33, dtype=torch.float8_e8m0fnu, device=DEV)):  # the same by tiles
+        dw = flux_amd.moe_wgrad(data((0, 1032), BF16, 1), data((0, 1040), BF16, 1) if kept is None else torch.empty(0, 1040, dtype=torch.float8_e4m3fn, device=DEV), counts([0] * 8), kept)
+        assert dw.shape == (8, 1032, 1040) and not dw.any()
+    assert not flux_amd.moe_dgrad(data((300, 2056), BF16, 1), data((2, 2056, 64), BF16, 2), splits).any()
     assert flux_amd.moe_checkpoint(x)[1].shape == (0, 2) and flux_amd.moe_swiglu(x).shape == (0, 32)
     x, w1, w2 = mlp_operands([0, 0], 0, 64, 32, BF16)
     flux_amd.moe_mlp(x, w1, w2, splits).sum().backward()
