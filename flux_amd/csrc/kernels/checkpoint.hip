@@ -226,12 +226,22 @@ __global__ __launch_bounds__(kThreads) void swiglu_backward_kernel(const RowsArg
   }
   const int64_t at = (p.row * a.cols + p.col) * 2;
   unpack<T>(load_some<T, PASS == 2>(a.grad + at, count), d);
+  // Gradient times value comes first: times the slope of a gate that closes, a small gradient would be below fp32.  Only where gradient times value is beyond fp32 the slope
+  // comes in between: there the gradient is over 1, and its product with a slope is in range.
+  float slope[8], most = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float s = sigmoid(g[i]), silu = g[i] * s;
+    const float s = sigmoid(g[i]), silu = g[i] * s, ud = d[i] * u[i];
     o[i] = silu * u[i];
     du[i] = d[i] * silu;
-    dg[i] = d[i] * (s * (1.f + g[i] * (1.f - s))) * u[i];  // (d u may be beyond fp32 where s is 0)
+    slope[i] = s * (1.f + g[i] * (1.f - s));
+    dg[i] = ud * slope[i];
+    most = fmaxf(most, fabsf(ud));
+  }
+  if (most == INFINITY) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (fabsf(d[i] * u[i]) == INFINITY) dg[i] = d[i] * slope[i] * u[i];
   }
   uint8_t *gx = a.grad_x + (p.row * 2 * a.cols + p.col) * 2;
   store_some<PASS != 0>(gx, pack<T>(dg), count);
