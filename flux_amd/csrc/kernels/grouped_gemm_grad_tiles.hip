@@ -163,11 +163,37 @@ __device__ __forceinline__ f32x4 sums_of(const f32x4 &acc) {
   return v;
 }
 
-// Sixteen bytes (BYTE: one, to a word) of each lane to LDS, from M0 on.  Not the builtin: with it the compiler lets every LDS read wait for all loads.
-template <bool BYTE>
-__device__ __forceinline__ void load_to_lds(uint32_t off, __amdgpu_buffer_rsrc_t rsrc) {
-  if constexpr (BYTE) asm volatile("buffer_load_ubyte %0, %1, 0 offen lds" : : "v"(off), "s"(rsrc) : "memory");
-  else asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(off), "s"(rsrc) : "memory");
+// Sixteen bytes (BYTE: one, to a word) of each lane to LDS, from base + AT on.  Not the builtin: with it the compiler lets every LDS read wait for all loads.  The load comes five wait
+// states after the statement's start: what a scalar register needs that a vector instruction wrote (v_readlane, with which the compiler brings back spilled ones: words of the buffer
+// among them), and it does not look into asm for that.
+template <bool BYTE, int AT>
+__device__ __forceinline__ void load_to_lds(uint32_t base, uint32_t off, __amdgpu_buffer_rsrc_t rsrc) {
+  if constexpr (BYTE) asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 3\n\tbuffer_load_ubyte %2, %3, 0 offen lds" : : "s"(base), "i"(AT), "v"(off), "s"(rsrc) : "memory", "scc");
+  else asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 3\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds" : : "s"(base), "i"(AT), "v"(off), "s"(rsrc) : "memory", "scc");
+}
+// The same behind two MFMAs, beside which the wait states cost little.  us, MFMA and load as statements without a wait / this / MFMA and load apart, the load with its wait: weights
+// 14336 x 4096, 16384 rows 1432 / 1435 / 1455 to 1480; 2048 x 7168 from 8 bits, 32768 rows 1046 / 1059 / 1063; input 1466 / 1467 / 1476 to 1488.
+template <bool F16, bool FIRST, bool BYTE, int AT>
+__device__ __forceinline__ void mfma_and_load(f32x4 &acc0, f32x4 &acc1, const u32x4 &c0, const u32x4 &c1, const u32x4 &r, uint32_t base, uint32_t off, __amdgpu_buffer_rsrc_t rsrc) {
+#define FLUXMI_MFMA_AND_LOAD(MFMA, D, LOAD)                                                                                                         \
+  asm volatile("s_add_u32 m0, %5, %6\n\t" MFMA " %0, %2, %4, " D("%0") "\n\ts_nop 1\n\t" MFMA " %1, %3, %4, " D("%1") "\n\t" LOAD                 \
+               " %7, %8, 0 offen lds"                                                                                                               \
+               : "+a"(acc0), "+a"(acc1) : "v"(c0), "v"(c1), "v"(r), "s"(base), "i"(AT), "v"(off), "s"(rsrc) : "memory", "scc")
+#define FLUXMI_SAME(x) x
+#define FLUXMI_ZERO(x) "0"
+#define FLUXMI_OF_SIZE(MFMA, D)                                             \
+  do {                                                                      \
+    if constexpr (BYTE) FLUXMI_MFMA_AND_LOAD(MFMA, D, "buffer_load_ubyte"); \
+    else FLUXMI_MFMA_AND_LOAD(MFMA, D, "buffer_load_dwordx4");              \
+  } while (0)
+  if constexpr (F16 && FIRST) FLUXMI_OF_SIZE("v_mfma_f32_16x16x32_f16", FLUXMI_ZERO);
+  else if constexpr (F16) FLUXMI_OF_SIZE("v_mfma_f32_16x16x32_f16", FLUXMI_SAME);
+  else if constexpr (FIRST) FLUXMI_OF_SIZE("v_mfma_f32_16x16x32_bf16", FLUXMI_ZERO);
+  else FLUXMI_OF_SIZE("v_mfma_f32_16x16x32_bf16", FLUXMI_SAME);
+#undef FLUXMI_MFMA_AND_LOAD
+#undef FLUXMI_OF_SIZE
+#undef FLUXMI_SAME
+#undef FLUXMI_ZERO
 }
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte == 0 ? 0x00400000u : (byte == 255 ? 0x7fc00000u : byte << 23)); }
 
@@ -371,15 +397,6 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
   };
   const uint32_t cdst = lds0 + wave * 4096, rdst = cdst + rows_at(G), codes = lds0 + codes_at() + wave * 2048, scales = lds0 + scales_at() + wave * 256;
   using std::integral_constant;
-  // M0 for fill Q of the step in slot SLOT: where it goes.  (Base and constant apart: 28 addresses would take as many registers, and what the compiler brings back
-  // from a vector register's lanes right before a load comes too late for it.)
-  auto set_target = [&](auto SLOT, auto Q) {
-    constexpr int slot = decltype(SLOT)::value, q = decltype(Q)::value;
-    constexpr bool row = q >= kColFills, code = !row && EIGHT && q < 2, scale = !row && EIGHT && q == 2;
-    constexpr int at = row ? slot * kSlot + (q - kColFills) * 1024 : (code ? slot * kCodeSlot + q * 1024 : (scale ? slot * kScaleSlot : slot * kSlot + q * 1024));
-    const uint32_t base = row ? rdst : (code ? codes : (scale ? scales : cdst));
-    asm volatile("s_add_u32 m0, %0, %1" : : "s"(base), "i"(at) : "memory", "scc");
-  };
 
   f32x4 acc[8][8];  // [row block][column block]
 
@@ -436,20 +453,21 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
     *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(value_at[i] + (slot % 2) * kSlot + h * 16) = value[i][h];
   };
 
-  auto fill = [&](auto Q) {
-    constexpr int q = decltype(Q)::value, r = q - kColFills;
-    if constexpr (r >= 0) load_to_lds<false>(roff[r < 0 ? 0 : r], rrsrc);
-    else if constexpr (EIGHT && q == 2) load_to_lds<true>(coff[2], srsrc);
-    else load_to_lds<false>(coff[q < 4 ? q : 0], crsrc);
+  // Fill Q of the step in slot SLOT, by `load`(bytes, where: base and constant, offsets, buffer).  (Base and constant apart: 28 addresses would take as many registers.)
+  auto fill_by = [&](auto SLOT, auto Q, auto &&load) {
+    constexpr int slot = decltype(SLOT)::value, q = decltype(Q)::value, r = q - kColFills;
+    if constexpr (r >= 0) load(std::false_type{}, rdst, integral_constant<int, slot * kSlot + (r < 0 ? 0 : r) * 1024>{}, roff[r < 0 ? 0 : r], rrsrc);
+    else if constexpr (EIGHT && q == 2) load(std::true_type{}, scales, integral_constant<int, slot * kScaleSlot>{}, coff[2], srsrc);
+    else if constexpr (EIGHT) load(std::false_type{}, codes, integral_constant<int, slot * kCodeSlot + q * 1024>{}, coff[q < 4 ? q : 0], crsrc);
+    else load(std::false_type{}, cdst, integral_constant<int, slot * kSlot + q * 1024>{}, coff[q < 4 ? q : 0], crsrc);
+  };
+  auto fill = [&](auto SLOT, auto Q) {
+    fill_by(SLOT, Q, [&](auto BYTE, uint32_t base, auto AT, uint32_t off, __amdgpu_buffer_rsrc_t rsrc) { load_to_lds<decltype(BYTE)::value, decltype(AT)::value>(base, off, rsrc); });
   };
   auto first_fills = [&]() {
     static_for<kSlots>([&](auto S) {
       next_buffers();
-      static_for<kFills>([&](auto Q) {
-        set_target(S, Q);
-        asm volatile("s_nop 0" : : : "memory");
-        fill(Q);
-      });
+      static_for<kFills>([&](auto Q) { fill(S, Q); });
     });
     next_buffers();
   };
@@ -526,11 +544,7 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
       static_for<8>([&](auto I) {
         constexpr int i = decltype(I)::value;
         static_for<kReads / 8>([&](auto R) { read_one(integral_constant<int, (u + 1) % kSlots>{}, integral_constant<int, i * (kReads / 8) + decltype(R)::value>{}, cn, rn); });
-        if constexpr (i < kFills) {
-          set_target(U, I);
-          asm volatile("s_nop 0" : : : "memory");
-          fill(I);
-        }
+        if constexpr (i < kFills) fill(U, I);
         if constexpr (i == 7) next_buffers();
         __builtin_amdgcn_sched_barrier(0);
         row_block<F16, decltype(FIRST)::value>(acc[i], cf, rf[i], i, row_blocks);
@@ -540,10 +554,14 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
       constexpr int t = decltype(T)::value, q = t / 8;
       conversion(U, T);
       if constexpr (t < 2 * kReads && t % 2 == 0) read_one(integral_constant<int, (u + 1) % kSlots>{}, integral_constant<int, t / 2>{}, cn, rn);
-      if constexpr (t % 8 == 3 && q < kFills) set_target(U, integral_constant<int, q>{});
-      if constexpr (t % 8 == 4 && q < kFills) fill(integral_constant<int, q>{});
       if constexpr (t == 62) next_buffers();
-      mfma<F16, decltype(FIRST)::value>(acc[t / 8][t % 8], cf[t % 8], rf[t / 8]);
+      if constexpr (t % 8 == 4 && q < kFills) {  // (MFMAs t and t + 1)
+        fill_by(U, integral_constant<int, q>{}, [&](auto BYTE, uint32_t base, auto AT, uint32_t off, __amdgpu_buffer_rsrc_t rsrc) {
+          mfma_and_load<F16, decltype(FIRST)::value, decltype(BYTE)::value, decltype(AT)::value>(acc[q][4], acc[q][5], cf[4], cf[5], rf[q], base, off, rsrc);
+        });
+      } else if constexpr (t % 8 != 5 || q >= kFills) {
+        mfma<F16, decltype(FIRST)::value>(acc[q][t % 8], cf[t % 8], rf[q]);
+      }
       __builtin_amdgcn_sched_barrier(0);
     });
     FLUXMI_LGKM0();
