@@ -206,6 +206,23 @@ struct Swiglu : torch::autograd::Function<Swiglu> {
   }
 };
 
+// The same with the codes and scales among the results, which have no gradients of their own.
+struct SwigluKept : torch::autograd::Function<SwigluKept> {
+  static variable_list forward(AutogradContext *ctx, const torch::Tensor &input) {
+    const auto [out, codes, scale] = swiglu(input, true);
+    ctx->mark_non_differentiable({codes, scale});
+    ctx->set_materialize_grads(false);  // (theirs would be zeros of 8 bits)
+    ctx->save_for_backward({codes, scale});
+    return {out, codes, scale};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    if (!grads[0].defined()) return {torch::Tensor()};
+    const torch::Tensor grad = incoming("moe_swiglu_checkpoint", grads);
+    const auto saved = ctx->get_saved_variables();
+    return {std::get<0>(swiglu_gradient(grad, saved[0], saved[1], false))};
+  }
+};
+
 // Of what lies between the two products the backward pass keeps the activation's input alone; its output is computed again beside the gradient.
 struct Mlp : torch::autograd::Function<Mlp> {
   static torch::Tensor forward(AutogradContext *ctx, const torch::Tensor &input, const torch::Tensor &weight1, const torch::Tensor &weight2,
@@ -322,6 +339,10 @@ std::tuple<torch::Tensor, torch::Tensor> moe_checkpoint(torch::Tensor input) {
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_swiglu_checkpoint(torch::Tensor input) {
   check_operand(input, "input", 2);
   TORCH_CHECK(input.size(1) % 2 == 0, "input must have gate and up columns, got ", input.size(1));
+  if (at::GradMode::is_enabled() && input.requires_grad()) {
+    const variable_list results = SwigluKept::apply(input);
+    return {results[0], results[1], results[2]};
+  }
   return swiglu(input, true);
 }
 

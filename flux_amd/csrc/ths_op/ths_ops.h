@@ -189,7 +189,8 @@ std::tuple<torch::Tensor, torch::Tensor> moe_unpermute_backward(torch::Tensor gr
 torch::Tensor moe_linear(torch::Tensor input, torch::Tensor weight, torch::Tensor splits, bool checkpoint);
 torch::Tensor moe_swiglu(torch::Tensor input, bool checkpoint);
 torch::Tensor moe_mlp(torch::Tensor input, torch::Tensor weight1, torch::Tensor weight2, torch::Tensor splits, bool checkpoint);
-// The gradients, for callers without autograd, and the 8 bits: e4m3 codes and a float8_e8m0fnu scale for every 32 values of a row.
+// The gradients, for callers without autograd, and the 8 bits: e4m3 codes and a float8_e8m0fnu scale for every 32 values of a row.  They record nothing, but for
+// moe_swiglu_checkpoint's first result, whose gradient is that of moe_swiglu with checkpoint.
 torch::Tensor moe_dgrad(torch::Tensor grad, torch::Tensor weight, torch::Tensor splits);
 torch::Tensor moe_wgrad(torch::Tensor grad, torch::Tensor input, torch::Tensor splits, std::optional<torch::Tensor> input_scale,
                         std::optional<torch::Tensor> output, bool accumulate, std::optional<at::ScalarType> output_dtype);
