@@ -207,7 +207,7 @@ __global__ __launch_bounds__(kThreads) void checkpoint_kernel(const RowsArgs a) 
   }
 }
 
-// KEPT: from codes and scales, otherwise from 16 bits.
+// KEPT: from codes and scales, otherwise from 16 bits.  Without a gradient: the activation alone.
 template <Row T, bool KEPT, int PASS>
 __global__ __launch_bounds__(kThreads) void swiglu_backward_kernel(const RowsArgs a) {
   const Place p = place_of(a);
@@ -225,6 +225,12 @@ __global__ __launch_bounds__(kThreads) void swiglu_backward_kernel(const RowsArg
     unpack<T>(load_some<T, PASS == 2>(x + static_cast<int64_t>(a.cols) * 2, count), u);
   }
   const int64_t at = (p.row * a.cols + p.col) * 2;
+  if (a.grad == nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = g[i] * sigmoid(g[i]) * u[i];
+    store_some<PASS != 0>(a.out + at, pack<T>(o), count);
+    return;
+  }
   unpack<T>(load_some<T, PASS == 2>(a.grad + at, count), d);
   // Gradient times value comes first: times the slope of a gate that closes, a small gradient would be below fp32.  Only where gradient times value is beyond fp32 the slope
   // comes in between: there the gradient is over 1, and its product with a slope is in range.
@@ -351,7 +357,7 @@ extern "C" int fluxmi_swiglu_backward(const void *grad, const void *x, const voi
   uint32_t grid;
   if (const int rc = plan_rows("swiglu_backward", &a, &grid)) return rc;
   if (grid == 0) return FLUXMI_OK;
-  FLUXMI_REQUIRE(grad && x && grad_x, FLUXMI_ERR_INVALID_ARG, "swiglu_backward: null pointer");
+  FLUXMI_REQUIRE(x && (grad || out) && (grad != nullptr) == (grad_x != nullptr), FLUXMI_ERR_INVALID_ARG, "swiglu_backward: null pointer");
   FLUXMI_REQUIRE(even(grad) && (x_scale != nullptr || even(x)) && even(grad_x) && even(out), FLUXMI_ERR_INVALID_ARG,
                  "swiglu_backward: a pointer is not aligned to its elements");
   a.grad = static_cast<const uint8_t *>(grad);
@@ -359,7 +365,7 @@ extern "C" int fluxmi_swiglu_backward(const void *grad, const void *x, const voi
   a.in_scale = static_cast<const uint8_t *>(x_scale);
   a.grad_x = static_cast<uint8_t *>(grad_x);
   a.out = static_cast<uint8_t *>(out);
-  by_half(type, rows * cols * (x_scale != nullptr ? 10 : 12), a.cols, [&](auto T, auto PASS) {
+  by_half(type, rows * cols * ((x_scale != nullptr ? 2 : 4) + (grad != nullptr ? 8 : 2)), a.cols, [&](auto T, auto PASS) {
     if (x_scale != nullptr) swiglu_backward_kernel<decltype(T)::value, true, decltype(PASS)::value><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
     else swiglu_backward_kernel<decltype(T)::value, false, decltype(PASS)::value><<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
   });

@@ -160,6 +160,16 @@ std::tuple<torch::Tensor, torch::Tensor> swiglu_gradient(const torch::Tensor &gr
   return {grad_input, out};
 }
 
+// The activation alone, from what swiglu_gradient has it from.
+torch::Tensor activation(const torch::Tensor &input, const torch::Tensor &scale, at::ScalarType dtype) {
+  const c10::DeviceGuard guard(input.device());
+  torch::Tensor out = empty_on(input, {input.size(0), input.size(1) / 2}, dtype);
+  check_status(fluxmi_swiglu_backward(nullptr, input.data_ptr(), scale.defined() ? scale.data_ptr() : nullptr, row_type(out), out.size(0), out.size(1), nullptr, out.data_ptr(),
+                                      current_stream()),
+               "fluxmi_swiglu_backward");
+  return out;
+}
+
 // ---- autograd -------------------------------------------------------------------------------------------------
 
 using torch::autograd::AutogradContext;
@@ -231,9 +241,7 @@ struct Mlp : torch::autograd::Function<Mlp> {
     const auto [x, x_scale] = kept_of(input, weight1.requires_grad(), checkpoint);
     const torch::Tensor hidden = product(input, weight1, splits);
     const auto [act, codes, scale] = swiglu(hidden, checkpoint);
-    ctx->save_for_backward({splits, x, x_scale, checkpoint ? codes : hidden, scale, input.requires_grad() ? weight1 : torch::Tensor(),
-                            below || weight2.requires_grad() ? weight2 : torch::Tensor()});
-    ctx->saved_data["below"] = below;
+    ctx->save_for_backward({splits, x, x_scale, checkpoint ? codes : hidden, scale, input.requires_grad() ? weight1 : torch::Tensor(), below ? weight2 : torch::Tensor()});
     ctx->saved_data["weight2"] = weight2.requires_grad();
     return product(act, weight2, splits);
   }
@@ -242,9 +250,10 @@ struct Mlp : torch::autograd::Function<Mlp> {
     const auto saved = ctx->get_saved_variables();
     const torch::Tensor &splits = saved[0], &x = saved[1], &x_scale = saved[2], &hidden = saved[3], &scale = saved[4], &weight1 = saved[5], &weight2 = saved[6];
     const bool want_weight2 = ctx->saved_data["weight2"].toBool();
-    // (the second weights' gradient alone still takes the activation, which comes with its input's gradient)
-    const auto [grad_hidden, act] = swiglu_gradient(input_gradient(grad, weight2, splits), hidden, scale, want_weight2);
-    torch::Tensor grad_input, grad_weight1, grad_weight2;
+    torch::Tensor grad_hidden, act, grad_input, grad_weight1, grad_weight2;
+    // (the second weights' gradient alone takes the activation, but no gradient of its input, which comes through those weights)
+    if (weight2.defined()) std::tie(grad_hidden, act) = swiglu_gradient(input_gradient(grad, weight2, splits), hidden, scale, want_weight2);
+    else act = activation(hidden, scale, grad.scalar_type());
     if (want_weight2) grad_weight2 = weight_gradient_like(grad, act, {}, splits);
     if (x.defined()) grad_weight1 = weight_gradient_like(grad_hidden, x, x_scale, splits);
     if (weight1.defined()) grad_input = input_gradient(grad_hidden, weight1, splits);

@@ -507,6 +507,7 @@ int fluxmi_moe_clear_rest(void *data, const int32_t *splits, int32_t nexperts, i
  *   fluxmi_swiglu            x [rows, 2 cols], gate and up halves -> out [rows, cols] = gate / (1 + exp(-gate)) * up; with codes and scale (both or
  *                            neither) also the checkpoint of x: codes [rows, 2 cols], scale [rows, 2 ceil(cols / 32)], each half in blocks of its own
  *   fluxmi_swiglu_backward   grad [rows, cols], x as above, or codes with x_scale -> grad_x [rows, 2 cols], and out again unless NULL
+ *                            (grad and grad_x NULL: out alone)
  *
  * `row_type` is FLUXMI_ROWS_BF16 or FLUXMI_ROWS_FP16, of x, out, grad and grad_x; what is between is fp32, rounded once: 1 / (1 + exp(-gate)) below 2^-126 (gate < -87.3) may be 0,
  * no product on the way to grad_x is below or beyond fp32 where the result is not.  Pointers are aligned to their elements; cols <= 2^30; a launch has no more than 2^32 threads, of which eight columns take one (more rows: FLUXMI_ERR_UNSUPPORTED).

@@ -62,3 +62,43 @@ def test_swiglu_checkpoint_refuses_what_the_activation_refuses():
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             flux_amd.moe_swiglu_checkpoint(x)[0].sum().backward()
     del alive
+
+
+# ---- the second weights alone ---------------------------------------------------------------------------------------
+
+
+def mlp_operands(splits, rest, hidden, ffn, dtype):
+    return (data((sum(splits) + rest, hidden), dtype, 1), data((len(splits), 2 * ffn, hidden), dtype, 2, hidden**-0.5), data((len(splits), hidden, ffn), dtype, 3, ffn**-0.5))
+
+
+@pytest.mark.parametrize("ckpt", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("splits,rest,hidden,ffn", [([20, 0, 11], 3, 64, 33), ([300, 70], 0, 128, 160), ([0, 0], 2, 8, 8)])
+def test_second_weights_alone(splits, rest, hidden, ffn, dtype, ckpt):
+    """Their gradient has the bits of a pass over everything, and the pass neither reads nor keeps the weights: they may change in between."""
+    x, w1, w2 = mlp_operands(splits, rest, hidden, ffn, dtype)
+    up = data((x.shape[0], hidden), dtype, 4)
+    whole = [t.clone().requires_grad_() for t in (x, w1, w2)]
+    flux_amd.moe_mlp(*whole, counts(splits), checkpoint=ckpt).backward(up)
+    alone = w2.clone().requires_grad_()
+    out = flux_amd.moe_mlp(x, w1, alone, counts(splits), checkpoint=ckpt)
+    with torch.no_grad():
+        alone.mul_(2)
+    out.backward(up)
+    assert torch.equal(alone.grad, whole[2].grad)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 31), (129, 2047), (40, 96)])
+def test_the_activation_alone(rows, cols, dtype):
+    """The C entry without a gradient: the bits that come beside one, and nothing else is written."""
+    from flux_amd import capi
+
+    x = data((rows, 2 * cols), dtype, 1, 3.0)
+    out, codes, scale = flux_amd.moe_swiglu_checkpoint(x)
+    grad = data((rows, cols), dtype, 2)
+    for given, its_scale in ((x, None), (codes, scale)):
+        want = flux_amd.moe_swiglu_backward(grad, given, its_scale)[1]
+        flat = torch.full((rows * cols + 16,), 7.0, dtype=dtype, device=DEV)
+        rc = capi.load().fluxmi_swiglu_backward(None, capi._ptr(given), capi._ptr(its_scale), capi._ROW_TYPES[dtype], rows, cols, None, capi._ptr(flat), capi._stream())
+        assert rc == 0 and torch.equal(flat[:rows * cols].view(rows, cols), want) and (flat[rows * cols:] == 7).all()
