@@ -198,8 +198,8 @@ struct Linear : torch::autograd::Function<Linear> {
     const torch::Tensor grad = incoming("moe_linear", grads);
     const auto saved = ctx->get_saved_variables();
     const torch::Tensor &splits = saved[0], &x = saved[1], &x_scale = saved[2], &weight = saved[3];
-    return {weight.defined() ? input_gradient(grad, weight, splits) : torch::Tensor(),
-            x.defined() ? weight_gradient_like(grad, x, x_scale, splits) : torch::Tensor(), {}, {}};
+    return {ctx->needs_input_grad(0) ? input_gradient(grad, weight, splits) : torch::Tensor(),
+            ctx->needs_input_grad(1) ? weight_gradient_like(grad, x, x_scale, splits) : torch::Tensor(), {}, {}};
   }
 };
 
@@ -233,7 +233,8 @@ struct SwigluKept : torch::autograd::Function<SwigluKept> {
   }
 };
 
-// Of what lies between the two products the backward pass keeps the activation's input alone; its output is computed again beside the gradient.
+// Of what lies between the two products the backward pass keeps the activation's input alone; its output is computed again beside the gradient.  A backward pass may be asked for fewer
+// gradients than the forward pass kept for (torch.autograd.grad), and computes those.
 struct Mlp : torch::autograd::Function<Mlp> {
   static torch::Tensor forward(AutogradContext *ctx, const torch::Tensor &input, const torch::Tensor &weight1, const torch::Tensor &weight2,
                                const torch::Tensor &splits, bool checkpoint) {
@@ -242,21 +243,20 @@ struct Mlp : torch::autograd::Function<Mlp> {
     const torch::Tensor hidden = product(input, weight1, splits);
     const auto [act, codes, scale] = swiglu(hidden, checkpoint);
     ctx->save_for_backward({splits, x, x_scale, checkpoint ? codes : hidden, scale, input.requires_grad() ? weight1 : torch::Tensor(), below ? weight2 : torch::Tensor()});
-    ctx->saved_data["weight2"] = weight2.requires_grad();
     return product(act, weight2, splits);
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const torch::Tensor grad = incoming("moe_mlp", grads);
     const auto saved = ctx->get_saved_variables();
     const torch::Tensor &splits = saved[0], &x = saved[1], &x_scale = saved[2], &hidden = saved[3], &scale = saved[4], &weight1 = saved[5], &weight2 = saved[6];
-    const bool want_weight2 = ctx->saved_data["weight2"].toBool();
+    const bool want_input = ctx->needs_input_grad(0), want_weight1 = ctx->needs_input_grad(1), want_weight2 = ctx->needs_input_grad(2);
     torch::Tensor grad_hidden, act, grad_input, grad_weight1, grad_weight2;
     // (the second weights' gradient alone takes the activation, but no gradient of its input, which comes through those weights)
-    if (weight2.defined()) std::tie(grad_hidden, act) = swiglu_gradient(input_gradient(grad, weight2, splits), hidden, scale, want_weight2);
-    else act = activation(hidden, scale, grad.scalar_type());
+    if (want_input || want_weight1) std::tie(grad_hidden, act) = swiglu_gradient(input_gradient(grad, weight2, splits), hidden, scale, want_weight2);
+    else if (want_weight2) act = activation(hidden, scale, grad.scalar_type());
     if (want_weight2) grad_weight2 = weight_gradient_like(grad, act, {}, splits);
-    if (x.defined()) grad_weight1 = weight_gradient_like(grad_hidden, x, x_scale, splits);
-    if (weight1.defined()) grad_input = input_gradient(grad_hidden, weight1, splits);
+    if (want_weight1) grad_weight1 = weight_gradient_like(grad_hidden, x, x_scale, splits);
+    if (want_input) grad_input = input_gradient(grad_hidden, weight1, splits);
     return {grad_input, grad_weight1, grad_weight2, {}, {}};
   }
 };

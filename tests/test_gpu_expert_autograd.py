@@ -102,3 +102,53 @@ def test_the_activation_alone(rows, cols, dtype):
         flat = torch.full((rows * cols + 16,), 7.0, dtype=dtype, device=DEV)
         rc = capi.load().fluxmi_swiglu_backward(None, capi._ptr(given), capi._ptr(its_scale), capi._ROW_TYPES[dtype], rows, cols, None, capi._ptr(flat), capi._stream())
         assert rc == 0 and torch.equal(flat[:rows * cols].view(rows, cols), want) and (flat[rows * cols:] == 7).all()
+
+
+# ---- backward passes that are asked for some of the gradients -------------------------------------------------------
+
+
+def allocated(call):
+    """A call's result, and the bytes that it allocated, freed ones among them."""
+    before = torch.cuda.memory_stats()["allocated_bytes.all.allocated"]
+    result = call()
+    return result, torch.cuda.memory_stats()["allocated_bytes.all.allocated"] - before
+
+
+@pytest.mark.parametrize("ckpt", [False, True])
+def test_gradients_that_are_not_asked_for_are_not_computed(ckpt):
+    """A weights' gradient that is left out leaves out its memory."""
+    splits, hidden, ffn = [5, 0, 9, 2], 512, 1024
+    leaves = [t.requires_grad_() for t in mlp_operands(splits, 0, hidden, ffn, BF16)]
+    x, w1, w2 = leaves
+    up, up1 = data((16, hidden), BF16, 4), data((16, 2 * ffn), BF16, 5)
+    out = flux_amd.moe_mlp(*leaves, counts(splits), checkpoint=ckpt)
+    whole, all_bytes = allocated(lambda: torch.autograd.grad(out, leaves, up))
+    for wanted in range(1, 7):
+        some = [i for i in range(3) if wanted >> i & 1]
+        out = flux_amd.moe_mlp(*leaves, counts(splits), checkpoint=ckpt)
+        got, its_bytes = allocated(lambda: torch.autograd.grad(out, [leaves[i] for i in some], up))
+        assert all(torch.equal(g, whole[i]) for g, i in zip(got, some))
+        assert its_bytes <= all_bytes - sum(t.numel() * 2 for i, t in enumerate(leaves) if i not in some)
+    out = flux_amd.moe_linear(x, w1, counts(splits), ckpt)
+    whole, all_bytes = allocated(lambda: torch.autograd.grad(out, [x, w1], up1))
+    for i, leaf in enumerate((x, w1)):
+        out = flux_amd.moe_linear(x, w1, counts(splits), ckpt)
+        got, its_bytes = allocated(lambda: torch.autograd.grad(out, [leaf], up1))
+        assert torch.equal(got[0], whole[i]) and its_bytes <= all_bytes - (w1 if i == 0 else x).numel() * 2
+
+
+def test_a_frozen_layer_before_one_that_learns():
+    """Gradients of intermediate results, of a graph in which some leaves want none, and of one leaf used twice."""
+    splits = counts([20, 13])
+    x, w1, w2 = mlp_operands([20, 13], 0, 64, 32, BF16)
+    x.requires_grad_()
+    middle = x * 2
+    out = flux_amd.moe_mlp(middle, w1, w2, splits)
+    up = data(out.shape, BF16, 4)
+    of_middle, = torch.autograd.grad(out, [middle], up, retain_graph=True)
+    of_x, = torch.autograd.grad(out, [x], up)
+    assert torch.equal(of_x, of_middle * 2)
+    w = data((2, 64, 64), BF16, 5, 0.1).requires_grad_()
+    y = flux_amd.moe_linear(flux_amd.moe_linear(x, w, splits), w, splits)
+    a, b = torch.autograd.grad(y, [x, w], up, retain_graph=True)
+    assert torch.equal(torch.autograd.grad(y, [w], up, retain_graph=True)[0], b) and torch.equal(torch.autograd.grad(y, [x], up)[0], a)
