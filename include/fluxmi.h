@@ -479,6 +479,7 @@ int fluxmi_grouped_gemm_mx_launch_info(const fluxmi_mx_gemm_args *args, fluxmi_m
  *
  * `row_type` (FLUXMI_ROWS_BF16 or FLUXMI_ROWS_FP16) is the type of grad [rows, n], weight, input [rows, k] and grad_input [rows, k]; grad_weight is of
  * `out_type`: that or FLUXMI_ROWS_FP32.  Sums are fp32, in an order that follows from the sizes, the row counts and the alignment alone, and are rounded once.
+ * (A subnormal factor counts as its type's least normal number in the rounding of a sum: the matrix unit aligns products by their factors' exponents.)
  * `splits`: DEVICE int32 row counts.  Negative ones are 0; what they have past `rows` does not exist.  Rows past the sum are not read by fluxmi_moe_wgrad.
  * Requirements: nexperts <= 1024; rows, n, k <= 2^24; operands aligned to their elements, grad_input to 8 bytes, grad_weight and workspace to 16.  Operands
  * that start on 16 bytes with n and k multiples of 8 are fast.
