@@ -13,7 +13,7 @@
 //
 // Memory bounds all of it: every byte is read and written once.  A lane has eight values of a row (16 bytes in, 8 out), four lanes a block, whose maximum they find among
 // themselves; rows of any length and start, whole vectors wherever eight values are left.  Of MI355X's 8 TB/s (a copy reaches 5.6, reading alone 6.9): swiglu with a checkpoint of
-// 16384 x 2 x 14336 bf16 303 us, 6.2 TB/s; its gradient from 8 bits 385 us, 6.1 TB/s; a checkpoint of 16384 x 4096 39 us, 5.3 TB/s; calls below 10 MB take 5 to 6 us, which is the
+// 16384 x 2 x 14336 bf16 304 us, 6.2 TB/s, without one 227, 6.2; its gradient from 8 bits 384 us, 6.1 TB/s, from 16 bits 494, 5.7; a checkpoint of 16384 x 4096 39 us, 5.3 TB/s; calls below 10 MB take 5 to 6 us, which is the
 // way through the call and not the memory.
 #include "rows.hpp"
 
@@ -285,6 +285,9 @@ int plan_rows(const char *who, RowsArgs *a, uint32_t *grid) {
 // f(type, PASS): 0, or results pass the caches by (1), or inputs as well (2).  A call of `bytes` in all; us with 0 / 1 / 2: swiglu with a checkpoint 16384 x 14336 339 / 326 / 304, 16384 x 4096
 // 94 / 78 / 87, 20000 x 1407 41 / 42 / 60; its gradient from 8 bits 414 / 392 / 386, 115 / 98 / 108, 89 / 56 / 86.  Inputs of a few hundred MB are still cached where they
 // were just made, and rows that do not start on lines would be fetched twice.
+// Around 96 MiB results in the caches are what a reader right behind the call gains by: 4096 columns, a call alone on inputs from memory and with a read of its results, 0 / 1: with a checkpoint 48 MiB
+// 12.7 / 11.5 and 15.2 / 15.6, 96 MiB 20.4 / 19.6 and 24.2 / 25.2, 192 MiB 37.3 / 35.6 and 42.1 / 44.7; gradient from 16 bits 11.8 / 9.9 and 20.6 / 20.6, 22.5 / 19.6 and 30.5 / 30.9, 39.0 / 36.4 and
+// 51.4 / 55.0; checkpoint alone 12.4 / 12.0 and 15.7 / 16.4, 21.9 / 21.1 and 27.4 / 28.0, 39.2 / 38.4 and 48.7 / 50.1.  From 1 GiB on, 0 / 1 / 2 of 1100 MiB, alone: 198 / 191 / 184, 200 / 196 / 189, 199 / 202 / 202.
 template <class F>
 void by_half(Row t, int64_t bytes, int32_t cols, F &&f) {
   const int pass = bytes < (int64_t{96} << 20) ? 0 : (bytes < (int64_t{1} << 30) || cols % 64 != 0 ? 1 : 2);

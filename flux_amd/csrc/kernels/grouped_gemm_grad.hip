@@ -11,7 +11,8 @@
 //
 // Here: pieces of 128 x 128 on four waves, one step in LDS and the next in registers, for operands of any width and start and for small products; the weights' sums are cut into parts
 // of 256 rows or more where pieces are few, so that the card is full.  Latency and barriers bound them: 8 experts 1024 x 1024, 2048 rows 15 us (weights), 26 (input); at the large
-// sizes of grouped_gemm_grad_tiles.hip, which computes what is larger, they take 2360 and 2460 where its tiles take 1430 and 1470.
+// sizes of grouped_gemm_grad_tiles.hip, which computes what is larger, they take 2360 and 2460 where its tiles take 1435 and 1470.  Operands that tiles refuse cost more: 8 experts
+// 14336 x 4092, 16384 rows 5130 (weights), 6130 (from 8 bits) and 6510 (input), most of it loads element by element; 14336 x 4096 with an input off 16 bytes 2820 (weights).
 #include "grouped_gemm_grad_tiles.hpp"
 
 namespace fluxmi {

@@ -11,14 +11,15 @@
 //    LDS held there reaches no result that is stored.
 //  * A checkpoint's codes and scale bytes (WEIGHT_8BIT) are fetched like the rest, and each wave turns what it fetched to values of 16 bits two steps ahead, in LDS, beside the
 //    MFMAs; the values are exact in the rows' type.
-//  * One workgroup to a compute unit computes several tiles, in turns or (weights, experts of different sizes) from a queue to each XCD.  The next tile's first four steps are
+//  * One workgroup to a compute unit computes several tiles, in turns or (weights of several experts, four turns or more) from a queue to each XCD.  The next tile's first four steps are
 //    requested before a tile's results go out, through a window in LDS and in whole lines.  The last turn's tiles are cut along the sum where that is cheaper, and joined in
 //    the parts' order: results have the same bits in every launch.
 //
-// What bounds it on MI355X (us): large products the board's power, 8 experts 14336 x 4096, 16384 rows: input 1470, weights 1430, 1.31 to 1.34 PFLOP/s, MFMA 70 to 79 % busy at 1.5 to 1.9 GHz
-// (zero operands reach 1.75 PFLOP/s).  Many small experts what lies between two tiles' sums, about 7 to each of 25 to 45: 64 skewed experts, 93000 rows, input 1408 x 2048 530, weights
-// 1400 x 2040 to fp32 607 (1408 x 2048, whose rows begin on lines, 560).  Weights from 8 bits, 32 experts 2048 x 7168 to fp32, 32768 rows: 1050, the conversion a tenth of it.  Few rows
-// the read of W: 74 rows on 8 experts 14336 x 4096 166, 5.7 TB/s.
+// What bounds it on MI355X (us): large products the board's power, 8 experts 14336 x 4096, 16384 rows: input 1470, weights 1435, 1.31 to 1.34 PFLOP/s, MFMA 77 and 68 % busy at 1.6 to 1.8 GHz
+// (zero operands reach 1.75 PFLOP/s).  Many small experts what lies between two tiles' sums, about 7 to each of 25 to 45, with MFMA 57 and 46 % busy: 64 skewed experts, 93000 rows, input
+// 1408 x 2048 525, weights 1400 x 2040 to fp32 606 (1408 x 2048, whose rows begin on lines, 560).  Weights from 8 bits, 32 experts 2048 x 7168 to fp32, 32768 rows: 1060, the conversion a
+// tenth of it, MFMA 39 % busy.  Few rows the read of W: 74 rows on 8 experts 14336 x 4096 167, 5.7 TB/s.  Results that are added to what is there wait for it store by store: the same
+// weights to bf16 2020, from 8 bits to fp32 1970, 1400 x 2040 to fp32 920.
 // Also built: without the window 1594 for weights (neighbouring lanes store to different rows); row blocks left out one by one in tiles of any height + 7 to 10 %; small and large
 // experts in turn from the queues 668 where the largest come first 631.
 #include "grouped_gemm_grad_tiles.hpp"
@@ -497,7 +498,8 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
   constexpr int kOpen = EIGHT ? kFills + 4 : 2 * kFills;
   // Loads and stores leave the counter in their order, also when the loads go to LDS from cold memory and a single store to the caches comes after them (measured: 3 G
   // words behind 1 to 96 stores, none missing).  A tile's first fills are requested before the stores of the tile before it, so that the first kFresh steps need not wait
-  // for those: kStores of them for 16 bits; twice as many for 32 bits, which with the fills are more than the counter holds: all fills are in before the first step.
+  // for those: kStores of them for 16 bits; twice as many for 32 bits, which with the fills are more than the counter holds: all fills are in before the first step.  (With queues the
+  // first wave waits for all of them before its first step: see where it asks for the next tile.)
   constexpr int kFresh = EIGHT ? 2 : 3, kStores = 32, kMostCounted = 62;
   static_assert(kOpen + kFills + kStores <= kMostCounted && 2 * kStores >= kMostCounted, "waits that the counter holds");
   int behind = 0;  // stores behind the first fills, times kStores
@@ -598,7 +600,8 @@ __global__ __launch_bounds__(kThreads, 1) void grad_tile_kernel(const TileArgs a
     if (rest < kStep && steps == 1) clear_rows(0);
     FLUXMI_LGKM0();
     __builtin_amdgcn_s_barrier();
-    // The next tile's number, asked for now and looked at when this one's sums are done.
+    // The next tile's number, which is looked at when this one's sums are done.  The compiler waits for it here, though, and with it for what the first wave has requested before: this
+    // tile's first fills and the last tile's stores; the other waves wait for it at the first step's barrier.
     int fetched = 0;
     if (!INPUT && args.queue != nullptr && threadIdx.x == 0) fetched = atomicAdd(args.queue + home * kQueueLine, 1);
     static_for<kReads>([&](auto R) { read_one(integral_constant<int, 0>{}, R, ca, ra); });
