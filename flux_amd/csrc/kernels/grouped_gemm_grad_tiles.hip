@@ -848,8 +848,8 @@ bool grad_tiles_are_faster(Grad g, int32_t nexperts, int64_t rows, int64_t n, in
   return flops >= 2.4e10 || most_tiles(g, nexperts, rows, n, k) >= 64;
 }
 
-// Experts of different sizes in several turns: a workgroup fetches its next tile when it has done with one.  The result has the same bits: a tile's sum is the same wherever
-// it is computed.
+// Several experts in four turns or more: a workgroup fetches its next tile when it has done with one.  The result has the same bits: a tile's sum is the same wherever
+// it is computed.  us, queue / turns: 64 skewed experts 1400 x 2040 to fp32 602 / 735; equal ones, 8 of 14336 x 4096 1400 / 1401, 32 of 2048 x 7168 from 8 bits 1047 / 1060.
 static bool by_queue(Grad g, int64_t nexperts, int64_t tiles, int grid) { return g != Grad::INPUT && nexperts > 1 && tiles >= 4 * static_cast<int64_t>(grid); }
 
 size_t grad_tiles_workspace_bytes(Grad g, int32_t nexperts, int64_t rows, int64_t n, int64_t k) {

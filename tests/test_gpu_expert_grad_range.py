@@ -92,3 +92,67 @@ def test_every_scale_byte(n, k):
     want[0] = 255.5
     want[1:] = torch.tensor([0.5 if byte[(i * 7) % rows] == 0 else 1.0 for i in range(1, n)])
     assert np.array_equal(got.numpy(), want.view(n, 1).expand(n, k).numpy())
+
+
+@pytest.mark.parametrize("kept", [False, True])
+def test_as_many_experts_as_there_may_be(kept):
+    """1024 of them by tiles: whole tables, and tiles from the queues."""
+    n, k, g = 264, 272, torch.Generator().manual_seed(1)
+    splits = torch.randint(0, 9, (1024,), generator=g).tolist()
+    splits[0], splits[1023] = 40, 33
+    rows, at = sum(splits) + 3, torch.tensor([0] + splits).cumsum(0).tolist()
+    on = torch.tensor(splits, dtype=torch.int32, device=DEV)
+    grad, x, w, scale = signs((rows, n), BF16, 1, (-3, 0)), signs((rows, k), BF16, 2, (-3, 0)), signs((1024, n, k), BF16, 3, (-3, 0)), None
+    x64 = x.double()
+    if kept:
+        x, scale = flux_amd.moe_checkpoint(x)
+        x64 = torch.from_numpy(checkpoint.values(x.view(torch.uint8).cpu().numpy(), scale.view(torch.uint8).cpu().numpy())).to(DEV)
+    dw, dx = flux_amd.moe_wgrad(grad, x, on, scale, output_dtype=F32), flux_amd.moe_dgrad(grad, w, on)
+    for e in range(1024):
+        g64, v = grad[at[e]:at[e + 1]].double(), x64[at[e]:at[e + 1]]
+        close(dw[e], g64.t() @ v, max(splits) * 2.0**-23 * (g64.abs().t() @ v.abs()))
+        if not kept:
+            close(dx[at[e]:at[e + 1]], g64 @ w[e].double(), n * 2.0**-23 * (g64.abs() @ w[e].double().abs()))
+    assert not dx[-3:].any()
+
+
+WIDE = (1 << 22) - 8  # the most that tiles take
+PLACES = [0, 1, 255, 256, 2097143, 2097152, WIDE - 257, WIDE - 8, WIDE - 1]
+
+
+def test_the_widest_sum_of_tiles():
+    """300 rows of the widest gradient: 256 of them are 2 GiB less 4 KiB.  Few values are not 0, so that the sums are short."""
+    grad, w = torch.zeros(300, WIDE, dtype=BF16, device=DEV), torch.zeros(1, WIDE, 264, dtype=BF16, device=DEV)
+    few, rows = signs((300, len(PLACES)), BF16, 1, (-3, 0)), signs((len(PLACES), 264), BF16, 2, (-3, 0))
+    grad[:, PLACES], w[0, PLACES] = few, rows
+    got = flux_amd.moe_dgrad(grad, w, torch.tensor([290], dtype=torch.int32, device=DEV))
+    a, b = few[:290].double(), rows.double()
+    close(got[:290], a @ b, len(PLACES) * 2.0**-23 * (a.abs() @ b.abs()))
+    assert not got[290:].any()
+
+
+@pytest.mark.parametrize("out", [BF16, F32])
+def test_the_widest_results_of_tiles(out):
+    """Rows of results of 8 or 16 MB: 256 of them end 8 KiB below 4 GiB in fp32."""
+    grad, x = signs((40, 264), BF16, 1, (-3, 0)), signs((40, WIDE), BF16, 2, (-3, 0))
+    total = torch.empty(1, 264, WIDE, dtype=out, device=DEV)
+    got = flux_amd.moe_wgrad(grad, x, torch.tensor([37], dtype=torch.int32, device=DEV), output=total)[0]
+    a = grad[:37].double()
+    for c in range(0, WIDE, 1 << 20):
+        b = x[:37, c:c + (1 << 20)].double()
+        close(got[:, c:c + (1 << 20)], a.t() @ b, 37 * 2.0**-23 * (a.abs().t() @ b.abs()))
+    old = got[:, PLACES].double()
+    flux_amd.moe_wgrad(grad, x, torch.tensor([37], dtype=torch.int32, device=DEV), output=total, accumulate=True)
+    b = x[:37, PLACES].double()
+    close(got[:, PLACES], old + a.t() @ b, 37 * 2.0**-23 * (a.abs().t() @ b.abs()) + 2.0**-23 * (old.abs() + (a.t() @ b).abs()))
+
+
+def test_the_tallest_results_of_tiles():
+    """Experts of 16384 tiles along their rows, from the queues."""
+    x, grad = signs((21, 136), BF16, 1, (-3, 0)), signs((21, WIDE), BF16, 2, (-3, 0))
+    got = flux_amd.moe_wgrad(grad, x, torch.tensor([9, 12], dtype=torch.int32, device=DEV))
+    for e, r in ((0, slice(0, 9)), (1, slice(9, 21))):
+        a = x[r].double()
+        for c in range(0, WIDE, 1 << 20):
+            b = grad[r, c:c + (1 << 20)].double()
+            close(got[e, c:c + (1 << 20)], b.t() @ a, 12 * 2.0**-23 * (b.abs().t() @ a.abs()))
